@@ -465,6 +465,44 @@ int ttk_dense_scale_f64(const double* A, int D, double* scale, void* stream);
 int ttk_chol_prepare_dense_f64(const double* A, int D, const double* scale, double ridge, const double* b, const double* w,
                                void* chol_ws, void* stream);
 
+/* ---- rows in front of a model, answers behind it (ttk_norm.hip, ttk_sample.hip) ----
+ * Type codes: 0 float64, 1 float32, 2 bfloat16, 3 float16.  Pointers of these entry points need the alignment of their
+ * elements only; ld* = distance of two rows in elements (0: one row for all), the elements of a row are consecutive.
+ *
+ * Dropout: element number e = offset (+ *offset_dev, a device integer read when the kernel runs, if not NULL) + index is
+ * kept iff word e mod 4 of Philox4x32-10 with key = seed and counter = (e div 4, 0, 0) is >= min(round(p 2^32), 2^32 - 1),
+ * and then divided by 1 - p; dropped elements are 0 whatever they held.  0 <= p <= 1, offset >= 0.  The same call on the
+ * gradient is the backward pass.  x == y is allowed. */
+int ttk_dropout(int dtype, const void* x, void* y, int64_t n, double p, uint64_t seed, int64_t offset,
+                const int64_t* offset_dev, void* stream);
+
+/* Layer norm over the last axis, dropout as its epilogue (p = 0: none; element number = offset + row cols + column):
+ *   y = drop((x - mean) rstd w + b),  rstd = 1 / sqrt(mean((x - mean)^2) + eps)
+ * x (rows, cols) with row distance ldx, w / b (cols) or NULL in wdtype (dtype, or float32 for 16-bit rows), y dense,
+ * mean / rstd (rows) in float32 (float64 for float64 rows). */
+int ttk_layer_norm(int dtype, int wdtype, const void* x, int64_t ldx, const void* w, const void* b, void* y, void* mean,
+                   void* rstd, int64_t rows, int cols, double eps, double p, uint64_t seed, int64_t offset,
+                   const int64_t* offset_dev, void* stream);
+
+/* Its backward pass: with g = drop(dy), a = g w, h = (x - mean) rstd
+ *   dx = rstd (a - mean_j(a) - h mean_j(a h)),  dw = sum_rows g h,  db = sum_rows g
+ * dx dense, dw / db (cols) in wdtype; each may be NULL.  ws: ttk_layer_norm_backward_ws_bytes bytes when dw or db is wanted
+ * (partial column sums, added in a fixed order). */
+int64_t ttk_layer_norm_backward_ws_bytes(int dtype, int64_t rows, int cols);
+int ttk_layer_norm_backward(int dtype, int wdtype, const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w,
+                            const void* mean, const void* rstd, void* dx, void* dw, void* db, int64_t rows, int cols, double p,
+                            uint64_t seed, int64_t offset, const int64_t* offset_dev, void* ws, int64_t ws_bytes, void* stream);
+
+/* One label a row drawn from softmax(logits / temperature) cut by top-k, then top-p, then min-p, with the row's random
+ * number u in [0, 1): the first index whose cumulative kept weight exceeds u times the total.  Ties in the cuts go to the
+ * lowest index; NaN counts as -inf, -inf is never drawn, +inf takes all; temperature <= 0: lowest index of the maximum;
+ * a row without a logit above -inf: -1.  top_k <= 0 or >= V, top_p >= 1, min_p <= 0 switch a cut off.
+ * u: one value a row, float64 when f64 != 0 else float32; temperature / top_p / min_p: the same type, one value a row, or
+ * NULL for the *_all value; top_k: one int32 a row or NULL. */
+int ttk_sample(int dtype, const void* logits, int64_t ld, const void* u, int f64, const void* temperature,
+               double temperature_all, const int32_t* top_k, int top_k_all, const void* top_p, double top_p_all,
+               const void* min_p, double min_p_all, int64_t* label, int64_t rows, int V, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

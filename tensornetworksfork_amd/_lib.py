@@ -10,13 +10,14 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("TTK_LIB_PATH") or os.path.join(_HERE, "libttk.so")   # (override: diagnostic builds)
 SRC_PATH = os.path.join(_HERE, "csrc", "ttk.hip")
-SRC_PATHS = [SRC_PATH, os.path.join(_HERE, "csrc", "ttk_dense.hip")]
+SRC_PATHS = [SRC_PATH] + [os.path.join(_HERE, "csrc", f) for f in ("ttk_dense.hip", "ttk_norm.hip", "ttk_sample.hip")]
 INCLUDE_DIR = os.path.join(os.path.dirname(_HERE), "include")
 
 _c_dp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _dbl = ctypes.c_double
+_u64 = ctypes.c_uint64
 
 # name -> (restype, argtypes); must list every symbol include/ttk.h declares
 SIGNATURES = {
@@ -109,6 +110,14 @@ SIGNATURES = {
     "ttk_rows_matvec_f64": (_int, [_c_dp, _c_dp, _c_dp, _c_dp, _i64, _int, _int, _c_dp, _i64, _c_dp]),
     "ttk_rows_rhs_f64": (_int, [_c_dp, _c_dp, _c_dp, _i64, _int, _int, _c_dp, _i64, _c_dp]),
     "ttk_lhl_f64": (_int, [_c_dp, _c_dp, _c_dp, _c_dp, _i64, _int, _int, _c_dp]),
+    "ttk_dropout": (_int, [_int, _c_dp, _c_dp, _i64, _dbl, _u64, _i64, _c_dp, _c_dp]),
+    "ttk_layer_norm": (_int, [_int, _int, _c_dp, _i64, _c_dp, _c_dp, _c_dp, _c_dp, _c_dp, _i64, _int, _dbl, _dbl, _u64, _i64,
+                              _c_dp, _c_dp]),
+    "ttk_layer_norm_backward_ws_bytes": (_i64, [_int, _i64, _int]),
+    "ttk_layer_norm_backward": (_int, [_int, _int, _c_dp, _i64, _c_dp, _i64, _c_dp, _c_dp, _c_dp, _c_dp, _c_dp, _c_dp, _i64,
+                                       _int, _dbl, _u64, _i64, _c_dp, _c_dp, _i64, _c_dp]),
+    "ttk_sample": (_int, [_int, _c_dp, _i64, _c_dp, _int, _c_dp, _dbl, _c_dp, _int, _c_dp, _dbl, _c_dp, _dbl, _c_dp, _i64, _int,
+                          _c_dp]),
 }
 
 _lib = None
@@ -119,16 +128,26 @@ class TTKError(RuntimeError):
 
 
 def build(force=False, verbose=False):
-    """Compile csrc/ttk.hip for gfx950 into libttk.so (cross-compiles without a GPU)."""
+    """Compile csrc/*.hip for gfx950 into libttk.so (cross-compiles without a GPU), one compiler process per source."""
     import subprocess
+    import tempfile
     if not force and os.path.exists(LIB_PATH) and os.path.getmtime(LIB_PATH) >= max(
             [os.path.getmtime(s) for s in SRC_PATHS] + [os.path.getmtime(os.path.join(INCLUDE_DIR, "ttk.h"))]):
         return LIB_PATH
-    cmd = ["hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-shared", "-fPIC", "-I", INCLUDE_DIR,
-           "-o", LIB_PATH] + SRC_PATHS
-    if verbose:
-        print(" ".join(cmd))
-    subprocess.run(cmd, check=True)
+    # (the packed float32 instructions the compiler forms by itself have given wrong results on this hardware)
+    flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+    with tempfile.TemporaryDirectory() as tmp:
+        objs = [os.path.join(tmp, os.path.basename(s) + ".o") for s in SRC_PATHS]
+        cmds = [["hipcc"] + flags + ["-I", INCLUDE_DIR, "-c", "-o", o, s] for s, o in zip(SRC_PATHS, objs)]
+        link = ["hipcc", "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB_PATH] + objs
+        if verbose:
+            print("\n".join(" ".join(c) for c in cmds + [link]))
+        procs = [subprocess.Popen(c) for c in cmds]
+        codes = [p.wait() for p in procs]
+        for c, rc in zip(cmds, codes):
+            if rc:
+                raise subprocess.CalledProcessError(rc, c)
+        subprocess.run(link, check=True)
     return LIB_PATH
 
 

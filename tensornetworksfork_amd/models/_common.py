@@ -4,6 +4,9 @@ from time import time
 import numpy as np
 import torch
 
+from .. import ops
+from ..tensor.norm import dropout, layer_norm
+
 
 def root_mean_squared_error_torch(y_true, y_pred):
     """sklearn's root_mean_squared_error (per-output RMSE, uniform average), evaluated
@@ -25,6 +28,18 @@ def error_rate_torch(y_true, y_pred):
     pred = torch.argmax(y_pred, dim=1)
     true = torch.argmax(y_true, dim=1) if (y_true.ndim > 1 and y_true.shape[1] > 1) else y_true.reshape(-1).to(pred.dtype)
     return 1.0 - (pred == true).double().mean().item()
+
+
+def sample_labels(scores, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Labels drawn from softmax(scores / temperature) (..., classes), cut by top-k, then top-p, then min-p, with the given
+    random numbers u (...) in [0, 1): int64 (...), -1 where a row has no score above -inf.  temperature 0: the argmax.
+    The parameters are numbers, or tensors with one value a row (ops.sample)."""
+    if isinstance(scores, torch.Tensor) and scores.ndim and not scores.is_contiguous():
+        try:
+            ops.rows_view(scores)
+        except ops._lib.TTKError:
+            scores = scores.contiguous()
+    return ops.sample(scores, u, temperature, top_k, top_p, min_p)
 
 
 class EarlyStopping:
@@ -87,3 +102,38 @@ def split_train_val(X, y, seed, validation_split):
     cut = int(n * (1 - validation_split))
     tr, va = idx[:cut], idx[cut:]
     return X[tr], y[tr], X[va], y[va]
+
+
+class RowFrontEnd:
+    """What the estimators do with raw rows before the model sees them: layer norm over the features (layer_norm=True, at
+    training and at prediction) and dropout of the training rows (probability dropout).  The mask is drawn once per fit()
+    from (seed, element number), since the sweeps keep the environments of the rows they were given; the next fit() of the
+    same estimator draws the next elements."""
+
+    def _init_front_end(self, layer_norm, dropout):
+        if not 0.0 <= float(dropout) < 1.0:
+            raise ValueError("dropout must be in [0, 1)")
+        self.layer_norm = bool(layer_norm)
+        self.dropout = float(dropout)
+        self._dropout_offset = 0
+
+    def _normalise(self, X):
+        return layer_norm(X) if self.layer_norm else X
+
+    def _drop(self, X):
+        if self.dropout == 0.0:
+            return X
+        offset, self._dropout_offset = self._dropout_offset, self._dropout_offset + X.numel()
+        return dropout(X, self.dropout, 0 if self.seed is None else int(self.seed), offset)
+
+    def sample(self, X, u=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, generator=None):
+        """One label per row of X drawn from the classifier's distribution over its classes (the last one is the reference
+        class of logit 0): NumPy int64.  u: the random numbers, one a row in [0, 1) (drawn from `generator` when None)."""
+        if self.task != 'classification':
+            raise ValueError("sample() needs task='classification'")
+        logits = self._logits(X) * float(getattr(self.bf, 'w', 1.0))
+        if u is None:
+            u = torch.rand(logits.shape[0], dtype=torch.float64, device=logits.device, generator=generator)
+        elif not isinstance(u, torch.Tensor):
+            u = torch.as_tensor(np.asarray(u, dtype=np.float64), device=logits.device)
+        return sample_labels(logits, u.to(logits.device), temperature, top_k, top_p, min_p).cpu().numpy()

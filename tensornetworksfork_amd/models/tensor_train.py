@@ -9,18 +9,19 @@ from ..tensor.bregman import SquareBregFunction
 from ..tensor.layers import (CPDLayer, CumSumLayer, TensorNetworkLayer, TensorTrainLayer,
                              TensorTrainLinearLayer)
 from ..tensor.network import SumOfNetworks
-from ._common import (EarlyStopping, error_rate_torch, root_mean_squared_error_torch, split_train_val, to_tensor64,
-                      unexplained_variance)
+from ._common import (EarlyStopping, RowFrontEnd, error_rate_torch, root_mean_squared_error_torch, sample_labels,
+                      split_train_val, to_tensor64, unexplained_variance)
 
-__all__ = ["TensorTrainRegressor", "EarlyStopping", "root_mean_squared_error_torch", "error_rate_torch",
+__all__ = ["TensorTrainRegressor", "EarlyStopping", "root_mean_squared_error_torch", "error_rate_torch", "sample_labels",
            "unexplained_variance"]
 
 
-class TensorTrainRegressor(BaseEstimator, RegressorMixin):
+class TensorTrainRegressor(RowFrontEnd, BaseEstimator, RegressorMixin):
     def __init__(self, N=3, r=8, output_dim=1, linear_dim=None, constrict_bond=False, perturb=False, seed=42,
                  device='cuda', bf=None, lr=1.0, eps_start=1.0, eps_decay=0.5, abs_err=1e-4, rel_err=1e-3,
                  batch_size=512, method='ridge_cholesky', num_swipes=30, model_type='tt', task='regression',
-                 train_operator=False, cum_sum=False, early_stopping=0, verbose=0):
+                 train_operator=False, cum_sum=False, early_stopping=0, verbose=0, layer_norm=False, dropout=0.0):
+        self._init_front_end(layer_norm, dropout)
         self.N = N
         self.r = r
         self.output_dim = output_dim
@@ -82,6 +83,10 @@ class TensorTrainRegressor(BaseEstimator, RegressorMixin):
         if self.verbose > 2:
             print("Number of parameters:", self._model.num_parameters())
 
+    def _on_features(self, fn, Xb):
+        """fn applied to the features of bias-augmented rows."""
+        return torch.cat((fn(Xb[:, :-1].contiguous()), Xb[:, -1:]), dim=1)
+
     def _with_bias(self, X):
         return torch.cat((X, torch.ones((X.shape[0], 1), dtype=torch.float64, device=X.device)), dim=1)
 
@@ -95,7 +100,7 @@ class TensorTrainRegressor(BaseEstimator, RegressorMixin):
         """Bias column, split, sweeps without gauge fixing, best-weights restore
         (models/tensor_train.py:212-296)."""
         X, y = to_tensor64(X, self.device), to_tensor64(y, self.device)
-        X = self._with_bias(X)
+        X = self._with_bias(self._normalise(X))
         if self._model is None:
             self.input_dim = X.shape[1]
             self._initialize_model()
@@ -110,7 +115,11 @@ class TensorTrainRegressor(BaseEstimator, RegressorMixin):
             X_val, y_val = to_tensor64(X_val, self.device), to_tensor64(y_val, self.device)
             X_train, y_train = X, y
             if X_val.shape[1] != X_train.shape[1]:
-                X_val = self._with_bias(X_val)
+                X_val = self._with_bias(self._normalise(X_val))
+            elif self.layer_norm:
+                X_val = self._on_features(self._normalise, X_val)
+        if self.dropout > 0.0:
+            X_train = self._on_features(self._drop, X_train)
         self._early_stopper = EarlyStopping(
             X_val, y_val, model_predict=self._predict_tensor, get_model_weights=self._model.node_states,
             loss_fn=root_mean_squared_error_torch if self.task == 'regression' else error_rate_torch,
@@ -124,9 +133,11 @@ class TensorTrainRegressor(BaseEstimator, RegressorMixin):
             self._model.load_node_states(self._early_stopper.best_state_dict, set_value=True)
         return self
 
+    def _logits(self, X):
+        return self._predict_tensor(self._with_bias(self._normalise(to_tensor64(X, self.device)))).detach()
+
     def predict(self, X):
-        X = to_tensor64(X, self.device)
-        return self._predict_tensor(self._with_bias(X)).detach().cpu().numpy()
+        return self._logits(X).cpu().numpy()
 
     def score(self, X, y_true):
         if not isinstance(y_true, np.ndarray):

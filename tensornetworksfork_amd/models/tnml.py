@@ -11,11 +11,11 @@ from .. import ops
 from ..tensor.bregman import SquareBregFunction
 from ..tensor.engine import PAIR_CLASS_MAX_P
 from ..tensor.layers import TensorTrainLayer
-from ._common import (EarlyStopping, error_rate_torch, root_mean_squared_error_torch, split_train_val, to_tensor64,
-                      unexplained_variance)
+from ._common import (EarlyStopping, RowFrontEnd, error_rate_torch, root_mean_squared_error_torch, sample_labels,
+                      split_train_val, to_tensor64, unexplained_variance)
 
 __all__ = ["TNMLRegressor", "EarlyStopping", "fbasis", "polynomial_basis", "root_mean_squared_error_torch",
-           "error_rate_torch", "unexplained_variance"]
+           "error_rate_torch", "sample_labels", "unexplained_variance"]
 
 
 def _on_device(X):
@@ -51,11 +51,12 @@ def polynomial_basis(X, degree=3):
     return [torch.stack([X[:, i] ** d for d in range(degree + 1)], dim=-1) for i in range(X.shape[-1])]
 
 
-class TNMLRegressor(BaseEstimator, RegressorMixin):
+class TNMLRegressor(RowFrontEnd, BaseEstimator, RegressorMixin):
     def __init__(self, r=8, output_dim=1, seed=42, device='cuda', bf=None, lr=1.0, eps_start=1.0, eps_decay=0.5,
                  abs_err=1e-6, rel_err=1e-4, batch_size=512, method='ridge_cholesky', num_swipes=30, model_type='tt',
                  task='regression', train_operator=False, early_stopping=0, basis='sin-cos', degree=3, verbose=0,
-                 constrict_bond=True):
+                 constrict_bond=True, layer_norm=False, dropout=0.0):
+        self._init_front_end(layer_norm, dropout)
         self.r = r
         self.input_dim = degree + 1 if basis == 'polynomial' else 2
         self.output_dim = output_dim
@@ -114,7 +115,8 @@ class TNMLRegressor(BaseEstimator, RegressorMixin):
         else:
             X_val, y_val = to_tensor64(X_val, self.device), to_tensor64(y_val, self.device)
             X_train, y_train = X, y
-        F_train, F_val = self._features(X_train), self._features(X_val)
+        X_train = self._drop(self._normalise(X_train))
+        F_train, F_val = self._features(X_train), self._features(self._normalise(X_val))
         self._early_stopper = EarlyStopping(
             F_val, y_val, model_predict=self._predict_tensor, get_model_weights=self._model.node_states,
             loss_fn=root_mean_squared_error_torch if self.task == 'regression' else error_rate_torch,
@@ -130,9 +132,11 @@ class TNMLRegressor(BaseEstimator, RegressorMixin):
             self._model.load_node_states(self._early_stopper.best_state_dict, set_value=True)
         return self
 
+    def _logits(self, X):
+        return self._predict_tensor(self._features(self._normalise(to_tensor64(X, self.device)))).detach()
+
     def predict(self, X):
-        X = to_tensor64(X, self.device)
-        return self._predict_tensor(self._features(X)).detach().cpu().numpy()
+        return self._logits(X).cpu().numpy()
 
     def score(self, X, y_true):
         if not isinstance(y_true, np.ndarray):

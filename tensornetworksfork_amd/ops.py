@@ -1079,3 +1079,184 @@ def patchify(images, kernel_size, stride, dtype=None):
     rc = _lib.lib().ttk_patchify(images.data_ptr(), S, Cin, H, W, k, st, types, out.data_ptr(), _stream(images))
     _lib.check(rc, "ttk_patchify")
     return out
+
+
+# ------------------------------------------------------------------ rows in front of a model, answers behind it
+ROW_TYPES = {torch.float64: 0, torch.float32: 1, torch.bfloat16: 2, torch.float16: 3}
+
+
+def _on(t):
+    """The launch device: `t`'s own, whichever is current."""
+    return torch.cuda.device(t.device)
+
+
+def _row_tensor(t, name, device=None):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise _lib.TTKError(f"{name}: expected a CUDA/HIP tensor (there is no CPU fallback)")
+    if t.dtype not in ROW_TYPES:
+        raise _lib.TTKError(f"{name}: expected float64, float32, bfloat16 or float16, got {t.dtype}")
+    if device is not None and t.device != device:
+        raise _lib.TTKError(f"{name}: expected a tensor on {device}, got {t.device}")
+    return t
+
+
+def rows_view(t, name="x"):
+    """(rows, cols, row distance) of a tensor whose last axis is consecutive in memory and whose other axes fold into one
+    row distance (contiguous tensors, column ranges of a wider matrix, one row broadcast to many)."""
+    if t.ndim == 0 or t.shape[-1] == 0:
+        raise _lib.TTKError(f"{name}: expected at least one axis and one column, got shape {tuple(t.shape)}")
+    rows, cols = t.numel() // t.shape[-1], t.shape[-1]
+    if cols > 0x7FFFFFFF:
+        raise _lib.TTKError(f"{name}: more than 2^31 - 1 columns")
+    if cols > 1 and t.stride(-1) != 1:
+        raise _lib.TTKError(f"{name}: expected consecutive elements along the last axis")
+    lead = [(n, s) for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n != 1]
+    if rows and any(lead[i][1] != lead[i + 1][0] * lead[i + 1][1] for i in range(len(lead) - 1)):
+        raise _lib.TTKError(f"{name}: the leading axes do not fold into rows of one distance (pass a contiguous tensor)")
+    return rows, cols, lead[-1][1] if lead else cols
+
+
+def _drop_args(p, seed, offset, device):
+    """(p, seed, offset, device pointer) of a dropout mask."""
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise _lib.TTKError(f"dropout: p must be in [0, 1], got {p}")
+    if isinstance(seed, torch.Tensor) or int(seed) != seed or not 0 <= int(seed) < 1 << 64:
+        raise _lib.TTKError("dropout: seed must be an integer in [0, 2^64)")
+    if isinstance(offset, torch.Tensor):
+        if offset.dtype != torch.int64 or offset.numel() != 1 or offset.device != device:
+            raise _lib.TTKError(f"dropout: an offset tensor must hold one int64 on {device}")
+        return p, int(seed), 0, offset.data_ptr()
+    if int(offset) != offset or not 0 <= int(offset) < 1 << 63:
+        raise _lib.TTKError("dropout: offset must be an integer in [0, 2^63) or an int64 device tensor")
+    return p, int(seed), int(offset), None
+
+
+def _norm_vector(v, name, x, cols):
+    """Pointer of a weight / bias: the rows' type, or float32 with 16-bit rows."""
+    if v is None:
+        return None
+    _row_tensor(v, name, x.device)
+    if tuple(v.shape) != (cols,) or not v.is_contiguous():
+        raise _lib.TTKError(f"{name}: expected a contiguous tensor of shape ({cols},), got {tuple(v.shape)}")
+    if v.dtype != x.dtype and not (v.dtype == torch.float32 and x.dtype in (torch.bfloat16, torch.float16)):
+        raise _lib.TTKError(f"{name}: expected {x.dtype}" + (" or float32" if x.dtype in (torch.bfloat16, torch.float16) else "")
+                            + f", got {v.dtype}")
+    return v.data_ptr()
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, p=0.0, seed=0, offset=0):
+    """Layer norm over the last axis, then dropout -> (y, mean, rstd); mean / rstd have x's leading shape and are float32
+    (float64 for float64 rows).  weight / bias: (cols,) of x's type, or float32 with 16-bit rows (both alike)."""
+    _row_tensor(x, "x")
+    rows, cols, ld = rows_view(x)
+    wp, bp = _norm_vector(weight, "weight", x, cols), _norm_vector(bias, "bias", x, cols)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise _lib.TTKError("layer_norm: weight and bias must have one type")
+    if not 0.0 <= float(eps) < float("inf"):
+        raise _lib.TTKError(f"layer_norm: eps must be finite and not negative, got {eps}")
+    p, seed, off, off_dev = _drop_args(p, seed, offset, x.device)
+    wt = weight if weight is not None else bias if bias is not None else x
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = torch.empty(x.shape[:-1], dtype=F64 if x.dtype == F64 else torch.float32, device=x.device)
+    rstd = torch.empty_like(mean)
+    if rows:
+        with _on(x):
+            rc = _lib.lib().ttk_layer_norm(ROW_TYPES[x.dtype], ROW_TYPES[wt.dtype], x.data_ptr(), ld, wp, bp, y.data_ptr(),
+                                           mean.data_ptr(), rstd.data_ptr(), rows, cols, float(eps), p, seed, off, off_dev,
+                                           _stream(x))
+        _lib.check(rc, "ttk_layer_norm")
+    return y, mean, rstd
+
+
+def layer_norm_backward(dy, x, mean, rstd, weight=None, p=0.0, seed=0, offset=0, need=(True, True, True), wdtype=None):
+    """Gradients (dx, dweight, dbias) of layer_norm for the gradient `dy` of its output; those not in `need` are None.
+    mean / rstd are what layer_norm returned, p / seed / offset what it was given.  dweight / dbias have the weight's type
+    (`wdtype`, or x's, where there is no weight)."""
+    _row_tensor(x, "x")
+    _row_tensor(dy, "dy", x.device)
+    if dy.dtype != x.dtype or dy.shape != x.shape:
+        raise _lib.TTKError(f"dy: expected {x.dtype} of shape {tuple(x.shape)}, got {dy.dtype} of shape {tuple(dy.shape)}")
+    rows, cols, ld = rows_view(x)
+    _, _, lddy = rows_view(dy, "dy")
+    wp = _norm_vector(weight, "weight", x, cols)
+    stat = F64 if x.dtype == F64 else torch.float32
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        _row_tensor(t, name, x.device)
+        if t.dtype != stat or tuple(t.shape) != tuple(x.shape[:-1]) or not t.is_contiguous():
+            raise _lib.TTKError(f"{name}: expected a contiguous {stat} tensor of shape {tuple(x.shape[:-1])}")
+    p, seed, off, off_dev = _drop_args(p, seed, offset, x.device)
+    wdt = weight.dtype if weight is not None else wdtype if wdtype is not None else x.dtype
+    if wdt != x.dtype and not (wdt == torch.float32 and x.dtype in (torch.bfloat16, torch.float16)):
+        raise _lib.TTKError(f"layer_norm_backward: gradients of type {wdt} do not go with rows of {x.dtype}")
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
+    make = torch.empty if rows else torch.zeros
+    dw = make((cols,), dtype=wdt, device=x.device) if need[1] else None
+    db = make((cols,), dtype=wdt, device=x.device) if need[2] else None
+    if rows and any(need):
+        L = _lib.lib()
+        ws, nbytes = None, 0
+        if need[1] or need[2]:
+            nbytes = int(L.ttk_layer_norm_backward_ws_bytes(ROW_TYPES[x.dtype], rows, cols))
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        ptr = [t.data_ptr() if t is not None else None for t in (dx, dw, db, ws)]
+        with _on(x):
+            rc = L.ttk_layer_norm_backward(ROW_TYPES[x.dtype], ROW_TYPES[wdt], dy.data_ptr(), lddy, x.data_ptr(), ld, wp,
+                                           mean.data_ptr(), rstd.data_ptr(), ptr[0], ptr[1], ptr[2], rows, cols, p, seed, off,
+                                           off_dev, ptr[3], nbytes, _stream(x))
+        _lib.check(rc, "ttk_layer_norm_backward")
+    return dx, dw, db
+
+
+def dropout(x, p, seed, offset=0):
+    """x with each element kept with probability 1 - p and divided by it, the others 0; element i (in memory order of the
+    contiguous x) is number offset + i of the mask that `seed` names.  The same call on a gradient is the backward pass."""
+    _row_tensor(x, "x")
+    if not x.is_contiguous():
+        raise _lib.TTKError("x: expected a contiguous tensor")
+    p, seed, off, off_dev = _drop_args(p, seed, offset, x.device)
+    y = torch.empty_like(x)
+    if x.numel():
+        with _on(x):
+            rc = _lib.lib().ttk_dropout(ROW_TYPES[x.dtype], x.data_ptr(), y.data_ptr(), x.numel(), p, seed, off, off_dev,
+                                        _stream(x))
+        _lib.check(rc, "ttk_dropout")
+    return y
+
+
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One label per row of `logits` (..., V), drawn from softmax(logits / temperature) cut by top-k, then top-p, then min-p
+    with the given random numbers u (...) in [0, 1) -> int64 (...).
+
+    Ties in the cuts go to the lowest index.  NaN counts as -inf, which is never drawn; a row of nothing else answers -1.
+    temperature 0 answers with the lowest index of the maximum.  u is float32 or float64; temperature, top_p and min_p are
+    numbers or tensors of u's type and shape, top_k a number (0: off) or an int32 tensor of u's shape.  Out-of-range values
+    inside tensors switch the cut off (top_k <= 0 or >= V, top_p >= 1, min_p <= 0) or are clamped (top_p <= 0 keeps one
+    element, min_p > 1 acts as 1, u outside [0, 1) answers with the first / last kept element)."""
+    _row_tensor(logits, "logits")
+    rows, V, ld = rows_view(logits, "logits")
+    shape = tuple(logits.shape[:-1])
+    if not isinstance(u, torch.Tensor) or u.dtype not in (torch.float32, F64) or u.device != logits.device \
+            or tuple(u.shape) != shape or not u.is_contiguous():
+        raise _lib.TTKError(f"u: expected a contiguous float32 / float64 tensor of shape {shape} on {logits.device}")
+
+    def param(v, name, dtype, ok):
+        if isinstance(v, torch.Tensor):
+            if v.dtype != dtype or v.device != logits.device or tuple(v.shape) != shape or not v.is_contiguous():
+                raise _lib.TTKError(f"{name}: expected a number or a contiguous {dtype} tensor of shape {shape} on {logits.device}")
+            return v.data_ptr(), 0
+        if not ok(v):
+            raise _lib.TTKError(f"{name}: {v} is out of range")
+        return None, v
+    tp, t = param(temperature, "temperature", u.dtype, lambda v: 0.0 <= v < float("inf"))
+    kp, k = param(top_k, "top_k", torch.int32, lambda v: int(v) == v and v >= 0)
+    pp, pv = param(top_p, "top_p", u.dtype, lambda v: 0.0 < v <= 1.0)
+    mp, mv = param(min_p, "min_p", u.dtype, lambda v: 0.0 <= v <= 1.0)
+    label = torch.empty(shape, dtype=torch.int64, device=logits.device)
+    if rows:
+        with _on(logits):
+            rc = _lib.lib().ttk_sample(ROW_TYPES[logits.dtype], logits.data_ptr(), ld, u.data_ptr(), int(u.dtype == F64), tp,
+                                       float(t), kp, min(int(k), 0x7FFFFFFF), pp, float(pv), mp, float(mv), label.data_ptr(),
+                                       rows, V, _stream(logits))
+        _lib.check(rc, "ttk_sample")
+    return label

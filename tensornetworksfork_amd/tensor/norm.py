@@ -1,0 +1,121 @@
+"""Layer norm and dropout of the rows a model learns from, differentiable (kernels: csrc/ttk_norm.hip).
+
+    rows -> layer_norm -> dropout -> TensorTrainLayer -> logits
+
+`layer_norm(..., p=...)` runs both in one pass over the rows; its backward pass returns the gradients of the rows, the
+weight and the bias.  The dropout mask is a function of (seed, offset + element number) and is never stored: the backward
+pass recomputes it, and a shard of a data set that passes the element number of its first row as `offset` draws the mask of
+the whole set.  `offset` may be an int64 device tensor of one element, read when the kernel runs: a captured graph draws a
+new mask on every replay if the graph (or the caller between replays) advances it.  Its value has to stay until the backward
+pass has run; changing it in place before that raises, as for any tensor autograd has saved.
+
+Gradients of gradients are not defined here (asking for them raises).
+"""
+import torch
+from torch import nn
+from torch.autograd.function import once_differentiable
+
+from .. import ops
+
+__all__ = ["layer_norm", "dropout", "LayerNorm", "Dropout"]
+
+
+def _rows(t):
+    """t, or a contiguous copy where its axes do not fold into rows of one distance."""
+    if not isinstance(t, torch.Tensor) or t.ndim == 0 or t.is_contiguous():
+        return t
+    try:
+        ops.rows_view(t)
+    except ops._lib.TTKError:
+        return t.contiguous()
+    return t
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, p, seed, offset):
+        y, mean, rstd = ops.layer_norm(x, weight, bias, eps, p, seed, offset)
+        off = offset if isinstance(offset, torch.Tensor) else None
+        ctx.save_for_backward(x, weight, mean, rstd, off)
+        ctx.wdtype = bias.dtype if weight is None and bias is not None else None
+        ctx.drop = (p, seed, None if off is not None else offset)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd, off = ctx.saved_tensors
+        p, seed, offset = ctx.drop
+        grads = ops.layer_norm_backward(_rows(dy), x, mean, rstd, weight, p, seed, offset if off is None else off,
+                                        need=ctx.needs_input_grad[:3], wdtype=ctx.wdtype)
+        return (*grads, None, None, None, None)
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, seed, offset):
+        off = offset if isinstance(offset, torch.Tensor) else None
+        ctx.save_for_backward(off)
+        ctx.drop = (p, seed, None if off is not None else offset)
+        return ops.dropout(x, p, seed, offset)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        off, = ctx.saved_tensors
+        p, seed, offset = ctx.drop
+        return ops.dropout(dy.contiguous(), p, seed, offset if off is None else off), None, None, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, p=0.0, seed=0, offset=0):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last axis, followed by dropout with probability p."""
+    return _LayerNorm.apply(_rows(x), weight, bias, eps, p, seed, offset)
+
+
+def dropout(x, p, seed, offset=0):
+    """Each element kept with probability 1 - p and divided by it; the mask is a function of (seed, offset + element)."""
+    return _Dropout.apply(x.contiguous() if isinstance(x, torch.Tensor) else x, p, seed, offset)
+
+
+class LayerNorm(nn.Module):
+    """Layer norm over the last axis of `cols` columns, with an optional learnable weight and bias, and dropout (probability
+    p, while training) as its epilogue.  Every training pass draws the next elements of the mask that `seed` names."""
+
+    def __init__(self, cols, eps=1e-5, affine=True, p=0.0, seed=0, device=None, dtype=None):
+        super().__init__()
+        self.cols, self.eps, self.p, self.seed = int(cols), float(eps), float(p), int(seed)
+        self.offset = 0
+        if affine:
+            self.weight = nn.Parameter(torch.ones(self.cols, device=device, dtype=dtype))
+            self.bias = nn.Parameter(torch.zeros(self.cols, device=device, dtype=dtype))
+        else:
+            self.register_parameter("weight", None)
+            self.register_parameter("bias", None)
+
+    def forward(self, x):
+        if x.ndim == 0 or x.shape[-1] != self.cols:
+            raise ops._lib.TTKError(f"LayerNorm: expected {self.cols} columns, got shape {tuple(x.shape)}")
+        if not self.training or self.p == 0.0:
+            return layer_norm(x, self.weight, self.bias, self.eps)
+        offset, self.offset = self.offset, self.offset + x.numel()
+        return layer_norm(x, self.weight, self.bias, self.eps, self.p, self.seed, offset)
+
+    def extra_repr(self):
+        return f"{self.cols}, eps={self.eps}, affine={self.weight is not None}, p={self.p}"
+
+
+class Dropout(nn.Module):
+    """Dropout while training; every training pass draws the next elements of the mask that `seed` names."""
+
+    def __init__(self, p, seed=0):
+        super().__init__()
+        self.p, self.seed, self.offset = float(p), int(seed), 0
+
+    def forward(self, x):
+        if not self.training or self.p == 0.0:
+            return x
+        offset, self.offset = self.offset, self.offset + x.numel()
+        return dropout(x, self.p, self.seed, offset)
+
+    def extra_repr(self):
+        return f"p={self.p}, seed={self.seed}"
