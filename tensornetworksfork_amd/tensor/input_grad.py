@@ -1,0 +1,89 @@
+"""Gradient of a tensor train with respect to its inputs, so that what stands in front of it (layer norm, dropout, any
+torch module) can be trained through it.
+
+Output y[s,c] = sum L[s,c,l] core[l,p,r] G[s,p] R[s,r] is linear in every site's feature vector G, so with the output's
+gradient g
+    dG[s,p] = sum_{l,r} (sum_c g[s,c] L[s,c,l]) core[l,p,r] R[s,r]
+which is an environment step with the core's feature axis in the place of its left bond; a conv or operator column then
+applies its feature node once more (one row GEMM).  Environments are the ones the forward pass's engine caches.
+"""
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import ops
+
+
+def _nodes(engine):
+    return [n for col in engine.cols for n in (col.A, col.F) if n is not None]
+
+
+class _Forward(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, layer, shared, *xs):
+        tn = layer.tensor_network
+        det = [x.detach() for x in xs]          # new objects: the engine's data-set cache never mistakes them for others
+        out = tn.forward(det[0] if shared else det)
+        if layer.labels is not None:
+            out.permute_first(*layer.labels)
+        ctx.engine, ctx.data, ctx.shared = tn._engine, tn._current, shared
+        ctx.nodes = [(n, n.tensor, n.tensor._version) for n in _nodes(tn._engine)]
+        ctx.like = [(x.dtype, x.device) for x in xs]
+        return out.tensor.detach()
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        eng, d = ctx.engine, ctx.data
+        if any(n.tensor is not t or t._version != v for n, t, v in ctx.nodes):
+            raise RuntimeError("a node of the tensor network has changed since the forward pass: its input gradient is gone")
+        eng.net._user_guard(d)
+        eng.sync(d)
+        g = ops.prep(dy.reshape(d.S, -1))
+        need = ctx.needs_input_grad[2:]
+        grads = [None] * len(need)
+        for k, col in enumerate(eng.cols):
+            at = 0 if ctx.shared else col.xin
+            if not need[at]:
+                continue
+            dx = _site_gradient(eng, d, k, g)
+            grads[at] = dx if grads[at] is None else grads[at] + dx
+        grads = [None if t is None else t.to(dtype=dt, device=dev) for t, (dt, dev) in zip(grads, ctx.like)]
+        return (None, None, *grads)
+
+
+def _site_gradient(eng, d, k, g):
+    """d (sum_s,c g y) / d x_k in x_k's own shape, float64."""
+    L, R = eng.left(d, k), eng.right(d, k)
+    core = eng.canonA(k).permute(1, 0, 2).contiguous()          # (p, rl, rr)
+    ca, cb, S, p = L.shape[0], R.shape[0], d.S, core.shape[0]
+    dG = [ops.env_step_right(R[b].contiguous(), ops.gl(g, L[a].contiguous()), core) for a in range(ca) for b in range(cb)]
+    col = eng.cols[k]
+    if col.kind == "plain":
+        return dG[0]
+    F = eng.canonF(k)
+    if col.kind == "conv":                                      # F (ca, px, cb):  dx[s,p,x] = sum_ab dG_ab[s,p] F[a,x,b]
+        A = torch.stack(dG, dim=2).reshape(S * p, ca * cb)
+        B = F.permute(0, 2, 1).reshape(ca * cb, -1).contiguous()
+        return ops.gemm_rows(A, B, B.shape[1]).reshape(S, p, -1)
+    A = torch.cat(dG, dim=1)                                    # F (ca, u, d, cb):  dx[s,d] = sum_abu dG_ab[s,u] F[a,u,d,b]
+    B = F.permute(0, 3, 1, 2).reshape(A.shape[1], -1).contiguous()
+    return ops.gemm_rows(A, B, B.shape[1])
+
+
+def wants_input_gradient(layer, x):
+    """Whether a forward pass of `layer` on `x` has to be recorded: grad mode, an input that requires it, a train whose
+    output carries its labels in the engine's order."""
+    from .engine import ChainEngine
+    xs = x if isinstance(x, (list, tuple)) else [x]
+    if not torch.is_grad_enabled() or not any(isinstance(t, torch.Tensor) and t.requires_grad for t in xs):
+        return False
+    tn = layer.tensor_network
+    if type(tn._engine) is not ChainEngine or tn._engine.cols is None:
+        return False
+    want = [lab for lab in (layer.labels or tn.output_labels) if lab in tn._engine.out_labels()]
+    return want == tn._engine.out_labels()
+
+
+def forward(layer, x):
+    shared = not isinstance(x, (list, tuple))
+    return _Forward.apply(layer, shared, *([x] if shared else x))

@@ -7,6 +7,7 @@ seeded layer starts from the same numbers as the reference.
 import torch
 import torch.nn as nn
 
+from . import input_grad
 from .network import TensorNetwork
 from .node import TensorNode
 
@@ -134,6 +135,9 @@ class TensorNetworkLayer(nn.Module):
         return super().cpu(*args, **kwargs)
 
     def forward(self, x, to_tensor=True):
+        """The network's output; differentiable with respect to inputs that require a gradient (tensor trains)."""
+        if to_tensor and input_grad.wants_input_gradient(self, x):
+            return input_grad.forward(self, x)
         out = self.tensor_network.forward(x)
         if self.labels is not None:
             out.permute_first(*self.labels)

@@ -17,6 +17,15 @@ SHAPES = [(1, 1), (3, 1), (1, 2), (5, 3), (70, 7), (1000, 8), (129, 16), (260, 1
           (19, 5120), (3, 8193), (700, 10007), (2, 16384), (2, 16385), (1, 32769), (3, 70001)]
 
 
+@pytest.fixture(autouse=True)
+def _float32_default():
+    """Other tests of the process may have left float64 as torch's default."""
+    old = torch.get_default_dtype()
+    torch.set_default_dtype(F32)
+    yield
+    torch.set_default_dtype(old)
+
+
 def _dev():
     assert torch.cuda.is_available(), "GPU tests need a HIP device"
     return torch.device("cuda:0")

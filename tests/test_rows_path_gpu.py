@@ -1,0 +1,227 @@
+"""Layer norm, dropout, a tensor train and label sampling as they are used together: the gradient through the train into the
+norm, the estimators with a front end, labels drawn from their answers."""
+import numpy as np
+import pytest
+import torch
+
+from tests import _row_oracles as R
+
+gpu = pytest.mark.gpu
+F64 = torch.float64
+TOL = 1e-10          # float64 kernels against float64 restatements, relative to the largest entry
+
+
+@pytest.fixture(autouse=True)
+def _double():
+    old = torch.get_default_dtype()
+    torch.set_default_dtype(F64)
+    yield
+    torch.set_default_dtype(old)
+
+
+def _dev():
+    assert torch.cuda.is_available(), "GPU tests need a HIP device"
+    return torch.device("cuda:0")
+
+
+def _close(a, b, tol=TOL):
+    a, b = a.detach().cpu().double(), b.detach().cpu().double()
+    assert a.shape == b.shape
+    assert float((a - b).abs().max()) <= tol * max(float(b.abs().max()), 1e-30)
+
+
+def _train(cores, xs):
+    """Plain train on the CPU: cores (rl, [c], p, rr) squeezed like the layer's, xs (S, p) -> (S, C)."""
+    N = len(cores)
+    env = None
+    for k, (A, x) in enumerate(zip(cores, xs)):
+        if k == 0:
+            A = A.reshape(-1, x.shape[1], A.shape[-1] if N > 1 else 1)          # (c, p, r)
+            env = torch.einsum("cpr,sp->scr", A, x)
+        else:
+            A = A.reshape(env.shape[2], x.shape[1], -1)
+            env = torch.einsum("scl,lpr,sp->scr", env, A, x)
+    return env.squeeze(-1)
+
+
+@gpu
+@pytest.mark.parametrize("N,r,p,C", [(1, 1, 4, 1), (2, 3, 5, 2), (4, 6, 3, 1), (5, 8, 7, 3), (3, 20, 18, 2), (16, 32, 6, 1)])
+def test_input_gradient_of_a_train(N, r, p, C):
+    from tensornetworksfork_amd.tensor.layers import TensorTrainLayer
+    dev = _dev()
+    layer = TensorTrainLayer(N, r, p, output_shape=C, seed=3)
+    cores = [n.tensor.clone() for n in layer.tensor_network.main_nodes]
+    layer = layer.to(dev)
+    g = torch.Generator().manual_seed(N)
+    xs = [torch.randn(37, p, generator=g) for _ in range(N)]
+    dy = torch.randn(37, C, generator=g)
+    ref_in = [x.clone().requires_grad_(True) for x in xs]
+    ref = _train(cores, ref_in)
+    ref_g = torch.autograd.grad((ref * dy).sum(), ref_in)
+    got_in = [x.to(dev).requires_grad_(True) for x in xs]
+    out = layer(got_in)
+    _close(out.reshape(37, C), ref)
+    for a, b in zip(torch.autograd.grad(out, got_in, dy.to(dev).reshape(out.shape)), ref_g):
+        _close(a, b)
+    # one tensor for every site, and only some inputs asked for
+    x1 = xs[0].clone().requires_grad_(True)
+    want, = torch.autograd.grad((_train(cores, [x1] * N) * dy).sum(), x1)
+    for form in (lambda t: t, lambda t: [t] * N):
+        xd = xs[0].to(dev).requires_grad_(True)
+        out = layer(form(xd))
+        got, = torch.autograd.grad(out, xd, dy.to(dev).reshape(out.shape))
+        _close(got, want)
+    if N > 1:
+        xd = xs[1].to(dev).requires_grad_(True)
+        out = layer([xs[0].to(dev), xd] + [x.to(dev) for x in xs[2:]])
+        got, = torch.autograd.grad(out, xd, dy.to(dev).reshape(out.shape))
+        _close(got, ref_g[1])
+    assert not layer([x.to(dev) for x in xs]).requires_grad
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["conv", "conv_bond", "linear"])
+def test_input_gradient_of_columns_with_feature_nodes(kind):
+    """Against differences of the forward pass: the output is a polynomial of degree one in each site's input, so central
+    differences carry rounding only (2^-53 |y| / h relative to gradients of y's size: 1e-11 at h = 1e-4, 1e-7 allowed)."""
+    from tensornetworksfork_amd.tensor.layers import TensorConvolutionTrainLayer, TensorTrainLinearLayer
+    dev = _dev()
+    torch.manual_seed(1)
+    if kind == "linear":
+        layer = TensorTrainLinearLayer(3, 4, 6, 5, output_shape=2, seed=2)
+        shapes = [(9, 6)] * 3
+    else:
+        layer = TensorConvolutionTrainLayer(3, 4, 7, 5, 2, convolution_bond=3 if kind == "conv_bond" else -1)
+        shapes = [(9, 7, 5)] * 3
+    layer = layer.to(dev)
+    g = torch.Generator().manual_seed(4)
+    xs = [torch.randn(*s, generator=g).to(dev) for s in shapes]
+    with torch.no_grad():
+        y0 = layer(xs)
+    dy = torch.randn(*y0.shape, generator=g).to(dev)
+    ins = [x.clone().requires_grad_(True) for x in xs]
+    grads = torch.autograd.grad(layer(ins), ins, dy)
+    for k in range(3):
+        assert grads[k].shape == xs[k].shape
+        scale = float(grads[k].abs().max())
+        for j in range(0, xs[k].numel(), 13):
+            vals = []
+            for h in (1e-4, -1e-4):
+                moved = [x.clone() for x in xs]
+                moved[k].reshape(-1)[j] += h
+                vals.append(float((layer(moved) * dy).sum()))
+            num = (vals[0] - vals[1]) / 2e-4
+            assert abs(num - float(grads[k].reshape(-1)[j])) <= 1e-7 * max(scale, float((y0 * dy).abs().sum())), (k, j)
+
+
+@gpu
+def test_a_node_that_changed_before_backward_is_noticed():
+    from tensornetworksfork_amd.tensor.layers import TensorTrainLayer
+    dev = _dev()
+    layer = TensorTrainLayer(3, 4, 5, output_shape=1, seed=3).to(dev)
+    x = torch.randn(8, 5, device=dev, requires_grad=True)
+    out = layer(x)
+    layer.tensor_network.main_nodes[1].tensor.mul_(2.0)
+    with pytest.raises(RuntimeError):
+        out.sum().backward()
+
+
+@gpu
+def test_norm_dropout_train_loss_backward_and_sampled_labels():
+    """rows -> LayerNorm(weight, bias, dropout) -> [features, 1] -> train -> cross entropy -> gradients of weight, bias and
+    rows, against the whole chain in 64 bits on the CPU with the same mask; then labels drawn from the logits."""
+    from tensornetworksfork_amd import ops
+    from tensornetworksfork_amd.models.tensor_train import sample_labels
+    from tensornetworksfork_amd.tensor.bregman import XEAutogradBregman
+    from tensornetworksfork_amd.tensor.layers import TensorTrainLayer
+    from tensornetworksfork_amd.tensor.norm import LayerNorm
+    dev = _dev()
+    S, F, N, C = 300, 13, 3, 4
+    g = torch.Generator().manual_seed(9)
+    rows = torch.randn(S, F, generator=g) * 3 + 1
+    target = torch.nn.functional.one_hot(torch.randint(0, C + 1, (S,), generator=g), C + 1).to(F64)
+    layer = TensorTrainLayer(N, 6, F + 1, output_shape=C, seed=1)
+    cores = [n.tensor.clone() for n in layer.tensor_network.main_nodes]
+    layer = layer.to(dev)
+    ln = LayerNorm(F, p=0.25, seed=31, device=dev, dtype=F64)
+    bf = XEAutogradBregman()
+    for step in range(3):
+        # the chain on the CPU
+        w, b = ln.weight.detach().cpu().requires_grad_(True), ln.bias.detach().cpu().requires_grad_(True)
+        xr = rows.clone().requires_grad_(True)
+        keep = R.keep_mask(S * F, 0.25, 31, step * S * F).reshape(S, F)
+        h = torch.nn.functional.layer_norm(xr, (F,), w, b, 1e-5)
+        h = torch.where(keep, h / 0.75, torch.zeros_like(h))
+        z = _train(cores, [torch.cat((h, torch.ones(S, 1)), 1)] * N)
+        loss = torch.nn.functional.cross_entropy(torch.cat((z, torch.zeros(S, 1)), 1), target.argmax(1), reduction="sum")
+        ref = torch.autograd.grad(loss, (xr, w, b))
+        # the framework
+        xd = rows.to(dev).requires_grad_(True)
+        feats = torch.cat((ln(xd), torch.ones(S, 1, device=dev)), dim=1)
+        logits = layer(feats)
+        l, dz, _ = bf(logits.detach(), target.to(dev))
+        _close(l.sum(), loss)
+        got = torch.autograd.grad(logits, (xd, ln.weight, ln.bias), dz)
+        for a, c in zip(got, ref):
+            _close(a, c, 1e-9)
+        with torch.no_grad():
+            ln.weight -= 1e-4 * got[1]
+            ln.bias -= 1e-4 * got[2]
+    ln.eval()
+    with torch.no_grad():
+        z = torch.cat((layer(torch.cat((ln(rows.to(dev)), torch.ones(S, 1, device=dev)), dim=1)), torch.zeros(S, 1, device=dev)), 1)
+    u = torch.rand(S, generator=g)
+    labels = sample_labels(z, u.to(dev), temperature=1.5, top_p=0.9).cpu()
+    for i in range(S):
+        want, margin = R.sample_row(z[i].cpu().numpy(), float(u[i]), T=1.5, P=0.9)
+        assert margin < 1e-9 or int(labels[i]) == want
+    assert torch.equal(sample_labels(z, u.to(dev), temperature=0.0).cpu(), z.argmax(1).cpu())
+    assert torch.equal(sample_labels(z.t().contiguous().t(), u.to(dev)), ops.sample(z.contiguous(), u.to(dev)))
+
+
+@gpu
+@pytest.mark.parametrize("which", ["tt", "tnml"])
+def test_estimators_with_a_front_end(which):
+    """fit(layer_norm, dropout) equals a plain fit on rows prepared by the oracles; predictions are of normalised rows;
+    sample() draws from the predicted distribution."""
+    from tensornetworksfork_amd.models.tensor_train import TensorTrainRegressor
+    from tensornetworksfork_amd.models.tnml import TNMLRegressor
+    from tensornetworksfork_amd.tensor.bregman import XEAutogradBregman
+    _dev()
+    rng = np.random.RandomState(0)
+    S, Fn, C = 400, 4, 3
+    X = rng.randn(S, Fn) * 2 + 1
+    cls = (X @ rng.randn(Fn, C)).argmax(1)
+    Y = np.eye(C)[cls]
+    kw = dict(r=4, output_dim=C - 1, bf=XEAutogradBregman(), num_swipes=2, task='classification', seed=7, early_stopping=3)
+
+    def make(**more):
+        if which == "tt":
+            return TensorTrainRegressor(N=3, **kw, **more)
+        return TNMLRegressor(basis='polynomial', degree=2, **kw, **more)
+    Xn = R.norm_forward(torch.tensor(X))[0].numpy()
+    e = make(layer_norm=True).fit(X, Y)
+    plain = make().fit(Xn, Y)
+    assert np.abs(e.predict(X) - plain.predict(Xn)).max() < 1e-6 * np.abs(plain.predict(Xn)).max()
+    # dropout: the training rows of the split, masked by element; validation and prediction rows stay
+    from tensornetworksfork_amd.models._common import split_train_val
+    Xt, Yt, Xv, Yv = split_train_val(torch.tensor(Xn), torch.tensor(Y), 7, 0.1)
+    Xd = R.dropout(Xt, 0.2, 7, 0)
+    d = make(layer_norm=True, dropout=0.2).fit(X, Y)
+    ref = make().fit(Xd.cuda(), Yt.cuda(), X_val=Xv.cuda(), y_val=Yv.cuda())
+    assert np.abs(d.predict(X) - ref.predict(Xn)).max() < 1e-6 * np.abs(ref.predict(Xn)).max()
+    assert d._dropout_offset == Xd.numel()
+    d.fit(X, Y)
+    assert d._dropout_offset == 2 * Xd.numel()
+    z = d.predict(X)
+    assert z.shape == (S, C)
+    u = rng.rand(S)
+    lab = d.sample(X, u, temperature=0.8, top_k=2)
+    for i in range(S):
+        want, margin = R.sample_row(z[i], u[i], T=0.8, k=2)
+        assert margin < 1e-9 or lab[i] == want
+    assert np.array_equal(d.sample(X, u, temperature=0.0), z.argmax(1))
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    a = d.sample(X, generator=gen)
+    assert a.shape == (S,) and a.min() >= 0 and a.max() < C
+    assert not np.array_equal(a, d.sample(X, generator=gen))

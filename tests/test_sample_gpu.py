@@ -16,6 +16,15 @@ CUTS = [dict(), dict(T=0.6), dict(k=1), dict(k=7), dict(P=0.9), dict(P=0.2, T=1.
         dict(k=1000, T=2.5), dict(T=0.0), dict(P=1e-12), dict(k=600, P=0.97, T=1.3), dict(M=1.0), dict(P=0.999, T=0.2)]
 
 
+@pytest.fixture(autouse=True)
+def _float32_default():
+    """Other tests of the process may have left float64 as torch's default."""
+    old = torch.get_default_dtype()
+    torch.set_default_dtype(F32)
+    yield
+    torch.set_default_dtype(old)
+
+
 def _dev():
     assert torch.cuda.is_available(), "GPU tests need a HIP device"
     return torch.device("cuda:0")
