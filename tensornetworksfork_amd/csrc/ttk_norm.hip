@@ -267,6 +267,241 @@ __global__ __launch_bounds__(1024) void ln_cols_sum_kernel(const A* __restrict__
 }
 
 // ---------------------------------------------------------------------------------------
+// Layer norm, rows held in registers: LANES lanes own a row, NV vectors of 16 bytes each (vector v of lane l starts at
+// column (v LANES + l) N).  One pass over memory: both statistics come from the registers, the variance from the centred
+// values.  LANES 16 and 64: several rows a workgroup, no barrier; 256 and more: a workgroup a row.
+//
+// The backward pass walks many rows a workgroup and keeps each lane's columns of dw and db in registers; they leave as one
+// partial row per workgroup (`part`: [workgroup][dw | db][cols]).
+// ---------------------------------------------------------------------------------------
+template <typename X, int LANES, int NV>
+__device__ __forceinline__ void load_row(Vec<X> (&v)[NV], const X* p, int lane, int cols, bool live) {
+  constexpr int N = Vec<X>::N;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * LANES + lane) * N;
+    if (live && c + N <= cols)
+      v[i].load(p + c);
+    else
+      v[i].load_some(p + c, live ? cols - c : 0);
+  }
+}
+
+template <typename X, int LANES, int NV>
+__device__ __forceinline__ void store_row(const Vec<X> (&v)[NV], X* p, int lane, int cols) {
+  constexpr int N = Vec<X>::N;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * LANES + lane) * N;
+    if (c + N <= cols)
+      v[i].store(p + c);
+    else
+      v[i].store_some(p + c, cols - c);
+  }
+}
+
+// N weights from column c on (missing ones 0)
+template <typename A, typename W, int N>
+__device__ __forceinline__ void load_weights(A (&out)[N], const W* w, int c, int cols) {
+  constexpr int M = Vec<W>::N;
+  if (N >= M && c + N <= cols) {
+#pragma unroll
+    for (int k = 0; k < N / M; ++k) {
+      Vec<W> t;
+      t.load(w + c + k * M);
+#pragma unroll
+      for (int j = 0; j < M; ++j) out[k * M + j] = (A)t.e[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) out[j] = c + j < cols ? (A)w[c + j] : A(0);
+  }
+}
+
+// sums over the LANES lanes of a row, in every lane
+template <int LANES, typename A>
+__device__ __forceinline__ void row_sum2(A& a, A& b, A* buf) {
+  if constexpr (LANES <= 64) {
+    a = lane_sum<LANES>(a);
+    b = lane_sum<LANES>(b);
+  } else {
+    block_sum2<LANES / 64>(a, b, buf);
+  }
+}
+template <int LANES, typename A>
+__device__ __forceinline__ A row_sum(A a, A* buf) {
+  if constexpr (LANES <= 64) {
+    return lane_sum<LANES>(a);
+  } else {
+    a = lane_sum<64>(a);
+    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = a;
+    __syncthreads();
+    a = A(0);
+#pragma unroll
+    for (int i = 0; i < LANES / 64; ++i) a += buf[i];
+    return a;
+  }
+}
+
+constexpr int group_threads(int lanes) { return lanes < 256 ? 256 : lanes; }
+
+template <typename X, typename W, int LANES, int NV>
+__global__ __launch_bounds__(group_threads(LANES)) void ln_fwd_group_kernel(
+    const X* __restrict__ x, int64_t ldx, const W* __restrict__ w, const W* __restrict__ b, X* __restrict__ y,
+    typename Acc<X>::type* __restrict__ mean_out, typename Acc<X>::type* __restrict__ rstd_out, int64_t rows, int cols, double eps,
+    Drop drop) {
+  typedef typename Acc<X>::type A;
+  constexpr int N = Vec<X>::N, RPB = group_threads(LANES) / LANES;
+  __shared__ A buf[2][LANES > 64 ? LANES / 64 : 1];
+  const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
+  const uint64_t e0 = drop_base(drop);
+  const A scale = (A)drop.scale;
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB) {
+    const int64_t row = r0 + sub;
+    const bool live = row < rows;
+    Vec<X> v[NV];
+    load_row<X, LANES, NV>(v, x + row * ldx, lane, cols, live);
+    A s = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < N; ++j) s += (A)v[i].e[j];
+    const A mean = row_sum<LANES>(s, buf[0]) / (A)cols;
+    A q = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const A d = (i * LANES + lane) * N + j < cols ? (A)v[i].e[j] - mean : A(0);
+        q += d * d;
+      }
+    const A rstd = A(1) / sqrt(row_sum<LANES>(q, buf[1]) / (A)cols + (A)eps);
+    if (!live) continue;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * LANES + lane) * N;
+      A h[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) h[j] = ((A)v[i].e[j] - mean) * rstd;
+      if (w) {
+        A t[N];
+        load_weights<A, W, N>(t, w, c, cols);
+#pragma unroll
+        for (int j = 0; j < N; ++j) h[j] *= t[j];
+      }
+      if (b) {
+        A t[N];
+        load_weights<A, W, N>(t, b, c, cols);
+#pragma unroll
+        for (int j = 0; j < N; ++j) h[j] += t[j];
+      }
+      if (drop.mode) {
+        const uint32_t bits = keep_bits<N>(drop, e0 + (uint64_t)row * cols + c);
+#pragma unroll
+        for (int j = 0; j < N; ++j) h[j] = (bits >> j & 1) ? h[j] * scale : A(0);
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[i].e[j] = (X)h[j];
+    }
+    store_row<X, LANES, NV>(v, y + row * cols, lane, cols);
+    if (lane == 0) mean_out[row] = mean, rstd_out[row] = rstd;
+  }
+}
+
+template <typename X, typename W, int LANES, int NV>
+__global__ __launch_bounds__(group_threads(LANES)) void ln_bwd_group_kernel(
+    const X* __restrict__ dy, int64_t lddy, const X* __restrict__ x, int64_t ldx, const W* __restrict__ w,
+    const typename Acc<X>::type* __restrict__ mean_in, const typename Acc<X>::type* __restrict__ rstd_in, X* __restrict__ dx,
+    typename Acc<X>::type* __restrict__ part, int64_t rows, int cols, Drop drop) {
+  typedef typename Acc<X>::type A;
+  constexpr int N = Vec<X>::N, RPB = group_threads(LANES) / LANES;
+  __shared__ A buf[2][LANES > 64 ? 2 * (LANES / 64) : 1];
+  const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
+  const uint64_t e0 = drop_base(drop);
+  const A scale = (A)drop.scale;
+  A aw[NV][N], ab[NV][N];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < N; ++j) aw[i][j] = ab[i][j] = A(0);
+  int turn = 0;
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB, turn ^= 1) {
+    const int64_t row = r0 + sub;
+    const bool live = row < rows;
+    Vec<X> xv[NV], gv[NV];
+    load_row<X, LANES, NV>(xv, x + row * ldx, lane, cols, live);
+    load_row<X, LANES, NV>(gv, dy + row * lddy, lane, cols, live);
+    const A mean = live ? mean_in[row] : A(0), rstd = live ? rstd_in[row] : A(0);
+    A s1 = 0, s2 = 0;
+    uint32_t bits[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * LANES + lane) * N;
+      bits[i] = drop.mode && live ? keep_bits<N>(drop, e0 + (uint64_t)row * cols + c) : ~0u;
+      A t[N];
+      if (w) load_weights<A, W, N>(t, w, c, cols);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        A g = (A)gv[i].e[j];
+        if (drop.mode) g = (bits[i] >> j & 1) ? g * scale : A(0);
+        const A h = c + j < cols ? ((A)xv[i].e[j] - mean) * rstd : A(0);
+        const A a = w ? g * t[j] : g;
+        s1 += a;
+        s2 += a * h;
+        aw[i][j] += g * h;
+        ab[i][j] += g;
+      }
+    }
+    if (!dx) continue;
+    row_sum2<LANES>(s1, s2, buf[turn]);
+    s1 /= (A)cols;
+    s2 /= (A)cols;
+    if (!live) continue;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * LANES + lane) * N;
+      A t[N];
+      if (w) load_weights<A, W, N>(t, w, c, cols);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        A g = (A)gv[i].e[j];
+        if (drop.mode) g = (bits[i] >> j & 1) ? g * scale : A(0);
+        const A h = ((A)xv[i].e[j] - mean) * rstd;
+        const A a = w ? g * t[j] : g;
+        gv[i].e[j] = (X)(rstd * (a - s1 - h * s2));
+      }
+    }
+    store_row<X, LANES, NV>(gv, dx + row * cols, lane, cols);
+  }
+  if (!part) return;
+  A* p = part + (int64_t)blockIdx.x * 2 * cols;
+  if constexpr (RPB == 1) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int c = (i * LANES + lane) * N + j;
+        if (c < cols) p[c] = aw[i][j], p[cols + c] = ab[i][j];
+      }
+  } else {      // the workgroup's row groups, one after the other
+    __shared__ A col[2][LANES * NV * N];
+    for (int g = 0; g < RPB; ++g) {
+      if (sub == g)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            const int c = (i * LANES + lane) * N + j;
+            col[0][c] = g ? col[0][c] + aw[i][j] : aw[i][j];
+            col[1][c] = g ? col[1][c] + ab[i][j] : ab[i][j];
+          }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < cols; c += 256) p[c] = col[0][c], p[cols + c] = col[1][c];
+  }
+}
+
+// ---------------------------------------------------------------------------------------
 // Dropout of a contiguous array
 // ---------------------------------------------------------------------------------------
 template <typename X>
@@ -317,13 +552,41 @@ bool types_ok(int dtype, int wdtype) {
   return dtype == wdtype ? dtype >= 0 && dtype <= 3 : (dtype == 2 || dtype == 3) && wdtype == 1;
 }
 
-// how the column sums of a backward pass are split over the rows
+// Which lanes own a row: as few as hold it in 16 elements a lane (8 of float64; the backward pass keeps two sums beside
+// each, and more does not fit the registers of a full workgroup).
+struct Layout {
+  int lanes, nv;     // lanes 0: longer than the registers hold, a workgroup walks the row
+};
+Layout row_layout(int dtype, int cols) {
+  const int n = dtype == 0 ? 2 : dtype == 1 ? 4 : 8;         // elements of a 16-byte vector
+  const int64_t nvec = ((int64_t)cols + n - 1) / n;
+  const bool half = n == 8;
+  if (nvec <= 16) return {16, 1};
+  if (nvec <= 32) return {16, 2};
+  if (nvec <= 64) return {64, 1};
+  if (nvec <= 128) return {64, 2};
+  if (nvec <= 256) return half ? Layout{256, 1} : Layout{64, 4};
+  if (nvec <= 512) return {256, 2};
+  if (nvec <= 1024) return half ? Layout{512, 2} : Layout{256, 4};
+  if (nvec <= 2048) return half ? Layout{1024, 2} : Layout{512, 4};
+  if (nvec <= 4096 && !half) return {1024, 4};
+  return {0, 0};
+}
+
+// workgroups of the backward pass: each leaves one partial row of column sums
+int bwd_groups(const Layout& l, int64_t rows) {
+  const int rpb = max(1, 256 / max(l.lanes, 1));
+  const int per_cu = l.lanes <= 256 ? 4 : l.lanes == 512 ? 2 : 1;
+  return (int)min((rows + rpb - 1) / rpb, (int64_t)(per_cu * CUS));
+}
+
+// column sums of rows the registers do not hold: a thread a column over a range of rows
 struct ColsPlan {
   int splits;
   int64_t rows_per_split;
 };
 ColsPlan cols_plan(int64_t rows, int cols) {
-  const int64_t tiles = (cols + 255) / 256;
+  const int64_t tiles = ((int64_t)cols + 255) / 256;
   int64_t s = min((int64_t)1024, max((int64_t)1, 8 * CUS / tiles));
   s = min(s, (rows + 15) / 16);
   ColsPlan p;
@@ -332,12 +595,60 @@ ColsPlan cols_plan(int64_t rows, int cols) {
   return p;
 }
 
+int bwd_parts(int dtype, int64_t rows, int cols) {
+  const Layout l = row_layout(dtype, cols);
+  return l.lanes ? bwd_groups(l, rows) : cols_plan(rows, cols).splits;
+}
+
+template <typename X>
+constexpr int type_code() {
+  return sizeof(X) == 8 ? 0 : sizeof(X) == 4 ? 1 : 2;      // (layouts depend on the size alone)
+}
+
+// K(LANES, NV) of a layout
+#define TTK_BY_LAYOUT(K)                                    \
+  if constexpr (sizeof(X) == 2) {                           \
+    switch (l.lanes * 16 + l.nv) {                          \
+      case 16 * 16 + 1: K(16, 1); break;                    \
+      case 16 * 16 + 2: K(16, 2); break;                    \
+      case 64 * 16 + 1: K(64, 1); break;                    \
+      case 64 * 16 + 2: K(64, 2); break;                    \
+      case 256 * 16 + 1: K(256, 1); break;                  \
+      case 256 * 16 + 2: K(256, 2); break;                  \
+      case 512 * 16 + 2: K(512, 2); break;                  \
+      case 1024 * 16 + 2: K(1024, 2); break;                \
+    }                                                       \
+  } else {                                                  \
+    switch (l.lanes * 16 + l.nv) {                          \
+      case 16 * 16 + 1: K(16, 1); break;                    \
+      case 16 * 16 + 2: K(16, 2); break;                    \
+      case 64 * 16 + 1: K(64, 1); break;                    \
+      case 64 * 16 + 2: K(64, 2); break;                    \
+      case 64 * 16 + 4: K(64, 4); break;                    \
+      case 256 * 16 + 2: K(256, 2); break;                  \
+      case 256 * 16 + 4: K(256, 4); break;                  \
+      case 512 * 16 + 4: K(512, 4); break;                  \
+      case 1024 * 16 + 4: K(1024, 4); break;                \
+    }                                                       \
+  }
+
 template <typename X, typename W>
 int ln_fwd(const void* x, int64_t ldx, const void* w, const void* b, void* y, void* mean, void* rstd, int64_t rows, int cols,
            double eps, const Drop& d, hipStream_t st) {
   typedef typename Acc<X>::type A;
-  hipLaunchKernelGGL((ln_fwd_long_kernel<X, W>), dim3((unsigned)min(rows, (int64_t)(4 * CUS))), dim3(LONG_THREADS), 0, st,
-                     (const X*)x, ldx, (const W*)w, (const W*)b, (X*)y, (A*)mean, (A*)rstd, rows, cols, eps, d);
+  const Layout l = row_layout(type_code<X>(), cols);
+  if (!l.lanes) {
+    hipLaunchKernelGGL((ln_fwd_long_kernel<X, W>), dim3((unsigned)min(rows, (int64_t)(4 * CUS))), dim3(LONG_THREADS), 0, st,
+                       (const X*)x, ldx, (const W*)w, (const W*)b, (X*)y, (A*)mean, (A*)rstd, rows, cols, eps, d);
+    return status();
+  }
+  const int rpb = max(1, 256 / l.lanes);
+  const dim3 grid((unsigned)min((rows + rpb - 1) / rpb, (int64_t)(16 * CUS)));
+#define K(LANES, NV)                                                                                                      \
+  hipLaunchKernelGGL((ln_fwd_group_kernel<X, W, LANES, NV>), grid, dim3(group_threads(LANES)), 0, st, (const X*)x, ldx,    \
+                     (const W*)w, (const W*)b, (X*)y, (A*)mean, (A*)rstd, rows, cols, eps, d)
+  TTK_BY_LAYOUT(K)
+#undef K
   return status();
 }
 
@@ -345,18 +656,29 @@ template <typename X, typename W>
 int ln_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, const void* mean, const void* rstd, void* dx,
            void* dw, void* db, int64_t rows, int cols, const Drop& d, void* ws, int64_t ws_bytes, hipStream_t st) {
   typedef typename Acc<X>::type A;
-  const ColsPlan cp = cols_plan(rows, cols);
-  if ((dw || db) && (!ws || ws_bytes < (int64_t)cp.splits * 2 * cols * (int64_t)sizeof(A))) return TTK_EWORKSPACE;
-  if (dx)
-    hipLaunchKernelGGL((ln_bwd_long_kernel<X, W>), dim3((unsigned)min(rows, (int64_t)(4 * CUS))), dim3(LONG_THREADS), 0, st,
-                       (const X*)dy, lddy, (const X*)x, ldx, (const W*)w, (const A*)mean, (const A*)rstd, (X*)dx, rows, cols, d);
-  if (dw || db) {
-    hipLaunchKernelGGL((ln_cols_kernel<X>), dim3((unsigned)((cols + 255) / 256), (unsigned)cp.splits), dim3(256), 0, st,
-                       (const X*)dy, lddy, (const X*)x, ldx, (const A*)mean, (const A*)rstd, (A*)ws, rows, cols,
-                       cp.rows_per_split, d);
-    hipLaunchKernelGGL((ln_cols_sum_kernel<A, W>), dim3((unsigned)((cols + 63) / 64), 2), dim3(1024), 0, st, (const A*)ws,
-                       cp.splits, cols, (W*)dw, (W*)db);
+  const Layout l = row_layout(type_code<X>(), cols);
+  const int parts = bwd_parts(type_code<X>(), rows, cols);
+  const bool sums = dw || db;
+  if (sums && (!ws || ws_bytes < (int64_t)parts * 2 * cols * (int64_t)sizeof(A))) return TTK_EWORKSPACE;
+  if (l.lanes && (dx || sums)) {
+#define K(LANES, NV)                                                                                                        \
+  hipLaunchKernelGGL((ln_bwd_group_kernel<X, W, LANES, NV>), dim3((unsigned)parts), dim3(group_threads(LANES)), 0, st,       \
+                     (const X*)dy, lddy, (const X*)x, ldx, (const W*)w, (const A*)mean, (const A*)rstd, (X*)dx,              \
+                     sums ? (A*)ws : (A*)nullptr, rows, cols, d)
+    TTK_BY_LAYOUT(K)
+#undef K
+  } else {
+    if (dx)
+      hipLaunchKernelGGL((ln_bwd_long_kernel<X, W>), dim3((unsigned)min(rows, (int64_t)(4 * CUS))), dim3(LONG_THREADS), 0, st,
+                         (const X*)dy, lddy, (const X*)x, ldx, (const W*)w, (const A*)mean, (const A*)rstd, (X*)dx, rows, cols, d);
+    if (sums)
+      hipLaunchKernelGGL((ln_cols_kernel<X>), dim3((unsigned)((cols + 255) / 256), (unsigned)parts), dim3(256), 0, st,
+                         (const X*)dy, lddy, (const X*)x, ldx, (const A*)mean, (const A*)rstd, (A*)ws, rows, cols,
+                         cols_plan(rows, cols).rows_per_split, d);
   }
+  if (sums)
+    hipLaunchKernelGGL((ln_cols_sum_kernel<A, W>), dim3((unsigned)((cols + 63) / 64), 2), dim3(1024), 0, st, (const A*)ws, parts,
+                       cols, (W*)dw, (W*)db);
   return status();
 }
 
@@ -389,7 +711,7 @@ int ttk_layer_norm(int dtype, int wdtype, const void* x, int64_t ldx, const void
 
 int64_t ttk_layer_norm_backward_ws_bytes(int dtype, int64_t rows, int cols) {
   if (dtype < 0 || dtype > 3 || rows < 1 || cols < 1) return TTK_EINVAL;
-  return (int64_t)cols_plan(rows, cols).splits * 2 * cols * (dtype == 0 ? 8 : 4);
+  return (int64_t)bwd_parts(dtype, rows, cols) * 2 * cols * (dtype == 0 ? 8 : 4);
 }
 
 int ttk_layer_norm_backward(int dtype, int wdtype, const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w,

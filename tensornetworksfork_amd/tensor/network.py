@@ -126,10 +126,10 @@ class TensorNetwork:
         user = torch.cuda.current_stream(device)
         pipe = TensorNetwork._pipe_streams.get(device)
         if pipe is None:
-            # High priority: streams of one priority share a few hardware queues in creation order, and behind the
-            # streams a collective library creates the pipeline stream can land on the caller's queue, which runs
-            # the two one after the other (measured on the multi-rank path: 0.3 ms per core update).
-            pipe = TensorNetwork._pipe_streams[device] = torch.cuda.Stream(device, priority=-1)
+            # Default priority: work on streams of different priorities has hung on this hardware.  (Streams of one
+            # priority share a few hardware queues in creation order, so behind a collective library's streams this one
+            # can land on the caller's queue, which runs the two one after the other.)
+            pipe = TensorNetwork._pipe_streams[device] = torch.cuda.Stream(device)
         return user, pipe
 
     def _user_guard(self, d=None, heavy=False):
