@@ -479,7 +479,7 @@ int ttk_dropout(int dtype, const void* x, void* y, int64_t n, double p, uint64_t
 /* Layer norm over the last axis, dropout as its epilogue (p = 0: none; element number = offset + row cols + column):
  *   y = drop((x - mean) rstd w + b),  rstd = 1 / sqrt(mean((x - mean)^2) + eps)
  * x (rows, cols) with row distance ldx, w / b (cols) or NULL in wdtype (dtype, or float32 for 16-bit rows), y dense,
- * mean / rstd (rows) in float32 (float64 for float64 rows). */
+ * mean / rstd (rows) in float32 (float64 for float64 rows), both NULL where they are not wanted. */
 int ttk_layer_norm(int dtype, int wdtype, const void* x, int64_t ldx, const void* w, const void* b, void* y, void* mean,
                    void* rstd, int64_t rows, int cols, double eps, double p, uint64_t seed, int64_t offset,
                    const int64_t* offset_dev, void* stream);

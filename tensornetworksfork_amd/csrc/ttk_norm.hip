@@ -73,21 +73,31 @@ __device__ __forceinline__ uint64_t drop_base(const Drop& d) {
   return (uint64_t)d.offset + (d.offset_dev ? (uint64_t)*d.offset_dev : 0ull);
 }
 
-// bit i = element 4 block + i is kept
-__device__ __forceinline__ uint32_t philox_keep4(const Drop& d, uint64_t block) {
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
+  return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);      // (the compiler keeps two xors by itself)
+}
+
+__device__ __forceinline__ void philox(const Drop& d, uint64_t block, uint32_t (&out)[4]) {
   uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32), c2 = 0, c3 = 0, k0 = d.k0, k1 = d.k1;
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const uint64_t p0 = (uint64_t)c0 * 0xD2511F53u, p1 = (uint64_t)c2 * 0xCD9E8D57u;
-    c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0;
+    c0 = xor3((uint32_t)(p1 >> 32), c1, k0);
     c1 = (uint32_t)p1;
-    c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1;
+    c2 = xor3((uint32_t)(p0 >> 32), c3, k1);
     c3 = (uint32_t)p0;
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }
+  out[0] = c0, out[1] = c1, out[2] = c2, out[3] = c3;
+}
+
+// bit i = element 4 block + i is kept
+__device__ __forceinline__ uint32_t philox_keep4(const Drop& d, uint64_t block) {
+  uint32_t w[4];
+  philox(d, block, w);
   const uint32_t t = d.threshold;
-  return (uint32_t)(c0 >= t) | ((uint32_t)(c1 >= t) << 1) | ((uint32_t)(c2 >= t) << 2) | ((uint32_t)(c3 >= t) << 3);
+  return (uint32_t)(w[0] >= t) | ((uint32_t)(w[1] >= t) << 1) | ((uint32_t)(w[2] >= t) << 2) | ((uint32_t)(w[3] >= t) << 3);
 }
 
 // bits of the N elements e, e + 1, ...
@@ -182,7 +192,7 @@ __global__ __launch_bounds__(LONG_THREADS) void ln_fwd_long_kernel(const X* __re
       if (drop.mode) v = (keep_bits<1>(drop, e0 + (uint64_t)row * cols + c) & 1) ? v * scale : A(0);
       y[row * cols + c] = (X)v;
     }
-    if (threadIdx.x == 0) mean_out[row] = mean, rstd_out[row] = rstd;
+    if (threadIdx.x == 0 && mean_out) mean_out[row] = mean, rstd_out[row] = rstd;
   }
 }
 
@@ -345,6 +355,20 @@ __device__ __forceinline__ A row_sum(A a, A* buf) {
 
 constexpr int group_threads(int lanes) { return lanes < 256 ? 256 : lanes; }
 
+// weights of a lane's columns; absent ones act as `none`
+template <typename A, typename W, int LANES, int NV, int N>
+__device__ __forceinline__ void lane_weights(A (&out)[NV][N], const W* w, int lane, int cols, A none) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (w) {
+      load_weights<A, W, N>(out[i], w, (i * LANES + lane) * N, cols);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) out[i][j] = none;
+    }
+  }
+}
+
 template <typename X, typename W, int LANES, int NV>
 __global__ __launch_bounds__(group_threads(LANES)) void ln_fwd_group_kernel(
     const X* __restrict__ x, int64_t ldx, const W* __restrict__ w, const W* __restrict__ b, X* __restrict__ y,
@@ -352,15 +376,26 @@ __global__ __launch_bounds__(group_threads(LANES)) void ln_fwd_group_kernel(
     Drop drop) {
   typedef typename Acc<X>::type A;
   constexpr int N = Vec<X>::N, RPB = group_threads(LANES) / LANES;
+  constexpr bool HOLD = NV * N <= 8;            // weights stay in registers
   __shared__ A buf[2][LANES > 64 ? LANES / 64 : 1];
   const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
   const uint64_t e0 = drop_base(drop);
   const A scale = (A)drop.scale;
-  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB) {
+  A wv[NV][N], bv[NV][N];
+  if constexpr (HOLD) {
+    lane_weights<A, W, LANES, NV, N>(wv, w, lane, cols, A(1));
+    lane_weights<A, W, LANES, NV, N>(bv, b, lane, cols, A(0));
+  }
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  Vec<X> next[NV];
+  load_row<X, LANES, NV>(next, x + ((int64_t)blockIdx.x * RPB + sub) * ldx, lane, cols, (int64_t)blockIdx.x * RPB + sub < rows);
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += step) {
     const int64_t row = r0 + sub;
     const bool live = row < rows;
     Vec<X> v[NV];
-    load_row<X, LANES, NV>(v, x + row * ldx, lane, cols, live);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = next[i];
+    if (r0 + step < rows) load_row<X, LANES, NV>(next, x + (row + step) * ldx, lane, cols, row + step < rows);
     A s = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -377,26 +412,17 @@ __global__ __launch_bounds__(group_threads(LANES)) void ln_fwd_group_kernel(
       }
     const A rstd = A(1) / sqrt(row_sum<LANES>(q, buf[1]) / (A)cols + (A)eps);
     if (!live) continue;
+    if constexpr (!HOLD) {
+      lane_weights<A, W, LANES, NV, N>(wv, w, lane, cols, A(1));
+      lane_weights<A, W, LANES, NV, N>(bv, b, lane, cols, A(0));
+    }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * LANES + lane) * N;
       A h[N];
 #pragma unroll
-      for (int j = 0; j < N; ++j) h[j] = ((A)v[i].e[j] - mean) * rstd;
-      if (w) {
-        A t[N];
-        load_weights<A, W, N>(t, w, c, cols);
-#pragma unroll
-        for (int j = 0; j < N; ++j) h[j] *= t[j];
-      }
-      if (b) {
-        A t[N];
-        load_weights<A, W, N>(t, b, c, cols);
-#pragma unroll
-        for (int j = 0; j < N; ++j) h[j] += t[j];
-      }
+      for (int j = 0; j < N; ++j) h[j] = ((A)v[i].e[j] - mean) * rstd * wv[i][j] + bv[i][j];
       if (drop.mode) {
-        const uint32_t bits = keep_bits<N>(drop, e0 + (uint64_t)row * cols + c);
+        const uint32_t bits = keep_bits<N>(drop, e0 + (uint64_t)row * cols + (i * LANES + lane) * N);
 #pragma unroll
         for (int j = 0; j < N; ++j) h[j] = (bits >> j & 1) ? h[j] * scale : A(0);
       }
@@ -404,7 +430,7 @@ __global__ __launch_bounds__(group_threads(LANES)) void ln_fwd_group_kernel(
       for (int j = 0; j < N; ++j) v[i].e[j] = (X)h[j];
     }
     store_row<X, LANES, NV>(v, y + row * cols, lane, cols);
-    if (lane == 0) mean_out[row] = mean, rstd_out[row] = rstd;
+    if (lane == 0 && mean_out) mean_out[row] = mean, rstd_out[row] = rstd;
   }
 }
 
@@ -415,37 +441,50 @@ __global__ __launch_bounds__(group_threads(LANES)) void ln_bwd_group_kernel(
     typename Acc<X>::type* __restrict__ part, int64_t rows, int cols, Drop drop) {
   typedef typename Acc<X>::type A;
   constexpr int N = Vec<X>::N, RPB = group_threads(LANES) / LANES;
+  constexpr bool HOLD = NV * N <= 8;
   __shared__ A buf[2][LANES > 64 ? 2 * (LANES / 64) : 1];
   const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
   const uint64_t e0 = drop_base(drop);
   const A scale = (A)drop.scale;
-  A aw[NV][N], ab[NV][N];
+  A aw[NV][N], ab[NV][N], wv[NV][N];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < N; ++j) aw[i][j] = ab[i][j] = A(0);
+  if constexpr (HOLD) lane_weights<A, W, LANES, NV, N>(wv, w, lane, cols, A(1));
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  Vec<X> nx[NV], ng[NV];
+  A nmean = 0, nrstd = 0;
+  auto fetch = [&](int64_t row) {
+    const bool live = row < rows;
+    load_row<X, LANES, NV>(nx, x + row * ldx, lane, cols, live);
+    load_row<X, LANES, NV>(ng, dy + row * lddy, lane, cols, live);
+    nmean = live ? mean_in[row] : A(0);
+    nrstd = live ? rstd_in[row] : A(0);
+  };
+  fetch((int64_t)blockIdx.x * RPB + sub);
   int turn = 0;
-  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB, turn ^= 1) {
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += step, turn ^= 1) {
     const int64_t row = r0 + sub;
     const bool live = row < rows;
     Vec<X> xv[NV], gv[NV];
-    load_row<X, LANES, NV>(xv, x + row * ldx, lane, cols, live);
-    load_row<X, LANES, NV>(gv, dy + row * lddy, lane, cols, live);
-    const A mean = live ? mean_in[row] : A(0), rstd = live ? rstd_in[row] : A(0);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) xv[i] = nx[i], gv[i] = ng[i];
+    const A mean = nmean, rstd = nrstd;
+    if (r0 + step < rows) fetch(row + step);
+    if constexpr (!HOLD) lane_weights<A, W, LANES, NV, N>(wv, w, lane, cols, A(1));
     A s1 = 0, s2 = 0;
     uint32_t bits[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * LANES + lane) * N;
-      bits[i] = drop.mode && live ? keep_bits<N>(drop, e0 + (uint64_t)row * cols + c) : ~0u;
-      A t[N];
-      if (w) load_weights<A, W, N>(t, w, c, cols);
+      if (drop.mode) bits[i] = live ? keep_bits<N>(drop, e0 + (uint64_t)row * cols + c) : 0u;
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         A g = (A)gv[i].e[j];
         if (drop.mode) g = (bits[i] >> j & 1) ? g * scale : A(0);
         const A h = c + j < cols ? ((A)xv[i].e[j] - mean) * rstd : A(0);
-        const A a = w ? g * t[j] : g;
+        const A a = g * wv[i][j];
         s1 += a;
         s2 += a * h;
         aw[i][j] += g * h;
@@ -459,16 +498,12 @@ __global__ __launch_bounds__(group_threads(LANES)) void ln_bwd_group_kernel(
     if (!live) continue;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * LANES + lane) * N;
-      A t[N];
-      if (w) load_weights<A, W, N>(t, w, c, cols);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         A g = (A)gv[i].e[j];
         if (drop.mode) g = (bits[i] >> j & 1) ? g * scale : A(0);
         const A h = ((A)xv[i].e[j] - mean) * rstd;
-        const A a = w ? g * t[j] : g;
-        gv[i].e[j] = (X)(rstd * (a - s1 - h * s2));
+        gv[i].e[j] = (X)(rstd * (g * wv[i][j] - s1 - h * s2));
       }
     }
     store_row<X, LANES, NV>(gv, dx + row * cols, lane, cols);
@@ -502,29 +537,245 @@ __global__ __launch_bounds__(group_threads(LANES)) void ln_bwd_group_kernel(
 }
 
 // ---------------------------------------------------------------------------------------
+// Layer norm of short dense rows: a wave takes 64 rows at once.  The tile (one contiguous piece of memory) goes through
+// the wave's own LDS with 16-byte accesses to memory, then each lane owns one row in registers and needs no other lane;
+// rows lie an odd number of words apart in LDS.  No barrier: a wave's LDS accesses stay in order.
+// ---------------------------------------------------------------------------------------
+constexpr int SHORT_WAVES = 4;
+
+// LDS position of flat element i of the tile: one word of padding a row when the row length is even (inv = 65536 / cols
+// rounded up: exact for the tile's i < 2048)
+__device__ __forceinline__ int short_pos(int i, int pad, int inv) { return pad ? i + (int)((uint32_t)i * (uint32_t)inv >> 16) : i; }
+
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+template <typename X, typename A>
+__device__ __forceinline__ void short_load(A* lds, const X* p, int n, int lane, int pad, int inv) {
+  constexpr int N = Vec<X>::N;
+  for (int i = lane * N; i < n; i += 64 * N) {
+    Vec<X> v;
+    if (i + N <= n)
+      v.load(p + i);
+    else
+      v.load_some(p + i, n - i);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (i + j < n) lds[short_pos(i + j, pad, inv)] = (A)v.e[j];
+  }
+}
+
+template <typename X, typename W, int NC>
+__global__ __launch_bounds__(64 * SHORT_WAVES) void ln_fwd_short_kernel(
+    const X* __restrict__ x, const W* __restrict__ w, const W* __restrict__ b, X* __restrict__ y,
+    typename Acc<X>::type* __restrict__ mean_out, typename Acc<X>::type* __restrict__ rstd_out, int64_t rows, int cols, double eps,
+    Drop drop) {
+  typedef typename Acc<X>::type A;
+  constexpr int N = Vec<X>::N;
+  __shared__ A tile[SHORT_WAVES][64 * (NC | 1)];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  A* lds = tile[wave];
+  const int pad = cols % 2 == 0, pitch = cols | 1, inv = (65536 + cols - 1) / cols;
+  const uint64_t e0 = drop_base(drop);
+  const A scale = (A)drop.scale;
+  const int64_t tiles = (rows + 63) / 64;
+  for (int64_t t = (int64_t)blockIdx.x * SHORT_WAVES + wave; t < tiles; t += (int64_t)gridDim.x * SHORT_WAVES) {
+    const int64_t row0 = t * 64;
+    const int nr = (int)min((int64_t)64, rows - row0), n = nr * cols;
+    short_load<X, A>(lds, x + row0 * cols, n, lane, pad, inv);
+    wave_lds_fence();
+    if (lane < nr) {
+      A v[NC], s = 0, q = 0;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        if (c < cols) v[c] = lds[lane * pitch + c], s += v[c];
+      const A mean = s / (A)cols;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        if (c < cols) v[c] -= mean, q += v[c] * v[c];
+      const A rstd = A(1) / sqrt(q / (A)cols + (A)eps);
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        if (c < cols) {
+          A h = v[c] * rstd;
+          if (w) h *= (A)w[c];
+          if (b) h += (A)b[c];
+          lds[lane * pitch + c] = h;
+        }
+      if (mean_out) mean_out[row0 + lane] = mean, rstd_out[row0 + lane] = rstd;
+    }
+    wave_lds_fence();
+    X* out = y + row0 * cols;
+    for (int i = lane * N; i < n; i += 64 * N) {
+      Vec<X> v;
+      const uint32_t bits = keep_bits<N>(drop, e0 + (uint64_t)row0 * cols + i);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        A h = i + j < n ? lds[short_pos(i + j, pad, inv)] : A(0);
+        if (drop.mode) h = (bits >> j & 1) ? h * scale : A(0);
+        v.e[j] = (X)h;
+      }
+      if (i + N <= n)
+        v.store(out + i);
+      else
+        v.store_some(out + i, n - i);
+    }
+    wave_lds_fence();
+  }
+}
+
+template <typename X, typename W, int NC>
+__global__ __launch_bounds__(64 * SHORT_WAVES) void ln_bwd_short_kernel(
+    const X* __restrict__ dy, const X* __restrict__ x, const W* __restrict__ w, const typename Acc<X>::type* __restrict__ mean_in,
+    const typename Acc<X>::type* __restrict__ rstd_in, X* __restrict__ dx, typename Acc<X>::type* __restrict__ part, int64_t rows,
+    int cols, Drop drop) {
+  typedef typename Acc<X>::type A;
+  constexpr int N = Vec<X>::N;
+  __shared__ A tile[SHORT_WAVES][2][64 * (NC | 1)];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  A *lx = tile[wave][0], *lg = tile[wave][1];
+  const int pad = cols % 2 == 0, pitch = cols | 1, inv = (65536 + cols - 1) / cols;
+  const uint64_t e0 = drop_base(drop);
+  const A scale = (A)drop.scale;
+  A aw[NC], ab[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) aw[c] = ab[c] = A(0);
+  const int64_t tiles = (rows + 63) / 64;
+  for (int64_t t = (int64_t)blockIdx.x * SHORT_WAVES + wave; t < tiles; t += (int64_t)gridDim.x * SHORT_WAVES) {
+    const int64_t row0 = t * 64;
+    const int nr = (int)min((int64_t)64, rows - row0), n = nr * cols;
+    short_load<X, A>(lx, x + row0 * cols, n, lane, pad, inv);
+    const X* gp = dy + row0 * cols;
+    for (int i = lane * N; i < n; i += 64 * N) {
+      Vec<X> v;
+      if (i + N <= n)
+        v.load(gp + i);
+      else
+        v.load_some(gp + i, n - i);
+      const uint32_t bits = keep_bits<N>(drop, e0 + (uint64_t)row0 * cols + i);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        A g = (A)v.e[j];
+        if (drop.mode) g = (bits >> j & 1) ? g * scale : A(0);
+        if (i + j < n) lg[short_pos(i + j, pad, inv)] = g;
+      }
+    }
+    wave_lds_fence();
+    if (lane < nr) {
+      const A mean = mean_in[row0 + lane], rstd = rstd_in[row0 + lane];
+      A h[NC], g[NC], s1 = 0, s2 = 0;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        if (c < cols) {
+          h[c] = (lx[lane * pitch + c] - mean) * rstd;
+          g[c] = lg[lane * pitch + c];
+          aw[c] += g[c] * h[c];
+          ab[c] += g[c];
+          if (w) g[c] *= (A)w[c];
+          s1 += g[c];
+          s2 += g[c] * h[c];
+        }
+      s1 /= (A)cols;
+      s2 /= (A)cols;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        if (c < cols) lg[lane * pitch + c] = rstd * (g[c] - s1 - h[c] * s2);
+    }
+    wave_lds_fence();
+    if (dx) {
+      X* out = dx + row0 * cols;
+      for (int i = lane * N; i < n; i += 64 * N) {
+        Vec<X> v;
+#pragma unroll
+        for (int j = 0; j < N; ++j) v.e[j] = (X)(i + j < n ? lg[short_pos(i + j, pad, inv)] : A(0));
+        if (i + N <= n)
+          v.store(out + i);
+        else
+          v.store_some(out + i, n - i);
+      }
+    }
+    wave_lds_fence();
+  }
+  if (!part) return;
+  __shared__ A red[SHORT_WAVES][2][NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+    if (c < cols) {
+      const A a = lane_sum<64>(aw[c]), g = lane_sum<64>(ab[c]);
+      if (lane == 0) red[wave][0][c] = a, red[wave][1][c] = g;
+    }
+  __syncthreads();
+  A* p = part + (int64_t)blockIdx.x * 2 * cols;
+  for (int c = threadIdx.x; c < 2 * cols; c += 64 * SHORT_WAVES) {
+    const int k = c >= cols, cc = c - k * cols;
+    A s = red[0][k][cc];
+#pragma unroll
+    for (int i = 1; i < SHORT_WAVES; ++i) s += red[i][k][cc];
+    p[c] = s;
+  }
+}
+
+// ---------------------------------------------------------------------------------------
 // Dropout of a contiguous array
 // ---------------------------------------------------------------------------------------
+// Threads own whole counter blocks: a thread's elements start where e is a multiple of 4 (memory alignment does not
+// matter, see Vec), so no block is computed twice; the first and the last vector of the array may be partial.
+template <typename X>
+struct DropChunk {
+  static constexpr int E = sizeof(X) == 2 ? 8 : 4;         // elements a thread takes at once
+};
+
 template <typename X>
 __global__ __launch_bounds__(256) void dropout_kernel(const X* x, X* y, int64_t n, Drop drop) {
   typedef typename Acc<X>::type A;
-  constexpr int N = Vec<X>::N;
+  constexpr int N = Vec<X>::N, E = DropChunk<X>::E, V = E / N;
   const uint64_t e0 = drop_base(drop);
+  const int s = (int)(e0 & 3);
+  const uint64_t b0 = e0 >> 2;
   const A scale = (A)drop.scale;
-  const int64_t step = (int64_t)gridDim.x * 256 * N;
-  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * N; i < n; i += step) {
-    Vec<X> v;
-    const int m = (int)min((int64_t)N, n - i);
-    if (m == N)
-      v.load(x + i);
-    else
-      v.load_some(x + i, m);
-    const uint32_t bits = keep_bits<N>(drop, e0 + (uint64_t)i);
+  const int64_t step = (int64_t)gridDim.x * 256 * E;
+  for (int64_t a = ((int64_t)blockIdx.x * 256 + threadIdx.x) * E; a - s < n; a += step) {
+    const int64_t i = a - s;                                // a thread's elements are i .. i + E - 1
+    const bool whole = i >= 0 && i + E <= n;
+    Vec<X> v[V];
+    if (whole) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) v.e[j] = (bits >> j & 1) ? (X)((A)v.e[j] * scale) : (X)A(0);
-    if (m == N)
-      v.store(y + i);
-    else
-      v.store_some(y + i, m);
+      for (int k = 0; k < V; ++k) v[k].load(x + i + k * N);
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k)
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[k].e[j] = i + k * N + j >= 0 && i + k * N + j < n ? x[i + k * N + j] : (X)A(0);
+    }
+    if (drop.mode == 1) {
+#pragma unroll
+      for (int q = 0; q < E / 4; ++q) {
+        uint32_t w[4];
+        philox(drop, b0 + (uint64_t)(a >> 2) + q, w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          X& t = v[(4 * q + j) / N].e[(4 * q + j) % N];
+          t = (X)(w[j] >= drop.threshold ? (A)t * scale : A(0));
+        }
+      }
+    } else if (drop.mode == 2) {
+#pragma unroll
+      for (int k = 0; k < V; ++k)
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[k].e[j] = (X)A(0);
+    }
+    if (whole) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k].store(y + i + k * N);
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k)
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (i + k * N + j >= 0 && i + k * N + j < n) y[i + k * N + j] = v[k].e[j];
+    }
   }
 }
 
@@ -552,31 +803,32 @@ bool types_ok(int dtype, int wdtype) {
   return dtype == wdtype ? dtype >= 0 && dtype <= 3 : (dtype == 2 || dtype == 3) && wdtype == 1;
 }
 
-// Which lanes own a row: as few as hold it in 16 elements a lane (8 of float64; the backward pass keeps two sums beside
-// each, and more does not fit the registers of a full workgroup).
+// Which lanes own a row.
 struct Layout {
-  int lanes, nv;     // lanes 0: longer than the registers hold, a workgroup walks the row
+  int lanes, nv;     // lanes 1: short dense rows, nv columns at most; lanes 0: longer than the registers hold
 };
-Layout row_layout(int dtype, int cols) {
+Layout row_layout(int dtype, int cols, bool dense) {
+  if (dense && cols <= (dtype == 0 ? 16 : 32)) return {1, (cols + 7) / 8 * 8};
   const int n = dtype == 0 ? 2 : dtype == 1 ? 4 : 8;         // elements of a 16-byte vector
   const int64_t nvec = ((int64_t)cols + n - 1) / n;
   const bool half = n == 8;
   if (nvec <= 16) return {16, 1};
-  if (nvec <= 32) return {16, 2};
+  if (nvec <= 32 && !half) return {16, 2};
   if (nvec <= 64) return {64, 1};
   if (nvec <= 128) return {64, 2};
   if (nvec <= 256) return half ? Layout{256, 1} : Layout{64, 4};
-  if (nvec <= 512) return {256, 2};
-  if (nvec <= 1024) return half ? Layout{512, 2} : Layout{256, 4};
-  if (nvec <= 2048) return half ? Layout{1024, 2} : Layout{512, 4};
+  if (nvec <= 512) return half ? Layout{512, 1} : Layout{256, 2};
+  if (nvec <= 1024) return half ? Layout{1024, 1} : Layout{512, 2};
+  if (nvec <= 2048) return {1024, 2};
   if (nvec <= 4096 && !half) return {1024, 4};
   return {0, 0};
 }
 
-// workgroups of the backward pass: each leaves one partial row of column sums
-int bwd_groups(const Layout& l, int64_t rows) {
-  const int rpb = max(1, 256 / max(l.lanes, 1));
-  const int per_cu = l.lanes <= 256 ? 4 : l.lanes == 512 ? 2 : 1;
+// Workgroups of a launch: as many as are resident at a time, each walks its share of the rows (the backward pass leaves
+// one partial row of column sums per workgroup).
+int row_groups(const Layout& l, int64_t rows, bool backward) {
+  const int64_t rpb = l.lanes == 1 ? 64 * SHORT_WAVES : max(1, 256 / l.lanes);
+  const int per_cu = l.lanes <= 256 ? (backward ? 4 : 8) : l.lanes == 512 ? (backward ? 2 : 4) : (backward ? 1 : 2);
   return (int)min((rows + rpb - 1) / rpb, (int64_t)(per_cu * CUS));
 }
 
@@ -595,9 +847,8 @@ ColsPlan cols_plan(int64_t rows, int cols) {
   return p;
 }
 
-int bwd_parts(int dtype, int64_t rows, int cols) {
-  const Layout l = row_layout(dtype, cols);
-  return l.lanes ? bwd_groups(l, rows) : cols_plan(rows, cols).splits;
+int bwd_parts(const Layout& l, int64_t rows, int cols) {
+  return l.lanes ? row_groups(l, rows, true) : cols_plan(rows, cols).splits;
 }
 
 template <typename X>
@@ -605,17 +856,27 @@ constexpr int type_code() {
   return sizeof(X) == 8 ? 0 : sizeof(X) == 4 ? 1 : 2;      // (layouts depend on the size alone)
 }
 
-// K(LANES, NV) of a layout
-#define TTK_BY_LAYOUT(K)                                    \
-  if constexpr (sizeof(X) == 2) {                           \
+// K(LANES, NV) of a layout, S(NC) of short rows
+#define TTK_BY_LAYOUT(K, S)                                 \
+  if (l.lanes == 1) {                                       \
+    switch (l.nv) {                                         \
+      case 8: S(8); break;                                  \
+      case 16: S(16); break;                                \
+      case 24:                                              \
+        if constexpr (sizeof(X) < 8) { S(24); }             \
+        break;                                              \
+      case 32:                                              \
+        if constexpr (sizeof(X) < 8) { S(32); }             \
+        break;                                              \
+    }                                                       \
+  } else if constexpr (sizeof(X) == 2) {                    \
     switch (l.lanes * 16 + l.nv) {                          \
       case 16 * 16 + 1: K(16, 1); break;                    \
-      case 16 * 16 + 2: K(16, 2); break;                    \
       case 64 * 16 + 1: K(64, 1); break;                    \
       case 64 * 16 + 2: K(64, 2); break;                    \
       case 256 * 16 + 1: K(256, 1); break;                  \
-      case 256 * 16 + 2: K(256, 2); break;                  \
-      case 512 * 16 + 2: K(512, 2); break;                  \
+      case 512 * 16 + 1: K(512, 1); break;                  \
+      case 1024 * 16 + 1: K(1024, 1); break;                \
       case 1024 * 16 + 2: K(1024, 2); break;                \
     }                                                       \
   } else {                                                  \
@@ -626,8 +887,8 @@ constexpr int type_code() {
       case 64 * 16 + 2: K(64, 2); break;                    \
       case 64 * 16 + 4: K(64, 4); break;                    \
       case 256 * 16 + 2: K(256, 2); break;                  \
-      case 256 * 16 + 4: K(256, 4); break;                  \
-      case 512 * 16 + 4: K(512, 4); break;                  \
+      case 512 * 16 + 2: K(512, 2); break;                  \
+      case 1024 * 16 + 2: K(1024, 2); break;                \
       case 1024 * 16 + 4: K(1024, 4); break;                \
     }                                                       \
   }
@@ -636,19 +897,22 @@ template <typename X, typename W>
 int ln_fwd(const void* x, int64_t ldx, const void* w, const void* b, void* y, void* mean, void* rstd, int64_t rows, int cols,
            double eps, const Drop& d, hipStream_t st) {
   typedef typename Acc<X>::type A;
-  const Layout l = row_layout(type_code<X>(), cols);
+  const Layout l = row_layout(type_code<X>(), cols, ldx == cols || rows == 1);
   if (!l.lanes) {
     hipLaunchKernelGGL((ln_fwd_long_kernel<X, W>), dim3((unsigned)min(rows, (int64_t)(4 * CUS))), dim3(LONG_THREADS), 0, st,
                        (const X*)x, ldx, (const W*)w, (const W*)b, (X*)y, (A*)mean, (A*)rstd, rows, cols, eps, d);
     return status();
   }
-  const int rpb = max(1, 256 / l.lanes);
-  const dim3 grid((unsigned)min((rows + rpb - 1) / rpb, (int64_t)(16 * CUS)));
+  const dim3 grid((unsigned)row_groups(l, rows, false));
 #define K(LANES, NV)                                                                                                      \
   hipLaunchKernelGGL((ln_fwd_group_kernel<X, W, LANES, NV>), grid, dim3(group_threads(LANES)), 0, st, (const X*)x, ldx,    \
                      (const W*)w, (const W*)b, (X*)y, (A*)mean, (A*)rstd, rows, cols, eps, d)
-  TTK_BY_LAYOUT(K)
+#define S(NC)                                                                                                             \
+  hipLaunchKernelGGL((ln_fwd_short_kernel<X, W, NC>), grid, dim3(64 * SHORT_WAVES), 0, st, (const X*)x, (const W*)w,       \
+                     (const W*)b, (X*)y, (A*)mean, (A*)rstd, rows, cols, eps, d)
+  TTK_BY_LAYOUT(K, S)
 #undef K
+#undef S
   return status();
 }
 
@@ -656,18 +920,23 @@ template <typename X, typename W>
 int ln_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, const void* mean, const void* rstd, void* dx,
            void* dw, void* db, int64_t rows, int cols, const Drop& d, void* ws, int64_t ws_bytes, hipStream_t st) {
   typedef typename Acc<X>::type A;
-  const Layout l = row_layout(type_code<X>(), cols);
-  const int parts = bwd_parts(type_code<X>(), rows, cols);
+  const Layout l = row_layout(type_code<X>(), cols, (ldx == cols && lddy == cols) || rows == 1);
+  const int parts = bwd_parts(l, rows, cols);
   const bool sums = dw || db;
   if (sums && (!ws || ws_bytes < (int64_t)parts * 2 * cols * (int64_t)sizeof(A))) return TTK_EWORKSPACE;
   if (l.lanes && (dx || sums)) {
-#define K(LANES, NV)                                                                                                        \
-  hipLaunchKernelGGL((ln_bwd_group_kernel<X, W, LANES, NV>), dim3((unsigned)parts), dim3(group_threads(LANES)), 0, st,       \
-                     (const X*)dy, lddy, (const X*)x, ldx, (const W*)w, (const A*)mean, (const A*)rstd, (X*)dx,              \
-                     sums ? (A*)ws : (A*)nullptr, rows, cols, d)
-    TTK_BY_LAYOUT(K)
+    A* part = sums ? (A*)ws : (A*)nullptr;
+#define K(LANES, NV)                                                                                                      \
+  hipLaunchKernelGGL((ln_bwd_group_kernel<X, W, LANES, NV>), dim3((unsigned)parts), dim3(group_threads(LANES)), 0, st,     \
+                     (const X*)dy, lddy, (const X*)x, ldx, (const W*)w, (const A*)mean, (const A*)rstd, (X*)dx, part,      \
+                     rows, cols, d)
+#define S(NC)                                                                                                             \
+  hipLaunchKernelGGL((ln_bwd_short_kernel<X, W, NC>), dim3((unsigned)parts), dim3(64 * SHORT_WAVES), 0, st, (const X*)dy,  \
+                     (const X*)x, (const W*)w, (const A*)mean, (const A*)rstd, (X*)dx, part, rows, cols, d)
+    TTK_BY_LAYOUT(K, S)
 #undef K
-  } else {
+#undef S
+  } else if (!l.lanes) {
     if (dx)
       hipLaunchKernelGGL((ln_bwd_long_kernel<X, W>), dim3((unsigned)min(rows, (int64_t)(4 * CUS))), dim3(LONG_THREADS), 0, st,
                          (const X*)dy, lddy, (const X*)x, ldx, (const W*)w, (const A*)mean, (const A*)rstd, (X*)dx, rows, cols, d);
@@ -702,7 +971,7 @@ int ttk_layer_norm(int dtype, int wdtype, const void* x, int64_t ldx, const void
                    int64_t rows, int cols, double eps, double p, uint64_t seed, int64_t offset, const int64_t* offset_dev,
                    void* stream) {
   Drop d;
-  if (!x || !y || !mean || !rstd || rows < 1 || cols < 1 || ldx < 0 || !(eps >= 0.0) || !types_ok(dtype, wdtype) ||
+  if (!x || !y || !mean != !rstd || rows < 1 || cols < 1 || ldx < 0 || !(eps >= 0.0) || !types_ok(dtype, wdtype) ||
       !make_drop(d, p, seed, offset, offset_dev))
     return TTK_EINVAL;
   hipStream_t st = (hipStream_t)stream;
@@ -711,7 +980,8 @@ int ttk_layer_norm(int dtype, int wdtype, const void* x, int64_t ldx, const void
 
 int64_t ttk_layer_norm_backward_ws_bytes(int dtype, int64_t rows, int cols) {
   if (dtype < 0 || dtype > 3 || rows < 1 || cols < 1) return TTK_EINVAL;
-  return (int64_t)bwd_parts(dtype, rows, cols) * 2 * cols * (dtype == 0 ? 8 : 4);
+  const int parts = max(bwd_parts(row_layout(dtype, cols, true), rows, cols), bwd_parts(row_layout(dtype, cols, false), rows, cols));
+  return (int64_t)parts * 2 * cols * (dtype == 0 ? 8 : 4);
 }
 
 int ttk_layer_norm_backward(int dtype, int wdtype, const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w,
@@ -730,8 +1000,8 @@ int ttk_dropout(int dtype, const void* x, void* y, int64_t n, double p, uint64_t
   Drop d;
   if (!x || !y || n < 1 || dtype < 0 || dtype > 3 || !make_drop(d, p, seed, offset, offset_dev)) return TTK_EINVAL;
   hipStream_t st = (hipStream_t)stream;
-  const int per = 256 * (dtype == 0 ? 2 : dtype == 1 ? 4 : 8);
-  const dim3 grid((unsigned)min((n + per - 1) / per, (int64_t)(16 * CUS)));
+  const int per = 256 * (dtype < 2 ? 4 : 8);
+  const dim3 grid((unsigned)min((n + 3 + per - 1) / per, (int64_t)(16 * CUS)));
   switch (dtype) {
     case 0: hipLaunchKernelGGL((dropout_kernel<double>), grid, dim3(256), 0, st, (const double*)x, (double*)y, n, d); break;
     case 1: hipLaunchKernelGGL((dropout_kernel<float>), grid, dim3(256), 0, st, (const float*)x, (float*)y, n, d); break;

@@ -1085,9 +1085,17 @@ def patchify(images, kernel_size, stride, dtype=None):
 ROW_TYPES = {torch.float64: 0, torch.float32: 1, torch.bfloat16: 2, torch.float16: 3}
 
 
-def _on(t):
-    """The launch device: `t`'s own, whichever is current."""
-    return torch.cuda.device(t.device)
+def _launch(what, device, *args):
+    """Calls an entry point on `device` (whichever is current) with the device's current stream as its last argument."""
+    fn = getattr(_lib.lib(), what)
+    at = device.index
+    if at == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(at))
+    else:
+        with torch.cuda.device(at):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(at))
+    if rc:
+        _lib.check(rc, what)
 
 
 def _row_tensor(t, name, device=None):
@@ -1105,7 +1113,10 @@ def rows_view(t, name="x"):
     row distance (contiguous tensors, column ranges of a wider matrix, one row broadcast to many)."""
     if t.ndim == 0 or t.shape[-1] == 0:
         raise _lib.TTKError(f"{name}: expected at least one axis and one column, got shape {tuple(t.shape)}")
-    rows, cols = t.numel() // t.shape[-1], t.shape[-1]
+    cols = t.shape[-1]
+    rows = t.numel() // cols
+    if cols <= 0x7FFFFFFF and t.is_contiguous():
+        return rows, cols, cols
     if cols > 0x7FFFFFFF:
         raise _lib.TTKError(f"{name}: more than 2^31 - 1 columns")
     if cols > 1 and t.stride(-1) != 1:
@@ -1145,9 +1156,9 @@ def _norm_vector(v, name, x, cols):
     return v.data_ptr()
 
 
-def layer_norm(x, weight=None, bias=None, eps=1e-5, p=0.0, seed=0, offset=0):
+def layer_norm(x, weight=None, bias=None, eps=1e-5, p=0.0, seed=0, offset=0, stats=True):
     """Layer norm over the last axis, then dropout -> (y, mean, rstd); mean / rstd have x's leading shape and are float32
-    (float64 for float64 rows).  weight / bias: (cols,) of x's type, or float32 with 16-bit rows (both alike)."""
+    (float64 for float64 rows), None when `stats` is False.  weight / bias: (cols,) of x's type, or float32 with 16-bit rows (both alike)."""
     _row_tensor(x, "x")
     rows, cols, ld = rows_view(x)
     wp, bp = _norm_vector(weight, "weight", x, cols), _norm_vector(bias, "bias", x, cols)
@@ -1158,14 +1169,13 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, p=0.0, seed=0, offset=0):
     p, seed, off, off_dev = _drop_args(p, seed, offset, x.device)
     wt = weight if weight is not None else bias if bias is not None else x
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = torch.empty(x.shape[:-1], dtype=F64 if x.dtype == F64 else torch.float32, device=x.device)
-    rstd = torch.empty_like(mean)
+    mean = rstd = None
+    if stats:
+        mean = torch.empty(x.shape[:-1], dtype=F64 if x.dtype == F64 else torch.float32, device=x.device)
+        rstd = torch.empty_like(mean)
     if rows:
-        with _on(x):
-            rc = _lib.lib().ttk_layer_norm(ROW_TYPES[x.dtype], ROW_TYPES[wt.dtype], x.data_ptr(), ld, wp, bp, y.data_ptr(),
-                                           mean.data_ptr(), rstd.data_ptr(), rows, cols, float(eps), p, seed, off, off_dev,
-                                           _stream(x))
-        _lib.check(rc, "ttk_layer_norm")
+        _launch("ttk_layer_norm", x.device, ROW_TYPES[x.dtype], ROW_TYPES[wt.dtype], x.data_ptr(), ld, wp, bp, y.data_ptr(),
+                mean.data_ptr() if stats else None, rstd.data_ptr() if stats else None, rows, cols, float(eps), p, seed, off, off_dev)
     return y, mean, rstd
 
 
@@ -1194,17 +1204,13 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, p=0.0, seed=0, offset=0,
     dw = make((cols,), dtype=wdt, device=x.device) if need[1] else None
     db = make((cols,), dtype=wdt, device=x.device) if need[2] else None
     if rows and any(need):
-        L = _lib.lib()
         ws, nbytes = None, 0
         if need[1] or need[2]:
-            nbytes = int(L.ttk_layer_norm_backward_ws_bytes(ROW_TYPES[x.dtype], rows, cols))
+            nbytes = int(_lib.lib().ttk_layer_norm_backward_ws_bytes(ROW_TYPES[x.dtype], rows, cols))
             ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
         ptr = [t.data_ptr() if t is not None else None for t in (dx, dw, db, ws)]
-        with _on(x):
-            rc = L.ttk_layer_norm_backward(ROW_TYPES[x.dtype], ROW_TYPES[wdt], dy.data_ptr(), lddy, x.data_ptr(), ld, wp,
-                                           mean.data_ptr(), rstd.data_ptr(), ptr[0], ptr[1], ptr[2], rows, cols, p, seed, off,
-                                           off_dev, ptr[3], nbytes, _stream(x))
-        _lib.check(rc, "ttk_layer_norm_backward")
+        _launch("ttk_layer_norm_backward", x.device, ROW_TYPES[x.dtype], ROW_TYPES[wdt], dy.data_ptr(), lddy, x.data_ptr(), ld, wp,
+                mean.data_ptr(), rstd.data_ptr(), ptr[0], ptr[1], ptr[2], rows, cols, p, seed, off, off_dev, ptr[3], nbytes)
     return dx, dw, db
 
 
@@ -1217,10 +1223,7 @@ def dropout(x, p, seed, offset=0):
     p, seed, off, off_dev = _drop_args(p, seed, offset, x.device)
     y = torch.empty_like(x)
     if x.numel():
-        with _on(x):
-            rc = _lib.lib().ttk_dropout(ROW_TYPES[x.dtype], x.data_ptr(), y.data_ptr(), x.numel(), p, seed, off, off_dev,
-                                        _stream(x))
-        _lib.check(rc, "ttk_dropout")
+        _launch("ttk_dropout", x.device, ROW_TYPES[x.dtype], x.data_ptr(), y.data_ptr(), x.numel(), p, seed, off, off_dev)
     return y
 
 
@@ -1254,9 +1257,6 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     mp, mv = param(min_p, "min_p", u.dtype, lambda v: 0.0 <= v <= 1.0)
     label = torch.empty(shape, dtype=torch.int64, device=logits.device)
     if rows:
-        with _on(logits):
-            rc = _lib.lib().ttk_sample(ROW_TYPES[logits.dtype], logits.data_ptr(), ld, u.data_ptr(), int(u.dtype == F64), tp,
-                                       float(t), kp, min(int(k), 0x7FFFFFFF), pp, float(pv), mp, float(mv), label.data_ptr(),
-                                       rows, V, _stream(logits))
-        _lib.check(rc, "ttk_sample")
+        _launch("ttk_sample", logits.device, ROW_TYPES[logits.dtype], logits.data_ptr(), ld, u.data_ptr(), int(u.dtype == F64), tp,
+                float(t), kp, min(int(k), 0x7FFFFFFF), pp, float(pv), mp, float(mv), label.data_ptr(), rows, V)
     return label

@@ -31,6 +31,11 @@ def _rows(t):
     return t
 
 
+def _recorded(*ts):
+    """Whether autograd has to remember the call."""
+    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in ts)
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, p, seed, offset):
@@ -69,12 +74,18 @@ class _Dropout(torch.autograd.Function):
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, p=0.0, seed=0, offset=0):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis, followed by dropout with probability p."""
-    return _LayerNorm.apply(_rows(x), weight, bias, eps, p, seed, offset)
+    x = _rows(x)
+    if not _recorded(x, weight, bias):
+        return ops.layer_norm(x, weight, bias, eps, p, seed, offset, stats=False)[0]
+    return _LayerNorm.apply(x, weight, bias, eps, p, seed, offset)
 
 
 def dropout(x, p, seed, offset=0):
     """Each element kept with probability 1 - p and divided by it; the mask is a function of (seed, offset + element)."""
-    return _Dropout.apply(x.contiguous() if isinstance(x, torch.Tensor) else x, p, seed, offset)
+    x = x.contiguous() if isinstance(x, torch.Tensor) else x
+    if not _recorded(x):
+        return ops.dropout(x, p, seed, offset)
+    return _Dropout.apply(x, p, seed, offset)
 
 
 class LayerNorm(nn.Module):
