@@ -46,10 +46,12 @@ __device__ __forceinline__ RowArgs row_args(const SampleArgs& a, int64_t row, in
 }
 
 // Unsigned integers in the order of the logits they stand for; -0 and +0 are one key, NaN is -inf.
+// LOW: that many low bits of a 16-bit logit's key are all 0 or all 1 (bits a float32 has and the logit has not).
 template <typename Z>
 struct Key {
   typedef uint32_t type;
   typedef float val_t;
+  static constexpr int LOW = sizeof(Z) == 4 ? 0 : __is_same(Z, __bf16) ? 16 : 13;
   static __device__ __forceinline__ float value(Z z) {
     const float f = (float)z;
     return f != f ? -__builtin_inff() : f + 0.0f;
@@ -63,6 +65,7 @@ template <>
 struct Key<double> {
   typedef uint64_t type;
   typedef double val_t;
+  static constexpr int LOW = 0;
   static __device__ __forceinline__ double value(double z) { return z != z ? -__builtin_inf() : z + 0.0; }
   static __device__ __forceinline__ uint64_t of(double f) {
     const uint64_t b = (uint64_t)__double_as_longlong(f);
@@ -70,181 +73,867 @@ struct Key<double> {
   }
 };
 
-template <typename T>
-__device__ __forceinline__ double weight(T z, T m, double temperature) {
-  return z == m ? 1.0 : exp(((double)z - (double)m) / temperature);
+// Weights relative to the row's largest logit: 2^((z - m) log2(e) / T) as 2^n times the Taylor polynomial of 2^f, |f| <= 1/2
+// (terms up to (f ln 2)^12 / 12!: relative error below 2e-16).  z == m gives exactly 1, -inf exactly 0.
+template <typename F>
+struct Weight {
+  F m;
+  double c;        // log2(e) / T
+  __device__ __forceinline__ Weight(F m_, double T) : m(m_), c(1.4426950408889634074 / T) {}
+  __device__ __forceinline__ double operator()(F z) const {
+    double t = ((double)z - (double)m) * c;
+    t = z == m ? 0.0 : t > -1100.0 ? t : -1100.0;
+    const double n = rint(t), f = t - n;
+    double p = 2.56784359934881958e-11;
+    p = fma(p, f, 4.44553827187081007e-10);
+    p = fma(p, f, 7.05491162080112088e-09);
+    p = fma(p, f, 1.01780860092396960e-07);
+    p = fma(p, f, 1.32154867901443053e-06);
+    p = fma(p, f, 1.52527338040598377e-05);
+    p = fma(p, f, 1.54035303933816061e-04);
+    p = fma(p, f, 1.33335581464284411e-03);
+    p = fma(p, f, 9.61812910762847688e-03);
+    p = fma(p, f, 5.55041086648215762e-02);
+    p = fma(p, f, 2.40226506959100694e-01);
+    p = fma(p, f, 6.93147180559945286e-01);
+    p = fma(p, f, 1.0);
+    return ldexp(p, (int)n);
+  }
+};
+
+// The row with an infinite maximum is the row of its +inf elements alone, all alike.
+template <typename F>
+__device__ __forceinline__ F finite(F z, bool top_inf) {
+  return top_inf ? (z == __builtin_inff() ? F(0) : F(-__builtin_inff())) : z;
 }
 
-constexpr int ROW_THREADS = 256;
-
 template <typename T>
-__device__ __forceinline__ T block_sum(T v, T* buf) {
+__device__ __forceinline__ T wave_sum(T v) {
 #pragma unroll
-  for (int s = 32; s > 0; s >>= 1) v += __shfl_xor(v, s);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = buf[0];
+  for (int s = 1; s < 64; s <<= 1) v += __shfl_xor(v, s);
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ T wave_max(T v) {
 #pragma unroll
-  for (int i = 1; i < ROW_THREADS / 64; ++i) v += buf[i];
+  for (int s = 1; s < 64; s <<= 1) {
+    const T o = __shfl_xor(v, s);
+    v = o > v ? o : v;
+  }
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {      // inclusive
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const T o = __shfl_up(v, s);
+    if (lane >= s) v += o;
+  }
   return v;
 }
 
-// index of the n-th (from 1) element of the row with key t
-template <typename Z>
-__device__ int nth_tie(const Z* z, int c0, int c1, typename Key<Z>::type t, int n, int* counts, int* found) {
-  int mine = 0;
-  for (int c = c0; c < c1; ++c) mine += Key<Z>::of(Key<Z>::value(z[c])) == t;
-  __syncthreads();
-  counts[threadIdx.x] = mine;
-  __syncthreads();
-  int before = 0;
-  for (int i = 0; i < (int)threadIdx.x; ++i) before += counts[i];
-  if (before < n && before + mine >= n)
-    for (int c = c0; c < c1; ++c)
-      if (Key<Z>::of(Key<Z>::value(z[c])) == t && ++before == n) *found = c;
-  __syncthreads();
-  return *found;
-}
+// ---------------------------------------------------------------------------------------
+// Few classes: a thread a row, everything in registers; an element's place in the order is counted against all others.
+// ---------------------------------------------------------------------------------------
+constexpr int FEW = 16;
 
-// One workgroup a row.  Thresholds are found bit by bit: the largest key t with enough elements (or weight) at or above it.
 template <typename Z>
-__global__ __launch_bounds__(ROW_THREADS) void sample_row_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args,
-                                                                 int64_t* __restrict__ label, int64_t rows, int V) {
-  typedef typename Key<Z>::type K;
+__global__ __launch_bounds__(64) void sample_few_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args,
+                                                        int64_t* __restrict__ label, int64_t rows, int V) {
   typedef typename Key<Z>::val_t F;
-  __shared__ double dbuf[ROW_THREADS];
-  __shared__ int ibuf[ROW_THREADS];
-  __shared__ F fbuf[ROW_THREADS / 64];
-  __shared__ int found;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int chunk = (V + ROW_THREADS - 1) / ROW_THREADS;
-  const int c0 = min(V, tid * chunk), c1 = min(V, c0 + chunk);
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const Z* z = logits + row * ld;
-    const RowArgs a = row_args(args, row, V);
-    F m = -__builtin_inff();
-    int at = V;
-    for (int c = c0; c < c1; ++c) {
-      const F f = Key<Z>::value(z[c]);
-      if (f > m) m = f, at = c;
-    }
-    const F mine = m;
+  const int64_t row = (int64_t)blockIdx.x * 64 + threadIdx.x;
+  if (row >= rows) return;
+  const Z* p = logits + row * ld;
+  F z[FEW], m = -__builtin_inff();
+  int first = -1;
 #pragma unroll
-    for (int s = 32; s > 0; s >>= 1) m = max(m, (F)__shfl_xor(m, s));
-    __syncthreads();
-    if (lane == 0) fbuf[tid >> 6] = m;
-    ibuf[tid] = mine == m ? at : V;
-    __syncthreads();
-    for (int i = 0; i < ROW_THREADS / 64; ++i) m = max(m, fbuf[i]);
-    if (!(m > -__builtin_inff()) || !(a.T > 0.0)) {
-      if (tid == 0) {
-        int first = V;
-        for (int i = 0; i < ROW_THREADS; ++i)
-          if (fbuf[i >> 6] == m) first = min(first, ibuf[i]);
-        label[row] = m > -__builtin_inff() ? first : -1;
-      }
-      __syncthreads();
-      continue;
-    }
-    K cut = 0;        // kept: key > cut, or key == cut and index <= icut
-    int icut = V;
-    if (a.k) {
-      for (int bit = 8 * (int)sizeof(K) - 1; bit >= 0; --bit) {
-        const K cand = cut | ((K)1 << bit);
-        int n = 0;
-        for (int c = c0; c < c1; ++c) n += Key<Z>::of(Key<Z>::value(z[c])) >= cand;
-        if (block_sum(n, ibuf) >= a.k) cut = cand;
-      }
-      int above = 0;
-      for (int c = c0; c < c1; ++c) above += Key<Z>::of(Key<Z>::value(z[c])) > cut;
-      above = block_sum(above, ibuf);
-      icut = nth_tie<Z>(z, c0, c1, cut, a.k - above, ibuf, &found);
+  for (int i = 0; i < FEW; ++i) z[i] = i < V ? Key<Z>::value(p[i]) : F(-__builtin_inff());
+#pragma unroll
+  for (int i = 0; i < FEW; ++i)
+    if (z[i] > m) m = z[i], first = i;
+  const RowArgs a = row_args(args, row, V);
+  if (first < 0 || !(a.T > 0.0)) {
+    label[row] = first;
+    return;
+  }
+  const bool inf = m == __builtin_inff();
+  if (inf) m = 0;
+  const Weight<F> weight(m, a.T);
+  double w[FEW];
+#pragma unroll
+  for (int i = 0; i < FEW; ++i) {
+    z[i] = finite(z[i], inf);
+    w[i] = i < V ? weight(z[i]) : 0.0;
+  }
+  if (a.k || a.P < 1.0) {
+    uint32_t kept = 0;
+    double total = 0;
+#pragma unroll
+    for (int i = 0; i < FEW; ++i) {
+      int rank = 0;
+#pragma unroll
+      for (int j = 0; j < FEW; ++j)
+        if (j != i) rank += j < i ? z[j] >= z[i] : z[j] > z[i];
+      if (!a.k || rank < a.k) kept |= 1u << i, total += w[i];
     }
     if (a.P < 1.0) {
-      K cut2 = 0;
-      double target = 0;
-      for (int bit = 8 * (int)sizeof(K); bit >= 0; --bit) {
-        const K cand = bit == 8 * (int)sizeof(K) ? (K)0 : cut2 | ((K)1 << bit);   // the first turn sums everything kept
-        double s = 0;
-        for (int c = c0; c < c1; ++c) {
-          const F f = Key<Z>::value(z[c]);
-          const K key = Key<Z>::of(f);
-          if (key >= cand && (key > cut || (key == cut && c <= icut))) s += weight(f, m, a.T);
-        }
-        s = block_sum(s, dbuf);
-        if (bit == 8 * (int)sizeof(K))
-          target = a.P * s;
-        else if (s >= target)
-          cut2 = cand;
-      }
-      double s = 0, wt = 0;
-      int ties = 0;
-      for (int c = c0; c < c1; ++c) {
-        const F f = Key<Z>::value(z[c]);
-        const K key = Key<Z>::of(f);
-        if (key > cut2) s += weight(f, m, a.T);
-        if (key == cut2 && (key > cut || c <= icut)) ++ties, wt = weight(f, m, a.T);
-      }
-      s = block_sum(s, dbuf);
-      ties = block_sum(ties, ibuf);
+      const double target = a.P * total;
+      uint32_t nucleus = 0;
 #pragma unroll
-      for (int i = 32; i > 0; i >>= 1) wt = max(wt, __shfl_xor(wt, i));
-      __syncthreads();
-      if (lane == 0) dbuf[tid >> 6] = wt;
-      __syncthreads();
-      for (int i = 0; i < ROW_THREADS / 64; ++i) wt = max(wt, dbuf[i]);
-      const double need = wt > 0 ? ceil((target - s) / wt) : 1.0;
-      const int n = need < 1.0 ? 1 : need > (double)ties ? ties : (int)need;
-      const int i2 = nth_tie<Z>(z, c0, c1, cut2, n, ibuf, &found);
-      cut = cut2;
-      icut = i2;
+      for (int i = 0; i < FEW; ++i) {
+        double before = 0;
+#pragma unroll
+        for (int j = 0; j < FEW; ++j)
+          if (j != i && (j < i ? z[j] >= z[i] : z[j] > z[i])) before += w[j];
+        if (before < target) nucleus |= 1u << i;
+      }
+      kept &= nucleus;
     }
-    double s = 0;
-    for (int c = c0; c < c1; ++c) {
-      const F f = Key<Z>::value(z[c]);
-      const K key = Key<Z>::of(f);
-      if (key > cut || (key == cut && c <= icut)) {
-        const double w = weight(f, m, a.T);
-        if (w >= a.M) s += w;
+#pragma unroll
+    for (int i = 0; i < FEW; ++i)
+      if (!(kept >> i & 1)) w[i] = 0;
+  }
+  double total = 0;
+#pragma unroll
+  for (int i = 0; i < FEW; ++i) {
+    if (!(w[i] >= a.M)) w[i] = 0;
+    total += w[i];
+  }
+  const double target = a.u * total;
+  double c = 0;
+  int pick = -1;
+  bool done = false;
+#pragma unroll
+  for (int i = 0; i < FEW; ++i) {
+    c += w[i];
+    if (!done && w[i] > 0) pick = i, done = c > target;
+  }
+  label[row] = pick;
+}
+
+// ---------------------------------------------------------------------------------------
+// Up to 64 E classes: a wave a row, E consecutive elements a lane.  Cuts are found bit by bit: the largest key t with
+// enough elements (or weight) at or above it.
+// ---------------------------------------------------------------------------------------
+template <typename Z, int E>
+__global__ __launch_bounds__(256) void sample_wave_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args,
+                                                          int64_t* __restrict__ label, int64_t rows, int V) {
+  typedef typename Key<Z>::type K;
+  typedef typename Key<Z>::val_t F;
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const Z* p = logits + row * ld;
+  const int e = (V + 63) / 64, c0 = lane * e;      // this lane's elements: c0 .. c0 + e - 1
+  F z[E], m = -__builtin_inff();
+  int first = 0x7FFFFFFF;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    z[i] = i < e && c0 + i < V ? Key<Z>::value(p[c0 + i]) : F(-__builtin_inff());
+    if (z[i] > m) m = z[i], first = c0 + i;
+  }
+  const F mine = m;
+  m = wave_max(m);
+  const RowArgs a = row_args(args, row, V);
+  if (!(m > -__builtin_inff()) || !(a.T > 0.0)) {
+    const uint64_t who = __ballot(mine == m);
+    const int f = __shfl(first, (int)__builtin_ctzll(who));
+    if (lane == 0) label[row] = m > -__builtin_inff() ? f : -1;
+    return;
+  }
+  const bool inf = m == __builtin_inff();
+  if (inf) m = 0;
+  const Weight<F> weight(m, a.T);
+  K key[E];
+  double w[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    z[i] = finite(z[i], inf);
+    key[i] = Key<Z>::of(z[i]);
+    w[i] = weight(z[i]);
+  }
+  constexpr int BITS = 8 * (int)sizeof(K), LOW = Key<Z>::LOW;
+  // keeps, of the elements with w > 0, those in front of the cut: key above t, or the first `ties` of those with key t
+  auto cut_at = [&](K t, int ties) {
+    int before = 0;
+    const K low = LOW ? (K)((1ull << LOW) - 1) : (K)0;
+    t |= low;
+#pragma unroll
+    for (int i = 0; i < E; ++i) before += w[i] > 0 && (K)(key[i] | low) == t;
+    before = wave_scan(before) - before;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const K k = key[i] | low;
+      if (k < t || (k == t && w[i] > 0 && before++ >= ties)) w[i] = 0;
+    }
+  };
+  if (a.k) {
+    K t = 0;
+    int above = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) all += __popcll(__ballot(z[i] > -__builtin_inff()));
+    if (all > a.k) {
+      for (int bit = BITS - 1; bit >= LOW; --bit) {
+        const K cand = t | ((K)1 << bit);
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) n += __popcll(__ballot(key[i] >= cand));
+        if (n >= a.k)
+          t = cand;
+        else
+          above = n;      // the last candidate with too few is the next key above the final t: what lies above t
+      }
+      // (elements of weight 0 lie below every other: they only matter as ties, where they are never drawn)
+      cut_at(t, a.k - above);
+    }
+  }
+  if (a.P < 1.0) {
+    double total = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) total += w[i];
+    total = wave_sum(total);
+    const double target = a.P * total;
+    K t = 0;
+    double above = 0;
+    for (int bit = BITS - 1; bit >= LOW; --bit) {
+      const K cand = t | ((K)1 << bit);
+      double s = 0;
+#pragma unroll
+      for (int i = 0; i < E; ++i) s += key[i] >= cand ? w[i] : 0.0;
+      s = wave_sum(s);
+      if (s >= target)
+        t = cand;
+      else
+        above = s;
+    }
+    double wt = 0;
+    const K low = LOW ? (K)((1ull << LOW) - 1) : (K)0;
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if ((K)(key[i] | low) == (K)(t | low) && w[i] > 0) wt = w[i];
+    wt = wave_max(wt);
+    const double need = wt > 0 ? ceil((target - above) / wt) : 1.0;
+    cut_at(t, need < 1.0 ? 1 : need > (double)V ? V : (int)need);
+  }
+  double s = 0;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    if (!(w[i] >= a.M)) w[i] = 0;
+    s += w[i];
+  }
+  const double upto = wave_scan(s), total = __shfl(upto, 63), target = a.u * total;
+  uint64_t who = __ballot(s > 0 && upto > target);
+  const bool last = who == 0;                       // u >= 1, or rounded up to it: the last kept element
+  if (last) who = __ballot(s > 0);
+  const int at = last ? 63 - (int)__builtin_clzll(who) : (int)__builtin_ctzll(who);
+  if (lane == at) {
+    double c = upto - s;
+    int pick = -1;
+    bool done = false;
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (!done && w[i] > 0) c += w[i], pick = c0 + i, done = !last && c > target;
+    label[row] = pick;
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Many classes: a workgroup a row.
+//
+// The row is read from memory once and from the caches a few times more:
+//   - the maximum (and its place, for temperature 0);
+//   - top-k up to 512: the k-th largest of the 1024 threads' own maxima bounds the k-th largest element from below, so the
+//     elements at or above that bound (a few more than k) are collected in LDS, sorted, cut and drawn from there;
+//   - otherwise each cut is found by histograms: weights (counts for top-k) are added into 2048 bins, the bin with the
+//     border is collected and sorted in LDS, or, where it holds too many, refined.  Weights enter as whole numbers
+//     (2^-S of the largest, S = 62 - log2 V, at most 51), so that sums do not depend on the order of the atomics;
+//   - the draw: float64 sums of the kept weights per segment of the row, their scan, and one wave over the segment that
+//     holds u times the total.
+// Elements of -inf do not exist for any of this.
+// ---------------------------------------------------------------------------------------
+constexpr int RT = 1024, RW = RT / 64, BINS = 2048, CAP = 2048, SEGS = 1024, BATCH = 4;
+
+template <typename Z>
+struct Chunk {
+  static constexpr int N = 16 / (int)sizeof(Z);
+  typedef uint32_t raw_t __attribute__((ext_vector_type(4), aligned(2)));
+  union {
+    uint32_t u[4];
+    Z e[N];
+  };
+};
+
+// Calls f(values, first index, segment) for every 16 bytes of the row; values behind the row are -inf.  A wave owns whole
+// segments; BATCH loads are in flight at a time.
+template <typename Z, typename Fn>
+__device__ __forceinline__ void walk(const Z* __restrict__ p, int V, int R, bool inf, Fn f) {
+  typedef typename Key<Z>::val_t F;
+  constexpr int N = Chunk<Z>::N;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int steps = (V + 64 * N - 1) / (64 * N);
+  for (int i0 = 0;; i0 += BATCH) {
+    int s0 = wave + RW * (i0 / R);
+    if ((int64_t)s0 * R >= steps) break;
+    Chunk<Z> c[BATCH];
+    int base[BATCH];
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      const int i = i0 + b, s = wave + RW * (i / R), t = s * R + i % R;
+      base[b] = t < steps ? (t * 64 + lane) * N : V;
+      if (base[b] + N <= V) {
+        const typename Chunk<Z>::raw_t r = *reinterpret_cast<const typename Chunk<Z>::raw_t*>(p + base[b]);
+        c[b].u[0] = r.x, c[b].u[1] = r.y, c[b].u[2] = r.z, c[b].u[3] = r.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) c[b].e[j] = base[b] + j < V ? p[base[b] + j] : (Z)(-__builtin_inff());
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      const int i = i0 + b, s = wave + RW * (i / R);
+      if (s * R + i % R < steps) {
+        F v[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = finite(Key<Z>::value(c[b].e[j]), inf);
+        f(v, base[b], s);
+      }
+    }
+  }
+}
+
+template <typename Z>
+struct RowShared {
+  typedef typename Key<Z>::type K;
+  typedef typename Key<Z>::val_t F;
+  union {
+    unsigned long long hist[BINS + 1];
+    struct {
+      uint64_t key[CAP];                                     // 32-bit keys: key << 32 | ~index
+      uint32_t nidx[sizeof(K) == 8 ? CAP : 1];               // 64-bit keys: ~index
+    } list;
+    double seg[SEGS];
+    int count[SEGS];
+  };
+  double wave_d[RW];
+  unsigned long long wave_u[RW];
+  int wave_n[2][RW];
+  F wave_f[RW];
+  K wave_lo[RW], wave_hi[RW];
+  int n, at, which, last;
+  unsigned long long above;
+  K cut_key;
+  int cut_idx;
+};
+
+template <typename T>
+__device__ __forceinline__ T block_scan(T v, T* buf, T& total) {      // inclusive; buf: RW values
+  const int wave = threadIdx.x >> 6;
+  v = wave_scan(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) buf[wave] = v;
+  __syncthreads();
+  T before = 0;
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < RW; ++i) {
+    if (i < wave) before += buf[i];
+    total += buf[i];
+  }
+  return v + before;
+}
+
+// an element of the list: what comes first sorts higher
+template <typename Z>
+__device__ __forceinline__ void list_put(RowShared<Z>& sh, int i, typename Key<Z>::type key, uint32_t nidx) {
+  if constexpr (sizeof(key) == 4) {
+    sh.list.key[i] = (uint64_t)key << 32 | nidx;
+  } else {
+    sh.list.key[i] = key;
+    sh.list.nidx[i] = nidx;
+  }
+}
+template <typename Z>
+__device__ __forceinline__ void list_get(const RowShared<Z>& sh, int i, typename Key<Z>::type& key, uint32_t& nidx) {
+  if constexpr (sizeof(key) == 4) {
+    key = (uint32_t)(sh.list.key[i] >> 32);
+    nidx = (uint32_t)sh.list.key[i];
+  } else {
+    key = sh.list.key[i];
+    nidx = sh.list.nidx[i];
+  }
+}
+
+// Bitonic sort of the first n2 (a power of two) elements, highest first: by (key, ~index), or by ~index alone.
+template <typename Z>
+__device__ void list_sort(RowShared<Z>& sh, int n2, bool by_index) {
+  typedef typename Key<Z>::type K;
+  for (int size = 2; size <= n2; size <<= 1)
+    for (int d = size >> 1; d > 0; d >>= 1) {
+      __syncthreads();
+      for (int t = threadIdx.x; t < n2 / 2; t += RT) {
+        const int i = 2 * t - (t & (d - 1)), j = i + d;
+        K ki, kj;
+        uint32_t ni, nj;
+        list_get<Z>(sh, i, ki, ni);
+        list_get<Z>(sh, j, kj, nj);
+        const bool less = by_index ? ni < nj : ki < kj || (ki == kj && ni < nj);
+        const bool more = by_index ? ni > nj : ki > kj || (ki == kj && ni > nj);
+        if ((i & size) ? more : less) {
+          list_put<Z>(sh, i, kj, nj);
+          list_put<Z>(sh, j, ki, ni);
+        }
+      }
+    }
+  __syncthreads();
+}
+
+// Collects the elements `in` accepts into the list (the first CAP that come) and returns how many there are; lo / hi: the
+// smallest and the largest of their keys.
+template <typename Z, typename In>
+__device__ int list_collect(RowShared<Z>& sh, const Z* p, int V, int R, bool inf, In in, typename Key<Z>::type& lo,
+                            typename Key<Z>::type& hi) {
+  typedef typename Key<Z>::type K;
+  typedef typename Key<Z>::val_t F;
+  constexpr int N = Chunk<Z>::N;
+  __syncthreads();
+  if (threadIdx.x == 0) sh.n = 0;
+  __syncthreads();
+  K l = ~(K)0, h = 0;
+  walk(p, V, R, inf, [&](const F(&v)[N], int base, int) {
+    uint32_t mask = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (in(v[j], base + j)) mask |= 1u << j;
+    if (mask) {
+      int at = atomicAdd(&sh.n, __popc(mask));
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (mask >> j & 1) {
+          const K k = Key<Z>::of(v[j]);
+          l = k < l ? k : l;
+          h = k > h ? k : h;
+          if (at < CAP) list_put<Z>(sh, at, k, ~(uint32_t)(base + j));
+          ++at;
+        }
+    }
+  });
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const K a = __shfl_xor(l, s), b = __shfl_xor(h, s);
+    l = a < l ? a : l;
+    h = b > h ? b : h;
+  }
+  if ((threadIdx.x & 63) == 0) sh.wave_lo[threadIdx.x >> 6] = l, sh.wave_hi[threadIdx.x >> 6] = h;
+  __syncthreads();
+  lo = sh.wave_lo[0], hi = sh.wave_hi[0];
+  for (int i = 1; i < RW; ++i) {
+    lo = sh.wave_lo[i] < lo ? sh.wave_lo[i] : lo;
+    hi = sh.wave_hi[i] > hi ? sh.wave_hi[i] : hi;
+  }
+  return sh.n;
+}
+
+// pads the list of c elements to a power of two with entries that sort last and returns it
+template <typename Z>
+__device__ int list_pad(RowShared<Z>& sh, int c) {
+  int n2 = 2;
+  while (n2 < c) n2 <<= 1;
+  for (int i = c + threadIdx.x; i < n2; i += RT) list_put<Z>(sh, i, 0, 0);
+  return n2;
+}
+
+// An element is kept when it does not come behind the cut.
+template <typename K>
+struct Cut {
+  K key;
+  int idx;
+  __device__ __forceinline__ bool keeps(K k, int i) const { return k > key || (k == key && i <= idx); }
+};
+
+template <typename Z>
+struct RowSampler {
+  typedef typename Key<Z>::type K;
+  typedef typename Key<Z>::val_t F;
+  static constexpr int N = Chunk<Z>::N;
+  RowShared<Z>& sh;
+  const Z* p;
+  int V, R;
+  bool inf;
+  Weight<F> weight;
+  double fixed;      // 2^S
+
+  __device__ __forceinline__ unsigned long long whole(double w) const {      // w 2^S, rounded; below 2^52
+    return (unsigned long long)__double_as_longlong(w * fixed + 0x1p52) - 0x4330000000000000ull;
+  }
+  static __device__ __forceinline__ F value_of(K k) {
+    if constexpr (sizeof(K) == 4)
+      return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+    else
+      return __longlong_as_double((int64_t)(k ^ ((k >> 63) ? 0x8000000000000000ull : ~0ull)));
+  }
+
+  // place of the n-th (from 1) kept element with key t
+  __device__ int nth_tie(const Cut<K>& cut, K t, int n) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < SEGS; i += RT) sh.count[i] = 0;
+    __syncthreads();
+    walk(p, V, R, inf, [&](const F(&v)[N], int base, int s) {
+      int c = 0;
+#pragma unroll
+      for (int j = 0; j < N; ++j) c += Key<Z>::of(v[j]) == t && cut.keeps(t, base + j);
+      c = wave_sum(c);
+      if ((threadIdx.x & 63) == 0) sh.count[s] += c;      // (a segment has one wave)
+    });
+    __syncthreads();
+    const int mine = sh.count[threadIdx.x];
+    unsigned long long total;
+    const int upto = (int)block_scan((unsigned long long)mine, sh.wave_u, total);
+    if (upto >= n && upto - mine < n) sh.which = threadIdx.x, sh.at = upto - mine;
+    __syncthreads();
+    const int s = sh.which;
+    int before = sh.at;
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      const int lane = threadIdx.x;
+      for (int r = 0; r < R; ++r) {
+        const int base = ((s * R + r) * 64 + lane) * N;
+        int c = 0;
+        for (int j = 0; j < N; ++j)
+          if (base + j < V) c += Key<Z>::of(finite(Key<Z>::value(p[base + j]), inf)) == t && cut.keeps(t, base + j);
+        const int incl = wave_scan(c);
+        if (before + incl >= n && before + incl - c < n) {
+          int k = before + incl - c;
+          for (int j = 0; j < N; ++j)
+            if (base + j < V && Key<Z>::of(finite(Key<Z>::value(p[base + j]), inf)) == t && cut.keeps(t, base + j) && ++k == n) sh.at = base + j;
+        }
+        before += __shfl(incl, 63);
       }
     }
     __syncthreads();
-    dbuf[tid] = s;
-    if (tid == 0) found = -1;
-    __syncthreads();
-    double before = 0, total = 0;
-    for (int i = 0; i < ROW_THREADS; ++i) {
-      if (i == tid) before = total;
-      total += dbuf[i];
-    }
-    const double target = a.u * total;
-    const bool last = !(target < total);  // u >= 1, or rounded up to it: the last kept element
-    if (s > 0 && (last ? before + s >= total : (before <= target && before + s > target))) {
-      int pick = -1;
-      double c = before;
-      for (int i = c0; i < c1; ++i) {
-        const F f = Key<Z>::value(z[i]);
-        const K key = Key<Z>::of(f);
-        if (!(key > cut || (key == cut && i <= icut))) continue;
-        const double w = weight(f, m, a.T);
-        if (!(w >= a.M) || !(w > 0)) continue;
-        pick = i;
-        c += w;
-        if (!last && c > target) break;
+    return sh.at;
+  }
+
+  // The cut of top-k (target elements) or, MASS, of top-p (share `target` of what `cut` keeps) among the elements `cut` keeps.
+  template <bool MASS>
+  __device__ Cut<K> select(Cut<K> cut, double target, double range) {
+    const K none = Key<Z>::of(F(-__builtin_inff()));
+    K a = none + 1, b = Key<Z>::of(weight.m);
+    bool linear = MASS;
+    const F slope = (F)fmin((double)BINS / range, 1e38);      // bins a unit of z, over `range` below the maximum
+    unsigned long long above = 0;
+    for (;;) {
+      __syncthreads();
+      for (int i = threadIdx.x; i <= BINS; i += RT) sh.hist[i] = 0;
+      __syncthreads();
+      int shift = 0;
+      if (!linear)
+        while (((b - a) >> shift) >= (K)BINS) ++shift;
+      unsigned long long beyond = 0;
+      walk(p, V, R, inf, [&](const F(&v)[N], int base, int) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const K k = Key<Z>::of(v[j]);
+          if (k <= none || !cut.keeps(k, base + j)) continue;
+          if (linear) {
+            const int bin = (int)fmin((weight.m - v[j]) * slope, F(BINS));
+            const unsigned long long q = whole(weight(v[j]));
+            if (bin < BINS)
+              atomicAdd(&sh.hist[bin], q);
+            else
+              beyond += q;
+          } else if (k >= a && k <= b) {
+            atomicAdd(&sh.hist[(int)((b - k) >> shift)], MASS ? whole(weight(v[j])) : 1ull);
+          }
+        }
+      });
+      if (linear) {
+        beyond = wave_sum(beyond);
+        if ((threadIdx.x & 63) == 0) atomicAdd(&sh.hist[BINS], beyond);
       }
-      found = pick;
+      __syncthreads();
+      const unsigned long long v0 = sh.hist[2 * threadIdx.x], v1 = sh.hist[2 * threadIdx.x + 1], over = sh.hist[BINS];
+      unsigned long long total;
+      const unsigned long long upto = above + block_scan(v0 + v1, sh.wave_u, total), from = upto - v0 - v1;
+      if (linear) target *= (double)(total + over);
+      if (threadIdx.x == 0 && (double)(above + total) < target) sh.which = linear ? BINS : -1, sh.above = above + total;
+      if ((double)from < target && (double)(from + v0) >= target) sh.which = 2 * threadIdx.x, sh.above = from;
+      if ((double)(from + v0) < target && (double)upto >= target) sh.which = 2 * threadIdx.x + 1, sh.above = from + v0;
+      __syncthreads();
+      const int bin = sh.which;
+      above = sh.above;
+      if (bin < 0) return cut;                        // fewer elements than asked for: all stay
+      const K bb = b - (linear ? (K)0 : (K)bin << shift), width = linear ? (K)0 : ((K)1 << shift) - 1;
+      K lo, hi;
+      const int c = list_collect<Z>(sh, p, V, R, inf, [&](F v, int i) {
+        const K k = Key<Z>::of(v);
+        if (k <= none || !cut.keeps(k, i)) return false;
+        return linear ? (int)fmin((weight.m - v) * slope, F(BINS)) == bin : k >= a && k <= bb && bb - k <= width;
+      }, lo, hi);
+      if (c <= CAP) {
+        const int n2 = list_pad<Z>(sh, c);
+        list_sort<Z>(sh, n2, false);
+        K key[2];
+        uint32_t nidx[2];
+        unsigned long long q[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int i = 2 * threadIdx.x + e;
+          if (i < c) {
+            list_get<Z>(sh, i, key[e], nidx[e]);
+            q[e] = MASS ? whole(weight(value_of(key[e]))) : 1ull;
+          }
+        }
+        unsigned long long sum;
+        unsigned long long before = above + block_scan(q[0] + q[1], sh.wave_u, sum) - q[0] - q[1];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {                 // the last element with less than the target in front of it
+          const int i = 2 * threadIdx.x + e;
+          if (i < c && (double)before < target && (i == c - 1 || (double)(before + q[e]) >= target))
+            sh.cut_key = key[e], sh.cut_idx = (int)~nidx[e];
+          before += q[e];
+        }
+        __syncthreads();
+        cut.key = sh.cut_key;
+        cut.idx = sh.cut_idx;
+        return cut;
+      }
+      if (lo == hi) {                                 // one value: its first elements
+        const double each = MASS ? (double)whole(weight(value_of(lo))) : 1.0;
+        const double need = ceil((target - (double)above) / each);
+        cut.idx = nth_tie(cut, lo, need < 1.0 ? 1 : need > (double)c ? c : (int)need);
+        cut.key = lo;
+        return cut;
+      }
+      a = lo, b = hi;
+      linear = false;
+    }
+  }
+
+  // the place, by index, where the running sum of the kept weights passes u times the total
+  __device__ int draw(const Cut<K>& cut, double u, double least) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < SEGS; i += RT) sh.seg[i] = 0;
+    if (threadIdx.x == 0) sh.which = SEGS, sh.last = -1;
+    __syncthreads();
+    walk(p, V, R, inf, [&](const F(&v)[N], int base, int s) {
+      double t = 0;
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (cut.keeps(Key<Z>::of(v[j]), base + j)) {
+          const double w = weight(v[j]);
+          if (w >= least) t += w;
+        }
+      t = wave_sum(t);
+      if ((threadIdx.x & 63) == 0) sh.seg[s] += t;      // (a segment has one wave)
+    });
+    __syncthreads();
+    const double mine = sh.seg[threadIdx.x];
+    double total;
+    const double upto = block_scan(mine, sh.wave_d, total), target = u * total;
+    if (mine > 0) {
+      if (upto > target) atomicMin(&sh.which, (int)threadIdx.x);
+      atomicMax(&sh.last, (int)threadIdx.x);
     }
     __syncthreads();
-    if (tid == 0) label[row] = found;
+    const bool last = sh.which == SEGS;                 // u >= 1, or rounded up to it: the last kept element
+    const int s = last ? sh.last : sh.which;
+    if ((int)threadIdx.x == s) sh.wave_d[0] = upto - mine;
     __syncthreads();
+    if (threadIdx.x < 64) {
+      const int lane = threadIdx.x;
+      double before = sh.wave_d[0];
+      int pick = -1, end = -1;                          // end: the last kept element so far
+      for (int r = 0; r < R && pick < 0; ++r) {
+        const int base = ((s * R + r) * 64 + lane) * N;
+        double w[N], t = 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          w[j] = 0;
+          if (base + j < V) {
+            const F v = finite(Key<Z>::value(p[base + j]), inf);
+            if (cut.keeps(Key<Z>::of(v), base + j)) {
+              w[j] = weight(v);
+              if (!(w[j] >= least)) w[j] = 0;
+              if (w[j] > 0) end = base + j;
+            }
+          }
+          t += w[j];
+        }
+        const double upto = before + wave_scan(t);
+        const uint64_t who = last ? 0 : __ballot(t > 0 && upto > target);
+        if (who) {
+          const int at = (int)__builtin_ctzll(who);
+          if (lane == at) {
+            double c = upto - t;
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+              if (w[j] > 0 && !(pick >= 0 && c > target)) c += w[j], pick = base + j;
+          }
+          pick = __shfl(pick, at);
+        }
+        before = __shfl(upto, 63);
+      }
+      end = wave_max(end);
+      if (lane == 0) sh.at = pick >= 0 ? pick : end;
+    }
+    __syncthreads();
+    return sh.at;
+  }
+
+  // top-k from the elements with keys from `bound` on, if the list holds them: true, and the label in `pick`
+  __device__ bool from_list(K bound, const RowArgs& a, int& pick) {
+    const K none = Key<Z>::of(F(-__builtin_inff()));
+    K lo, hi;
+    const int c = list_collect<Z>(sh, p, V, R, inf, [&](F v, int) {
+      const K k = Key<Z>::of(v);
+      return k >= bound && k > none;
+    }, lo, hi);
+    if (c > CAP) return false;
+    const int n2 = list_pad<Z>(sh, c);
+    list_sort<Z>(sh, n2, false);
+    const int kk = min(a.k, c);
+    double w[2], total;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = 2 * threadIdx.x + e;
+      K k;
+      uint32_t n;
+      w[e] = 0;
+      if (i < kk) {
+        list_get<Z>(sh, i, k, n);
+        w[e] = weight(value_of(k));
+      }
+    }
+    const double from = block_scan(w[0] + w[1], sh.wave_d, total) - w[0] - w[1], target = a.P * total;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = 2 * threadIdx.x + e;
+      const bool front = a.P >= 1.0 || i == 0 || (e ? from + w[0] : from) < target;
+      if (i < n2 && !(i < kk && front && w[e] >= a.M)) list_put<Z>(sh, i, 0, 0);
+    }
+    list_sort<Z>(sh, n2, true);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = 2 * threadIdx.x + e;
+      K k;
+      uint32_t n = 0;
+      w[e] = 0;
+      if (i < n2) list_get<Z>(sh, i, k, n);
+      if (n) w[e] = weight(value_of(k));
+    }
+    if (threadIdx.x == 0) sh.which = CAP, sh.last = -1;
+    const double upto = block_scan(w[0] + w[1], sh.wave_d, total), t = a.u * total;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (w[e] > 0) {
+        const int i = 2 * threadIdx.x + e;
+        if ((e ? upto : upto - w[1]) > t) atomicMin(&sh.which, i);
+        atomicMax(&sh.last, i);
+      }
+    __syncthreads();
+    K k;
+    uint32_t n;
+    list_get<Z>(sh, sh.which == CAP ? sh.last : sh.which, k, n);
+    pick = (int)~n;
+    return true;
+  }
+};
+
+template <typename Z>
+__global__ __launch_bounds__(RT) void sample_row_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args,
+                                                        int64_t* __restrict__ label, int64_t rows, int V) {
+  typedef typename Key<Z>::type K;
+  typedef typename Key<Z>::val_t F;
+  constexpr int N = Chunk<Z>::N;
+  __shared__ RowShared<Z> sh;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int steps = (V + 64 * N - 1) / (64 * N), R = (steps + SEGS - 1) / SEGS;
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const Z* p = logits + row * ld;
+    const RowArgs a = row_args(args, row, V);
+    F mine = -__builtin_inff();
+    int at = V;                                        // the 16 bytes it was first seen in
+    walk(p, V, R, false, [&](const F(&v)[N], int base, int) {
+      F t = v[0];
+#pragma unroll
+      for (int j = 1; j < N; ++j) t = v[j] > t ? v[j] : t;
+      if (t > mine) mine = t, at = base;
+    });
+    F m = wave_max(mine);
+    __syncthreads();
+    if (lane == 0) sh.wave_f[wave] = m;
+    if (threadIdx.x == 0) sh.at = V;
+    __syncthreads();
+    for (int i = 0; i < RW; ++i) m = sh.wave_f[i] > m ? sh.wave_f[i] : m;
+    if (!(m > -__builtin_inff()) || !(a.T > 0.0)) {
+      if (mine == m && at < V) {
+        int j = 0;
+        while (Key<Z>::value(p[at + j]) != m) ++j;
+        atomicMin(&sh.at, at + j);
+      }
+      __syncthreads();
+      if (threadIdx.x == 0) label[row] = m > -__builtin_inff() ? sh.at : -1;
+      continue;
+    }
+    const bool inf = m == __builtin_inff();
+    mine = finite(mine, inf);
+    if (inf) m = 0;
+    const int S = min(51, 30 + (int)__builtin_clz(V));      // 62 - log2 V, rounded down
+    RowSampler<Z> r = {sh, p, V, R, inf, Weight<F>(m, a.T), ldexp(1.0, S)};
+    int pick = -1;
+    bool done = false;
+    Cut<K> cut = {Key<Z>::of(F(-__builtin_inff())), -1};
+    if (a.k) {
+      if (a.k <= RT / 2) {
+        // the k-th largest of the threads' maxima, its upper 16 (64-bit keys: 24) bits
+        const K key = Key<Z>::of(mine);
+        K bound = 0;
+        constexpr int BITS = 8 * (int)sizeof(K), END = BITS - (BITS == 64 ? 24 : 16);
+        int turn = 0;
+        for (int bit = BITS - 1; bit >= END; --bit, turn ^= 1) {
+          const K cand = bound | ((K)1 << bit);
+          const int c = __popcll(__ballot(key >= cand));
+          if (lane == 0) sh.wave_n[turn][wave] = c;
+          __syncthreads();
+          int n = 0;
+#pragma unroll
+          for (int i = 0; i < RW; ++i) n += sh.wave_n[turn][i];
+          if (n >= a.k) bound = cand;
+        }
+        done = r.from_list(bound, a, pick);
+      }
+      if (!done) cut = r.template select<false>(cut, (double)a.k, 1.0);
+    }
+    if (!done) {
+      // what lies further below the maximum than ln(V / (1 - P)) weighs less than 1 - P of the total: no bins for it
+      if (a.P < 1.0) cut = r.template select<true>(cut, a.P, a.T * log((double)V / (1.0 - a.P)));
+      pick = r.draw(cut, a.u, a.M);
+    }
+    if (threadIdx.x == 0) label[row] = pick;
   }
 }
 
 template <typename Z>
 int launch(const void* logits, int64_t ld, const SampleArgs& a, int64_t* label, int64_t rows, int V, hipStream_t st) {
-  hipLaunchKernelGGL((sample_row_kernel<Z>), dim3((unsigned)min(rows, (int64_t)65536)), dim3(ROW_THREADS), 0, st,
-                     (const Z*)logits, ld, a, label, rows, V);
+  const Z* z = (const Z*)logits;
+  if (V <= FEW) {
+    if ((rows + 63) / 64 > 0x7FFFFFFF) return TTK_EINVAL;
+    hipLaunchKernelGGL((sample_few_kernel<Z>), dim3((unsigned)((rows + 63) / 64)), dim3(64), 0, st, z, ld, a, label, rows, V);
+  } else if (V <= 1024) {
+    const int64_t groups = (rows + 3) / 4;
+    if (groups > 0x7FFFFFFF) return TTK_EINVAL;
+    const dim3 grid((unsigned)groups);
+    if (V <= 128)
+      hipLaunchKernelGGL((sample_wave_kernel<Z, 2>), grid, dim3(256), 0, st, z, ld, a, label, rows, V);
+    else if (V <= 512)
+      hipLaunchKernelGGL((sample_wave_kernel<Z, 8>), grid, dim3(256), 0, st, z, ld, a, label, rows, V);
+    else
+      hipLaunchKernelGGL((sample_wave_kernel<Z, 16>), grid, dim3(256), 0, st, z, ld, a, label, rows, V);
+  } else {
+    hipLaunchKernelGGL((sample_row_kernel<Z>), dim3((unsigned)min(rows, (int64_t)65536)), dim3(RT), 0, st, z, ld, a, label, rows,
+                       V);
+  }
   return hipGetLastError() == hipSuccess ? TTK_OK : TTK_ELAUNCH;
 }
 
@@ -255,7 +944,7 @@ extern "C" {
 int ttk_sample(int dtype, const void* logits, int64_t ld, const void* u, int f64, const void* temperature, double temperature_all,
                const int32_t* top_k, int top_k_all, const void* top_p, double top_p_all, const void* min_p, double min_p_all,
                int64_t* label, int64_t rows, int V, void* stream) {
-  if (!logits || !u || !label || rows < 1 || V < 1 || ld < 0) return TTK_EINVAL;
+  if (!logits || !u || !label || rows < 1 || V < 1 || V > (1 << 30) || ld < 0) return TTK_EINVAL;
   const SampleArgs a = {u, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all, top_k_all, f64};
   hipStream_t st = (hipStream_t)stream;
   switch (dtype) {
