@@ -52,12 +52,9 @@ struct Key {
   typedef uint32_t type;
   typedef float val_t;
   static constexpr int LOW = sizeof(Z) == 4 ? 0 : __is_same(Z, __bf16) ? 16 : 13;
-  static __device__ __forceinline__ float value(Z z) {
-    const float f = (float)z;
-    return f != f ? -__builtin_inff() : f + 0.0f;
-  }
+  static __device__ __forceinline__ float value(Z z) { return fmaxf((float)z, -__builtin_inff()); }
   static __device__ __forceinline__ uint32_t of(float f) {
-    const uint32_t b = __float_as_uint(f);
+    const uint32_t b = __float_as_uint(f + 0.0f);
     return b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u);
   }
 };
@@ -66,9 +63,9 @@ struct Key<double> {
   typedef uint64_t type;
   typedef double val_t;
   static constexpr int LOW = 0;
-  static __device__ __forceinline__ double value(double z) { return z != z ? -__builtin_inf() : z + 0.0; }
+  static __device__ __forceinline__ double value(double z) { return fmax(z, -__builtin_inf()); }
   static __device__ __forceinline__ uint64_t of(double f) {
-    const uint64_t b = (uint64_t)__double_as_longlong(f);
+    const uint64_t b = (uint64_t)__double_as_longlong(f + 0.0);
     return b ^ ((b >> 63) ? ~0ull : 0x8000000000000000ull);
   }
 };
@@ -107,11 +104,41 @@ __device__ __forceinline__ F finite(F z, bool top_inf) {
   return top_inf ? (z == __builtin_inff() ? F(0) : F(-__builtin_inff())) : z;
 }
 
+// One step of a scan over the wave: v + (v of the lane CTRL names, 0 where there is none), in the rows of ROWS.
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T scan_step(T v) {
+  union {
+    T t;
+    int u[sizeof(T) / 4];
+  } a, b;
+  a.t = v;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 4; ++i) b.u[i] = __builtin_amdgcn_update_dpp(0, a.u[i], CTRL, ROWS, 0xf, ROWS == 0xf);
+  return v + b.t;
+}
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {      // inclusive
+  v = scan_step<0x111, 0xf>(v);      // 1, 2, 4, 8 lanes back within 16
+  v = scan_step<0x112, 0xf>(v);
+  v = scan_step<0x114, 0xf>(v);
+  v = scan_step<0x118, 0xf>(v);
+  v = scan_step<0x142, 0xa>(v);      // lane 15 to the next 16 lanes
+  return scan_step<0x143, 0xc>(v);   // lane 31 to the upper 32
+}
+template <typename T>
+__device__ __forceinline__ T from_lane(T v, int lane) {      // lane: the same in every lane
+  union {
+    T t;
+    int u[sizeof(T) / 4];
+  } a;
+  a.t = v;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 4; ++i) a.u[i] = __builtin_amdgcn_readlane(a.u[i], lane);
+  return a.t;
+}
 template <typename T>
 __device__ __forceinline__ T wave_sum(T v) {
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) v += __shfl_xor(v, s);
-  return v;
+  return from_lane(wave_scan(v), 63);
 }
 template <typename T>
 __device__ __forceinline__ T wave_max(T v) {
@@ -119,16 +146,6 @@ __device__ __forceinline__ T wave_max(T v) {
   for (int s = 1; s < 64; s <<= 1) {
     const T o = __shfl_xor(v, s);
     v = o > v ? o : v;
-  }
-  return v;
-}
-template <typename T>
-__device__ __forceinline__ T wave_scan(T v) {      // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const T o = __shfl_up(v, s);
-    if (lane >= s) v += o;
   }
   return v;
 }
@@ -352,7 +369,7 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const Z* __restrict__ 
 //     holds u times the total.
 // Elements of -inf do not exist for any of this.
 // ---------------------------------------------------------------------------------------
-constexpr int RT = 1024, RW = RT / 64, BINS = 2048, CAP = 2048, SEGS = 1024, BATCH = 4;
+constexpr int RT = 1024, RW = RT / 64, BINS = 2048, CAP = 2048, SEGS = 1024;
 
 template <typename Z>
 struct Chunk {
@@ -364,43 +381,74 @@ struct Chunk {
   };
 };
 
-// Calls f(values, first index, segment) for every 16 bytes of the row; values behind the row are -inf.  A wave owns whole
-// segments; BATCH loads are in flight at a time.
-template <typename Z, typename Fn>
-__device__ __forceinline__ void walk(const Z* __restrict__ p, int V, int R, bool inf, Fn f) {
+// A row as the waves of its workgroup see it: steps of 64 x 16 bytes, R steps a segment, wave w owns segments w, w + RW, ...
+template <typename Z>
+struct RowView {
+  const Z* p;
+  int V, steps, R;
+  bool inf;        // the maximum is +inf
+};
+
+// The 16 bytes of this lane in step t.  Behind the row's end the last 16 bytes are read again (a row has more than that).
+template <typename Z>
+__device__ __forceinline__ int chunk_base(const RowView<Z>& row, int t) {
+  return min((t * 64 + (int)(threadIdx.x & 63)) * Chunk<Z>::N, row.V - Chunk<Z>::N);
+}
+template <typename Z>
+__device__ __forceinline__ void load_chunk(Chunk<Z>& c, const RowView<Z>& row, int t) {
+  const typename Chunk<Z>::raw_t r = *reinterpret_cast<const typename Chunk<Z>::raw_t*>(row.p + chunk_base(row, t));
+  c.u[0] = r.x, c.u[1] = r.y, c.u[2] = r.z, c.u[3] = r.w;
+}
+// Its values; those another lane has already are -inf.  NaN stays: every comparison below is false for it, which is what
+// -inf would get.
+template <typename Z>
+__device__ __forceinline__ void chunk_values(typename Key<Z>::val_t (&v)[Chunk<Z>::N], const Chunk<Z>& c, const RowView<Z>& row,
+                                             int t) {
   typedef typename Key<Z>::val_t F;
   constexpr int N = Chunk<Z>::N;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int steps = (V + 64 * N - 1) / (64 * N);
-  for (int i0 = 0;; i0 += BATCH) {
-    int s0 = wave + RW * (i0 / R);
-    if ((int64_t)s0 * R >= steps) break;
-    Chunk<Z> c[BATCH];
-    int base[BATCH];
 #pragma unroll
-    for (int b = 0; b < BATCH; ++b) {
-      const int i = i0 + b, s = wave + RW * (i / R), t = s * R + i % R;
-      base[b] = t < steps ? (t * 64 + lane) * N : V;
-      if (base[b] + N <= V) {
-        const typename Chunk<Z>::raw_t r = *reinterpret_cast<const typename Chunk<Z>::raw_t*>(p + base[b]);
-        c[b].u[0] = r.x, c[b].u[1] = r.y, c[b].u[2] = r.z, c[b].u[3] = r.w;
-      } else {
+  for (int j = 0; j < N; ++j) v[j] = (F)c.e[j];
+  if (t == row.steps - 1) {
+    const int again = (t * 64 + (int)(threadIdx.x & 63)) * N - chunk_base(row, t);
 #pragma unroll
-        for (int j = 0; j < N; ++j) c[b].e[j] = base[b] + j < V ? p[base[b] + j] : (Z)(-__builtin_inff());
-      }
-    }
+    for (int j = 0; j < N; ++j)
+      if (j < again) v[j] = -__builtin_inff();
+  }
+  if (row.inf)
 #pragma unroll
-    for (int b = 0; b < BATCH; ++b) {
-      const int i = i0 + b, s = wave + RW * (i / R);
-      if (s * R + i % R < steps) {
-        F v[N];
-#pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = finite(Key<Z>::value(c[b].e[j]), inf);
-        f(v, base[b], s);
-      }
-    }
+    for (int j = 0; j < N; ++j) v[j] = finite(v[j], true);
+}
+
+// Calls f(values, first index) for every 16 bytes of the row and end(segment) after a wave's last step of a segment.  The
+// next three steps are under way while one is worked on.
+template <typename Z, typename Fn, typename End>
+__device__ __forceinline__ void walk(const RowView<Z>& row, Fn f, End end) {
+  constexpr int N = Chunk<Z>::N;
+  int s = threadIdx.x >> 6, r = 0, ls = s, lr = 0;      // the step at work, the step to load next
+  Chunk<Z> q[4];
+  auto load = [&](Chunk<Z>& c) {
+    load_chunk<Z>(c, row, ls * row.R + lr);
+    if (++lr == row.R) lr = 0, ls += RW;
+  };
+  load(q[0]);
+  load(q[1]);
+  load(q[2]);
+#pragma unroll 1
+  for (int t = s * row.R; t < row.steps;) {
+    load(q[3]);
+    typename Key<Z>::val_t v[N];
+    chunk_values<Z>(v, q[0], row, t);
+    f(v, chunk_base(row, t));
+    q[0] = q[1], q[1] = q[2], q[2] = q[3];
+    const bool full = ++r == row.R;
+    if (full || t + 1 >= row.steps) end(s);
+    if (full) r = 0, s += RW;
+    t = s * row.R + r;
   }
 }
+struct NoEnd {
+  __device__ __forceinline__ void operator()(int) const {}
+};
 
 template <typename Z>
 struct RowShared {
@@ -415,6 +463,7 @@ struct RowShared {
     double seg[SEGS];
     int count[SEGS];
   };
+  double pow2[32];
   double wave_d[RW];
   unsigned long long wave_u[RW];
   int wave_n[2][RW];
@@ -424,6 +473,30 @@ struct RowShared {
   unsigned long long above;
   K cut_key;
   int cut_idx;
+};
+
+// The weight of Weight, with 2^(n / 32) from a table: 2^((z - m) log2(e) / T) = 2^(n div 32) pow2[n mod 32] 2^(f / 32),
+// |f| <= 1/2, the last factor by its Taylor polynomial (relative error below 3e-15).  The 32 doubles lie in 64 different
+// LDS banks.  m is finite.
+template <typename F>
+struct RowWeight {
+  double m, c;
+  const double* pow2;
+  __device__ __forceinline__ RowWeight(F m_, double T, const double* table)
+      : m((double)m_), c(fmin(32 * 1.4426950408889634074 / T, 1e300)), pow2(table) {}
+  __device__ __forceinline__ double operator()(F z) const {
+    double t = ((double)z - m) * c;
+    t = t > -35200.0 ? t : -35200.0;
+    const double s = t + 0x1.8p52, f = t - (s - 0x1.8p52);
+    const int n = (int)(uint32_t)__double_as_longlong(s);
+    double p = 3.97370998454941544e-11;
+    p = fma(p, f, 9.17256270182464302e-09);
+    p = fma(p, f, 1.69385097243718189e-06);
+    p = fma(p, f, 2.34596198202246772e-04);
+    p = fma(p, f, 2.16608493924982902e-02);
+    p = fma(p, f, 1.0);
+    return ldexp(p * pow2[n & 31], n >> 5);
+  }
 };
 
 template <typename T>
@@ -464,14 +537,22 @@ __device__ __forceinline__ void list_get(const RowShared<Z>& sh, int i, typename
   }
 }
 
-// Bitonic sort of the first n2 (a power of two) elements, highest first: by (key, ~index), or by ~index alone.
+// Bitonic sort of the first n2 (a power of two) elements, highest first: by (key, ~index), or by ~index alone.  A wave
+// exchanges within its own 128 elements while the distance is at most 64: only longer ones need the workgroup's barrier.
 template <typename Z>
-__device__ void list_sort(RowShared<Z>& sh, int n2, bool by_index) {
+__device__ __forceinline__ void list_sort(RowShared<Z>& sh, int n2, bool by_index) {
   typedef typename Key<Z>::type K;
+  __syncthreads();
   for (int size = 2; size <= n2; size <<= 1)
     for (int d = size >> 1; d > 0; d >>= 1) {
-      __syncthreads();
-      for (int t = threadIdx.x; t < n2 / 2; t += RT) {
+      if (d > 64)
+        __syncthreads();
+      else {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      }
+      const int t = threadIdx.x;
+      if (t < n2 / 2) {
         const int i = 2 * t - (t & (d - 1)), j = i + d;
         K ki, kj;
         uint32_t ni, nj;
@@ -484,6 +565,7 @@ __device__ void list_sort(RowShared<Z>& sh, int n2, bool by_index) {
           list_put<Z>(sh, j, ki, ni);
         }
       }
+      if (d > 64) __syncthreads();
     }
   __syncthreads();
 }
@@ -491,8 +573,7 @@ __device__ void list_sort(RowShared<Z>& sh, int n2, bool by_index) {
 // Collects the elements `in` accepts into the list (the first CAP that come) and returns how many there are; lo / hi: the
 // smallest and the largest of their keys.
 template <typename Z, typename In>
-__device__ int list_collect(RowShared<Z>& sh, const Z* p, int V, int R, bool inf, In in, typename Key<Z>::type& lo,
-                            typename Key<Z>::type& hi) {
+__device__ int list_collect(RowShared<Z>& sh, const RowView<Z>& row, In in, typename Key<Z>::type& lo, typename Key<Z>::type& hi) {
   typedef typename Key<Z>::type K;
   typedef typename Key<Z>::val_t F;
   constexpr int N = Chunk<Z>::N;
@@ -500,7 +581,7 @@ __device__ int list_collect(RowShared<Z>& sh, const Z* p, int V, int R, bool inf
   if (threadIdx.x == 0) sh.n = 0;
   __syncthreads();
   K l = ~(K)0, h = 0;
-  walk(p, V, R, inf, [&](const F(&v)[N], int base, int) {
+  walk<Z>(row, [&](const F(&v)[N], int base) {
     uint32_t mask = 0;
 #pragma unroll
     for (int j = 0; j < N; ++j)
@@ -517,7 +598,7 @@ __device__ int list_collect(RowShared<Z>& sh, const Z* p, int V, int R, bool inf
           ++at;
         }
     }
-  });
+  }, NoEnd());
 #pragma unroll
   for (int s = 1; s < 64; s <<= 1) {
     const K a = __shfl_xor(l, s), b = __shfl_xor(h, s);
@@ -543,12 +624,12 @@ __device__ int list_pad(RowShared<Z>& sh, int c) {
   return n2;
 }
 
-// An element is kept when it does not come behind the cut.
-template <typename K>
+// What is kept: the elements that do not come behind (v, idx) in the order.
+template <typename F>
 struct Cut {
-  K key;
+  F v;
   int idx;
-  __device__ __forceinline__ bool keeps(K k, int i) const { return k > key || (k == key && i <= idx); }
+  __device__ __forceinline__ bool keeps(F z, int i) const { return z > v || (z == v && i <= idx); }
 };
 
 template <typename Z>
@@ -557,10 +638,9 @@ struct RowSampler {
   typedef typename Key<Z>::val_t F;
   static constexpr int N = Chunk<Z>::N;
   RowShared<Z>& sh;
-  const Z* p;
-  int V, R;
-  bool inf;
-  Weight<F> weight;
+  RowView<Z> row;
+  F m;
+  RowWeight<F> weight;
   double fixed;      // 2^S
 
   __device__ __forceinline__ unsigned long long whole(double w) const {      // w 2^S, rounded; below 2^52
@@ -573,17 +653,19 @@ struct RowSampler {
       return __longlong_as_double((int64_t)(k ^ ((k >> 63) ? 0x8000000000000000ull : ~0ull)));
   }
 
-  // place of the n-th (from 1) kept element with key t
-  __device__ int nth_tie(const Cut<K>& cut, K t, int n) {
+  // place of the n-th (from 1) kept element that equals t
+  __device__ __forceinline__ int nth_tie(const Cut<F>& cut, F t, int n) {
     __syncthreads();
     for (int i = threadIdx.x; i < SEGS; i += RT) sh.count[i] = 0;
     __syncthreads();
-    walk(p, V, R, inf, [&](const F(&v)[N], int base, int s) {
-      int c = 0;
+    int c = 0;
+    walk<Z>(row, [&](const F(&v)[N], int base) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) c += Key<Z>::of(v[j]) == t && cut.keeps(t, base + j);
+      for (int j = 0; j < N; ++j) c += v[j] == t && cut.keeps(t, base + j);
+    }, [&](int s) {
       c = wave_sum(c);
-      if ((threadIdx.x & 63) == 0) sh.count[s] += c;      // (a segment has one wave)
+      if ((threadIdx.x & 63) == 0) sh.count[s] = c;
+      c = 0;
     });
     __syncthreads();
     const int mine = sh.count[threadIdx.x];
@@ -594,31 +676,33 @@ struct RowSampler {
     const int s = sh.which;
     int before = sh.at;
     __syncthreads();
-    if (threadIdx.x < 64) {
-      const int lane = threadIdx.x;
-      for (int r = 0; r < R; ++r) {
-        const int base = ((s * R + r) * 64 + lane) * N;
-        int c = 0;
-        for (int j = 0; j < N; ++j)
-          if (base + j < V) c += Key<Z>::of(finite(Key<Z>::value(p[base + j]), inf)) == t && cut.keeps(t, base + j);
-        const int incl = wave_scan(c);
-        if (before + incl >= n && before + incl - c < n) {
-          int k = before + incl - c;
+    if (threadIdx.x < 64)
+      for (int r = 0; r < row.R && s * row.R + r < row.steps; ++r) {
+        Chunk<Z> q;
+        F v[N];
+        load_chunk<Z>(q, row, s * row.R + r);
+        chunk_values<Z>(v, q, row, s * row.R + r);
+        const int base = chunk_base(row, s * row.R + r);
+        int mine = 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) mine += v[j] == t && cut.keeps(t, base + j);
+        const int upto = wave_scan(mine);
+        int k = before + upto - mine;
+        if (k < n && k + mine >= n)
+#pragma unroll
           for (int j = 0; j < N; ++j)
-            if (base + j < V && Key<Z>::of(finite(Key<Z>::value(p[base + j]), inf)) == t && cut.keeps(t, base + j) && ++k == n) sh.at = base + j;
-        }
-        before += __shfl(incl, 63);
+            if (v[j] == t && cut.keeps(t, base + j) && ++k == n) sh.at = base + j;
+        before += from_lane(upto, 63);
       }
-    }
     __syncthreads();
     return sh.at;
   }
 
   // The cut of top-k (target elements) or, MASS, of top-p (share `target` of what `cut` keeps) among the elements `cut` keeps.
   template <bool MASS>
-  __device__ Cut<K> select(Cut<K> cut, double target, double range) {
-    const K none = Key<Z>::of(F(-__builtin_inff()));
-    K a = none + 1, b = Key<Z>::of(weight.m);
+  __device__ __forceinline__ Cut<F> select(Cut<F> cut, double target, double range) {
+    const F none = -__builtin_inff();
+    K a = Key<Z>::of(none) + 1, b = Key<Z>::of(m);
     bool linear = MASS;
     const F slope = (F)fmin((double)BINS / range, 1e38);      // bins a unit of z, over `range` below the maximum
     unsigned long long above = 0;
@@ -630,26 +714,30 @@ struct RowSampler {
       if (!linear)
         while (((b - a) >> shift) >= (K)BINS) ++shift;
       unsigned long long beyond = 0;
-      walk(p, V, R, inf, [&](const F(&v)[N], int base, int) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const K k = Key<Z>::of(v[j]);
-          if (k <= none || !cut.keeps(k, base + j)) continue;
-          if (linear) {
-            const int bin = (int)fmin((weight.m - v[j]) * slope, F(BINS));
-            const unsigned long long q = whole(weight(v[j]));
-            if (bin < BINS)
-              atomicAdd(&sh.hist[bin], q);
-            else
-              beyond += q;
-          } else if (k >= a && k <= b) {
-            atomicAdd(&sh.hist[(int)((b - k) >> shift)], MASS ? whole(weight(v[j])) : 1ull);
-          }
-        }
-      });
       if (linear) {
+        walk<Z>(row, [&](const F(&v)[N], int base) {
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+            if (v[j] > none && cut.keeps(v[j], base + j)) {
+              const int bin = (int)fmin((m - v[j]) * slope, F(BINS));
+              const unsigned long long q = whole(weight(v[j]));
+              if (bin < BINS)
+                atomicAdd(&sh.hist[bin], q);
+              else
+                beyond += q;
+            }
+        }, NoEnd());
         beyond = wave_sum(beyond);
         if ((threadIdx.x & 63) == 0) atomicAdd(&sh.hist[BINS], beyond);
+      } else {
+        walk<Z>(row, [&](const F(&v)[N], int base) {
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            const K k = Key<Z>::of(v[j]);
+            if (k >= a && k <= b && cut.keeps(v[j], base + j))
+              atomicAdd(&sh.hist[(int)((b - k) >> shift)], MASS ? whole(weight(v[j])) : 1ull);
+          }
+        }, NoEnd());
       }
       __syncthreads();
       const unsigned long long v0 = sh.hist[2 * threadIdx.x], v1 = sh.hist[2 * threadIdx.x + 1], over = sh.hist[BINS];
@@ -665,10 +753,11 @@ struct RowSampler {
       if (bin < 0) return cut;                        // fewer elements than asked for: all stay
       const K bb = b - (linear ? (K)0 : (K)bin << shift), width = linear ? (K)0 : ((K)1 << shift) - 1;
       K lo, hi;
-      const int c = list_collect<Z>(sh, p, V, R, inf, [&](F v, int i) {
+      const int c = list_collect<Z>(sh, row, [&](F v, int i) {
+        if (!(v > none) || !cut.keeps(v, i)) return false;
+        if (linear) return (int)fmin((m - v) * slope, F(BINS)) == bin;
         const K k = Key<Z>::of(v);
-        if (k <= none || !cut.keeps(k, i)) return false;
-        return linear ? (int)fmin((weight.m - v) * slope, F(BINS)) == bin : k >= a && k <= bb && bb - k <= width;
+        return k >= a && k <= bb && bb - k <= width;
       }, lo, hi);
       if (c <= CAP) {
         const int n2 = list_pad<Z>(sh, c);
@@ -694,16 +783,13 @@ struct RowSampler {
           before += q[e];
         }
         __syncthreads();
-        cut.key = sh.cut_key;
-        cut.idx = sh.cut_idx;
-        return cut;
+        return {value_of(sh.cut_key), sh.cut_idx};
       }
       if (lo == hi) {                                 // one value: its first elements
-        const double each = MASS ? (double)whole(weight(value_of(lo))) : 1.0;
+        const F v = value_of(lo);
+        const double each = MASS ? (double)whole(weight(v)) : 1.0;
         const double need = ceil((target - (double)above) / each);
-        cut.idx = nth_tie(cut, lo, need < 1.0 ? 1 : need > (double)c ? c : (int)need);
-        cut.key = lo;
-        return cut;
+        return {v, nth_tie(cut, v, need < 1.0 ? 1 : need > (double)c ? c : (int)need)};
       }
       a = lo, b = hi;
       linear = false;
@@ -711,21 +797,22 @@ struct RowSampler {
   }
 
   // the place, by index, where the running sum of the kept weights passes u times the total
-  __device__ int draw(const Cut<K>& cut, double u, double least) {
+  __device__ __forceinline__ int draw(const Cut<F>& cut, double u, double least) {
     __syncthreads();
     for (int i = threadIdx.x; i < SEGS; i += RT) sh.seg[i] = 0;
     if (threadIdx.x == 0) sh.which = SEGS, sh.last = -1;
     __syncthreads();
-    walk(p, V, R, inf, [&](const F(&v)[N], int base, int s) {
-      double t = 0;
+    double sum = 0;
+    walk<Z>(row, [&](const F(&v)[N], int base) {
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (cut.keeps(Key<Z>::of(v[j]), base + j)) {
-          const double w = weight(v[j]);
-          if (w >= least) t += w;
-        }
-      t = wave_sum(t);
-      if ((threadIdx.x & 63) == 0) sh.seg[s] += t;      // (a segment has one wave)
+      for (int j = 0; j < N; ++j) {
+        const double w = weight(v[j]);
+        sum += cut.keeps(v[j], base + j) && w >= least ? w : 0.0;
+      }
+    }, [&](int s) {
+      sum = wave_sum(sum);
+      if ((threadIdx.x & 63) == 0) sh.seg[s] = sum;
+      sum = 0;
     });
     __syncthreads();
     const double mine = sh.seg[threadIdx.x];
@@ -744,35 +831,31 @@ struct RowSampler {
       const int lane = threadIdx.x;
       double before = sh.wave_d[0];
       int pick = -1, end = -1;                          // end: the last kept element so far
-      for (int r = 0; r < R && pick < 0; ++r) {
-        const int base = ((s * R + r) * 64 + lane) * N;
+      for (int r = 0; r < row.R && s * row.R + r < row.steps && pick < 0; ++r) {
+        const int base = chunk_base(row, s * row.R + r);
+        Chunk<Z> q;
+        F v[N];
+        load_chunk<Z>(q, row, s * row.R + r);
+        chunk_values<Z>(v, q, row, s * row.R + r);
         double w[N], t = 0;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-          w[j] = 0;
-          if (base + j < V) {
-            const F v = finite(Key<Z>::value(p[base + j]), inf);
-            if (cut.keeps(Key<Z>::of(v), base + j)) {
-              w[j] = weight(v);
-              if (!(w[j] >= least)) w[j] = 0;
-              if (w[j] > 0) end = base + j;
-            }
-          }
+          w[j] = weight(v[j]);
+          if (!(cut.keeps(v[j], base + j) && w[j] >= least)) w[j] = 0;
+          if (w[j] > 0) end = base + j;
           t += w[j];
         }
         const double upto = before + wave_scan(t);
         const uint64_t who = last ? 0 : __ballot(t > 0 && upto > target);
         if (who) {
           const int at = (int)__builtin_ctzll(who);
-          if (lane == at) {
-            double c = upto - t;
+          double c = upto - t;
 #pragma unroll
-            for (int j = 0; j < N; ++j)
-              if (w[j] > 0 && !(pick >= 0 && c > target)) c += w[j], pick = base + j;
-          }
-          pick = __shfl(pick, at);
+          for (int j = 0; j < N; ++j)
+            if (w[j] > 0 && !(pick >= 0 && c > target)) c += w[j], pick = base + j;
+          pick = from_lane(pick, at);
         }
-        before = __shfl(upto, 63);
+        before = from_lane(upto, 63);
       }
       end = wave_max(end);
       if (lane == 0) sh.at = pick >= 0 ? pick : end;
@@ -781,14 +864,11 @@ struct RowSampler {
     return sh.at;
   }
 
-  // top-k from the elements with keys from `bound` on, if the list holds them: true, and the label in `pick`
-  __device__ bool from_list(K bound, const RowArgs& a, int& pick) {
-    const K none = Key<Z>::of(F(-__builtin_inff()));
+  // top-k from the elements at or above `bound`, if the list holds them: true, and the label in `pick`
+  __device__ __forceinline__ bool from_list(F bound, const RowArgs& a, int& pick) {
+    const F none = -__builtin_inff();
     K lo, hi;
-    const int c = list_collect<Z>(sh, p, V, R, inf, [&](F v, int) {
-      const K k = Key<Z>::of(v);
-      return k >= bound && k > none;
-    }, lo, hi);
+    const int c = list_collect<Z>(sh, row, [&](F v, int) { return v >= bound && v > none; }, lo, hi);
     if (c > CAP) return false;
     const int n2 = list_pad<Z>(sh, c);
     list_sort<Z>(sh, n2, false);
@@ -848,42 +928,45 @@ __global__ __launch_bounds__(RT) void sample_row_kernel(const Z* __restrict__ lo
   constexpr int N = Chunk<Z>::N;
   __shared__ RowShared<Z> sh;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int steps = (V + 64 * N - 1) / (64 * N), R = (steps + SEGS - 1) / SEGS;
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const Z* p = logits + row * ld;
-    const RowArgs a = row_args(args, row, V);
+  const int steps = (V + 64 * N - 1) / (64 * N);
+  // segments of up to 4 steps where every wave still gets several, more only where there are more than SEGS of them
+  const int R = max((steps + SEGS - 1) / SEGS, max(1, min(4, steps / (4 * RW))));
+  if (threadIdx.x < 32) sh.pow2[threadIdx.x] = exp2((double)threadIdx.x / 32.0);
+  for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
+    const RowArgs a = row_args(args, i, V);
+    RowView<Z> row = {logits + i * ld, V, steps, R, false};
     F mine = -__builtin_inff();
     int at = V;                                        // the 16 bytes it was first seen in
-    walk(p, V, R, false, [&](const F(&v)[N], int base, int) {
-      F t = v[0];
+    walk<Z>(row, [&](const F(&v)[N], int base) {
+      F t = mine;
 #pragma unroll
-      for (int j = 1; j < N; ++j) t = v[j] > t ? v[j] : t;
+      for (int j = 0; j < N; ++j) t = v[j] > t ? v[j] : t;
       if (t > mine) mine = t, at = base;
-    });
+    }, NoEnd());
     F m = wave_max(mine);
     __syncthreads();
     if (lane == 0) sh.wave_f[wave] = m;
     if (threadIdx.x == 0) sh.at = V;
     __syncthreads();
-    for (int i = 0; i < RW; ++i) m = sh.wave_f[i] > m ? sh.wave_f[i] : m;
+    for (int j = 0; j < RW; ++j) m = sh.wave_f[j] > m ? sh.wave_f[j] : m;
     if (!(m > -__builtin_inff()) || !(a.T > 0.0)) {
       if (mine == m && at < V) {
         int j = 0;
-        while (Key<Z>::value(p[at + j]) != m) ++j;
+        while (Key<Z>::value(row.p[at + j]) != m) ++j;
         atomicMin(&sh.at, at + j);
       }
       __syncthreads();
-      if (threadIdx.x == 0) label[row] = m > -__builtin_inff() ? sh.at : -1;
+      if (threadIdx.x == 0) label[i] = m > -__builtin_inff() ? sh.at : -1;
       continue;
     }
-    const bool inf = m == __builtin_inff();
-    mine = finite(mine, inf);
-    if (inf) m = 0;
+    row.inf = m == __builtin_inff();
+    mine = finite(mine, row.inf);
+    if (row.inf) m = 0;
     const int S = min(51, 30 + (int)__builtin_clz(V));      // 62 - log2 V, rounded down
-    RowSampler<Z> r = {sh, p, V, R, inf, Weight<F>(m, a.T), ldexp(1.0, S)};
+    RowSampler<Z> r = {sh, row, m, RowWeight<F>(m, a.T, sh.pow2), ldexp(1.0, S)};
     int pick = -1;
     bool done = false;
-    Cut<K> cut = {Key<Z>::of(F(-__builtin_inff())), -1};
+    Cut<F> cut = {-__builtin_inff(), -1};
     if (a.k) {
       if (a.k <= RT / 2) {
         // the k-th largest of the threads' maxima, its upper 16 (64-bit keys: 24) bits
@@ -898,10 +981,11 @@ __global__ __launch_bounds__(RT) void sample_row_kernel(const Z* __restrict__ lo
           __syncthreads();
           int n = 0;
 #pragma unroll
-          for (int i = 0; i < RW; ++i) n += sh.wave_n[turn][i];
+          for (int j = 0; j < RW; ++j) n += sh.wave_n[turn][j];
           if (n >= a.k) bound = cand;
         }
-        done = r.from_list(bound, a, pick);
+        const K none = Key<Z>::of(F(-__builtin_inff()));
+        done = r.from_list(r.value_of(bound > none ? bound : none), a, pick);
       }
       if (!done) cut = r.template select<false>(cut, (double)a.k, 1.0);
     }
@@ -910,7 +994,7 @@ __global__ __launch_bounds__(RT) void sample_row_kernel(const Z* __restrict__ lo
       if (a.P < 1.0) cut = r.template select<true>(cut, a.P, a.T * log((double)V / (1.0 - a.P)));
       pick = r.draw(cut, a.u, a.M);
     }
-    if (threadIdx.x == 0) label[row] = pick;
+    if (threadIdx.x == 0) label[i] = pick;
   }
 }
 
