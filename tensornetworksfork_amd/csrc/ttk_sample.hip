@@ -701,7 +701,7 @@ struct RowSampler {
   // The cut of top-k (target elements) or, MASS, of top-p (share `target` of what `cut` keeps) among the elements `cut` keeps.
   template <bool MASS>
   __device__ __forceinline__ Cut<F> select(Cut<F> cut, double target, double range) {
-    const F none = -__builtin_inff();
+    constexpr F none = -__builtin_inff();
     K a = Key<Z>::of(none) + 1, b = Key<Z>::of(m);
     bool linear = MASS;
     const F slope = (F)fmin((double)BINS / range, 1e38);      // bins a unit of z, over `range` below the maximum
@@ -716,16 +716,18 @@ struct RowSampler {
       unsigned long long beyond = 0;
       if (linear) {
         walk<Z>(row, [&](const F(&v)[N], int base) {
+          int bin[N];
+          unsigned long long q[N];
+#pragma unroll
+          for (int j = 0; j < N; ++j) {               // without branches: the eight chains overlap
+            const F z = cut.keeps(v[j], base + j) ? v[j] : none;
+            bin[j] = (int)fmin((m - z) * slope, F(BINS));
+            q[j] = whole(weight(z));
+            beyond += bin[j] < BINS ? 0ull : q[j];
+          }
 #pragma unroll
           for (int j = 0; j < N; ++j)
-            if (v[j] > none && cut.keeps(v[j], base + j)) {
-              const int bin = (int)fmin((m - v[j]) * slope, F(BINS));
-              const unsigned long long q = whole(weight(v[j]));
-              if (bin < BINS)
-                atomicAdd(&sh.hist[bin], q);
-              else
-                beyond += q;
-            }
+            if (bin[j] < BINS) atomicAdd(&sh.hist[bin[j]], q[j]);
         }, NoEnd());
         beyond = wave_sum(beyond);
         if ((threadIdx.x & 63) == 0) atomicAdd(&sh.hist[BINS], beyond);
@@ -805,9 +807,9 @@ struct RowSampler {
     double sum = 0;
     walk<Z>(row, [&](const F(&v)[N], int base) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const double w = weight(v[j]);
-        sum += cut.keeps(v[j], base + j) && w >= least ? w : 0.0;
+      for (int j = 0; j < N; ++j) {                   // without branches: the eight chains overlap
+        const double w = weight(cut.keeps(v[j], base + j) ? v[j] : -__builtin_inff());
+        sum += w >= least ? w : 0.0;
       }
     }, [&](int s) {
       sum = wave_sum(sum);
