@@ -116,8 +116,9 @@ SIGNATURES = {
     "ttk_layer_norm_backward_ws_bytes": (_i64, [_int, _i64, _int]),
     "ttk_layer_norm_backward": (_int, [_int, _int, _c_dp, _i64, _c_dp, _i64, _c_dp, _c_dp, _c_dp, _c_dp, _c_dp, _c_dp, _i64,
                                        _int, _dbl, _u64, _i64, _c_dp, _c_dp, _i64, _c_dp]),
+    "ttk_sample_ws_bytes": (_i64, [_int, _i64, _int]),
     "ttk_sample": (_int, [_int, _c_dp, _i64, _c_dp, _int, _c_dp, _dbl, _c_dp, _int, _c_dp, _dbl, _c_dp, _dbl, _c_dp, _i64, _int,
-                          _c_dp]),
+                          _c_dp, _i64, _c_dp]),
 }
 
 _lib = None

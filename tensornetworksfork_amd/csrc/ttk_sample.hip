@@ -356,20 +356,25 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const Z* __restrict__ 
 }
 
 // ---------------------------------------------------------------------------------------
-// Many classes: a workgroup a row.
+// Many classes: a few launches over all rows, a row split over workgroups where rows are few.
 //
-// The row is read from memory once and from the caches a few times more:
-//   - the maximum (and its place, for temperature 0);
-//   - top-k up to 512: the k-th largest of the 1024 threads' own maxima bounds the k-th largest element from below, so the
-//     elements at or above that bound (a few more than k) are collected in LDS, sorted, cut and drawn from there;
-//   - otherwise each cut is found by histograms: weights (counts for top-k) are added into 2048 bins, the bin with the
-//     border is collected and sorted in LDS, or, where it holds too many, refined.  Weights enter as whole numbers
-//     (2^-S of the largest, S = 62 - log2 V, at most 51), so that sums do not depend on the order of the atomics;
-//   - the draw: float64 sums of the kept weights per segment of the row, their scan, and one wave over the segment that
-//     holds u times the total.
-// Elements of -inf do not exist for any of this.
+//   maxima    the largest logit of each of up to 1024 groups of a row's elements (their largest is m; the k-th largest bounds
+//             the k-th largest element from below)
+//   collect   top-k: the elements at or above that bound, a few more than k, into the row's list
+//   counts    top-p: how many elements lie in each of 4096 bins below m.  A bin's weight is known to the width of a bin from
+//             its count, so the cumulative weight is bounded from both sides, and
+//   window    the border of top-p lies in a narrow window of bins
+//   sums      every weight once: float64 sums of the kept ones per segment of the row, and of the rest; the window's elements
+//             go into the row's list
+//   finish    a workgroup a row: sorts the list in LDS, cuts it, and draws from it or from the segment sums
+// Rows whose list does not hold what it should (top-k above what the groups bound, thousands of equal logits) are done by
+// `slow_row`: cuts by histograms over the whole row, refined until the bin with the border fits the list.
+//
+// Elements of -inf do not exist for any of this, nor do weights below 2^-1000 of the largest; min-p is a bound on the value,
+// m + T ln(min_p).  Sums are added in a fixed order, counts are whole numbers, lists are sorted: the label does not depend on
+// the order in which workgroups run.
 // ---------------------------------------------------------------------------------------
-constexpr int RT = 1024, RW = RT / 64, BINS = 2048, CAP = 2048, SEGS = 1024;
+constexpr int RT = 1024, RW = RT / 64, BINS = 2048, COUNTS = 4096, CAP = 2048, SEGS = 1024, GROUPS = 1024, LONG_CAP = 8192;
 
 template <typename Z>
 struct Chunk {
@@ -381,18 +386,19 @@ struct Chunk {
   };
 };
 
-// A row as the waves of its workgroup see it: steps of 64 x 16 bytes, R steps a segment, wave w owns segments w, w + RW, ...
+// A row as a wave sees it: steps of 64 x 16 bytes, R steps a segment; the wave owns segments first, first + stride, ...
 template <typename Z>
 struct RowView {
   const Z* p;
-  int V, steps, R;
+  int V, steps, R, first, stride;
   bool inf;        // the maximum is +inf
 };
 
 // The 16 bytes of this lane in step t.  Behind the row's end the last 16 bytes are read again (a row has more than that).
 template <typename Z>
 __device__ __forceinline__ int chunk_base(const RowView<Z>& row, int t) {
-  return min((t * 64 + (int)(threadIdx.x & 63)) * Chunk<Z>::N, row.V - Chunk<Z>::N);
+  const int64_t at = ((int64_t)t * 64 + (int)(threadIdx.x & 63)) * Chunk<Z>::N;
+  return (int)min(at, (int64_t)(row.V - Chunk<Z>::N));
 }
 template <typename Z>
 __device__ __forceinline__ void load_chunk(Chunk<Z>& c, const RowView<Z>& row, int t) {
@@ -409,7 +415,7 @@ __device__ __forceinline__ void chunk_values(typename Key<Z>::val_t (&v)[Chunk<Z
 #pragma unroll
   for (int j = 0; j < N; ++j) v[j] = (F)c.e[j];
   if (t == row.steps - 1) {
-    const int again = (t * 64 + (int)(threadIdx.x & 63)) * N - chunk_base(row, t);
+    const int64_t again = ((int64_t)t * 64 + (int)(threadIdx.x & 63)) * N - chunk_base(row, t);
 #pragma unroll
     for (int j = 0; j < N; ++j)
       if (j < again) v[j] = -__builtin_inff();
@@ -424,11 +430,11 @@ __device__ __forceinline__ void chunk_values(typename Key<Z>::val_t (&v)[Chunk<Z
 template <typename Z, typename Fn, typename End>
 __device__ __forceinline__ void walk(const RowView<Z>& row, Fn f, End end) {
   constexpr int N = Chunk<Z>::N;
-  int s = threadIdx.x >> 6, r = 0, ls = s, lr = 0;      // the step at work, the step to load next
+  int s = row.first, r = 0, ls = s, lr = 0;      // the step at work, the step to load next
   Chunk<Z> q[4];
   auto load = [&](Chunk<Z>& c) {
     load_chunk<Z>(c, row, ls * row.R + lr);
-    if (++lr == row.R) lr = 0, ls += RW;
+    if (++lr == row.R) lr = 0, ls += row.stride;
   };
   load(q[0]);
   load(q[1]);
@@ -442,7 +448,7 @@ __device__ __forceinline__ void walk(const RowView<Z>& row, Fn f, End end) {
     q[0] = q[1], q[1] = q[2], q[2] = q[3];
     const bool full = ++r == row.R;
     if (full || t + 1 >= row.steps) end(s);
-    if (full) r = 0, s += RW;
+    if (full) r = 0, s += row.stride;
     t = s * row.R + r;
   }
 }
@@ -455,19 +461,18 @@ struct RowShared {
   typedef typename Key<Z>::type K;
   typedef typename Key<Z>::val_t F;
   union {
-    unsigned long long hist[BINS + 1];
+    unsigned long long hist[BINS];
+    uint32_t counts[COUNTS];
     struct {
       uint64_t key[CAP];                                     // 32-bit keys: key << 32 | ~index
       uint32_t nidx[sizeof(K) == 8 ? CAP : 1];               // 64-bit keys: ~index
     } list;
-    double seg[SEGS];
     int count[SEGS];
   };
+  double seg[SEGS];
   double pow2[32];
   double wave_d[RW];
   unsigned long long wave_u[RW];
-  int wave_n[2][RW];
-  F wave_f[RW];
   K wave_lo[RW], wave_hi[RW];
   int n, at, which, last;
   unsigned long long above;
@@ -477,16 +482,17 @@ struct RowShared {
 
 // The weight of Weight, with 2^(n / 32) from a table: 2^((z - m) log2(e) / T) = 2^(n div 32) pow2[n mod 32] 2^(f / 32),
 // |f| <= 1/2, the last factor by its Taylor polynomial (relative error below 3e-15).  The 32 doubles lie in 64 different
-// LDS banks.  m is finite.
+// LDS banks.  m is finite; an element that is not kept weighs 0, one that is lies at most 1000 / log2(e) T below m.
 template <typename F>
 struct RowWeight {
   double m, c;
   const double* pow2;
   __device__ __forceinline__ RowWeight(F m_, double T, const double* table)
       : m((double)m_), c(fmin(32 * 1.4426950408889634074 / T, 1e300)), pow2(table) {}
-  __device__ __forceinline__ double operator()(F z) const {
-    double t = ((double)z - m) * c;
-    t = t > -35200.0 ? t : -35200.0;
+  __device__ __forceinline__ double operator()(F z, bool keep) const {
+    const int64_t b = __double_as_longlong(((double)z - m) * c);
+    const int hi = keep ? (int)(b >> 32) : (int)0xC0E13000;      // -35200: 2^-1100, which is 0
+    const double t = __longlong_as_double((int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)b));
     const double s = t + 0x1.8p52, f = t - (s - 0x1.8p52);
     const int n = (int)(uint32_t)__double_as_longlong(s);
     double p = 3.97370998454941544e-11;
@@ -537,36 +543,87 @@ __device__ __forceinline__ void list_get(const RowShared<Z>& sh, int i, typename
   }
 }
 
-// Bitonic sort of the first n2 (a power of two) elements, highest first: by (key, ~index), or by ~index alone.  A wave
-// exchanges within its own 128 elements while the distance is at most 64: only longer ones need the workgroup's barrier.
+// Bitonic sort of the first n2 (a power of two, at least 128) elements, highest first: by (key, ~index), or by ~index
+// alone.  Wave w holds elements 128 w + lane and 128 w + 64 + lane in registers; distances up to 64 are exchanged there,
+// longer ones through LDS.
+template <typename Z>
+struct Item {
+  typedef typename Key<Z>::type K;
+  K k;
+  uint32_t n;
+};
+template <typename Z>
+__device__ __forceinline__ bool in_front(const Item<Z>& a, const Item<Z>& b, bool by_index) {
+  if constexpr (sizeof(a.k) == 4) {
+    const uint64_t x = by_index ? a.n : (uint64_t)a.k << 32 | a.n, y = by_index ? b.n : (uint64_t)b.k << 32 | b.n;
+    return x > y;
+  } else {
+    return by_index ? a.n > b.n : a.k > b.k || (a.k == b.k && a.n > b.n);
+  }
+}
 template <typename Z>
 __device__ __forceinline__ void list_sort(RowShared<Z>& sh, int n2, bool by_index) {
-  typedef typename Key<Z>::type K;
+  const int lane = threadIdx.x & 63, i0 = (threadIdx.x >> 6) * 128 + lane;
+  const bool mine = i0 - lane < n2;      // (the same in a wave)
+  Item<Z> e[2];
   __syncthreads();
-  for (int size = 2; size <= n2; size <<= 1)
-    for (int d = size >> 1; d > 0; d >>= 1) {
-      if (d > 64)
-        __syncthreads();
-      else {
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+  if (mine) {
+    list_get<Z>(sh, i0, e[0].k, e[0].n);
+    list_get<Z>(sh, i0 + 64, e[1].k, e[1].n);
+  }
+#pragma unroll 1
+  for (int size = 2; size <= n2; size <<= 1) {
+    if (size > 128) {
+      if (mine) {
+        list_put<Z>(sh, i0, e[0].k, e[0].n);
+        list_put<Z>(sh, i0 + 64, e[1].k, e[1].n);
       }
-      const int t = threadIdx.x;
-      if (t < n2 / 2) {
-        const int i = 2 * t - (t & (d - 1)), j = i + d;
-        K ki, kj;
-        uint32_t ni, nj;
-        list_get<Z>(sh, i, ki, ni);
-        list_get<Z>(sh, j, kj, nj);
-        const bool less = by_index ? ni < nj : ki < kj || (ki == kj && ni < nj);
-        const bool more = by_index ? ni > nj : ki > kj || (ki == kj && ni > nj);
-        if ((i & size) ? more : less) {
-          list_put<Z>(sh, i, kj, nj);
-          list_put<Z>(sh, j, ki, ni);
+#pragma unroll 1
+      for (int d = size >> 1; d > 64; d >>= 1) {
+        __syncthreads();
+        const int t = threadIdx.x;
+        if (t < n2 / 2) {
+          const int i = 2 * t - (t & (d - 1)), j = i + d;
+          Item<Z> a, b;
+          list_get<Z>(sh, i, a.k, a.n);
+          list_get<Z>(sh, j, b.k, b.n);
+          if ((i & size) ? in_front<Z>(a, b, by_index) : in_front<Z>(b, a, by_index)) {
+            list_put<Z>(sh, i, b.k, b.n);
+            list_put<Z>(sh, j, a.k, a.n);
+          }
         }
       }
-      if (d > 64) __syncthreads();
+      __syncthreads();
+      if (mine) {
+        list_get<Z>(sh, i0, e[0].k, e[0].n);
+        list_get<Z>(sh, i0 + 64, e[1].k, e[1].n);
+      }
     }
+    if (mine) {
+      if (size >= 128) {
+        const bool swap = (i0 & size) ? in_front<Z>(e[0], e[1], by_index) : in_front<Z>(e[1], e[0], by_index);
+        const Item<Z> x = e[0];
+        e[0] = swap ? e[1] : e[0];
+        e[1] = swap ? x : e[1];
+      }
+#pragma unroll 1
+      for (int d = min(size >> 1, 32); d > 0; d >>= 1) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int i = i0 + 64 * h;
+          Item<Z> o;
+          o.k = __shfl_xor(e[h].k, d);
+          o.n = __shfl_xor(e[h].n, d);
+          const bool first = ((i & d) == 0) == ((i & size) == 0);      // takes the one in front
+          if (first ? in_front<Z>(o, e[h], by_index) : in_front<Z>(e[h], o, by_index)) e[h] = o;
+        }
+      }
+    }
+  }
+  if (mine) {
+    list_put<Z>(sh, i0, e[0].k, e[0].n);
+    list_put<Z>(sh, i0 + 64, e[1].k, e[1].n);
+  }
   __syncthreads();
 }
 
@@ -581,7 +638,7 @@ __device__ int list_collect(RowShared<Z>& sh, const RowView<Z>& row, In in, type
   if (threadIdx.x == 0) sh.n = 0;
   __syncthreads();
   K l = ~(K)0, h = 0;
-  walk<Z>(row, [&](const F(&v)[N], int base) {
+  walk<Z>(row, [&](F(&v)[N], int base) {
     uint32_t mask = 0;
 #pragma unroll
     for (int j = 0; j < N; ++j)
@@ -618,18 +675,83 @@ __device__ int list_collect(RowShared<Z>& sh, const RowView<Z>& row, In in, type
 // pads the list of c elements to a power of two with entries that sort last and returns it
 template <typename Z>
 __device__ int list_pad(RowShared<Z>& sh, int c) {
-  int n2 = 2;
+  int n2 = 128;
   while (n2 < c) n2 <<= 1;
   for (int i = c + threadIdx.x; i < n2; i += RT) list_put<Z>(sh, i, 0, 0);
   return n2;
 }
 
-// What is kept: the elements that do not come behind (v, idx) in the order.
+template <typename F>
+__device__ __forceinline__ F next_up(F v) {      // v not NaN, not +inf
+  if constexpr (sizeof(F) == 4) {
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    return v == 0 ? __uint_as_float(1u) : __uint_as_float(b >> 31 ? b - 1 : b + 1);
+  } else {
+    const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
+    return v == 0 ? __longlong_as_double(1) : __longlong_as_double((int64_t)(b >> 63 ? b - 1 : b + 1));
+  }
+}
+template <typename F>
+__device__ __forceinline__ F round_up(double x) {      // the smallest F not below x, finite
+  F f = (F)x;
+  if ((double)f < x) f = next_up(f);
+  return f;
+}
+
+// What is kept: the elements that do not come behind (v, idx) in the order, and are not below `floor`.
 template <typename F>
 struct Cut {
   F v;
   int idx;
   __device__ __forceinline__ bool keeps(F z, int i) const { return z > v || (z == v && i <= idx); }
+};
+
+// The same as one comparison an element: z is kept iff z >= the limit of its 16 bytes, but for those the index splits.
+template <typename F>
+struct Limit {
+  F with, without;      // limits where elements that equal v are kept, and where they are not
+  int idx;
+  __device__ __forceinline__ Limit(const Cut<F>& c, F floor) : idx(c.idx) {
+    const F up = next_up(c.v);
+    with = c.idx < 0 || c.v < floor ? (up > floor ? up : floor) : c.v;
+    without = up > floor ? up : floor;
+  }
+  template <int N>
+  __device__ __forceinline__ F of(F (&z)[N], int base) const {
+    const bool split = base <= idx && base + N - 1 > idx;
+    if (__any(split)) {
+      if (split)
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (base + j > idx && z[j] < without) z[j] = -__builtin_inff();
+    }
+    return base > idx ? without : with;
+  }
+};
+
+template <typename Z>
+__device__ __forceinline__ typename Key<Z>::val_t value_of(typename Key<Z>::type k) {
+  if constexpr (sizeof(k) == 4)
+    return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+  else
+    return __longlong_as_double((int64_t)(k ^ ((k >> 63) ? 0x8000000000000000ull : ~0ull)));
+}
+
+// What one row's largest logit and parameters say about its elements.
+template <typename Z>
+struct RowScale {
+  typedef typename Key<Z>::val_t F;
+  F m;
+  bool inf;
+  F floor, least;      // below `floor` weights are 0 (finite: -inf is below it); below `least` min-p drops
+  __device__ __forceinline__ RowScale(typename Key<Z>::type key, const RowArgs& a) {
+    m = value_of<Z>(key);
+    inf = m == __builtin_inff();
+    if (inf) m = 0;
+    floor = round_up<F>((double)m - 693.147 * a.T);
+    least = a.M > 0 ? round_up<F>((double)m + a.T * log(a.M)) : floor;
+    if (least < floor) least = floor;
+  }
 };
 
 template <typename Z>
@@ -641,17 +763,7 @@ struct RowSampler {
   RowView<Z> row;
   F m;
   RowWeight<F> weight;
-  double fixed;      // 2^S
-
-  __device__ __forceinline__ unsigned long long whole(double w) const {      // w 2^S, rounded; below 2^52
-    return (unsigned long long)__double_as_longlong(w * fixed + 0x1p52) - 0x4330000000000000ull;
-  }
-  static __device__ __forceinline__ F value_of(K k) {
-    if constexpr (sizeof(K) == 4)
-      return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
-    else
-      return __longlong_as_double((int64_t)(k ^ ((k >> 63) ? 0x8000000000000000ull : ~0ull)));
-  }
+  F floor;
 
   // place of the n-th (from 1) kept element that equals t
   __device__ __forceinline__ int nth_tie(const Cut<F>& cut, F t, int n) {
@@ -659,7 +771,7 @@ struct RowSampler {
     for (int i = threadIdx.x; i < SEGS; i += RT) sh.count[i] = 0;
     __syncthreads();
     int c = 0;
-    walk<Z>(row, [&](const F(&v)[N], int base) {
+    walk<Z>(row, [&](F(&v)[N], int base) {
 #pragma unroll
       for (int j = 0; j < N; ++j) c += v[j] == t && cut.keeps(t, base + j);
     }, [&](int s) {
@@ -677,6 +789,7 @@ struct RowSampler {
     int before = sh.at;
     __syncthreads();
     if (threadIdx.x < 64)
+#pragma unroll 1
       for (int r = 0; r < row.R && s * row.R + r < row.steps; ++r) {
         Chunk<Z> q;
         F v[N];
@@ -698,68 +811,49 @@ struct RowSampler {
     return sh.at;
   }
 
-  // The cut of top-k (target elements) or, MASS, of top-p (share `target` of what `cut` keeps) among the elements `cut` keeps.
+  // The cut of top-k (`target` elements) or, MASS, of top-p (the share `target` of the weight) among the elements `cut` keeps.
   template <bool MASS>
-  __device__ __forceinline__ Cut<F> select(Cut<F> cut, double target, double range) {
-    constexpr F none = -__builtin_inff();
-    K a = Key<Z>::of(none) + 1, b = Key<Z>::of(m);
-    bool linear = MASS;
-    const F slope = (F)fmin((double)BINS / range, 1e38);      // bins a unit of z, over `range` below the maximum
+  __device__ __forceinline__ Cut<F> select(Cut<F> cut, double target) {
+    K a = Key<Z>::of(MASS ? floor : -__builtin_inff()) + (MASS ? 0 : 1), b = Key<Z>::of(m);
+    const double fixed = ldexp(1.0, min(51, 30 + (int)__builtin_clz(row.V)));      // 2^S
+    auto whole = [&](double w) {                                                   // w 2^S, rounded; below 2^52
+      return (unsigned long long)__double_as_longlong(w * fixed + 0x1p52) - 0x4330000000000000ull;
+    };
     unsigned long long above = 0;
+    bool share = MASS;                                // the target is still to be multiplied by the total
+#pragma unroll 1
     for (;;) {
       __syncthreads();
-      for (int i = threadIdx.x; i <= BINS; i += RT) sh.hist[i] = 0;
+      for (int i = threadIdx.x; i < BINS; i += RT) sh.hist[i] = 0;
       __syncthreads();
       int shift = 0;
-      if (!linear)
-        while (((b - a) >> shift) >= (K)BINS) ++shift;
-      unsigned long long beyond = 0;
-      if (linear) {
-        walk<Z>(row, [&](const F(&v)[N], int base) {
-          int bin[N];
-          unsigned long long q[N];
+      while (((b - a) >> shift) >= (K)BINS) ++shift;
+      walk<Z>(row, [&](F(&v)[N], int base) {
 #pragma unroll
-          for (int j = 0; j < N; ++j) {               // without branches: the eight chains overlap
-            const F z = cut.keeps(v[j], base + j) ? v[j] : none;
-            bin[j] = (int)fmin((m - z) * slope, F(BINS));
-            q[j] = whole(weight(z));
-            beyond += bin[j] < BINS ? 0ull : q[j];
-          }
-#pragma unroll
-          for (int j = 0; j < N; ++j)
-            if (bin[j] < BINS) atomicAdd(&sh.hist[bin[j]], q[j]);
-        }, NoEnd());
-        beyond = wave_sum(beyond);
-        if ((threadIdx.x & 63) == 0) atomicAdd(&sh.hist[BINS], beyond);
-      } else {
-        walk<Z>(row, [&](const F(&v)[N], int base) {
-#pragma unroll
-          for (int j = 0; j < N; ++j) {
-            const K k = Key<Z>::of(v[j]);
-            if (k >= a && k <= b && cut.keeps(v[j], base + j))
-              atomicAdd(&sh.hist[(int)((b - k) >> shift)], MASS ? whole(weight(v[j])) : 1ull);
-          }
-        }, NoEnd());
-      }
+        for (int j = 0; j < N; ++j) {
+          const K k = Key<Z>::of(v[j]);
+          if (k >= a && k <= b && cut.keeps(v[j], base + j))
+            atomicAdd(&sh.hist[(int)((b - k) >> shift)], MASS ? whole(weight(v[j], true)) : 1ull);
+        }
+      }, NoEnd());
       __syncthreads();
-      const unsigned long long v0 = sh.hist[2 * threadIdx.x], v1 = sh.hist[2 * threadIdx.x + 1], over = sh.hist[BINS];
+      const unsigned long long v0 = sh.hist[2 * threadIdx.x], v1 = sh.hist[2 * threadIdx.x + 1];
       unsigned long long total;
       const unsigned long long upto = above + block_scan(v0 + v1, sh.wave_u, total), from = upto - v0 - v1;
-      if (linear) target *= (double)(total + over);
-      if (threadIdx.x == 0 && (double)(above + total) < target) sh.which = linear ? BINS : -1, sh.above = above + total;
+      if (share) target *= (double)total;
+      share = false;
+      if (threadIdx.x == 0 && (double)(above + total) < target) sh.which = -1, sh.above = above;
       if ((double)from < target && (double)(from + v0) >= target) sh.which = 2 * threadIdx.x, sh.above = from;
       if ((double)(from + v0) < target && (double)upto >= target) sh.which = 2 * threadIdx.x + 1, sh.above = from + v0;
       __syncthreads();
       const int bin = sh.which;
       above = sh.above;
       if (bin < 0) return cut;                        // fewer elements than asked for: all stay
-      const K bb = b - (linear ? (K)0 : (K)bin << shift), width = linear ? (K)0 : ((K)1 << shift) - 1;
+      const K bb = b - ((K)bin << shift), width = ((K)1 << shift) - 1;
       K lo, hi;
       const int c = list_collect<Z>(sh, row, [&](F v, int i) {
-        if (!(v > none) || !cut.keeps(v, i)) return false;
-        if (linear) return (int)fmin((m - v) * slope, F(BINS)) == bin;
         const K k = Key<Z>::of(v);
-        return k >= a && k <= bb && bb - k <= width;
+        return k >= a && k <= bb && bb - k <= width && cut.keeps(v, i);
       }, lo, hi);
       if (c <= CAP) {
         const int n2 = list_pad<Z>(sh, c);
@@ -772,7 +866,7 @@ struct RowSampler {
           const int i = 2 * threadIdx.x + e;
           if (i < c) {
             list_get<Z>(sh, i, key[e], nidx[e]);
-            q[e] = MASS ? whole(weight(value_of(key[e]))) : 1ull;
+            q[e] = MASS ? whole(weight(value_of<Z>(key[e]), true)) : 1ull;
           }
         }
         unsigned long long sum;
@@ -785,38 +879,40 @@ struct RowSampler {
           before += q[e];
         }
         __syncthreads();
-        return {value_of(sh.cut_key), sh.cut_idx};
+        return {value_of<Z>(sh.cut_key), sh.cut_idx};
       }
       if (lo == hi) {                                 // one value: its first elements
-        const F v = value_of(lo);
-        const double each = MASS ? (double)whole(weight(v)) : 1.0;
+        const F v = value_of<Z>(lo);
+        const double each = MASS ? (double)whole(weight(v, true)) : 1.0;
         const double need = ceil((target - (double)above) / each);
         return {v, nth_tie(cut, v, need < 1.0 ? 1 : need > (double)c ? c : (int)need)};
       }
       a = lo, b = hi;
-      linear = false;
     }
   }
 
-  // the place, by index, where the running sum of the kept weights passes u times the total
-  __device__ __forceinline__ int draw(const Cut<F>& cut, double u, double least) {
+  // Sums of the kept weights by segment.
+  __device__ __forceinline__ void segment_sums(const Cut<F>& cut, F least) {
     __syncthreads();
-    for (int i = threadIdx.x; i < SEGS; i += RT) sh.seg[i] = 0;
-    if (threadIdx.x == 0) sh.which = SEGS, sh.last = -1;
+    sh.seg[threadIdx.x] = 0;
     __syncthreads();
+    const Limit<F> limit(cut, least > floor ? least : floor);
     double sum = 0;
-    walk<Z>(row, [&](const F(&v)[N], int base) {
+    walk<Z>(row, [&](F(&v)[N], int base) {
+      const F lim = limit.template of<N>(v, base);
 #pragma unroll
-      for (int j = 0; j < N; ++j) {                   // without branches: the eight chains overlap
-        const double w = weight(cut.keeps(v[j], base + j) ? v[j] : -__builtin_inff());
-        sum += w >= least ? w : 0.0;
-      }
+      for (int j = 0; j < N; ++j) sum += weight(v[j], v[j] >= lim);
     }, [&](int s) {
       sum = wave_sum(sum);
       if ((threadIdx.x & 63) == 0) sh.seg[s] = sum;
       sum = 0;
     });
     __syncthreads();
+  }
+
+  // the place, by index, where the running sum of the kept weights passes u times the total (sh.seg holds their sums)
+  __device__ __forceinline__ int draw(const Cut<F>& cut, F least, double u) {
+    if (threadIdx.x == 0) sh.which = SEGS, sh.last = -1;
     const double mine = sh.seg[threadIdx.x];
     double total;
     const double upto = block_scan(mine, sh.wave_d, total), target = u * total;
@@ -831,19 +927,21 @@ struct RowSampler {
     __syncthreads();
     if (threadIdx.x < 64) {
       const int lane = threadIdx.x;
+      const Limit<F> limit(cut, least > floor ? least : floor);
       double before = sh.wave_d[0];
       int pick = -1, end = -1;                          // end: the last kept element so far
+#pragma unroll 1
       for (int r = 0; r < row.R && s * row.R + r < row.steps && pick < 0; ++r) {
         const int base = chunk_base(row, s * row.R + r);
         Chunk<Z> q;
         F v[N];
         load_chunk<Z>(q, row, s * row.R + r);
         chunk_values<Z>(v, q, row, s * row.R + r);
+        const F lim = limit.template of<N>(v, base);
         double w[N], t = 0;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-          w[j] = weight(v[j]);
-          if (!(cut.keeps(v[j], base + j) && w[j] >= least)) w[j] = 0;
+          w[j] = weight(v[j], v[j] >= lim);
           if (w[j] > 0) end = base + j;
           t += w[j];
         }
@@ -865,161 +963,631 @@ struct RowSampler {
     __syncthreads();
     return sh.at;
   }
+};
 
-  // top-k from the elements at or above `bound`, if the list holds them: true, and the label in `pick`
-  __device__ __forceinline__ bool from_list(F bound, const RowArgs& a, int& pick) {
-    const F none = -__builtin_inff();
-    K lo, hi;
-    const int c = list_collect<Z>(sh, row, [&](F v, int) { return v >= bound && v > none; }, lo, hi);
-    if (c > CAP) return false;
-    const int n2 = list_pad<Z>(sh, c);
-    list_sort<Z>(sh, n2, false);
-    const int kk = min(a.k, c);
-    double w[2], total;
+// Any row of more than 1024 classes with temperature above 0, by one workgroup.  Not inlined: a row in a thousand comes here,
+// and its registers would cost every other.
+template <typename Z>
+__device__ __attribute__((noinline)) int slow_row(const Z* p, int V, int R, typename Key<Z>::type top, double u, double T, double P,
+                                                  double M, int k) {
+  typedef typename Key<Z>::val_t F;
+  __shared__ RowShared<Z> sh;
+  const RowArgs a = {u, T, P, M, k};
+  const RowScale<Z> sc(top, a);
+  __syncthreads();
+  if (threadIdx.x < 32) sh.pow2[threadIdx.x] = exp2((double)threadIdx.x / 32.0);
+  constexpr int N = Chunk<Z>::N;
+  const RowView<Z> row = {p, V, (int)(((int64_t)V + 64 * N - 1) / (64 * N)), R, (int)(threadIdx.x >> 6), RW, sc.inf};
+  RowSampler<Z> r = {sh, row, sc.m, RowWeight<F>(sc.m, T, sh.pow2), sc.floor};
+  Cut<F> cut = {-__builtin_inff(), -1};
+  if (k) cut = r.template select<false>(cut, (double)k);
+  if (P < 1.0) cut = r.template select<true>(cut, P);
+  r.segment_sums(cut, sc.least);
+  return r.draw(cut, sc.least, u);
+}
+
+// ---- the launches -------------------------------------------------------------------------------------------------
+
+struct Geometry {
+  int V, steps, R, segs, per_seg;      // per_seg: groups a segment (a power of two)
+  int most;                            // top-k up to this many is taken from the list
+};
+
+template <typename Z>
+Geometry geometry(int V) {
+  constexpr int N = Chunk<Z>::N;
+  Geometry g;
+  g.V = V;
+  g.steps = (int)(((int64_t)V + 64 * N - 1) / (64 * N));
+  g.R = (g.steps + SEGS - 1) / SEGS;
+  g.segs = (g.steps + g.R - 1) / g.R;
+  g.per_seg = 64;
+  while (g.per_seg * g.segs > GROUPS) g.per_seg /= 2;
+  // k of n groups' maxima bound the k-th largest by an element with about -n ln(1 - k / n) above it
+  const int groups = g.per_seg * g.segs;
+  g.most = V <= LONG_CAP ? V : groups - groups / 32;
+  return g;
+}
+
+// A row's part of the workspace.
+template <typename Z>
+struct RowWork {
+  typedef typename Key<Z>::type K;
+  K maxima[GROUPS];
+  uint32_t counts[COUNTS];
+  double seg[SEGS], above[SEGS], rest[SEGS];      // kept for certain; those before min-p; the others
+  K key[LONG_CAP];
+  uint32_t idx[LONG_CAP];
+  int n;                                          // elements that asked for a place in the list
+  int first, last;                                // window: bins; first > last: none was found
+};
+
+enum Path { DONE_BY_MAX, LIST, WINDOW, PLAIN, SLOW };
+
+__device__ __forceinline__ Path row_path(const RowArgs& a, const Geometry& g) {
+  if (!(a.T > 0.0)) return DONE_BY_MAX;
+  if (a.k) return a.k <= g.most ? LIST : SLOW;
+  return a.P < 1.0 ? WINDOW : PLAIN;
+}
+
+constexpr int TB = 256, TW = TB / 64;
+
+// the largest key of the groups' maxima, in every thread of a workgroup of WAVES waves
+template <int WAVES, typename K>
+__device__ __forceinline__ K largest(const K* maxima, int n, K* buf) {
+  K m = 0;
+  for (int i = threadIdx.x; i < n; i += WAVES * 64) m = maxima[i] > m ? maxima[i] : m;
+  m = wave_max(m);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = buf[0];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int i = 2 * threadIdx.x + e;
-      K k;
-      uint32_t n;
-      w[e] = 0;
-      if (i < kk) {
-        list_get<Z>(sh, i, k, n);
-        w[e] = weight(value_of(k));
-      }
+  for (int i = 1; i < WAVES; ++i) m = buf[i] > m ? buf[i] : m;
+  return m;
+}
+
+template <typename Z>
+__global__ __launch_bounds__(TB) void row_maxima_kernel(const Z* __restrict__ logits, int64_t ld, Geometry g,
+                                                        RowWork<Z>* __restrict__ work) {
+  typedef typename Key<Z>::val_t F;
+  constexpr int N = Chunk<Z>::N;
+  RowWork<Z>& w = work[blockIdx.y];
+  const int lane = threadIdx.x & 63;
+  if (blockIdx.x == 0 && threadIdx.x == 0) w.n = 0, w.first = 1, w.last = 0;
+  for (int i = blockIdx.x * TB + threadIdx.x; i < COUNTS; i += gridDim.x * TB) w.counts[i] = 0;
+  const RowView<Z> row = {logits + (int64_t)blockIdx.y * ld, g.V, g.steps, g.R, (int)(blockIdx.x * TW + (threadIdx.x >> 6)),
+                          (int)(gridDim.x * TW), false};
+  F mine = -__builtin_inff();
+  const int wide = 64 / g.per_seg;
+  walk<Z>(row, [&](F(&v)[N], int) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) mine = v[j] > mine ? v[j] : mine;
+  }, [&](int s) {
+    for (int d = 1; d < wide; d <<= 1) {
+      const F o = __shfl_xor(mine, d);
+      mine = o > mine ? o : mine;
     }
-    const double from = block_scan(w[0] + w[1], sh.wave_d, total) - w[0] - w[1], target = a.P * total;
+    if (lane % wide == 0) w.maxima[s * g.per_seg + lane / wide] = Key<Z>::of(mine);
+    mine = -__builtin_inff();
+  });
+}
+
+// Places for the lanes' `mask`ed elements in the row's list: the first one of this lane.
+__device__ __forceinline__ int list_places(int* n, uint32_t mask) {
+  const int c = __popc(mask), upto = wave_scan(c), all = from_lane(upto, 63);
+  int at = 0;
+  if ((threadIdx.x & 63) == 0) at = atomicAdd(n, all);
+  return from_lane(at, 0) + upto - c;
+}
+
+template <typename Z>
+__global__ __launch_bounds__(TB) void row_collect_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args, Geometry g,
+                                                         RowWork<Z>* __restrict__ work, int64_t row0) {
+  typedef typename Key<Z>::type K;
+  typedef typename Key<Z>::val_t F;
+  constexpr int N = Chunk<Z>::N;
+  __shared__ K buf[TW];
+  __shared__ int counts[2][TW];
+  RowWork<Z>& w = work[blockIdx.y];
+  const RowArgs a = row_args(args, row0 + blockIdx.y, g.V);
+  if (row_path(a, g) != LIST) return;
+  const int groups = g.segs * g.per_seg;
+  const K top = largest<TW>(w.maxima, groups, buf);
+  const RowScale<Z> sc(top, a);
+  K bound = 0;
+  if (a.k <= groups) {      // the k-th largest of the maxima, its upper 16 (64-bit keys: 24) bits
+    K key[GROUPS / TB];
+#pragma unroll
+    for (int i = 0; i < GROUPS / TB; ++i) {
+      const int at = i * TB + threadIdx.x;
+      key[i] = at < groups ? w.maxima[at] : (K)0;
+      if (sc.inf) key[i] = Key<Z>::of(finite(value_of<Z>(key[i]), true));
+    }
+    constexpr int BITS = 8 * (int)sizeof(K), END = BITS - (BITS == 64 ? 24 : 16);
+    int turn = 0;
+#pragma unroll 1
+    for (int bit = BITS - 1; bit >= END; --bit, turn ^= 1) {
+      const K cand = bound | ((K)1 << bit);
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < GROUPS / TB; ++i) c += __popcll(__ballot(key[i] >= cand));
+      if ((threadIdx.x & 63) == 0) counts[turn][threadIdx.x >> 6] = c;
+      __syncthreads();
+      c = 0;
+#pragma unroll
+      for (int i = 0; i < TW; ++i) c += counts[turn][i];
+      if (c >= a.k) bound = cand;
+    }
+  }
+  const K lowest = Key<Z>::of(sc.floor);
+  const F lim = bound > lowest ? value_of<Z>(bound) : sc.floor;
+  const RowView<Z> row = {logits + (int64_t)blockIdx.y * ld, g.V, g.steps, g.R, (int)(blockIdx.x * TW + (threadIdx.x >> 6)),
+                          (int)(gridDim.x * TW), sc.inf};
+  walk<Z>(row, [&](F(&v)[N], int base) {
+    uint32_t mask = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) mask |= (uint32_t)(v[j] >= lim) << j;
+    if (__any(mask != 0)) {
+      int at = list_places(&w.n, mask);
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (mask >> j & 1) {
+          if (at < LONG_CAP) w.key[at] = Key<Z>::of(v[j]), w.idx[at] = (uint32_t)(base + j);
+          ++at;
+        }
+    }
+  }, NoEnd());
+}
+
+// Bins over what can matter of a row cut by top-p: what lies further below the maximum than ln(V / (1 - P)) weighs less than
+// 1 - P of the total.
+template <typename F>
+__device__ __forceinline__ F bin_slope(const RowArgs& a, int V) {
+  return (F)fmin((double)COUNTS / (a.T * log((double)V / (1.0 - a.P))), 1e38);
+}
+
+// The bins the border of top-p must lie in, from the counts (`all` elements at or above the floor): a bin's weight lies
+// between its count times the weights of its edges, moved out by a hundredth of a bin for the roundings of the bin number.
+__device__ __forceinline__ void find_window(const uint32_t* counts, int beyond, double slope, const RowArgs& a, double* buf,
+                                            int* found) {
+  constexpr int PER = COUNTS / RT;
+  const double step = 1.0 / (slope * a.T);
+  double least[PER], most[PER], sl = 0, sm = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int bin = PER * threadIdx.x + i;
+    const double n = (double)counts[bin];
+    least[i] = n * exp(-((double)bin + 1.01) * step);
+    most[i] = n * exp(-((double)bin - 0.01) * step);
+    sl += least[i];
+    sm += most[i];
+  }
+  double total_least, total_most;
+  double ul = block_scan(sl, buf, total_least) - sl;
+  double um = block_scan(sm, buf, total_most) - sm;
+  total_most += (double)beyond * exp(-((double)COUNTS - 0.01) * step);
+  __syncthreads();
+  if (threadIdx.x == 0) found[0] = COUNTS, found[1] = COUNTS;
+  __syncthreads();
+  const double early = a.P * total_least * (1 - 1e-9), late = a.P * total_most * (1 + 1e-9);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    ul += least[i];
+    um += most[i];
+    if (um >= early) atomicMin(&found[0], PER * (int)threadIdx.x + i);
+    if (ul >= late) atomicMin(&found[1], PER * (int)threadIdx.x + i);
+  }
+  __syncthreads();
+}
+
+// counts; where a row has one workgroup, its window too (`n` of the row's work holds, meanwhile, the elements behind the bins)
+template <typename Z>
+__global__ __launch_bounds__(RT) void row_counts_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args, Geometry g,
+                                                        RowWork<Z>* __restrict__ work, int64_t row0) {
+  typedef typename Key<Z>::type K;
+  typedef typename Key<Z>::val_t F;
+  constexpr int N = Chunk<Z>::N;
+  __shared__ uint32_t counts[COUNTS];
+  __shared__ K buf[RW];
+  __shared__ double dbuf[RW];
+  __shared__ int beyond, found[2];
+  RowWork<Z>& w = work[blockIdx.y];
+  const RowArgs a = row_args(args, row0 + blockIdx.y, g.V);
+  if (row_path(a, g) != WINDOW) return;
+  for (int i = threadIdx.x; i < COUNTS; i += RT) counts[i] = 0;
+  if (threadIdx.x == 0) beyond = 0;
+  const RowScale<Z> sc(largest<RW>(w.maxima, g.segs * g.per_seg, buf), a);
+  const F slope = bin_slope<F>(a, g.V);
+  const RowView<Z> row = {logits + (int64_t)blockIdx.y * ld, g.V, g.steps, g.R, (int)(blockIdx.x * RW + (threadIdx.x >> 6)),
+                          (int)(gridDim.x * RW), sc.inf};
+  int behind = 0;
+  walk<Z>(row, [&](F(&v)[N], int) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const F x = (sc.m - v[j]) * slope;
+      const bool in = x < F(COUNTS);
+      if (v[j] >= sc.floor && in) atomicAdd(&counts[(int)x], 1u);
+      behind += v[j] >= sc.floor && !in;
+    }
+  }, NoEnd());
+  behind = wave_sum(behind);
+  if ((threadIdx.x & 63) == 0 && behind) atomicAdd(&beyond, behind);
+  __syncthreads();
+  if (gridDim.x == 1) {
+    find_window(counts, beyond, (double)slope, a, dbuf, found);
+    if (threadIdx.x == 0) w.first = found[0], w.last = found[1] < COUNTS ? found[1] : -1;
+    return;
+  }
+  for (int i = threadIdx.x; i < COUNTS; i += RT)
+    if (counts[i]) atomicAdd(&w.counts[i], counts[i]);
+  if (threadIdx.x == 0 && beyond) atomicAdd(&w.n, beyond);
+}
+
+template <typename Z>
+__global__ __launch_bounds__(RT) void row_window_kernel(SampleArgs args, Geometry g, RowWork<Z>* __restrict__ work, int64_t row0) {
+  typedef typename Key<Z>::val_t F;
+  __shared__ double dbuf[RW];
+  __shared__ int found[2];
+  RowWork<Z>& w = work[blockIdx.x];
+  const RowArgs a = row_args(args, row0 + blockIdx.x, g.V);
+  if (row_path(a, g) != WINDOW) return;
+  find_window(w.counts, w.n, (double)bin_slope<F>(a, g.V), a, dbuf, found);
+  if (threadIdx.x == 0) w.first = found[0], w.last = found[1] < COUNTS ? found[1] : -1, w.n = 0;
+}
+
+template <typename Z>
+__global__ __launch_bounds__(TB) void row_sums_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args, Geometry g,
+                                                      RowWork<Z>* __restrict__ work, int64_t row0) {
+  typedef typename Key<Z>::type K;
+  typedef typename Key<Z>::val_t F;
+  constexpr int N = Chunk<Z>::N;
+  __shared__ K buf[TW];
+  __shared__ double pow2[32];
+  RowWork<Z>& w = work[blockIdx.y];
+  const RowArgs a = row_args(args, row0 + blockIdx.y, g.V);
+  const Path path = row_path(a, g);
+  if (path != PLAIN && path != WINDOW) return;
+  if (path == WINDOW && w.first > w.last) return;
+  if (threadIdx.x < 32) pow2[threadIdx.x] = exp2((double)threadIdx.x / 32.0);
+  const RowScale<Z> sc(largest<TW>(w.maxima, g.segs * g.per_seg, buf), a);      // (its barriers cover pow2)
+  const RowWeight<F> weight(sc.m, a.T, pow2);
+  const RowView<Z> row = {logits + (int64_t)blockIdx.y * ld, g.V, g.steps, g.R, (int)(blockIdx.x * TW + (threadIdx.x >> 6)),
+                          (int)(gridDim.x * TW), sc.inf};
+  double sum = 0;
+  if (path == PLAIN) {
+    walk<Z>(row, [&](F(&v)[N], int) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) sum += weight(v[j], v[j] >= sc.least);
+    }, [&](int s) {
+      sum = wave_sum(sum);
+      if ((threadIdx.x & 63) == 0) w.seg[s] = sum;
+      sum = 0;
+    });
+    return;
+  }
+  const F slope = bin_slope<F>(a, g.V), top = F(w.first), bottom = F(w.last + 1);
+  double above = 0, rest = 0;
+  walk<Z>(row, [&](F(&v)[N], int base) {
+    uint32_t mask = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const F x = (sc.m - v[j]) * slope;
+      const bool is = v[j] >= sc.floor;
+      const double t = weight(v[j], is), c = x < top ? t : 0.0;
+      above += c;
+      rest += t - c;
+      sum += v[j] >= sc.least ? c : 0.0;
+      mask |= (uint32_t)(is && x >= top && x < bottom) << j;
+    }
+    if (__any(mask != 0)) {
+      int at = list_places(&w.n, mask);
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (mask >> j & 1) {
+          if (at < CAP) w.key[at] = Key<Z>::of(v[j]), w.idx[at] = (uint32_t)(base + j);
+          ++at;
+        }
+    }
+  }, [&](int s) {
+    sum = wave_sum(sum);
+    above = wave_sum(above);
+    rest = wave_sum(rest);
+    if ((threadIdx.x & 63) == 0) w.seg[s] = sum, w.above[s] = above, w.rest[s] = rest;
+    sum = above = rest = 0;
+  });
+}
+
+// The row's list, of which LDS holds c <= CAP elements (or all of n2 with the places behind them empty), to the label.
+template <typename Z>
+struct Finish {
+  typedef typename Key<Z>::type K;
+  typedef typename Key<Z>::val_t F;
+  RowShared<Z>& sh;
+  const RowWork<Z>& w;
+  const Geometry& g;
+
+  // top-k, top-p and min-p of a sorted list that holds at least the k first elements; the draw
+  __device__ __forceinline__ int from_list(int c, int n2, const RowArgs& a, const RowScale<Z>& sc, const RowWeight<F>& weight) {
+    const int kk = min(a.k, c);
+    double t[2], total;
+    K k[2];
+    uint32_t n[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int i = 2 * threadIdx.x + e;
-      const bool front = a.P >= 1.0 || i == 0 || (e ? from + w[0] : from) < target;
-      if (i < n2 && !(i < kk && front && w[e] >= a.M)) list_put<Z>(sh, i, 0, 0);
+      k[e] = 0, n[e] = 0;
+      if (i < kk) list_get<Z>(sh, i, k[e], n[e]);
+      t[e] = weight(value_of<Z>(k[e]), i < kk);
+    }
+    const double from = block_scan(t[0] + t[1], sh.wave_d, total) - t[0] - t[1], target = a.P * total;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = 2 * threadIdx.x + e;
+      const bool front = a.P >= 1.0 || i == 0 || (e ? from + t[0] : from) < target;
+      if (i < n2 && !(i < kk && front && value_of<Z>(k[e]) >= sc.least)) list_put<Z>(sh, i, 0, 0);
     }
     list_sort<Z>(sh, n2, true);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int i = 2 * threadIdx.x + e;
-      K k;
-      uint32_t n = 0;
-      w[e] = 0;
-      if (i < n2) list_get<Z>(sh, i, k, n);
-      if (n) w[e] = weight(value_of(k));
+      k[e] = 0, n[e] = 0;
+      if (i < n2) list_get<Z>(sh, i, k[e], n[e]);
+      t[e] = weight(value_of<Z>(k[e]), n[e] != 0);
     }
     if (threadIdx.x == 0) sh.which = CAP, sh.last = -1;
-    const double upto = block_scan(w[0] + w[1], sh.wave_d, total), t = a.u * total;
+    const double upto = block_scan(t[0] + t[1], sh.wave_d, total), at = a.u * total;
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-      if (w[e] > 0) {
+      if (n[e]) {
         const int i = 2 * threadIdx.x + e;
-        if ((e ? upto : upto - w[1]) > t) atomicMin(&sh.which, i);
+        if ((e ? upto : upto - t[1]) > at) atomicMin(&sh.which, i);
         atomicMax(&sh.last, i);
       }
     __syncthreads();
-    K k;
-    uint32_t n;
-    list_get<Z>(sh, sh.which == CAP ? sh.last : sh.which, k, n);
-    pick = (int)~n;
+    list_get<Z>(sh, sh.which == CAP ? sh.last : sh.which, k[0], n[0]);
+    return (int)~n[0];
+  }
+
+  // A list of c <= LONG_CAP elements down to the LDS list: those from the bin on that holds the k-th largest (bins of equal
+  // width over the keys from `lo` to `hi`).  Returns how many, or more than CAP.
+  __device__ __forceinline__ int shorten(int c, int k, K hi) {
+    K lo = hi;
+    for (int i = threadIdx.x; i < c; i += RT) lo = w.key[i] < lo ? w.key[i] : lo;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+      const K o = __shfl_xor(lo, s);
+      lo = o < lo ? o : lo;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.wave_lo[threadIdx.x >> 6] = lo;
+    for (int i = threadIdx.x; i < COUNTS; i += RT) sh.counts[i] = 0;
+    if (threadIdx.x == 0) sh.n = 0, sh.which = COUNTS - 1;
+    __syncthreads();
+    for (int i = 0; i < RW; ++i) lo = sh.wave_lo[i] < lo ? sh.wave_lo[i] : lo;
+    int shift = 0;
+    while (((hi - lo) >> shift) >= (K)COUNTS) ++shift;
+    for (int i = threadIdx.x; i < c; i += RT) atomicAdd(&sh.counts[(int)((hi - w.key[i]) >> shift)], 1u);
+    __syncthreads();
+    constexpr int PER = COUNTS / RT;
+    unsigned long long mine = 0, total;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) mine += sh.counts[PER * threadIdx.x + i];
+    unsigned long long upto = block_scan(mine, sh.wave_u, total) - mine;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      upto += sh.counts[PER * threadIdx.x + i];
+      if (upto >= (unsigned long long)k) atomicMin(&sh.which, PER * (int)threadIdx.x + i);
+    }
+    __syncthreads();
+    const int bin = sh.which;
+    __syncthreads();
+    for (int i = threadIdx.x; i < c; i += RT)
+      if ((int)((hi - w.key[i]) >> shift) <= bin) {
+        const int at = atomicAdd(&sh.n, 1);
+        if (at < CAP) list_put<Z>(sh, at, w.key[i], ~w.idx[i]);
+      }
+    __syncthreads();
+    return sh.n;
+  }
+
+  // The cut of top-p from the window's sorted list of c elements; its kept ones join the sums of their segments.  False: the
+  // border is not in the list.
+  __device__ __forceinline__ bool from_window(int c, int n2, const RowArgs& a, const RowScale<Z>& sc, const RowWeight<F>& weight,
+                                              Cut<F>& cut) {
+    double above, rest;
+    block_scan((int)threadIdx.x < g.segs ? w.above[threadIdx.x] : 0.0, sh.wave_d, above);
+    block_scan((int)threadIdx.x < g.segs ? w.rest[threadIdx.x] : 0.0, sh.wave_d, rest);
+    const double target = a.P * (above + rest);
+    K k[2];
+    uint32_t n[2];
+    double t[2] = {0, 0}, total;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = 2 * threadIdx.x + e;
+      if (i < c) {
+        list_get<Z>(sh, i, k[e], n[e]);
+        t[e] = weight(value_of<Z>(k[e]), true);
+      }
+    }
+    const double from = above + (block_scan(t[0] + t[1], sh.wave_d, total) - t[0] - t[1]);
+    if (above > 0 && !(above < target)) return false;
+    if (!(above + total >= target * (1 - 1e-12))) return false;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {      // the last element with less than the target in front of it
+      const int i = 2 * threadIdx.x + e;
+      const bool in = i < c && (i == 0 || (e ? from + t[0] : from) < target);
+      const bool next = i + 1 < c && (e ? from + t[0] + t[1] : from + t[0]) < target;
+      if (in && !next) sh.cut_key = k[e], sh.cut_idx = (int)~n[e];
+    }
+    __syncthreads();
+    cut = {value_of<Z>(sh.cut_key), sh.cut_idx};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = 2 * threadIdx.x + e;
+      if (i < c && !(cut.keeps(value_of<Z>(k[e]), (int)~n[e]) && value_of<Z>(k[e]) >= sc.least)) list_put<Z>(sh, i, 0, 0);
+    }
+    list_sort<Z>(sh, n2, true);
+    if ((int)threadIdx.x < g.segs) {
+      const int64_t span = (int64_t)g.R * 64 * Chunk<Z>::N, start = threadIdx.x * span;
+      int lo = 0, hi = n2;             // the first list place whose index is at least `start`
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        list_get<Z>(sh, mid, k[0], n[0]);
+        if (n[0] && (int64_t)(uint32_t)~n[0] < start)
+          lo = mid + 1;
+        else
+          hi = mid;
+      }
+      double add = 0;
+      for (; lo < n2; ++lo) {
+        list_get<Z>(sh, lo, k[0], n[0]);
+        if (!n[0] || (int64_t)(uint32_t)~n[0] >= start + span) break;
+        add += weight(value_of<Z>(k[0]), true);
+      }
+      sh.seg[threadIdx.x] += add;
+    }
+    __syncthreads();
     return true;
   }
 };
 
 template <typename Z>
-__global__ __launch_bounds__(RT) void sample_row_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args,
-                                                        int64_t* __restrict__ label, int64_t rows, int V) {
+__global__ __launch_bounds__(RT) void row_finish_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args, Geometry g,
+                                                        RowWork<Z>* __restrict__ work, int64_t* __restrict__ label, int64_t row0) {
   typedef typename Key<Z>::type K;
   typedef typename Key<Z>::val_t F;
   constexpr int N = Chunk<Z>::N;
   __shared__ RowShared<Z> sh;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int steps = (V + 64 * N - 1) / (64 * N);
-  // segments of up to 4 steps where every wave still gets several, more only where there are more than SEGS of them
-  const int R = max((steps + SEGS - 1) / SEGS, max(1, min(4, steps / (4 * RW))));
+  const int64_t i = row0 + blockIdx.x;
+  const RowWork<Z>& w = work[blockIdx.x];
+  const RowArgs a = row_args(args, i, g.V);
+  const Z* p = logits + (int64_t)blockIdx.x * ld;
   if (threadIdx.x < 32) sh.pow2[threadIdx.x] = exp2((double)threadIdx.x / 32.0);
-  for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
-    const RowArgs a = row_args(args, i, V);
-    RowView<Z> row = {logits + i * ld, V, steps, R, false};
-    F mine = -__builtin_inff();
-    int at = V;                                        // the 16 bytes it was first seen in
-    walk<Z>(row, [&](const F(&v)[N], int base) {
-      F t = mine;
-#pragma unroll
-      for (int j = 0; j < N; ++j) t = v[j] > t ? v[j] : t;
-      if (t > mine) mine = t, at = base;
-    }, NoEnd());
-    F m = wave_max(mine);
-    __syncthreads();
-    if (lane == 0) sh.wave_f[wave] = m;
-    if (threadIdx.x == 0) sh.at = V;
-    __syncthreads();
-    for (int j = 0; j < RW; ++j) m = sh.wave_f[j] > m ? sh.wave_f[j] : m;
-    if (!(m > -__builtin_inff()) || !(a.T > 0.0)) {
-      if (mine == m && at < V) {
-        int j = 0;
-        while (Key<Z>::value(row.p[at + j]) != m) ++j;
-        atomicMin(&sh.at, at + j);
-      }
-      __syncthreads();
-      if (threadIdx.x == 0) label[i] = m > -__builtin_inff() ? sh.at : -1;
-      continue;
-    }
-    row.inf = m == __builtin_inff();
-    mine = finite(mine, row.inf);
-    if (row.inf) m = 0;
-    const int S = min(51, 30 + (int)__builtin_clz(V));      // 62 - log2 V, rounded down
-    RowSampler<Z> r = {sh, row, m, RowWeight<F>(m, a.T, sh.pow2), ldexp(1.0, S)};
-    int pick = -1;
-    bool done = false;
-    Cut<F> cut = {-__builtin_inff(), -1};
-    if (a.k) {
-      if (a.k <= RT / 2) {
-        // the k-th largest of the threads' maxima, its upper 16 (64-bit keys: 24) bits
-        const K key = Key<Z>::of(mine);
-        K bound = 0;
-        constexpr int BITS = 8 * (int)sizeof(K), END = BITS - (BITS == 64 ? 24 : 16);
-        int turn = 0;
-        for (int bit = BITS - 1; bit >= END; --bit, turn ^= 1) {
-          const K cand = bound | ((K)1 << bit);
-          const int c = __popcll(__ballot(key >= cand));
-          if (lane == 0) sh.wave_n[turn][wave] = c;
-          __syncthreads();
-          int n = 0;
-#pragma unroll
-          for (int j = 0; j < RW; ++j) n += sh.wave_n[turn][j];
-          if (n >= a.k) bound = cand;
-        }
-        const K none = Key<Z>::of(F(-__builtin_inff()));
-        done = r.from_list(r.value_of(bound > none ? bound : none), a, pick);
-      }
-      if (!done) cut = r.template select<false>(cut, (double)a.k, 1.0);
-    }
-    if (!done) {
-      // what lies further below the maximum than ln(V / (1 - P)) weighs less than 1 - P of the total: no bins for it
-      if (a.P < 1.0) cut = r.template select<true>(cut, a.P, a.T * log((double)V / (1.0 - a.P)));
-      pick = r.draw(cut, a.u, a.M);
-    }
-    if (threadIdx.x == 0) label[i] = pick;
+  const int groups = g.segs * g.per_seg;
+  const K top = largest<RW>(w.maxima, groups, sh.wave_hi);
+  if (!(value_of<Z>(top) > -__builtin_inff())) {
+    if (threadIdx.x == 0) label[i] = -1;
+    return;
   }
+  const Path path = row_path(a, g);
+  const RowScale<Z> sc(top, a);
+  const RowWeight<F> weight(sc.m, a.T, sh.pow2);
+  RowView<Z> row = {p, g.V, g.steps, g.R, 0, 1, sc.inf};
+  Finish<Z> fin = {sh, w, g};
+  int pick = -1;
+  if (path == DONE_BY_MAX) {
+    // the first segment with the maximum, by one wave
+    if (threadIdx.x == 0) sh.which = groups, sh.at = g.V;
+    __syncthreads();
+    for (int j = threadIdx.x; j < groups; j += RT)
+      if (w.maxima[j] == top) atomicMin(&sh.which, j);
+    __syncthreads();
+    const int s = sh.which / g.per_seg;
+    const F m = value_of<Z>(top);
+    row.inf = false;
+    if (threadIdx.x < 64)
+#pragma unroll 1
+      for (int r = 0; r < g.R && s * g.R + r < g.steps; ++r) {
+        Chunk<Z> q;
+        F v[N];
+        load_chunk<Z>(q, row, s * g.R + r);
+        chunk_values<Z>(v, q, row, s * g.R + r);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (v[j] == m) atomicMin(&sh.at, chunk_base(row, s * g.R + r) + j);
+      }
+    __syncthreads();
+    pick = sh.at;
+  } else if (path == LIST) {
+    int c = w.n;
+    if (c > CAP && c <= LONG_CAP)
+      c = fin.shorten(c, a.k, Key<Z>::of(sc.m));
+    else
+      for (int j = threadIdx.x; j < min(c, CAP); j += RT) list_put<Z>(sh, j, w.key[j], ~w.idx[j]);
+    if (c <= CAP) {
+      const int n2 = list_pad<Z>(sh, c);
+      list_sort<Z>(sh, n2, false);
+      pick = fin.from_list(c, n2, a, sc, weight);
+    } else {
+      pick = slow_row<Z>(p, g.V, g.R, top, a.u, a.T, a.P, a.M, a.k);
+    }
+  } else if (path == SLOW) {
+    pick = slow_row<Z>(p, g.V, g.R, top, a.u, a.T, a.P, a.M, a.k);
+  } else {
+    Cut<F> cut = {-__builtin_inff(), -1};
+    bool good = true;
+    sh.seg[threadIdx.x] = (int)threadIdx.x < g.segs ? w.seg[threadIdx.x] : 0.0;
+    if (path == WINDOW) {
+      const int c = w.n;
+      good = w.first <= w.last && c > 0 && c <= CAP;
+      if (good) {
+        for (int j = threadIdx.x; j < c; j += RT) list_put<Z>(sh, j, w.key[j], ~w.idx[j]);
+        const int n2 = list_pad<Z>(sh, c);
+        list_sort<Z>(sh, n2, false);
+        good = fin.from_window(c, n2, a, sc, weight, cut);
+      }
+    }
+    if (good) {
+      RowSampler<Z> r = {sh, row, sc.m, weight, sc.floor};
+      pick = r.draw(cut, sc.least, a.u);
+    } else {
+      pick = slow_row<Z>(p, g.V, g.R, top, a.u, a.T, a.P, a.M, a.k);
+    }
+  }
+  if (threadIdx.x == 0) label[i] = pick;
 }
 
+constexpr int64_t ROW_BATCH = 512;      // rows that share the workspace
+
 template <typename Z>
-int launch(const void* logits, int64_t ld, const SampleArgs& a, int64_t* label, int64_t rows, int V, hipStream_t st) {
-  const Z* z = (const Z*)logits;
-  if (V <= FEW) {
-    if ((rows + 63) / 64 > 0x7FFFFFFF) return TTK_EINVAL;
-    hipLaunchKernelGGL((sample_few_kernel<Z>), dim3((unsigned)((rows + 63) / 64)), dim3(64), 0, st, z, ld, a, label, rows, V);
-  } else if (V <= 1024) {
-    const int64_t groups = (rows + 3) / 4;
-    if (groups > 0x7FFFFFFF) return TTK_EINVAL;
-    const dim3 grid((unsigned)groups);
-    if (V <= 128)
-      hipLaunchKernelGGL((sample_wave_kernel<Z, 2>), grid, dim3(256), 0, st, z, ld, a, label, rows, V);
-    else if (V <= 512)
-      hipLaunchKernelGGL((sample_wave_kernel<Z, 8>), grid, dim3(256), 0, st, z, ld, a, label, rows, V);
-    else
-      hipLaunchKernelGGL((sample_wave_kernel<Z, 16>), grid, dim3(256), 0, st, z, ld, a, label, rows, V);
-  } else {
-    hipLaunchKernelGGL((sample_row_kernel<Z>), dim3((unsigned)min(rows, (int64_t)65536)), dim3(RT), 0, st, z, ld, a, label, rows,
-                       V);
+int launch_rows(const Z* z, int64_t ld, const SampleArgs& a, int64_t* label, int64_t rows, int V, void* ws, int64_t ws_bytes,
+                hipStream_t st) {
+  if (!ws || ws_bytes < min(rows, ROW_BATCH) * (int64_t)sizeof(RowWork<Z>)) return TTK_EWORKSPACE;
+  RowWork<Z>* work = (RowWork<Z>*)ws;
+  const Geometry g = geometry<Z>(V);
+  // what the rows can need (parameters of their own: anything)
+  const bool any_t = a.temperature || a.temperature_all > 0.0, any_k = a.top_k || (a.top_k_all > 0 && a.top_k_all < V);
+  const bool all_k = !a.top_k && any_k, any_p = a.top_p || a.top_p_all < 1.0;
+  for (int64_t r0 = 0; r0 < rows; r0 += ROW_BATCH) {
+    const int64_t n = min(ROW_BATCH, rows - r0);
+    const Z* p = z + r0 * ld;
+    // workgroups a row: enough to fill the machine, each wave with a segment at least
+    const int split = (int)max((int64_t)1, min((int64_t)(g.segs + TW - 1) / TW, (1024 + n - 1) / n));
+    const int wide = (int)max((int64_t)1, min((int64_t)(g.segs + RW - 1) / RW, (256 + n - 1) / n));
+    const dim3 grid((unsigned)split, (unsigned)n), big((unsigned)wide, (unsigned)n);
+    hipLaunchKernelGGL((row_maxima_kernel<Z>), grid, dim3(TB), 0, st, p, ld, g, work);
+    if (any_t && any_k) hipLaunchKernelGGL((row_collect_kernel<Z>), grid, dim3(TB), 0, st, p, ld, a, g, work, r0);
+    if (any_t && !all_k) {
+      if (any_p) {
+        hipLaunchKernelGGL((row_counts_kernel<Z>), big, dim3(RT), 0, st, p, ld, a, g, work, r0);
+        if (wide > 1) hipLaunchKernelGGL((row_window_kernel<Z>), dim3((unsigned)n), dim3(RT), 0, st, a, g, work, r0);
+      }
+      hipLaunchKernelGGL((row_sums_kernel<Z>), grid, dim3(TB), 0, st, p, ld, a, g, work, r0);
+    }
+    hipLaunchKernelGGL((row_finish_kernel<Z>), dim3((unsigned)n), dim3(RT), 0, st, p, ld, a, g, work, label, r0);
   }
+  return hipGetLastError() == hipSuccess ? TTK_OK : TTK_ELAUNCH;
+}
+
+constexpr int WAVE_ROW = 1024;      // rows up to this long: a wave a row, no workspace
+
+template <typename Z>
+int launch(const void* logits, int64_t ld, const SampleArgs& a, int64_t* label, int64_t rows, int V, void* ws, int64_t ws_bytes,
+           hipStream_t st) {
+  const Z* z = (const Z*)logits;
+  if (V > WAVE_ROW) return launch_rows<Z>(z, ld, a, label, rows, V, ws, ws_bytes, st);
+  const int64_t groups = V <= FEW ? (rows + 63) / 64 : (rows + 3) / 4;
+  if (groups > 0x7FFFFFFF) return TTK_EINVAL;
+  const dim3 grid((unsigned)groups);
+  if (V <= FEW)
+    hipLaunchKernelGGL((sample_few_kernel<Z>), grid, dim3(64), 0, st, z, ld, a, label, rows, V);
+  else if (V <= 128)
+    hipLaunchKernelGGL((sample_wave_kernel<Z, 2>), grid, dim3(256), 0, st, z, ld, a, label, rows, V);
+  else if (V <= 512)
+    hipLaunchKernelGGL((sample_wave_kernel<Z, 8>), grid, dim3(256), 0, st, z, ld, a, label, rows, V);
+  else
+    hipLaunchKernelGGL((sample_wave_kernel<Z, 16>), grid, dim3(256), 0, st, z, ld, a, label, rows, V);
   return hipGetLastError() == hipSuccess ? TTK_OK : TTK_ELAUNCH;
 }
 
@@ -1027,17 +1595,23 @@ int launch(const void* logits, int64_t ld, const SampleArgs& a, int64_t* label, 
 
 extern "C" {
 
+int64_t ttk_sample_ws_bytes(int dtype, int64_t rows, int V) {
+  if (dtype < 0 || dtype > 3 || rows < 1 || V < 1 || V > (1 << 30)) return TTK_EINVAL;
+  if (V <= WAVE_ROW) return 0;
+  return min(rows, ROW_BATCH) * (int64_t)(dtype == 0 ? sizeof(RowWork<double>) : sizeof(RowWork<float>));
+}
+
 int ttk_sample(int dtype, const void* logits, int64_t ld, const void* u, int f64, const void* temperature, double temperature_all,
                const int32_t* top_k, int top_k_all, const void* top_p, double top_p_all, const void* min_p, double min_p_all,
-               int64_t* label, int64_t rows, int V, void* stream) {
+               int64_t* label, int64_t rows, int V, void* ws, int64_t ws_bytes, void* stream) {
   if (!logits || !u || !label || rows < 1 || V < 1 || V > (1 << 30) || ld < 0) return TTK_EINVAL;
   const SampleArgs a = {u, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all, top_k_all, f64};
   hipStream_t st = (hipStream_t)stream;
   switch (dtype) {
-    case 0: return launch<double>(logits, ld, a, label, rows, V, st);
-    case 1: return launch<float>(logits, ld, a, label, rows, V, st);
-    case 2: return launch<__bf16>(logits, ld, a, label, rows, V, st);
-    case 3: return launch<_Float16>(logits, ld, a, label, rows, V, st);
+    case 0: return launch<double>(logits, ld, a, label, rows, V, ws, ws_bytes, st);
+    case 1: return launch<float>(logits, ld, a, label, rows, V, ws, ws_bytes, st);
+    case 2: return launch<__bf16>(logits, ld, a, label, rows, V, ws, ws_bytes, st);
+    case 3: return launch<_Float16>(logits, ld, a, label, rows, V, ws, ws_bytes, st);
   }
   return TTK_EINVAL;
 }

@@ -1257,6 +1257,11 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     mp, mv = param(min_p, "min_p", u.dtype, lambda v: 0.0 <= v <= 1.0)
     label = torch.empty(shape, dtype=torch.int64, device=logits.device)
     if rows:
+        if V > 1 << 30:
+            raise _lib.TTKError("logits: more than 2^30 classes")
+        nbytes = int(_lib.lib().ttk_sample_ws_bytes(ROW_TYPES[logits.dtype], rows, V))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
         _launch("ttk_sample", logits.device, ROW_TYPES[logits.dtype], logits.data_ptr(), ld, u.data_ptr(), int(u.dtype == F64), tp,
-                float(t), kp, min(int(k), 0x7FFFFFFF), pp, float(pv), mp, float(mv), label.data_ptr(), rows, V)
+                float(t), kp, min(int(k), 0x7FFFFFFF), pp, float(pv), mp, float(mv), label.data_ptr(), rows, V,
+                ws.data_ptr() if nbytes else None, nbytes)
     return label

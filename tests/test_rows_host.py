@@ -30,7 +30,7 @@ def test_library_refuses_bad_arguments_before_any_launch():
                                                         st=None), **k}.values())
     dr = lambda **k: L.ttk_dropout(*{**dict(dt=1, x=P, y=P, n=4, p=0.5, seed=0, off=0, offd=None, st=None), **k}.values())  # noqa: E731
     sm = lambda **k: L.ttk_sample(*{**dict(dt=1, z=P, ld=4, u=P, f64=0, t=None, ta=1.0, k=None, ka=0, p=None, pa=1.0, m=None,  # noqa: E731
-                                           ma=0.0, out=P, rows=2, V=4, st=None), **k}.values())
+                                           ma=0.0, out=P, rows=2, V=4, ws=None, n=0, st=None), **k}.values())
     nan = float("nan")
     for k in (dict(x=None), dict(y=None), dict(m=None), dict(r=None), dict(rows=0), dict(cols=0), dict(ld=-1), dict(eps=-1.0),
               dict(eps=nan), dict(dt=4), dict(dt=0, wdt=1), dict(dt=1, wdt=2), dict(dt=-1, wdt=-1), dict(p=1.5), dict(p=nan), dict(off=-1)):
@@ -41,8 +41,11 @@ def test_library_refuses_bad_arguments_before_any_launch():
     assert bw(ws=None) == -2 and bw(n=8) == -2
     for k in (dict(x=None), dict(y=None), dict(n=0), dict(dt=7), dict(p=2.0), dict(off=-1)):
         assert dr(**k) == -1, k
-    for k in (dict(z=None), dict(u=None), dict(out=None), dict(rows=0), dict(V=0), dict(ld=-2), dict(dt=9)):
+    for k in (dict(z=None), dict(u=None), dict(out=None), dict(rows=0), dict(V=0), dict(ld=-2), dict(dt=9), dict(V=(1 << 30) + 1)):
         assert sm(**k) == -1, k
+    need = L.ttk_sample_ws_bytes(1, 2, 5000)
+    assert need > 0 and sm(V=5000) == -2 and sm(V=5000, ws=P, n=need - 1) == -2
+    assert L.ttk_sample_ws_bytes(1, 7, 1024) == 0 and L.ttk_sample_ws_bytes(4, 7, 9) == -1 and L.ttk_sample_ws_bytes(1, 0, 9) == -1
     assert L.ttk_layer_norm_backward_ws_bytes(1, 0, 4) == -1 and L.ttk_layer_norm_backward_ws_bytes(9, 4, 4) == -1
     assert L.ttk_layer_norm_backward_ws_bytes(1, 5, 7) >= 2 * 7 * 4
 
