@@ -1285,7 +1285,7 @@ __global__ __launch_bounds__(TB) void row_sums_kernel(const Z* __restrict__ logi
 #pragma unroll
       for (int j = 0; j < N; ++j)
         if (mask >> j & 1) {
-          if (at < CAP) w.key[at] = Key<Z>::of(v[j]), w.idx[at] = (uint32_t)(base + j);
+          if (at < LONG_CAP) w.key[at] = Key<Z>::of(v[j]), w.idx[at] = (uint32_t)(base + j);
           ++at;
         }
     }
@@ -1298,157 +1298,174 @@ __global__ __launch_bounds__(TB) void row_sums_kernel(const Z* __restrict__ logi
   });
 }
 
-// The row's list, of which LDS holds c <= CAP elements (or all of n2 with the places behind them empty), to the label.
+// Cuts of a row from its list of c <= LONG_CAP elements (in the workspace), by the workgroup that finishes the row.
 template <typename Z>
 struct Finish {
   typedef typename Key<Z>::type K;
   typedef typename Key<Z>::val_t F;
   RowShared<Z>& sh;
   const RowWork<Z>& w;
-  const Geometry& g;
+  int c;
+  RowWeight<F> weight;
+  double fixed;                 // 2^S, see `whole`
 
-  // top-k, top-p and min-p of a sorted list that holds at least the k first elements; the draw
-  __device__ __forceinline__ int from_list(int c, int n2, const RowArgs& a, const RowScale<Z>& sc, const RowWeight<F>& weight) {
-    const int kk = min(a.k, c);
-    double t[2], total;
-    K k[2];
-    uint32_t n[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int i = 2 * threadIdx.x + e;
-      k[e] = 0, n[e] = 0;
-      if (i < kk) list_get<Z>(sh, i, k[e], n[e]);
-      t[e] = weight(value_of<Z>(k[e]), i < kk);
-    }
-    const double from = block_scan(t[0] + t[1], sh.wave_d, total) - t[0] - t[1], target = a.P * total;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int i = 2 * threadIdx.x + e;
-      const bool front = a.P >= 1.0 || i == 0 || (e ? from + t[0] : from) < target;
-      if (i < n2 && !(i < kk && front && value_of<Z>(k[e]) >= sc.least)) list_put<Z>(sh, i, 0, 0);
-    }
-    list_sort<Z>(sh, n2, true);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int i = 2 * threadIdx.x + e;
-      k[e] = 0, n[e] = 0;
-      if (i < n2) list_get<Z>(sh, i, k[e], n[e]);
-      t[e] = weight(value_of<Z>(k[e]), n[e] != 0);
-    }
-    if (threadIdx.x == 0) sh.which = CAP, sh.last = -1;
-    const double upto = block_scan(t[0] + t[1], sh.wave_d, total), at = a.u * total;
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      if (n[e]) {
-        const int i = 2 * threadIdx.x + e;
-        if ((e ? upto : upto - t[1]) > at) atomicMin(&sh.which, i);
-        atomicMax(&sh.last, i);
-      }
-    __syncthreads();
-    list_get<Z>(sh, sh.which == CAP ? sh.last : sh.which, k[0], n[0]);
-    return (int)~n[0];
+  // Sums that must not depend on an order are whole numbers: weights times 2^S, rounded; below 2^52 each.
+  __device__ __forceinline__ unsigned long long whole(double x) const {
+    return (unsigned long long)__double_as_longlong(x * fixed + 0x1p52) - 0x4330000000000000ull;
   }
 
-  // A list of c <= LONG_CAP elements down to the LDS list: those from the bin on that holds the k-th largest (bins of equal
-  // width over the keys from `lo` to `hi`).  Returns how many, or more than CAP.
-  __device__ __forceinline__ int shorten(int c, int k, K hi) {
-    K lo = hi;
-    for (int i = threadIdx.x; i < c; i += RT) lo = w.key[i] < lo ? w.key[i] : lo;
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-      const K o = __shfl_xor(lo, s);
-      lo = o < lo ? o : lo;
+  // The cut behind the last element with less than `target` in front of it, of the list's elements that `cut` keeps: in
+  // number, or, MASS, in weight (in units of 2^-S), of which `above0` lies in front of all of them (share: target is a share
+  // of that and theirs).  False where the list does not hold it.
+  template <bool MASS>
+  __device__ __forceinline__ bool list_cut(Cut<F>& cut, double target, bool share, double above0) {
+    unsigned long long above = MASS ? (unsigned long long)(above0 * fixed) : 0ull;
+    K lo = ~(K)0, hi = 0;
+    for (int i = threadIdx.x; i < c; i += RT) {
+      const K k = w.key[i];
+      if (cut.keeps(value_of<Z>(k), (int)w.idx[i])) lo = k < lo ? k : lo, hi = k > hi ? k : hi;
     }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.wave_lo[threadIdx.x >> 6] = lo;
-    for (int i = threadIdx.x; i < COUNTS; i += RT) sh.counts[i] = 0;
-    if (threadIdx.x == 0) sh.n = 0, sh.which = COUNTS - 1;
-    __syncthreads();
-    for (int i = 0; i < RW; ++i) lo = sh.wave_lo[i] < lo ? sh.wave_lo[i] : lo;
-    int shift = 0;
-    while (((hi - lo) >> shift) >= (K)COUNTS) ++shift;
-    for (int i = threadIdx.x; i < c; i += RT) atomicAdd(&sh.counts[(int)((hi - w.key[i]) >> shift)], 1u);
-    __syncthreads();
-    constexpr int PER = COUNTS / RT;
-    unsigned long long mine = 0, total;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) mine += sh.counts[PER * threadIdx.x + i];
-    unsigned long long upto = block_scan(mine, sh.wave_u, total) - mine;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      upto += sh.counts[PER * threadIdx.x + i];
-      if (upto >= (unsigned long long)k) atomicMin(&sh.which, PER * (int)threadIdx.x + i);
-    }
-    __syncthreads();
-    const int bin = sh.which;
-    __syncthreads();
-    for (int i = threadIdx.x; i < c; i += RT)
-      if ((int)((hi - w.key[i]) >> shift) <= bin) {
-        const int at = atomicAdd(&sh.n, 1);
-        if (at < CAP) list_put<Z>(sh, at, w.key[i], ~w.idx[i]);
+    block_range(lo, hi);
+#pragma unroll 1
+    for (;;) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < BINS; i += RT) sh.hist[i] = 0;
+      if (threadIdx.x == 0) sh.which = -1, sh.n = 0;
+      __syncthreads();
+      int shift = 0;
+      while (((hi - lo) >> shift) >= (K)BINS) ++shift;
+      for (int i = threadIdx.x; i < c; i += RT) {
+        const K k = w.key[i];
+        if (k >= lo && k <= hi && cut.keeps(value_of<Z>(k), (int)w.idx[i]))
+          atomicAdd(&sh.hist[(int)((hi - k) >> shift)], MASS ? whole(weight(value_of<Z>(k), true)) : 1ull);
       }
-    __syncthreads();
-    return sh.n;
+      __syncthreads();
+      const unsigned long long v0 = sh.hist[2 * threadIdx.x], v1 = sh.hist[2 * threadIdx.x + 1];
+      unsigned long long total;
+      const unsigned long long upto = above + block_scan(v0 + v1, sh.wave_u, total), from = upto - v0 - v1;
+      if (share) target *= (double)(above + total);
+      share = false;
+      // (the first element is kept whatever lies in front of it)
+      const unsigned long long v[2] = {v0, v1};
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const unsigned long long f = e ? from + v0 : from;
+        if (v[e] && ((double)f < target || f == above) && (double)(f + v[e]) >= target) sh.which = 2 * threadIdx.x + e, sh.above = f;
+      }
+      __syncthreads();
+      const int bin = sh.which;
+      if (bin < 0) return false;
+      const K top = hi - ((K)bin << shift);
+      const K span = ((K)1 << shift) - 1, bottom = top - lo > span ? top - span : lo;
+      above = sh.above;
+      K l = ~(K)0, h = 0;
+      __syncthreads();
+      for (int i = threadIdx.x; i < c; i += RT) {
+        const K k = w.key[i];
+        const uint32_t at = w.idx[i];
+        if (k >= bottom && k <= top && cut.keeps(value_of<Z>(k), (int)at)) {
+          const int place = atomicAdd(&sh.n, 1);
+          if (place < CAP) list_put<Z>(sh, place, k, ~at);
+          l = k < l ? k : l;
+          h = k > h ? k : h;
+        }
+      }
+      block_range(l, h);
+      const int n = sh.n;
+      if (n <= CAP) break;
+      if (l == h) return false;
+      lo = l, hi = h;
+    }
+    const int n = sh.n, n2 = list_pad<Z>(sh, n);
+    list_sort<Z>(sh, n2, false);
+    sorted_cut<MASS>(cut, n, target, above);
+    return true;
   }
 
-  // The cut of top-p from the window's sorted list of c elements; its kept ones join the sums of their segments.  False: the
-  // border is not in the list.
-  __device__ __forceinline__ bool from_window(int c, int n2, const RowArgs& a, const RowScale<Z>& sc, const RowWeight<F>& weight,
-                                              Cut<F>& cut) {
-    double above, rest;
-    block_scan((int)threadIdx.x < g.segs ? w.above[threadIdx.x] : 0.0, sh.wave_d, above);
-    block_scan((int)threadIdx.x < g.segs ? w.rest[threadIdx.x] : 0.0, sh.wave_d, rest);
-    const double target = a.P * (above + rest);
-    K k[2];
-    uint32_t n[2];
-    double t[2] = {0, 0}, total;
+  // the same for the n elements of the sorted LDS list
+  template <bool MASS>
+  __device__ __forceinline__ void sorted_cut(Cut<F>& cut, int n, double target, unsigned long long above) {
+    K key[2];
+    uint32_t nidx[2];
+    unsigned long long q[2] = {0, 0}, sum;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int i = 2 * threadIdx.x + e;
-      if (i < c) {
-        list_get<Z>(sh, i, k[e], n[e]);
-        t[e] = weight(value_of<Z>(k[e]), true);
+      if (i < n) {
+        list_get<Z>(sh, i, key[e], nidx[e]);
+        q[e] = MASS ? whole(weight(value_of<Z>(key[e]), true)) : 1ull;
       }
     }
-    const double from = above + (block_scan(t[0] + t[1], sh.wave_d, total) - t[0] - t[1]);
-    if (above > 0 && !(above < target)) return false;
-    if (!(above + total >= target * (1 - 1e-12))) return false;
+    unsigned long long before = above + block_scan(q[0] + q[1], sh.wave_u, sum) - q[0] - q[1];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {      // the last element with less than the target in front of it
+    for (int e = 0; e < 2; ++e) {
       const int i = 2 * threadIdx.x + e;
-      const bool in = i < c && (i == 0 || (e ? from + t[0] : from) < target);
-      const bool next = i + 1 < c && (e ? from + t[0] + t[1] : from + t[0]) < target;
-      if (in && !next) sh.cut_key = k[e], sh.cut_idx = (int)~n[e];
+      if (i < n && ((double)before < target || i == 0) && (i == n - 1 || (double)(before + q[e]) >= target))
+        sh.cut_key = key[e], sh.cut_idx = (int)~nidx[e];
+      before += q[e];
     }
     __syncthreads();
     cut = {value_of<Z>(sh.cut_key), sh.cut_idx};
+    __syncthreads();
+  }
+
+  __device__ __forceinline__ void block_range(K& lo, K& hi) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int i = 2 * threadIdx.x + e;
-      if (i < c && !(cut.keeps(value_of<Z>(k[e]), (int)~n[e]) && value_of<Z>(k[e]) >= sc.least)) list_put<Z>(sh, i, 0, 0);
-    }
-    list_sort<Z>(sh, n2, true);
-    if ((int)threadIdx.x < g.segs) {
-      const int64_t span = (int64_t)g.R * 64 * Chunk<Z>::N, start = threadIdx.x * span;
-      int lo = 0, hi = n2;             // the first list place whose index is at least `start`
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        list_get<Z>(sh, mid, k[0], n[0]);
-        if (n[0] && (int64_t)(uint32_t)~n[0] < start)
-          lo = mid + 1;
-        else
-          hi = mid;
-      }
-      double add = 0;
-      for (; lo < n2; ++lo) {
-        list_get<Z>(sh, lo, k[0], n[0]);
-        if (!n[0] || (int64_t)(uint32_t)~n[0] >= start + span) break;
-        add += weight(value_of<Z>(k[0]), true);
-      }
-      sh.seg[threadIdx.x] += add;
+    for (int s = 1; s < 64; s <<= 1) {
+      const K a = __shfl_xor(lo, s), b = __shfl_xor(hi, s);
+      lo = a < lo ? a : lo;
+      hi = b > hi ? b : hi;
     }
     __syncthreads();
-    return true;
+    if ((threadIdx.x & 63) == 0) sh.wave_lo[threadIdx.x >> 6] = lo, sh.wave_hi[threadIdx.x >> 6] = hi;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < RW; ++i) {
+      lo = sh.wave_lo[i] < lo ? sh.wave_lo[i] : lo;
+      hi = sh.wave_hi[i] > hi ? sh.wave_hi[i] : hi;
+    }
+  }
+
+  // top-k and top-p of a list that holds the k first elements
+  __device__ __forceinline__ bool top_cut(Cut<F>& cut, const RowArgs& a) {
+    if (c <= 256) {            // few enough to sort at once
+      for (int i = threadIdx.x; i < c; i += RT) list_put<Z>(sh, i, w.key[i], ~w.idx[i]);
+      list_sort<Z>(sh, list_pad<Z>(sh, c), false);
+      const int kk = min(a.k, c);
+      if (a.P < 1.0) {
+        const int i = 2 * threadIdx.x;
+        double t = 0;
+        unsigned long long sum;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          K k = 0;
+          uint32_t n;
+          if (i + e < kk) list_get<Z>(sh, i + e, k, n);
+          t += i + e < kk ? (double)whole(weight(value_of<Z>(k), true)) : 0.0;
+        }
+        block_scan((unsigned long long)t, sh.wave_u, sum);
+        sorted_cut<true>(cut, kk, a.P * (double)sum, 0);
+      } else {
+        sorted_cut<false>(cut, kk, (double)kk, 0);
+      }
+      return true;
+    }
+    if (c > a.k && !list_cut<false>(cut, (double)a.k, false, 0)) return false;
+    return !(a.P < 1.0) || list_cut<true>(cut, a.P, true, 0);
+  }
+
+  // the list's elements that `cut` keeps and that are not below `least` join their segments' sums
+  __device__ __forceinline__ void join_segments(const Cut<F>& cut, F least, int span) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < SEGS; i += RT) sh.hist[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < c; i += RT) {
+      const F v = value_of<Z>(w.key[i]);
+      const uint32_t at = w.idx[i];
+      if (v >= least && cut.keeps(v, (int)at)) atomicAdd(&sh.hist[at / (uint32_t)span], whole(weight(v, true)));
+    }
+    __syncthreads();
+    sh.seg[threadIdx.x] += (double)sh.hist[threadIdx.x] / fixed;
   }
 };
 
@@ -1472,9 +1489,7 @@ __global__ __launch_bounds__(RT) void row_finish_kernel(const Z* __restrict__ lo
   }
   const Path path = row_path(a, g);
   const RowScale<Z> sc(top, a);
-  const RowWeight<F> weight(sc.m, a.T, sh.pow2);
   RowView<Z> row = {p, g.V, g.steps, g.R, 0, 1, sc.inf};
-  Finish<Z> fin = {sh, w, g};
   int pick = -1;
   if (path == DONE_BY_MAX) {
     // the first segment with the maximum, by one wave
@@ -1499,36 +1514,25 @@ __global__ __launch_bounds__(RT) void row_finish_kernel(const Z* __restrict__ lo
       }
     __syncthreads();
     pick = sh.at;
-  } else if (path == LIST) {
-    int c = w.n;
-    if (c > CAP && c <= LONG_CAP)
-      c = fin.shorten(c, a.k, Key<Z>::of(sc.m));
-    else
-      for (int j = threadIdx.x; j < min(c, CAP); j += RT) list_put<Z>(sh, j, w.key[j], ~w.idx[j]);
-    if (c <= CAP) {
-      const int n2 = list_pad<Z>(sh, c);
-      list_sort<Z>(sh, n2, false);
-      pick = fin.from_list(c, n2, a, sc, weight);
-    } else {
-      pick = slow_row<Z>(p, g.V, g.R, top, a.u, a.T, a.P, a.M, a.k);
-    }
-  } else if (path == SLOW) {
-    pick = slow_row<Z>(p, g.V, g.R, top, a.u, a.T, a.P, a.M, a.k);
   } else {
+    const RowWeight<F> weight(sc.m, a.T, sh.pow2);
+    // S: the sum of V weights stays below 2^63
+    Finish<Z> fin = {sh, w, w.n, weight, ldexp(1.0, min(51, 30 + (int)__builtin_clz(g.V)))};
     Cut<F> cut = {-__builtin_inff(), -1};
-    bool good = true;
-    sh.seg[threadIdx.x] = (int)threadIdx.x < g.segs ? w.seg[threadIdx.x] : 0.0;
-    if (path == WINDOW) {
-      const int c = w.n;
-      good = w.first <= w.last && c > 0 && c <= CAP;
-      if (good) {
-        for (int j = threadIdx.x; j < c; j += RT) list_put<Z>(sh, j, w.key[j], ~w.idx[j]);
-        const int n2 = list_pad<Z>(sh, c);
-        list_sort<Z>(sh, n2, false);
-        good = fin.from_window(c, n2, a, sc, weight, cut);
-      }
+    const bool listed = fin.c > 0 && fin.c <= LONG_CAP;
+    bool good = path == PLAIN;
+    sh.seg[threadIdx.x] = (path == PLAIN || path == WINDOW) && (int)threadIdx.x < g.segs ? w.seg[threadIdx.x] : 0.0;
+    if (path == LIST) {
+      good = listed && fin.top_cut(cut, a);
+    } else if (path == WINDOW && listed && w.first <= w.last) {
+      double above, rest;
+      block_scan((int)threadIdx.x < g.segs ? w.above[threadIdx.x] : 0.0, sh.wave_d, above);
+      block_scan((int)threadIdx.x < g.segs ? w.rest[threadIdx.x] : 0.0, sh.wave_d, rest);
+      // (rest holds the window's elements, which list_cut counts by itself)
+      good = fin.template list_cut<true>(cut, a.P * (above + rest) * fin.fixed, false, above);
     }
     if (good) {
+      if (path != PLAIN) fin.join_segments(cut, sc.least, g.R * 64 * N);
       RowSampler<Z> r = {sh, row, sc.m, weight, sc.floor};
       pick = r.draw(cut, sc.least, a.u);
     } else {
