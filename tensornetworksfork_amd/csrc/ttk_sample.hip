@@ -361,9 +361,10 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const Z* __restrict__ 
 //   maxima    the largest logit of each of up to 1024 groups of a row's elements (their largest is m; the k-th largest bounds
 //             the k-th largest element from below)
 //   collect   top-k: the elements at or above that bound, a few more than k, into the row's list
-//   counts    top-p: how many elements lie in each of 4096 bins below m.  A bin's weight is known to the width of a bin from
-//             its count, so the cumulative weight is bounded from both sides, and
-//   window    the border of top-p lies in a narrow window of bins
+//   counts    top-p: the number of elements in each of 4096 bins below m and the sum of their places within the bin.  The
+//             bin's weight follows to second order in its width (relative 1e-5), so the cumulative weight is bounded from both
+//             sides, and
+//   window    the border of top-p lies in a window of a few bins
 //   sums      every weight once: float64 sums of the kept ones per segment of the row, and of the rest; the window's elements
 //             go into the row's list
 //   finish    a workgroup a row: sorts the list in LDS, cuts it, and draws from it or from the segment sums
@@ -462,7 +463,6 @@ struct RowShared {
   typedef typename Key<Z>::val_t F;
   union {
     unsigned long long hist[BINS];
-    uint32_t counts[COUNTS];
     struct {
       uint64_t key[CAP];                                     // 32-bit keys: key << 32 | ~index
       uint32_t nidx[sizeof(K) == 8 ? CAP : 1];               // 64-bit keys: ~index
@@ -1005,7 +1005,7 @@ Geometry geometry(int V) {
   while (g.per_seg * g.segs > GROUPS) g.per_seg /= 2;
   // k of n groups' maxima bound the k-th largest by an element with about -n ln(1 - k / n) above it
   const int groups = g.per_seg * g.segs;
-  g.most = V <= LONG_CAP ? V : groups - groups / 32;
+  g.most = V <= LONG_CAP ? V : groups - groups / 128;
   return g;
 }
 
@@ -1014,7 +1014,7 @@ template <typename Z>
 struct RowWork {
   typedef typename Key<Z>::type K;
   K maxima[GROUPS];
-  uint32_t counts[COUNTS];
+  unsigned long long counts[COUNTS];              // number << 33 + sum of the places within the bin
   double seg[SEGS], above[SEGS], rest[SEGS];      // kept for certain; those before min-p; the others
   K key[LONG_CAP];
   uint32_t idx[LONG_CAP];
@@ -1140,33 +1140,37 @@ __global__ __launch_bounds__(TB) void row_collect_kernel(const Z* __restrict__ l
   }, NoEnd());
 }
 
-// Bins over what can matter of a row cut by top-p: what lies further below the maximum than ln(V / (1 - P)) weighs less than
-// 1 - P of the total.
+// Bins over what matters of a row cut by top-p: what lies further below the maximum than ln(V / (1 - P)) weighs less than
+// 1 - P of the total, and five units more make what lies behind the bins weigh nothing against a bin.
 template <typename F>
 __device__ __forceinline__ F bin_slope(const RowArgs& a, int V) {
-  return (F)fmin((double)COUNTS / (a.T * log((double)V / (1.0 - a.P))), 1e38);
+  return (F)fmin((double)COUNTS / (a.T * (log((double)V / (1.0 - a.P)) + 5.0)), 1e38);
 }
+// Places within a bin are counted in units of 2^-place_bits: V of them stay below 2^33.
+__device__ __forceinline__ int place_bits(int V) { return min(10, 1 + (int)__builtin_clz(V)); }
 
-// The bins the border of top-p must lie in, from the counts (`all` elements at or above the floor): a bin's weight lies
-// between its count times the weights of its edges, moved out by a hundredth of a bin for the roundings of the bin number.
-__device__ __forceinline__ void find_window(const uint32_t* counts, int beyond, double slope, const RowArgs& a, double* buf,
-                                            int* found) {
+// The bins the border of top-p must lie in.  With step = width of a bin in units of T, an element at place f of bin b weighs
+// e^(-(b + f) step), and e^(-y) lies between 1 - y and 1 - y + y^2 / 2; places are known to their unit and to the roundings of
+// the bin number (below 4096 2^-22 of a bin).
+__device__ __forceinline__ void find_window(const unsigned long long* counts, int beyond, double slope, const RowArgs& a, int V,
+                                            double* buf, int* found) {
   constexpr int PER = COUNTS / RT;
-  const double step = 1.0 / (slope * a.T);
+  const double step = 1.0 / (slope * a.T), unit = ldexp(1.0, -place_bits(V));
   double least[PER], most[PER], sl = 0, sm = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int bin = PER * threadIdx.x + i;
-    const double n = (double)counts[bin];
-    least[i] = n * exp(-((double)bin + 1.01) * step);
-    most[i] = n * exp(-((double)bin - 0.01) * step);
+    const double n = (double)(counts[bin] >> 33), f = (double)(counts[bin] & 0x1FFFFFFFFull) * unit;
+    const double low = fmax(f - 0.001 * n, 0.0), high = f + (unit + 0.001) * n, e = exp(-(double)bin * step);
+    least[i] = e * fmax(n - step * high, 0.0);
+    most[i] = e * (n - step * low + 0.5 * step * step * high);
     sl += least[i];
     sm += most[i];
   }
   double total_least, total_most;
   double ul = block_scan(sl, buf, total_least) - sl;
   double um = block_scan(sm, buf, total_most) - sm;
-  total_most += (double)beyond * exp(-((double)COUNTS - 0.01) * step);
+  total_most += (double)beyond * exp(-((double)COUNTS - 0.001) * step);
   __syncthreads();
   if (threadIdx.x == 0) found[0] = COUNTS, found[1] = COUNTS;
   __syncthreads();
@@ -1188,7 +1192,7 @@ __global__ __launch_bounds__(RT) void row_counts_kernel(const Z* __restrict__ lo
   typedef typename Key<Z>::type K;
   typedef typename Key<Z>::val_t F;
   constexpr int N = Chunk<Z>::N;
-  __shared__ uint32_t counts[COUNTS];
+  __shared__ unsigned long long counts[COUNTS];
   __shared__ K buf[RW];
   __shared__ double dbuf[RW];
   __shared__ int beyond, found[2];
@@ -1198,7 +1202,7 @@ __global__ __launch_bounds__(RT) void row_counts_kernel(const Z* __restrict__ lo
   for (int i = threadIdx.x; i < COUNTS; i += RT) counts[i] = 0;
   if (threadIdx.x == 0) beyond = 0;
   const RowScale<Z> sc(largest<RW>(w.maxima, g.segs * g.per_seg, buf), a);
-  const F slope = bin_slope<F>(a, g.V);
+  const F slope = bin_slope<F>(a, g.V), units = (F)(1 << place_bits(g.V));
   const RowView<Z> row = {logits + (int64_t)blockIdx.y * ld, g.V, g.steps, g.R, (int)(blockIdx.x * RW + (threadIdx.x >> 6)),
                           (int)(gridDim.x * RW), sc.inf};
   int behind = 0;
@@ -1207,7 +1211,9 @@ __global__ __launch_bounds__(RT) void row_counts_kernel(const Z* __restrict__ lo
     for (int j = 0; j < N; ++j) {
       const F x = (sc.m - v[j]) * slope;
       const bool in = x < F(COUNTS);
-      if (v[j] >= sc.floor && in) atomicAdd(&counts[(int)x], 1u);
+      const int bin = (int)x;
+      const uint32_t place = (uint32_t)((x - (F)bin) * units);
+      if (v[j] >= sc.floor && in) atomicAdd(&counts[bin], (1ull << 33) + place);
       behind += v[j] >= sc.floor && !in;
     }
   }, NoEnd());
@@ -1215,7 +1221,7 @@ __global__ __launch_bounds__(RT) void row_counts_kernel(const Z* __restrict__ lo
   if ((threadIdx.x & 63) == 0 && behind) atomicAdd(&beyond, behind);
   __syncthreads();
   if (gridDim.x == 1) {
-    find_window(counts, beyond, (double)slope, a, dbuf, found);
+    find_window(counts, beyond, (double)slope, a, g.V, dbuf, found);
     if (threadIdx.x == 0) w.first = found[0], w.last = found[1] < COUNTS ? found[1] : -1;
     return;
   }
@@ -1232,7 +1238,7 @@ __global__ __launch_bounds__(RT) void row_window_kernel(SampleArgs args, Geometr
   RowWork<Z>& w = work[blockIdx.x];
   const RowArgs a = row_args(args, row0 + blockIdx.x, g.V);
   if (row_path(a, g) != WINDOW) return;
-  find_window(w.counts, w.n, (double)bin_slope<F>(a, g.V), a, dbuf, found);
+  find_window(w.counts, w.n, (double)bin_slope<F>(a, g.V), a, g.V, dbuf, found);
   if (threadIdx.x == 0) w.first = found[0], w.last = found[1] < COUNTS ? found[1] : -1, w.n = 0;
 }
 
