@@ -471,7 +471,7 @@ struct RowShared {
   };
   double seg[SEGS];
   double pow2[32];
-  double wave_d[RW];
+  double wave_d[RW], seg_before;
   unsigned long long wave_u[RW];
   K wave_lo[RW], wave_hi[RW];
   int n, at, which, last;
@@ -912,56 +912,60 @@ struct RowSampler {
 
   // the place, by index, where the running sum of the kept weights passes u times the total (sh.seg holds their sums)
   __device__ __forceinline__ int draw(const Cut<F>& cut, F least, double u) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (threadIdx.x == 0) sh.which = SEGS, sh.last = -1;
     const double mine = sh.seg[threadIdx.x];
     double total;
     const double upto = block_scan(mine, sh.wave_d, total), target = u * total;
-    if (mine > 0) {
-      if (upto > target) atomicMin(&sh.which, (int)threadIdx.x);
-      atomicMax(&sh.last, (int)threadIdx.x);
-    }
+    const uint64_t over = __ballot(mine > 0 && upto > target), any = __ballot(mine > 0);
+    if (over && lane == (int)__builtin_ctzll(over)) atomicMin(&sh.which, (int)threadIdx.x);
+    if (any && lane == 63 - (int)__builtin_clzll(any)) atomicMax(&sh.last, (int)threadIdx.x);
     __syncthreads();
     const bool last = sh.which == SEGS;                 // u >= 1, or rounded up to it: the last kept element
     const int s = last ? sh.last : sh.which;
-    if ((int)threadIdx.x == s) sh.wave_d[0] = upto - mine;
+    if ((int)threadIdx.x == s) sh.seg_before = upto - mine;
+    if (threadIdx.x == 0) sh.at = -1, sh.n = -1;        // the answer; the last kept element so far
     __syncthreads();
-    if (threadIdx.x < 64) {
-      const int lane = threadIdx.x;
-      const Limit<F> limit(cut, least > floor ? least : floor);
-      double before = sh.wave_d[0];
-      int pick = -1, end = -1;                          // end: the last kept element so far
+    double before = sh.seg_before;
+    const Limit<F> limit(cut, least > floor ? least : floor);
 #pragma unroll 1
-      for (int r = 0; r < row.R && s * row.R + r < row.steps && pick < 0; ++r) {
-        const int base = chunk_base(row, s * row.R + r);
+    for (int r0 = 0; r0 < row.R; r0 += RW) {            // a step a wave
+      const int r = r0 + wave, step = s * row.R + r;
+      const bool in = r < row.R && step < row.steps;
+      const int base = in ? chunk_base(row, step) : 0;
+      double w[N], t = 0;
+      int end = -1;
+      if (in) {
         Chunk<Z> q;
         F v[N];
-        load_chunk<Z>(q, row, s * row.R + r);
-        chunk_values<Z>(v, q, row, s * row.R + r);
+        load_chunk<Z>(q, row, step);
+        chunk_values<Z>(v, q, row, step);
         const F lim = limit.template of<N>(v, base);
-        double w[N], t = 0;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
           w[j] = weight(v[j], v[j] >= lim);
           if (w[j] > 0) end = base + j;
           t += w[j];
         }
-        const double upto = before + wave_scan(t);
-        const uint64_t who = last ? 0 : __ballot(t > 0 && upto > target);
-        if (who) {
-          const int at = (int)__builtin_ctzll(who);
-          double c = upto - t;
-#pragma unroll
-          for (int j = 0; j < N; ++j)
-            if (w[j] > 0 && !(pick >= 0 && c > target)) c += w[j], pick = base + j;
-          pick = from_lane(pick, at);
-        }
-        before = from_lane(upto, 63);
       }
-      end = wave_max(end);
-      if (lane == 0) sh.at = pick >= 0 ? pick : end;
+      double all;
+      const double upto = before + block_scan(t, sh.wave_d, all);
+      const uint64_t who = last ? 0 : __ballot(t > 0 && upto > target);
+      if (who && lane == (int)__builtin_ctzll(who)) {
+        double c = upto - t;
+        int pick = -1;
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (w[j] > 0 && !(pick >= 0 && c > target)) c += w[j], pick = base + j;
+        atomicMin((unsigned int*)&sh.at, (unsigned int)pick);      // (-1 is the largest)
+      }
+      const uint64_t some = __ballot(end >= 0);
+      if (some && lane == 63 - (int)__builtin_clzll(some)) atomicMax(&sh.n, end);
+      __syncthreads();
+      if (sh.at >= 0) break;
+      before += all;
     }
-    __syncthreads();
-    return sh.at;
+    return sh.at >= 0 ? sh.at : sh.n;
   }
 };
 
@@ -999,7 +1003,7 @@ Geometry geometry(int V) {
   Geometry g;
   g.V = V;
   g.steps = (int)(((int64_t)V + 64 * N - 1) / (64 * N));
-  g.R = (g.steps + SEGS - 1) / SEGS;
+  g.R = max((g.steps + SEGS - 1) / SEGS, max(1, min(4, g.steps / 64)));
   g.segs = (g.steps + g.R - 1) / g.R;
   g.per_seg = 64;
   while (g.per_seg * g.segs > GROUPS) g.per_seg /= 2;
@@ -1088,7 +1092,7 @@ __global__ __launch_bounds__(TB) void row_collect_kernel(const Z* __restrict__ l
   typedef typename Key<Z>::val_t F;
   constexpr int N = Chunk<Z>::N;
   __shared__ K buf[TW];
-  __shared__ int counts[2][TW];
+  __shared__ uint64_t counts[2][TW];
   RowWork<Z>& w = work[blockIdx.y];
   const RowArgs a = row_args(args, row0 + blockIdx.y, g.V);
   if (row_path(a, g) != LIST) return;
@@ -1107,17 +1111,21 @@ __global__ __launch_bounds__(TB) void row_collect_kernel(const Z* __restrict__ l
     constexpr int BITS = 8 * (int)sizeof(K), END = BITS - (BITS == 64 ? 24 : 16);
     int turn = 0;
 #pragma unroll 1
-    for (int bit = BITS - 1; bit >= END; --bit, turn ^= 1) {
-      const K cand = bound | ((K)1 << bit);
-      int c = 0;
+    for (int bit = BITS - 2; bit >= END; bit -= 2, turn ^= 1) {      // two bits at a time
+      uint32_t c[3] = {0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < GROUPS / TB; ++i) c += __popcll(__ballot(key[i] >= cand));
-      if ((threadIdx.x & 63) == 0) counts[turn][threadIdx.x >> 6] = c;
+      for (int i = 0; i < GROUPS / TB; ++i)
+#pragma unroll
+        for (int j = 0; j < 3; ++j) c[j] += __popcll(__ballot(key[i] >= (bound | (K)(j + 1) << bit)));
+      if ((threadIdx.x & 63) == 0) counts[turn][threadIdx.x >> 6] = c[0] | (uint64_t)c[1] << 20 | (uint64_t)c[2] << 40;
       __syncthreads();
-      c = 0;
+      uint64_t all = 0;
 #pragma unroll
-      for (int i = 0; i < TW; ++i) c += counts[turn][i];
-      if (c >= a.k) bound = cand;
+      for (int i = 0; i < TW; ++i) all += counts[turn][i];
+      K digit = 0;
+#pragma unroll
+      for (int j = 0; j < 3; ++j) digit += (int)(all >> (20 * j) & 0xFFFFF) >= a.k;
+      bound |= digit << bit;
     }
   }
   const K lowest = Key<Z>::of(sc.floor);
@@ -1177,10 +1185,10 @@ __device__ __forceinline__ void find_window(const unsigned long long* counts, in
   const double early = a.P * total_least * (1 - 1e-9), late = a.P * total_most * (1 + 1e-9);
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
+    if (um < early && um + most[i] >= early) atomicMin(&found[0], PER * (int)threadIdx.x + i);
+    if (ul < late && ul + least[i] >= late) atomicMin(&found[1], PER * (int)threadIdx.x + i);
     ul += least[i];
     um += most[i];
-    if (um >= early) atomicMin(&found[0], PER * (int)threadIdx.x + i);
-    if (ul >= late) atomicMin(&found[1], PER * (int)threadIdx.x + i);
   }
   __syncthreads();
 }
@@ -1192,7 +1200,7 @@ __global__ __launch_bounds__(RT) void row_counts_kernel(const Z* __restrict__ lo
   typedef typename Key<Z>::type K;
   typedef typename Key<Z>::val_t F;
   constexpr int N = Chunk<Z>::N;
-  __shared__ unsigned long long counts[COUNTS];
+  __shared__ unsigned long long counts[COUNTS + 64];      // the last 64: elements that are not counted
   __shared__ K buf[RW];
   __shared__ double dbuf[RW];
   __shared__ int beyond, found[2];
@@ -1206,16 +1214,21 @@ __global__ __launch_bounds__(RT) void row_counts_kernel(const Z* __restrict__ lo
   const RowView<Z> row = {logits + (int64_t)blockIdx.y * ld, g.V, g.steps, g.R, (int)(blockIdx.x * RW + (threadIdx.x >> 6)),
                           (int)(gridDim.x * RW), sc.inf};
   int behind = 0;
+  const int none = COUNTS + (int)(threadIdx.x & 63);
   walk<Z>(row, [&](F(&v)[N], int) {
+    int bin[N];
+    uint32_t place[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const F x = (sc.m - v[j]) * slope;
-      const bool in = x < F(COUNTS);
-      const int bin = (int)x;
-      const uint32_t place = (uint32_t)((x - (F)bin) * units);
-      if (v[j] >= sc.floor && in) atomicAdd(&counts[bin], (1ull << 33) + place);
-      behind += v[j] >= sc.floor && !in;
+      const bool in = x < F(COUNTS), is = v[j] >= sc.floor;
+      const int b = (int)x;
+      place[j] = (uint32_t)((x - (F)b) * units);
+      bin[j] = in && is ? b : none;
+      behind += is && !in;
     }
+#pragma unroll
+    for (int j = 0; j < N; ++j) atomicAdd(&counts[bin[j]], (1ull << 33) | place[j]);
   }, NoEnd());
   behind = wave_sum(behind);
   if ((threadIdx.x & 63) == 0 && behind) atomicAdd(&beyond, behind);
@@ -1476,7 +1489,7 @@ struct Finish {
 };
 
 template <typename Z>
-__global__ __launch_bounds__(RT) void row_finish_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args, Geometry g,
+__global__ __launch_bounds__(RT, 8) void row_finish_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args, Geometry g,
                                                         RowWork<Z>* __restrict__ work, int64_t* __restrict__ label, int64_t row0) {
   typedef typename Key<Z>::type K;
   typedef typename Key<Z>::val_t F;
