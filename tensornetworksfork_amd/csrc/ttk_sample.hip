@@ -367,15 +367,19 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const Z* __restrict__ 
 //   window    the border of top-p lies in a window of a few bins
 //   sums      every weight once: float64 sums of the kept ones per segment of the row, and of the rest; the window's elements
 //             go into the row's list
-//   finish    a workgroup a row: sorts the list in LDS, cuts it, and draws from it or from the segment sums
-// Rows whose list does not hold what it should (top-k above what the groups bound, thousands of equal logits) are done by
-// `slow_row`: cuts by histograms over the whole row, refined until the bin with the border fits the list.
+//   finish    a workgroup a row: the cut, by histograms of the list refined until the bin with the border can be sorted in LDS;
+//             what the cut keeps of the list joins the segment sums; the segment where their running sum passes u times the
+//             total, and the element in it
+//   slow      the rows whose list does not hold what it should (top-k above what the groups bound, thousands of equal
+//             logits): the same cuts by histograms over the whole row
 //
 // Elements of -inf do not exist for any of this, nor do weights below 2^-1000 of the largest; min-p is a bound on the value,
 // m + T ln(min_p).  Sums are added in a fixed order, counts are whole numbers, lists are sorted: the label does not depend on
 // the order in which workgroups run.
 // ---------------------------------------------------------------------------------------
-constexpr int RT = 1024, RW = RT / 64, BINS = 2048, COUNTS = 4096, CAP = 2048, SEGS = 1024, GROUPS = 1024, LONG_CAP = 8192;
+constexpr int BINS = 2048, COUNTS = 4096, SEGS = 1024, GROUPS = 1024, LIST_CAP = 8192;
+constexpr int TB = 256, TW = TB / 64;      // threads and waves of the passes and of `finish`
+constexpr int RT = 1024, RW = RT / 64;     // of `counts`, `window` and `slow`
 
 template <typename Z>
 struct Chunk {
@@ -426,8 +430,8 @@ __device__ __forceinline__ void chunk_values(typename Key<Z>::val_t (&v)[Chunk<Z
     for (int j = 0; j < N; ++j) v[j] = finite(v[j], true);
 }
 
-// Calls f(values, first index) for every 16 bytes of the row and end(segment) after a wave's last step of a segment.  The
-// next three steps are under way while one is worked on.
+// Calls f(values, first index) for every 16 bytes of the wave's part of the row and end(segment) after its last step of a
+// segment.  The next three steps are under way while one is worked on.
 template <typename Z, typename Fn, typename End>
 __device__ __forceinline__ void walk(const RowView<Z>& row, Fn f, End end) {
   constexpr int N = Chunk<Z>::N;
@@ -457,10 +461,11 @@ struct NoEnd {
   __device__ __forceinline__ void operator()(int) const {}
 };
 
-template <typename Z>
+// LDS of a workgroup of T threads that cuts a row and draws from it.
+template <typename Z, int T>
 struct RowShared {
   typedef typename Key<Z>::type K;
-  typedef typename Key<Z>::val_t F;
+  static constexpr int CAP = 2 * T;
   union {
     unsigned long long hist[BINS];
     struct {
@@ -471,14 +476,18 @@ struct RowShared {
   };
   double seg[SEGS];
   double pow2[32];
-  double wave_d[RW], seg_before;
-  unsigned long long wave_u[RW];
-  K wave_lo[RW], wave_hi[RW];
+  double wave_d[T / 64], seg_before;
+  unsigned long long wave_u[T / 64];
+  K wave_lo[T / 64], wave_hi[T / 64];
   int n, at, which, last;
   unsigned long long above;
   K cut_key;
   int cut_idx;
 };
+
+__device__ __forceinline__ void fill_pow2(double* pow2) {
+  if (threadIdx.x < 32) pow2[threadIdx.x] = exp2((double)threadIdx.x / 32.0);
+}
 
 // The weight of Weight, with 2^(n / 32) from a table: 2^((z - m) log2(e) / T) = 2^(n div 32) pow2[n mod 32] 2^(f / 32),
 // |f| <= 1/2, the last factor by its Taylor polynomial (relative error below 3e-15).  The 32 doubles lie in 64 different
@@ -505,78 +514,106 @@ struct RowWeight {
   }
 };
 
-template <typename T>
-__device__ __forceinline__ T block_scan(T v, T* buf, T& total) {      // inclusive; buf: RW values
+// Weights as whole numbers of 2^-S: sums that do not depend on an order.  S = 62 - log2 V, at most 51: the sum of V of them
+// stays below 2^63.
+struct Whole {
+  double fixed;      // 2^S
+  __device__ __forceinline__ explicit Whole(int V) : fixed(ldexp(1.0, min(51, 30 + (int)__builtin_clz(V)))) {}
+  __device__ __forceinline__ unsigned long long operator()(double w) const {      // w <= 1, rounded
+    return (unsigned long long)__double_as_longlong(w * fixed + 0x1p52) - 0x4330000000000000ull;
+  }
+};
+
+template <int T, typename A>
+__device__ __forceinline__ A block_scan(A v, A* buf, A& total) {      // inclusive; buf: T / 64 values
   const int wave = threadIdx.x >> 6;
   v = wave_scan(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 63) buf[wave] = v;
   __syncthreads();
-  T before = 0;
+  A before = 0;
   total = 0;
 #pragma unroll
-  for (int i = 0; i < RW; ++i) {
+  for (int i = 0; i < T / 64; ++i) {
     if (i < wave) before += buf[i];
     total += buf[i];
   }
   return v + before;
 }
 
-// an element of the list: what comes first sorts higher
-template <typename Z>
-__device__ __forceinline__ void list_put(RowShared<Z>& sh, int i, typename Key<Z>::type key, uint32_t nidx) {
-  if constexpr (sizeof(key) == 4) {
-    sh.list.key[i] = (uint64_t)key << 32 | nidx;
-  } else {
-    sh.list.key[i] = key;
-    sh.list.nidx[i] = nidx;
+template <int T, typename K>
+__device__ __forceinline__ void block_range(K& lo, K& hi, K* buf_lo, K* buf_hi) {
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const K a = __shfl_xor(lo, s), b = __shfl_xor(hi, s);
+    lo = a < lo ? a : lo;
+    hi = b > hi ? b : hi;
   }
-}
-template <typename Z>
-__device__ __forceinline__ void list_get(const RowShared<Z>& sh, int i, typename Key<Z>::type& key, uint32_t& nidx) {
-  if constexpr (sizeof(key) == 4) {
-    key = (uint32_t)(sh.list.key[i] >> 32);
-    nidx = (uint32_t)sh.list.key[i];
-  } else {
-    key = sh.list.key[i];
-    nidx = sh.list.nidx[i];
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) buf_lo[threadIdx.x >> 6] = lo, buf_hi[threadIdx.x >> 6] = hi;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < T / 64; ++i) {
+    lo = buf_lo[i] < lo ? buf_lo[i] : lo;
+    hi = buf_hi[i] > hi ? buf_hi[i] : hi;
   }
 }
 
-// Bitonic sort of the first n2 (a power of two, at least 128) elements, highest first: by (key, ~index), or by ~index
-// alone.  Wave w holds elements 128 w + lane and 128 w + 64 + lane in registers; distances up to 64 are exchanged there,
-// longer ones through LDS.
+// ---- the LDS list: at most 2 T elements; what comes first sorts higher -------------------------------------------
+
 template <typename Z>
 struct Item {
   typedef typename Key<Z>::type K;
   K k;
-  uint32_t n;
+  uint32_t n;        // ~index
 };
 template <typename Z>
-__device__ __forceinline__ bool in_front(const Item<Z>& a, const Item<Z>& b, bool by_index) {
-  if constexpr (sizeof(a.k) == 4) {
-    const uint64_t x = by_index ? a.n : (uint64_t)a.k << 32 | a.n, y = by_index ? b.n : (uint64_t)b.k << 32 | b.n;
-    return x > y;
+__device__ __forceinline__ bool in_front(const Item<Z>& a, const Item<Z>& b) {
+  if constexpr (sizeof(a.k) == 4)
+    return ((uint64_t)a.k << 32 | a.n) > ((uint64_t)b.k << 32 | b.n);
+  else
+    return a.k > b.k || (a.k == b.k && a.n > b.n);
+}
+template <typename Z, int T>
+__device__ __forceinline__ void list_put(RowShared<Z, T>& sh, int i, const Item<Z>& e) {
+  if constexpr (sizeof(e.k) == 4) {
+    sh.list.key[i] = (uint64_t)e.k << 32 | e.n;
   } else {
-    return by_index ? a.n > b.n : a.k > b.k || (a.k == b.k && a.n > b.n);
+    sh.list.key[i] = e.k;
+    sh.list.nidx[i] = e.n;
   }
 }
-template <typename Z>
-__device__ __forceinline__ void list_sort(RowShared<Z>& sh, int n2, bool by_index) {
+template <typename Z, int T>
+__device__ __forceinline__ Item<Z> list_get(const RowShared<Z, T>& sh, int i) {
+  if constexpr (sizeof(typename Key<Z>::type) == 4)
+    return {(uint32_t)(sh.list.key[i] >> 32), (uint32_t)sh.list.key[i]};
+  else
+    return {sh.list.key[i], sh.list.nidx[i]};
+}
+
+// Bitonic sort of the first n elements (n <= 2 T), the first in front.  Wave w holds elements 128 w + lane and 128 w + 64 +
+// lane in registers; distances up to 64 are exchanged there, longer ones through LDS.
+template <typename Z, int T>
+__device__ __forceinline__ void list_sort(RowShared<Z, T>& sh, int n) {
+  int n2 = 128;
+  while (n2 < n) n2 <<= 1;
   const int lane = threadIdx.x & 63, i0 = (threadIdx.x >> 6) * 128 + lane;
   const bool mine = i0 - lane < n2;      // (the same in a wave)
   Item<Z> e[2];
   __syncthreads();
-  if (mine) {
-    list_get<Z>(sh, i0, e[0].k, e[0].n);
-    list_get<Z>(sh, i0 + 64, e[1].k, e[1].n);
-  }
+  if (mine)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const Item<Z> none = {0, 0};       // sorts last
+      e[h] = i0 + 64 * h < n ? list_get<Z, T>(sh, i0 + 64 * h) : none;
+    }
 #pragma unroll 1
   for (int size = 2; size <= n2; size <<= 1) {
     if (size > 128) {
+      __syncthreads();
       if (mine) {
-        list_put<Z>(sh, i0, e[0].k, e[0].n);
-        list_put<Z>(sh, i0 + 64, e[1].k, e[1].n);
+        list_put<Z, T>(sh, i0, e[0]);
+        list_put<Z, T>(sh, i0 + 64, e[1]);
       }
 #pragma unroll 1
       for (int d = size >> 1; d > 64; d >>= 1) {
@@ -584,24 +621,22 @@ __device__ __forceinline__ void list_sort(RowShared<Z>& sh, int n2, bool by_inde
         const int t = threadIdx.x;
         if (t < n2 / 2) {
           const int i = 2 * t - (t & (d - 1)), j = i + d;
-          Item<Z> a, b;
-          list_get<Z>(sh, i, a.k, a.n);
-          list_get<Z>(sh, j, b.k, b.n);
-          if ((i & size) ? in_front<Z>(a, b, by_index) : in_front<Z>(b, a, by_index)) {
-            list_put<Z>(sh, i, b.k, b.n);
-            list_put<Z>(sh, j, a.k, a.n);
+          const Item<Z> a = list_get<Z, T>(sh, i), b = list_get<Z, T>(sh, j);
+          if ((i & size) ? in_front<Z>(a, b) : in_front<Z>(b, a)) {
+            list_put<Z, T>(sh, i, b);
+            list_put<Z, T>(sh, j, a);
           }
         }
       }
       __syncthreads();
       if (mine) {
-        list_get<Z>(sh, i0, e[0].k, e[0].n);
-        list_get<Z>(sh, i0 + 64, e[1].k, e[1].n);
+        e[0] = list_get<Z, T>(sh, i0);
+        e[1] = list_get<Z, T>(sh, i0 + 64);
       }
     }
     if (mine) {
       if (size >= 128) {
-        const bool swap = (i0 & size) ? in_front<Z>(e[0], e[1], by_index) : in_front<Z>(e[1], e[0], by_index);
+        const bool swap = (i0 & size) ? in_front<Z>(e[0], e[1]) : in_front<Z>(e[1], e[0]);
         const Item<Z> x = e[0];
         e[0] = swap ? e[1] : e[0];
         e[1] = swap ? x : e[1];
@@ -615,119 +650,37 @@ __device__ __forceinline__ void list_sort(RowShared<Z>& sh, int n2, bool by_inde
           o.k = __shfl_xor(e[h].k, d);
           o.n = __shfl_xor(e[h].n, d);
           const bool first = ((i & d) == 0) == ((i & size) == 0);      // takes the one in front
-          if (first ? in_front<Z>(o, e[h], by_index) : in_front<Z>(e[h], o, by_index)) e[h] = o;
+          if (first ? in_front<Z>(o, e[h]) : in_front<Z>(e[h], o)) e[h] = o;
         }
       }
     }
   }
+  __syncthreads();
   if (mine) {
-    list_put<Z>(sh, i0, e[0].k, e[0].n);
-    list_put<Z>(sh, i0 + 64, e[1].k, e[1].n);
+    list_put<Z, T>(sh, i0, e[0]);
+    list_put<Z, T>(sh, i0 + 64, e[1]);
   }
   __syncthreads();
 }
 
-// Collects the elements `in` accepts into the list (the first CAP that come) and returns how many there are; lo / hi: the
-// smallest and the largest of their keys.
-template <typename Z, typename In>
-__device__ int list_collect(RowShared<Z>& sh, const RowView<Z>& row, In in, typename Key<Z>::type& lo, typename Key<Z>::type& hi) {
-  typedef typename Key<Z>::type K;
-  typedef typename Key<Z>::val_t F;
-  constexpr int N = Chunk<Z>::N;
-  __syncthreads();
-  if (threadIdx.x == 0) sh.n = 0;
-  __syncthreads();
-  K l = ~(K)0, h = 0;
-  walk<Z>(row, [&](F(&v)[N], int base) {
-    uint32_t mask = 0;
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (in(v[j], base + j)) mask |= 1u << j;
-    if (mask) {
-      int at = atomicAdd(&sh.n, __popc(mask));
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (mask >> j & 1) {
-          const K k = Key<Z>::of(v[j]);
-          l = k < l ? k : l;
-          h = k > h ? k : h;
-          if (at < CAP) list_put<Z>(sh, at, k, ~(uint32_t)(base + j));
-          ++at;
-        }
-    }
-  }, NoEnd());
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const K a = __shfl_xor(l, s), b = __shfl_xor(h, s);
-    l = a < l ? a : l;
-    h = b > h ? b : h;
-  }
-  if ((threadIdx.x & 63) == 0) sh.wave_lo[threadIdx.x >> 6] = l, sh.wave_hi[threadIdx.x >> 6] = h;
-  __syncthreads();
-  lo = sh.wave_lo[0], hi = sh.wave_hi[0];
-  for (int i = 1; i < RW; ++i) {
-    lo = sh.wave_lo[i] < lo ? sh.wave_lo[i] : lo;
-    hi = sh.wave_hi[i] > hi ? sh.wave_hi[i] : hi;
-  }
-  return sh.n;
-}
-
-// pads the list of c elements to a power of two with entries that sort last and returns it
-template <typename Z>
-__device__ int list_pad(RowShared<Z>& sh, int c) {
-  int n2 = 128;
-  while (n2 < c) n2 <<= 1;
-  for (int i = c + threadIdx.x; i < n2; i += RT) list_put<Z>(sh, i, 0, 0);
-  return n2;
-}
+// ---- cuts ---------------------------------------------------------------------------------------------------------
 
 template <typename F>
 __device__ __forceinline__ F next_up(F v) {      // v not NaN, not +inf
   if constexpr (sizeof(F) == 4) {
-    const uint32_t b = __float_as_uint(v + 0.0f);
+    const uint32_t b = __float_as_uint(v);
     return v == 0 ? __uint_as_float(1u) : __uint_as_float(b >> 31 ? b - 1 : b + 1);
   } else {
-    const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
     return v == 0 ? __longlong_as_double(1) : __longlong_as_double((int64_t)(b >> 63 ? b - 1 : b + 1));
   }
 }
 template <typename F>
-__device__ __forceinline__ F round_up(double x) {      // the smallest F not below x, finite
+__device__ __forceinline__ F round_up(double x) {      // the smallest finite F not below x
   F f = (F)x;
-  if ((double)f < x) f = next_up(f);
+  if ((double)f < x || f == -__builtin_inff()) f = next_up(f);
   return f;
 }
-
-// What is kept: the elements that do not come behind (v, idx) in the order, and are not below `floor`.
-template <typename F>
-struct Cut {
-  F v;
-  int idx;
-  __device__ __forceinline__ bool keeps(F z, int i) const { return z > v || (z == v && i <= idx); }
-};
-
-// The same as one comparison an element: z is kept iff z >= the limit of its 16 bytes, but for those the index splits.
-template <typename F>
-struct Limit {
-  F with, without;      // limits where elements that equal v are kept, and where they are not
-  int idx;
-  __device__ __forceinline__ Limit(const Cut<F>& c, F floor) : idx(c.idx) {
-    const F up = next_up(c.v);
-    with = c.idx < 0 || c.v < floor ? (up > floor ? up : floor) : c.v;
-    without = up > floor ? up : floor;
-  }
-  template <int N>
-  __device__ __forceinline__ F of(F (&z)[N], int base) const {
-    const bool split = base <= idx && base + N - 1 > idx;
-    if (__any(split)) {
-      if (split)
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-          if (base + j > idx && z[j] < without) z[j] = -__builtin_inff();
-    }
-    return base > idx ? without : with;
-  }
-};
 
 template <typename Z>
 __device__ __forceinline__ typename Key<Z>::val_t value_of(typename Key<Z>::type k) {
@@ -754,16 +707,695 @@ struct RowScale {
   }
 };
 
-template <typename Z>
+// What is kept: the elements that do not come behind (v, idx) in the order.
+template <typename F>
+struct Cut {
+  F v;
+  int idx;
+  __device__ __forceinline__ bool keeps(F z, int i) const { return z > v || (z == v && i <= idx); }
+};
+
+// The same, of elements not below `floor`, as one comparison an element: z is kept iff z >= the limit of its 16 bytes, but
+// for the 16 bytes that the index splits.
+template <typename F>
+struct Limit {
+  F with, without;      // limits where elements that equal v are kept, and where they are not
+  int idx;
+  __device__ __forceinline__ Limit(const Cut<F>& c, F floor) : idx(c.idx) {
+    const F up = next_up(c.v);
+    without = up > floor ? up : floor;
+    with = c.idx < 0 || c.v < floor ? without : c.v;
+  }
+  template <int N>
+  __device__ __forceinline__ F of(F (&z)[N], int base) const {
+    const bool split = base <= idx && base + N - 1 > idx;
+    if (__any(split)) {
+      if (split)
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (base + j > idx && z[j] < without) z[j] = -__builtin_inff();
+    }
+    return base > idx ? without : with;
+  }
+};
+
+// ---- one row by one workgroup of T threads ------------------------------------------------------------------------
+
+template <typename Z, int T>
 struct RowSampler {
   typedef typename Key<Z>::type K;
   typedef typename Key<Z>::val_t F;
-  static constexpr int N = Chunk<Z>::N;
-  RowShared<Z>& sh;
+  static constexpr int N = Chunk<Z>::N, CAP = RowShared<Z, T>::CAP, PB = BINS / T, PS = SEGS / T;
+  RowShared<Z, T>& sh;
   RowView<Z> row;
-  F m;
+  RowScale<Z> sc;
   RowWeight<F> weight;
-  F floor;
+  Whole whole;
+
+  // The bin (of the histogram in LDS) where the running sum, which starts at `above`, first reaches the target (or, share, the
+  // target times the sum of all), and in sh.above what lies in front of it; -1 if there is none.
+  __device__ __forceinline__ int border_bin(unsigned long long above, double& target, bool share) {
+    unsigned long long v[PB], mine = 0, total;
+#pragma unroll
+    for (int e = 0; e < PB; ++e) v[e] = sh.hist[PB * threadIdx.x + e], mine += v[e];
+    if (threadIdx.x == 0) sh.which = -1;
+    unsigned long long from = above + block_scan<T>(mine, sh.wave_u, total) - mine;
+    if (share) target *= (double)(above + total);
+#pragma unroll
+    for (int e = 0; e < PB; ++e) {
+      // (the very first element is kept whatever the target)
+      if (v[e] && ((double)from < target || from == above) && (double)(from + v[e]) >= target)
+        sh.which = PB * threadIdx.x + e, sh.above = from;
+      from += v[e];
+    }
+    __syncthreads();
+    return sh.which;
+  }
+
+  // The cut behind the last of the n sorted elements of the LDS list with less than the target in front of it.
+  template <bool MASS>
+  __device__ __forceinline__ Cut<F> sorted_cut(int n, double target, unsigned long long above) {
+    Item<Z> e[2];
+    unsigned long long q[2] = {0, 0}, sum;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (2 * (int)threadIdx.x + h < n) {
+        e[h] = list_get<Z, T>(sh, 2 * threadIdx.x + h);
+        q[h] = MASS ? whole(weight(value_of<Z>(e[h].k), true)) : 1ull;
+      }
+    unsigned long long before = above + block_scan<T>(q[0] + q[1], sh.wave_u, sum) - q[0] - q[1];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = 2 * threadIdx.x + h;
+      if (i < n && ((double)before < target || i == 0) && (i == n - 1 || (double)(before + q[h]) >= target))
+        sh.cut_key = e[h].k, sh.cut_idx = (int)~e[h].n;
+      before += q[h];
+    }
+    __syncthreads();
+    const Cut<F> cut = {value_of<Z>(sh.cut_key), sh.cut_idx};
+    __syncthreads();
+    return cut;
+  }
+
+  // The place, by index, where the running sum of the kept weights passes u times the total; sh.seg holds their sums.
+  __device__ __forceinline__ int draw(const Cut<F>& cut, double u) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __syncthreads();
+    double v[PS], mine = 0, total;
+#pragma unroll
+    for (int e = 0; e < PS; ++e) v[e] = sh.seg[PS * threadIdx.x + e], mine += v[e];
+    if (threadIdx.x == 0) sh.which = SEGS, sh.last = -1, sh.at = -1, sh.n = -1;
+    const double from = block_scan<T>(mine, sh.wave_d, total) - mine, target = u * total;
+    double upto = from;
+    int first = SEGS, last = -1;
+#pragma unroll
+    for (int e = 0; e < PS; ++e) {
+      upto += v[e];
+      if (v[e] > 0) {
+        if (upto > target) first = min(first, PS * (int)threadIdx.x + e);
+        last = PS * threadIdx.x + e;
+      }
+    }
+    const uint64_t over = __ballot(first < SEGS), any = __ballot(last >= 0);
+    if (over && lane == (int)__builtin_ctzll(over)) atomicMin(&sh.which, first);
+    if (any && lane == 63 - (int)__builtin_clzll(any)) atomicMax(&sh.last, last);
+    __syncthreads();
+    const bool to_end = sh.which == SEGS;               // u >= 1, or rounded up to it: the last kept element
+    const int s = to_end ? sh.last : sh.which;
+    if ((int)threadIdx.x == s / PS) {
+      upto = from;
+#pragma unroll
+      for (int e = 0; e < PS; ++e)
+        if (e < s % PS) upto += v[e];
+      sh.seg_before = upto;
+    }
+    __syncthreads();
+    double before = sh.seg_before;
+    const Limit<F> limit(cut, sc.least);
+#pragma unroll 1
+    for (int r0 = 0; r0 < row.R; r0 += T / 64) {        // a step a wave
+      const int r = r0 + wave, step = s * row.R + r;
+      const bool in = r < row.R && step < row.steps;
+      const int base = in ? chunk_base(row, step) : 0;
+      double w[N], t = 0, all;
+      int end = -1;                                     // the last kept element so far
+      if (in) {
+        Chunk<Z> q;
+        F z[N];
+        load_chunk<Z>(q, row, step);
+        chunk_values<Z>(z, q, row, step);
+        const F lim = limit.template of<N>(z, base);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          w[j] = weight(z[j], z[j] >= lim);
+          if (w[j] > 0) end = base + j;
+          t += w[j];
+        }
+      }
+      const double upto = before + block_scan<T>(t, sh.wave_d, all);
+      const uint64_t who = to_end ? 0 : __ballot(t > 0 && upto > target);
+      if (who && lane == (int)__builtin_ctzll(who)) {
+        double c = upto - t;
+        int pick = -1;
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (w[j] > 0 && !(pick >= 0 && c > target)) c += w[j], pick = base + j;
+        atomicMin((unsigned int*)&sh.at, (unsigned int)pick);      // (-1 is the largest)
+      }
+      const uint64_t some = __ballot(end >= 0);
+      if (some && lane == 63 - (int)__builtin_clzll(some)) atomicMax(&sh.n, end);
+      __syncthreads();
+      if (sh.at >= 0) break;
+      before += all;
+    }
+    return sh.at >= 0 ? sh.at : sh.n;
+  }
+};
+
+// ---- launches -----------------------------------------------------------------------------------------------------
+
+struct Geometry {
+  int V, steps, R, segs, per_seg;      // per_seg: groups a segment (a power of two)
+  int most;                            // top-k up to this many is taken from the list
+};
+
+template <typename Z>
+Geometry geometry(int V, int64_t rows) {
+  constexpr int N = Chunk<Z>::N;
+  Geometry g;
+  g.V = V;
+  g.steps = (int)(((int64_t)V + 64 * N - 1) / (64 * N));
+  // segments of up to 4 steps where the machine has work enough without shorter ones
+  g.R = max((g.steps + SEGS - 1) / SEGS, rows * g.steps >= 16384 ? max(1, min(4, g.steps / 64)) : 1);
+  g.segs = (g.steps + g.R - 1) / g.R;
+  g.per_seg = 64;
+  while (g.per_seg * g.segs > GROUPS) g.per_seg /= 2;
+  // the k-th largest of n groups' maxima has about -n ln(1 - k / n) elements at or above it
+  const int groups = g.per_seg * g.segs;
+  g.most = V <= LIST_CAP ? V : groups - groups / 128;
+  return g;
+}
+
+// A row's part of the workspace.
+template <typename Z>
+struct RowWork {
+  typedef typename Key<Z>::type K;
+  K maxima[GROUPS];
+  unsigned long long counts[COUNTS];              // number << 33 + sum of the places within the bin
+  double seg[SEGS], above[SEGS], total[SEGS];     // what is kept for certain; that before min-p; all
+  K key[LIST_CAP];
+  uint32_t idx[LIST_CAP];
+  int n;                                          // elements that asked for a place in the list
+  int first, last;                                // window: bins; first > last: none was found
+};
+
+enum Path { BY_MAX, LIST, WINDOW, PLAIN, SLOW };
+
+__device__ __forceinline__ Path row_path(const RowArgs& a, const Geometry& g) {
+  if (!(a.T > 0.0)) return BY_MAX;
+  if (a.k) return a.k <= g.most ? LIST : SLOW;
+  return a.P < 1.0 ? WINDOW : PLAIN;
+}
+
+// the part of a row that wave number `wave` of `waves` owns
+template <typename Z>
+__device__ __forceinline__ RowView<Z> row_part(const Z* p, const Geometry& g, int wave, int waves, bool inf) {
+  return {p, g.V, g.steps, g.R, wave, waves, inf};
+}
+
+// the largest key of the groups' maxima, in every thread of a workgroup of T threads
+template <int T, typename K>
+__device__ __forceinline__ K largest(const K* maxima, int n, K* buf) {
+  K m = 0;
+#pragma unroll
+  for (int i = 0; i < GROUPS / T; ++i) {
+    const int at = i * T + threadIdx.x;
+    const K k = at < n ? maxima[at] : (K)0;
+    m = k > m ? k : m;
+  }
+  m = wave_max(m);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = buf[0];
+#pragma unroll
+  for (int i = 1; i < T / 64; ++i) m = buf[i] > m ? buf[i] : m;
+  return m;
+}
+
+template <typename Z>
+__global__ __launch_bounds__(TB) void row_maxima_kernel(const Z* __restrict__ logits, int64_t ld, Geometry g,
+                                                        RowWork<Z>* __restrict__ work) {
+  typedef typename Key<Z>::val_t F;
+  constexpr int N = Chunk<Z>::N;
+  RowWork<Z>& w = work[blockIdx.y];
+  const int lane = threadIdx.x & 63, wide = 64 / g.per_seg;
+  if (blockIdx.x == 0 && threadIdx.x == 0) w.n = 0, w.first = 1, w.last = 0;
+  for (int i = blockIdx.x * TB + threadIdx.x; i < COUNTS; i += gridDim.x * TB) w.counts[i] = 0;
+  F mine = -__builtin_inff();
+  walk<Z>(row_part(logits + (int64_t)blockIdx.y * ld, g, blockIdx.x * TW + (threadIdx.x >> 6), gridDim.x * TW, false),
+          [&](F(&v)[N], int) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) mine = v[j] > mine ? v[j] : mine;
+          },
+          [&](int s) {
+            for (int d = 1; d < wide; d <<= 1) {
+              const F o = __shfl_xor(mine, d);
+              mine = o > mine ? o : mine;
+            }
+            if (lane % wide == 0) w.maxima[s * g.per_seg + lane / wide] = Key<Z>::of(mine);
+            mine = -__builtin_inff();
+          });
+}
+
+// Puts the `mask`ed elements of the wave's 16-byte pieces into the row's list.
+template <typename Z, int N>
+__device__ __forceinline__ void list_add(RowWork<Z>& w, const typename Key<Z>::val_t (&v)[N], int base, uint32_t mask) {
+  const int c = __popc(mask), upto = wave_scan(c), all = from_lane(upto, 63);
+  int at = 0;
+  if ((threadIdx.x & 63) == 0) at = atomicAdd(&w.n, all);
+  at = from_lane(at, 0) + upto - c;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (mask >> j & 1) {
+      if (at < LIST_CAP) w.key[at] = Key<Z>::of(v[j]), w.idx[at] = (uint32_t)(base + j);
+      ++at;
+    }
+}
+
+template <typename Z>
+__global__ __launch_bounds__(TB) void row_collect_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args, Geometry g,
+                                                         RowWork<Z>* __restrict__ work, int64_t row0) {
+  typedef typename Key<Z>::type K;
+  typedef typename Key<Z>::val_t F;
+  constexpr int N = Chunk<Z>::N;
+  __shared__ K buf[TW];
+  __shared__ uint64_t counts[2][TW];
+  RowWork<Z>& w = work[blockIdx.y];
+  const RowArgs a = row_args(args, row0 + blockIdx.y, g.V);
+  if (row_path(a, g) != LIST) return;
+  const int groups = g.segs * g.per_seg;
+  const RowScale<Z> sc(largest<TB>(w.maxima, groups, buf), a);
+  K bound = 0;
+  if (a.k <= groups) {      // the k-th largest of the maxima, its upper 16 (64-bit keys: 24) bits, two at a time
+    K key[GROUPS / TB];
+#pragma unroll
+    for (int i = 0; i < GROUPS / TB; ++i) {
+      const int at = i * TB + threadIdx.x;
+      key[i] = at < groups ? w.maxima[at] : (K)0;
+      if (sc.inf) key[i] = Key<Z>::of(finite(value_of<Z>(key[i]), true));
+    }
+    constexpr int BITS = 8 * (int)sizeof(K), END = BITS - (BITS == 64 ? 24 : 16);
+    int turn = 0;
+#pragma unroll 1
+    for (int bit = BITS - 2; bit >= END; bit -= 2, turn ^= 1) {
+      uint32_t c[3] = {0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < GROUPS / TB; ++i)
+#pragma unroll
+        for (int j = 0; j < 3; ++j) c[j] += __popcll(__ballot(key[i] >= (bound | (K)(j + 1) << bit)));
+      if ((threadIdx.x & 63) == 0) counts[turn][threadIdx.x >> 6] = c[0] | (uint64_t)c[1] << 20 | (uint64_t)c[2] << 40;
+      __syncthreads();
+      uint64_t all = 0;
+#pragma unroll
+      for (int i = 0; i < TW; ++i) all += counts[turn][i];
+      K digit = 0;
+#pragma unroll
+      for (int j = 0; j < 3; ++j) digit += (int)(all >> (20 * j) & 0xFFFFF) >= a.k;
+      bound |= digit << bit;
+    }
+  }
+  const F lim = bound > Key<Z>::of(sc.floor) ? value_of<Z>(bound) : sc.floor;
+  walk<Z>(row_part(logits + (int64_t)blockIdx.y * ld, g, blockIdx.x * TW + (threadIdx.x >> 6), gridDim.x * TW, sc.inf),
+          [&](F(&v)[N], int base) {
+            uint32_t mask = 0;
+#pragma unroll
+            for (int j = 0; j < N; ++j) mask |= (uint32_t)(v[j] >= lim) << j;
+            if (__any(mask != 0)) list_add<Z, N>(w, v, base, mask);
+          },
+          NoEnd());
+}
+
+// Bins over what matters of a row cut by top-p: what lies further below the maximum than ln(V / (1 - P)) weighs less than
+// 1 - P of the total, and five units more make what lies behind the bins weigh nothing against a bin.
+template <typename F>
+__device__ __forceinline__ F bin_slope(const RowArgs& a, int V) {
+  return (F)fmin((double)COUNTS / (a.T * (log((double)V / (1.0 - a.P)) + 5.0)), 1e38);
+}
+// Places within a bin are counted in units of 2^-place_bits: V of them stay below 2^33.
+__device__ __forceinline__ int place_bits(int V) { return min(10, 1 + (int)__builtin_clz(V)); }
+
+// The bins the border of top-p must lie in.  With step = width of a bin in units of T, an element at place f of bin b weighs
+// e^(-(b + f) step), and e^(-y) lies between 1 - y and 1 - y + y^2 / 2; places are known to their unit and to the roundings of
+// the bin number (below 4096 2^-22 of a bin).
+__device__ __forceinline__ void find_window(const unsigned long long* counts, int beyond, double slope, const RowArgs& a, int V,
+                                            double* buf, int* found) {
+  constexpr int PER = COUNTS / RT;
+  const double step = 1.0 / (slope * a.T), unit = ldexp(1.0, -place_bits(V));
+  double least[PER], most[PER], sl = 0, sm = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int bin = PER * threadIdx.x + i;
+    const double n = (double)(counts[bin] >> 33), f = (double)(counts[bin] & 0x1FFFFFFFFull) * unit;
+    const double low = fmax(f - 0.001 * n, 0.0), high = f + (unit + 0.001) * n, e = exp(-(double)bin * step);
+    least[i] = e * fmax(n - step * high, 0.0);
+    most[i] = e * (n - step * low + 0.5 * step * step * high);
+    sl += least[i];
+    sm += most[i];
+  }
+  double total_least, total_most;
+  double ul = block_scan<RT>(sl, buf, total_least) - sl;
+  double um = block_scan<RT>(sm, buf, total_most) - sm;
+  total_most += (double)beyond * exp(-((double)COUNTS - 0.001) * step);
+  if (threadIdx.x == 0) found[0] = found[1] = COUNTS;
+  __syncthreads();
+  const double early = a.P * total_least * (1 - 1e-9), late = a.P * total_most * (1 + 1e-9);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (um < early && um + most[i] >= early) atomicMin(&found[0], PER * (int)threadIdx.x + i);
+    if (ul < late && ul + least[i] >= late) atomicMin(&found[1], PER * (int)threadIdx.x + i);
+    ul += least[i];
+    um += most[i];
+  }
+  __syncthreads();
+}
+
+// counts; where a row has one workgroup, its window too (`n` of the row's work holds, meanwhile, the elements behind the bins)
+template <typename Z>
+__global__ __launch_bounds__(RT) void row_counts_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args, Geometry g,
+                                                        RowWork<Z>* __restrict__ work, int64_t row0) {
+  typedef typename Key<Z>::type K;
+  typedef typename Key<Z>::val_t F;
+  constexpr int N = Chunk<Z>::N;
+  __shared__ unsigned long long counts[COUNTS + 64];      // the last 64: elements that are not counted
+  __shared__ K buf[RW];
+  __shared__ double dbuf[RW];
+  __shared__ int beyond, found[2];
+  RowWork<Z>& w = work[blockIdx.y];
+  const RowArgs a = row_args(args, row0 + blockIdx.y, g.V);
+  if (row_path(a, g) != WINDOW) return;
+  for (int i = threadIdx.x; i < COUNTS; i += RT) counts[i] = 0;
+  if (threadIdx.x == 0) beyond = 0;
+  const RowScale<Z> sc(largest<RT>(w.maxima, g.segs * g.per_seg, buf), a);      // (its barriers cover the zeros)
+  const F slope = bin_slope<F>(a, g.V), units = (F)(1 << place_bits(g.V));
+  int behind = 0;
+  const int none = COUNTS + (int)(threadIdx.x & 63);
+  walk<Z>(row_part(logits + (int64_t)blockIdx.y * ld, g, blockIdx.x * RW + (threadIdx.x >> 6), gridDim.x * RW, sc.inf),
+          [&](F(&v)[N], int) {
+            int bin[N];
+            uint32_t place[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) {      // without branches: the chains overlap
+              const F x = (sc.m - v[j]) * slope;
+              const bool in = x < F(COUNTS), is = v[j] >= sc.floor;
+              const int b = (int)x;
+              place[j] = (uint32_t)((x - (F)b) * units);
+              bin[j] = in && is ? b : none;
+              behind += is && !in;
+            }
+#pragma unroll
+            for (int j = 0; j < N; ++j) atomicAdd(&counts[bin[j]], (1ull << 33) | place[j]);
+          },
+          NoEnd());
+  behind = wave_sum(behind);
+  if ((threadIdx.x & 63) == 0 && behind) atomicAdd(&beyond, behind);
+  __syncthreads();
+  if (gridDim.x == 1) {
+    find_window(counts, beyond, (double)slope, a, g.V, dbuf, found);
+    if (threadIdx.x == 0) w.first = found[0], w.last = found[1] < COUNTS ? found[1] : -1;
+    return;
+  }
+  for (int i = threadIdx.x; i < COUNTS; i += RT)
+    if (counts[i]) atomicAdd(&w.counts[i], counts[i]);
+  if (threadIdx.x == 0 && beyond) atomicAdd(&w.n, beyond);
+}
+
+template <typename Z>
+__global__ __launch_bounds__(RT) void row_window_kernel(SampleArgs args, Geometry g, RowWork<Z>* __restrict__ work, int64_t row0) {
+  typedef typename Key<Z>::val_t F;
+  __shared__ double dbuf[RW];
+  __shared__ int found[2];
+  RowWork<Z>& w = work[blockIdx.x];
+  const RowArgs a = row_args(args, row0 + blockIdx.x, g.V);
+  if (row_path(a, g) != WINDOW) return;
+  find_window(w.counts, w.n, (double)bin_slope<F>(a, g.V), a, g.V, dbuf, found);
+  if (threadIdx.x == 0) w.first = found[0], w.last = found[1] < COUNTS ? found[1] : -1, w.n = 0;
+}
+
+// The sums of a row that top-p cuts: MIN_P where the elements min-p drops are summed apart.
+template <typename Z, bool MIN_P>
+__device__ __forceinline__ void window_sums(const RowView<Z>& row, const RowScale<Z>& sc, const RowArgs& a,
+                                            const RowWeight<typename Key<Z>::val_t>& weight, RowWork<Z>& w) {
+  typedef typename Key<Z>::val_t F;
+  constexpr int N = Chunk<Z>::N;
+  const F slope = bin_slope<F>(a, row.V), top = F(w.first), bottom = F(w.last + 1);
+  double sum = 0, above = 0, total = 0;
+  walk<Z>(row,
+          [&](F(&v)[N], int base) {
+            uint32_t mask = 0;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+              const F x = (sc.m - v[j]) * slope;
+              const bool is = v[j] >= sc.floor;
+              const double t = weight(v[j], is), c = x < top ? t : 0.0;
+              total += t;
+              above += c;
+              if (MIN_P) sum += v[j] >= sc.least ? c : 0.0;
+              mask |= (uint32_t)(is && x >= top && x < bottom) << j;
+            }
+            if (__any(mask != 0)) list_add<Z, N>(w, v, base, mask);
+          },
+          [&](int s) {
+            total = wave_sum(total);
+            above = wave_sum(above);
+            if (MIN_P) sum = wave_sum(sum);
+            if ((threadIdx.x & 63) == 0) w.seg[s] = MIN_P ? sum : above, w.above[s] = above, w.total[s] = total;
+            sum = above = total = 0;
+          });
+}
+
+template <typename Z>
+__global__ __launch_bounds__(TB) void row_sums_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args, Geometry g,
+                                                      RowWork<Z>* __restrict__ work, int64_t row0) {
+  typedef typename Key<Z>::type K;
+  typedef typename Key<Z>::val_t F;
+  constexpr int N = Chunk<Z>::N;
+  __shared__ K buf[TW];
+  __shared__ double pow2[32];
+  RowWork<Z>& w = work[blockIdx.y];
+  const RowArgs a = row_args(args, row0 + blockIdx.y, g.V);
+  const Path path = row_path(a, g);
+  if ((path != PLAIN && path != WINDOW) || (path == WINDOW && w.first > w.last)) return;
+  fill_pow2(pow2);
+  const RowScale<Z> sc(largest<TB>(w.maxima, g.segs * g.per_seg, buf), a);      // (its barriers cover pow2)
+  const RowWeight<F> weight(sc.m, a.T, pow2);
+  const RowView<Z> row = row_part(logits + (int64_t)blockIdx.y * ld, g, blockIdx.x * TW + (threadIdx.x >> 6), gridDim.x * TW, sc.inf);
+  if (path == PLAIN) {
+    double sum = 0;
+    walk<Z>(row,
+            [&](F(&v)[N], int) {
+#pragma unroll
+              for (int j = 0; j < N; ++j) sum += weight(v[j], v[j] >= sc.least);
+            },
+            [&](int s) {
+              sum = wave_sum(sum);
+              if ((threadIdx.x & 63) == 0) w.seg[s] = sum;
+              sum = 0;
+            });
+  } else if (a.M > 0) {
+    window_sums<Z, true>(row, sc, a, weight, w);
+  } else {
+    window_sums<Z, false>(row, sc, a, weight, w);
+  }
+}
+
+// Cuts of a row from its list of c <= LIST_CAP elements (in the workspace).
+template <typename Z>
+struct ListCut : RowSampler<Z, TB> {
+  typedef RowSampler<Z, TB> Base;
+  typedef typename Key<Z>::type K;
+  typedef typename Key<Z>::val_t F;
+  using Base::sh;
+  using Base::weight;
+  using Base::whole;
+  const RowWork<Z>& w;
+  int c;
+  __device__ __forceinline__ ListCut(const Base& b, const RowWork<Z>& work) : Base(b), w(work), c(work.n) {}
+
+  // The cut behind the last element with less than `target` in front of it, of the list's elements that `cut` keeps: in
+  // number, or, MASS, in weight (units of 2^-S), of which `above` lies in front of all of them (share: target is a share of
+  // theirs).  False where the list does not hold it.
+  template <bool MASS>
+  __device__ __forceinline__ bool cut_at(Cut<F>& cut, double target, bool share, unsigned long long above) {
+    K lo = ~(K)0, hi = 0;
+    for (int i = threadIdx.x; i < c; i += TB) {
+      const K k = w.key[i];
+      if (cut.keeps(value_of<Z>(k), (int)w.idx[i])) lo = k < lo ? k : lo, hi = k > hi ? k : hi;
+    }
+    block_range<TB>(lo, hi, sh.wave_lo, sh.wave_hi);
+#pragma unroll 1
+    for (;;) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < BINS; i += TB) sh.hist[i] = 0;
+      if (threadIdx.x == 0) sh.n = 0;
+      __syncthreads();
+      int shift = 0;
+      while (((hi - lo) >> shift) >= (K)BINS) ++shift;
+      for (int i = threadIdx.x; i < c; i += TB) {
+        const K k = w.key[i];
+        if (k >= lo && k <= hi && cut.keeps(value_of<Z>(k), (int)w.idx[i]))
+          atomicAdd(&sh.hist[(int)((hi - k) >> shift)], MASS ? whole(weight(value_of<Z>(k), true)) : 1ull);
+      }
+      __syncthreads();
+      const int bin = this->border_bin(above, target, share);
+      share = false;
+      if (bin < 0) return false;
+      above = sh.above;
+      const K top = hi - ((K)bin << shift), span = ((K)1 << shift) - 1, bottom = top - lo > span ? top - span : lo;
+      __syncthreads();
+      K l = ~(K)0, h = 0;
+      for (int i = threadIdx.x; i < c; i += TB) {
+        const K k = w.key[i];
+        const uint32_t at = w.idx[i];
+        if (k >= bottom && k <= top && cut.keeps(value_of<Z>(k), (int)at)) {
+          const int place = atomicAdd(&sh.n, 1);
+          if (place < Base::CAP) list_put<Z, TB>(sh, place, {k, ~at});
+          l = k < l ? k : l;
+          h = k > h ? k : h;
+        }
+      }
+      block_range<TB>(l, h, sh.wave_lo, sh.wave_hi);
+      if (sh.n <= Base::CAP) break;
+      if (l == h) return false;
+      lo = l, hi = h;
+    }
+    const int n = sh.n;
+    list_sort<Z, TB>(sh, n);
+    cut = this->template sorted_cut<MASS>(n, target, above);
+    return true;
+  }
+
+  // top-k and top-p of a list that holds the k first elements
+  __device__ __forceinline__ bool top_cut(Cut<F>& cut, const RowArgs& a) {
+    if (c <= 256) {            // few enough to sort at once
+      for (int i = threadIdx.x; i < c; i += TB) list_put<Z, TB>(sh, i, {w.key[i], ~w.idx[i]});
+      list_sort<Z, TB>(sh, c);
+      const int kk = min(a.k, c);
+      if (!(a.P < 1.0)) {
+        const Item<Z> e = list_get<Z, TB>(sh, kk - 1);
+        cut = {value_of<Z>(e.k), (int)~e.n};
+        __syncthreads();
+        return true;
+      }
+      unsigned long long q = 0, sum;
+      if ((int)threadIdx.x < kk) q = whole(weight(value_of<Z>(list_get<Z, TB>(sh, threadIdx.x).k), true));
+      block_scan<TB>(q, sh.wave_u, sum);
+      cut = this->template sorted_cut<true>(kk, a.P * (double)sum, 0);
+      return true;
+    }
+    if (c > a.k && !cut_at<false>(cut, (double)a.k, false, 0)) return false;
+    return !(a.P < 1.0) || cut_at<true>(cut, a.P, true, 0);
+  }
+
+  // the list's elements that `cut` and min-p keep join their segments' sums
+  __device__ __forceinline__ void join_segments(const Cut<F>& cut) {
+    const int span = this->row.R * 64 * Base::N;
+    __syncthreads();
+    for (int i = threadIdx.x; i < SEGS; i += TB) sh.hist[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < c; i += TB) {
+      const F v = value_of<Z>(w.key[i]);
+      const uint32_t at = w.idx[i];
+      if (v >= this->sc.least && cut.keeps(v, (int)at)) atomicAdd(&sh.hist[at / (uint32_t)span], whole(weight(v, true)));
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < SEGS; i += TB) sh.seg[i] += (double)sh.hist[i] / whole.fixed;
+  }
+};
+
+constexpr int64_t NOT_YET = -2;      // the label of a row that `slow` has to do
+
+template <typename Z>
+__global__ __launch_bounds__(TB) void row_finish_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args, Geometry g,
+                                                        RowWork<Z>* __restrict__ work, int64_t* __restrict__ label, int64_t row0) {
+  typedef typename Key<Z>::type K;
+  typedef typename Key<Z>::val_t F;
+  constexpr int N = Chunk<Z>::N;
+  __shared__ RowShared<Z, TB> sh;
+  const int64_t i = row0 + blockIdx.x;
+  const RowWork<Z>& w = work[blockIdx.x];
+  const RowArgs a = row_args(args, i, g.V);
+  const Path path = row_path(a, g);
+  const Z* p = logits + (int64_t)blockIdx.x * ld;
+  fill_pow2(sh.pow2);
+  for (int s = threadIdx.x; s < SEGS; s += TB) sh.seg[s] = (path == PLAIN || path == WINDOW) && s < g.segs ? w.seg[s] : 0.0;
+  const int groups = g.segs * g.per_seg;
+  const K top = largest<TB>(w.maxima, groups, sh.wave_hi);
+  if (!(value_of<Z>(top) > -__builtin_inff())) {
+    if (threadIdx.x == 0) label[i] = -1;
+    return;
+  }
+  int64_t pick = NOT_YET;
+  if (path == BY_MAX) {
+    // the first segment with the maximum, by one wave
+    if (threadIdx.x == 0) sh.which = groups, sh.at = g.V;
+    __syncthreads();
+    for (int j = threadIdx.x; j < groups; j += TB)
+      if (w.maxima[j] == top) atomicMin(&sh.which, j);
+    __syncthreads();
+    const int s = sh.which / g.per_seg;
+    const F m = value_of<Z>(top);
+    const RowView<Z> row = row_part(p, g, 0, 1, false);
+    if (threadIdx.x < 64)
+#pragma unroll 1
+      for (int r = 0; r < g.R && s * g.R + r < g.steps; ++r) {
+        Chunk<Z> q;
+        F v[N];
+        load_chunk<Z>(q, row, s * g.R + r);
+        chunk_values<Z>(v, q, row, s * g.R + r);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (v[j] == m) atomicMin(&sh.at, chunk_base(row, s * g.R + r) + j);
+      }
+    __syncthreads();
+    pick = sh.at;
+  } else if (path != SLOW) {
+    const RowScale<Z> sc(top, a);
+    const RowSampler<Z, TB> sampler = {sh, row_part(p, g, 0, 1, sc.inf), sc, RowWeight<F>(sc.m, a.T, sh.pow2), Whole(g.V)};
+    ListCut<Z> row(sampler, w);
+    Cut<F> cut = {-__builtin_inff(), -1};
+    bool good = path == PLAIN;
+    if (row.c > 0 && row.c <= LIST_CAP) {
+      if (path == LIST) good = row.top_cut(cut, a);
+      if (path == WINDOW && w.first <= w.last) {
+        double above = 0, total = 0, all_above, all;
+        for (int s = threadIdx.x; s < g.segs; s += TB) above += w.above[s], total += w.total[s];
+        block_scan<TB>(above, sh.wave_d, all_above);
+        block_scan<TB>(total, sh.wave_d, all);
+        good = row.template cut_at<true>(cut, a.P * all * row.whole.fixed, false, (unsigned long long)(all_above * row.whole.fixed));
+      }
+    }
+    if (good) {
+      if (path != PLAIN) row.join_segments(cut);
+      pick = row.draw(cut, a.u);
+    }
+  }
+  if (threadIdx.x == 0) label[i] = pick;
+}
+
+// ---- rows that the lists do not hold ------------------------------------------------------------------------------
+
+template <typename Z>
+struct RowCut : RowSampler<Z, RT> {
+  typedef RowSampler<Z, RT> Base;
+  typedef typename Key<Z>::type K;
+  typedef typename Key<Z>::val_t F;
+  static constexpr int N = Base::N;
+  using Base::row;
+  using Base::sh;
+  using Base::weight;
+  using Base::whole;
+  __device__ __forceinline__ explicit RowCut(const Base& b) : Base(b) {}
 
   // place of the n-th (from 1) kept element that equals t
   __device__ __forceinline__ int nth_tie(const Cut<F>& cut, F t, int n) {
@@ -771,18 +1403,20 @@ struct RowSampler {
     for (int i = threadIdx.x; i < SEGS; i += RT) sh.count[i] = 0;
     __syncthreads();
     int c = 0;
-    walk<Z>(row, [&](F(&v)[N], int base) {
+    walk<Z>(row,
+            [&](F(&v)[N], int base) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) c += v[j] == t && cut.keeps(t, base + j);
-    }, [&](int s) {
-      c = wave_sum(c);
-      if ((threadIdx.x & 63) == 0) sh.count[s] = c;
-      c = 0;
-    });
+              for (int j = 0; j < N; ++j) c += v[j] == t && cut.keeps(t, base + j);
+            },
+            [&](int s) {
+              c = wave_sum(c);
+              if ((threadIdx.x & 63) == 0) sh.count[s] = c;
+              c = 0;
+            });
     __syncthreads();
-    const int mine = sh.count[threadIdx.x];
+    const int mine = sh.count[threadIdx.x];      // (as many segments as threads)
     unsigned long long total;
-    const int upto = (int)block_scan((unsigned long long)mine, sh.wave_u, total);
+    const int upto = (int)block_scan<RT>((unsigned long long)mine, sh.wave_u, total);
     if (upto >= n && upto - mine < n) sh.which = threadIdx.x, sh.at = upto - mine;
     __syncthreads();
     const int s = sh.which;
@@ -814,72 +1448,62 @@ struct RowSampler {
   // The cut of top-k (`target` elements) or, MASS, of top-p (the share `target` of the weight) among the elements `cut` keeps.
   template <bool MASS>
   __device__ __forceinline__ Cut<F> select(Cut<F> cut, double target) {
-    K a = Key<Z>::of(MASS ? floor : -__builtin_inff()) + (MASS ? 0 : 1), b = Key<Z>::of(m);
-    const double fixed = ldexp(1.0, min(51, 30 + (int)__builtin_clz(row.V)));      // 2^S
-    auto whole = [&](double w) {                                                   // w 2^S, rounded; below 2^52
-      return (unsigned long long)__double_as_longlong(w * fixed + 0x1p52) - 0x4330000000000000ull;
-    };
+    K a = MASS ? Key<Z>::of(this->sc.floor) : Key<Z>::of(-__builtin_inff()) + 1, b = Key<Z>::of(this->sc.m);
     unsigned long long above = 0;
-    bool share = MASS;                                // the target is still to be multiplied by the total
+    bool share = MASS;
 #pragma unroll 1
     for (;;) {
       __syncthreads();
       for (int i = threadIdx.x; i < BINS; i += RT) sh.hist[i] = 0;
+      if (threadIdx.x == 0) sh.n = 0;
       __syncthreads();
       int shift = 0;
       while (((b - a) >> shift) >= (K)BINS) ++shift;
-      walk<Z>(row, [&](F(&v)[N], int base) {
+      walk<Z>(row,
+              [&](F(&v)[N], int base) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const K k = Key<Z>::of(v[j]);
-          if (k >= a && k <= b && cut.keeps(v[j], base + j))
-            atomicAdd(&sh.hist[(int)((b - k) >> shift)], MASS ? whole(weight(v[j], true)) : 1ull);
-        }
-      }, NoEnd());
+                for (int j = 0; j < N; ++j) {
+                  const K k = Key<Z>::of(v[j]);
+                  if (k >= a && k <= b && cut.keeps(v[j], base + j))
+                    atomicAdd(&sh.hist[(int)((b - k) >> shift)], MASS ? whole(weight(v[j], true)) : 1ull);
+                }
+              },
+              NoEnd());
       __syncthreads();
-      const unsigned long long v0 = sh.hist[2 * threadIdx.x], v1 = sh.hist[2 * threadIdx.x + 1];
-      unsigned long long total;
-      const unsigned long long upto = above + block_scan(v0 + v1, sh.wave_u, total), from = upto - v0 - v1;
-      if (share) target *= (double)total;
+      const int bin = this->border_bin(above, target, share);
       share = false;
-      if (threadIdx.x == 0 && (double)(above + total) < target) sh.which = -1, sh.above = above;
-      if ((double)from < target && (double)(from + v0) >= target) sh.which = 2 * threadIdx.x, sh.above = from;
-      if ((double)(from + v0) < target && (double)upto >= target) sh.which = 2 * threadIdx.x + 1, sh.above = from + v0;
-      __syncthreads();
-      const int bin = sh.which;
-      above = sh.above;
       if (bin < 0) return cut;                        // fewer elements than asked for: all stay
-      const K bb = b - ((K)bin << shift), width = ((K)1 << shift) - 1;
-      K lo, hi;
-      const int c = list_collect<Z>(sh, row, [&](F v, int i) {
-        const K k = Key<Z>::of(v);
-        return k >= a && k <= bb && bb - k <= width && cut.keeps(v, i);
-      }, lo, hi);
-      if (c <= CAP) {
-        const int n2 = list_pad<Z>(sh, c);
-        list_sort<Z>(sh, n2, false);
-        K key[2];
-        uint32_t nidx[2];
-        unsigned long long q[2] = {0, 0};
+      above = sh.above;
+      const K top = b - ((K)bin << shift), span = ((K)1 << shift) - 1, bottom = top - a > span ? top - span : a;
+      __syncthreads();
+      K lo = ~(K)0, hi = 0;
+      walk<Z>(row,
+              [&](F(&v)[N], int base) {
+                uint32_t mask = 0;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int i = 2 * threadIdx.x + e;
-          if (i < c) {
-            list_get<Z>(sh, i, key[e], nidx[e]);
-            q[e] = MASS ? whole(weight(value_of<Z>(key[e]), true)) : 1ull;
-          }
-        }
-        unsigned long long sum;
-        unsigned long long before = above + block_scan(q[0] + q[1], sh.wave_u, sum) - q[0] - q[1];
+                for (int j = 0; j < N; ++j) {
+                  const K k = Key<Z>::of(v[j]);
+                  mask |= (uint32_t)(k >= bottom && k <= top && cut.keeps(v[j], base + j)) << j;
+                }
+                if (mask) {
+                  int at = atomicAdd(&sh.n, __popc(mask));
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {                 // the last element with less than the target in front of it
-          const int i = 2 * threadIdx.x + e;
-          if (i < c && (double)before < target && (i == c - 1 || (double)(before + q[e]) >= target))
-            sh.cut_key = key[e], sh.cut_idx = (int)~nidx[e];
-          before += q[e];
-        }
-        __syncthreads();
-        return {value_of<Z>(sh.cut_key), sh.cut_idx};
+                  for (int j = 0; j < N; ++j)
+                    if (mask >> j & 1) {
+                      const K k = Key<Z>::of(v[j]);
+                      lo = k < lo ? k : lo;
+                      hi = k > hi ? k : hi;
+                      if (at < Base::CAP) list_put<Z, RT>(sh, at, {k, ~(uint32_t)(base + j)});
+                      ++at;
+                    }
+                }
+              },
+              NoEnd());
+      block_range<RT>(lo, hi, sh.wave_lo, sh.wave_hi);
+      const int c = sh.n;
+      if (c <= Base::CAP) {
+        list_sort<Z, RT>(sh, c);
+        return this->template sorted_cut<MASS>(c, target, above);
       }
       if (lo == hi) {                                 // one value: its first elements
         const F v = value_of<Z>(lo);
@@ -891,673 +1515,45 @@ struct RowSampler {
     }
   }
 
-  // Sums of the kept weights by segment.
-  __device__ __forceinline__ void segment_sums(const Cut<F>& cut, F least) {
+  __device__ __forceinline__ void segment_sums(const Cut<F>& cut) {
     __syncthreads();
-    sh.seg[threadIdx.x] = 0;
+    for (int i = threadIdx.x; i < SEGS; i += RT) sh.seg[i] = 0;
     __syncthreads();
-    const Limit<F> limit(cut, least > floor ? least : floor);
+    const Limit<F> limit(cut, this->sc.least);
     double sum = 0;
-    walk<Z>(row, [&](F(&v)[N], int base) {
-      const F lim = limit.template of<N>(v, base);
+    walk<Z>(row,
+            [&](F(&v)[N], int base) {
+              const F lim = limit.template of<N>(v, base);
 #pragma unroll
-      for (int j = 0; j < N; ++j) sum += weight(v[j], v[j] >= lim);
-    }, [&](int s) {
-      sum = wave_sum(sum);
-      if ((threadIdx.x & 63) == 0) sh.seg[s] = sum;
-      sum = 0;
-    });
-    __syncthreads();
-  }
-
-  // the place, by index, where the running sum of the kept weights passes u times the total (sh.seg holds their sums)
-  __device__ __forceinline__ int draw(const Cut<F>& cut, F least, double u) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (threadIdx.x == 0) sh.which = SEGS, sh.last = -1;
-    const double mine = sh.seg[threadIdx.x];
-    double total;
-    const double upto = block_scan(mine, sh.wave_d, total), target = u * total;
-    const uint64_t over = __ballot(mine > 0 && upto > target), any = __ballot(mine > 0);
-    if (over && lane == (int)__builtin_ctzll(over)) atomicMin(&sh.which, (int)threadIdx.x);
-    if (any && lane == 63 - (int)__builtin_clzll(any)) atomicMax(&sh.last, (int)threadIdx.x);
-    __syncthreads();
-    const bool last = sh.which == SEGS;                 // u >= 1, or rounded up to it: the last kept element
-    const int s = last ? sh.last : sh.which;
-    if ((int)threadIdx.x == s) sh.seg_before = upto - mine;
-    if (threadIdx.x == 0) sh.at = -1, sh.n = -1;        // the answer; the last kept element so far
-    __syncthreads();
-    double before = sh.seg_before;
-    const Limit<F> limit(cut, least > floor ? least : floor);
-#pragma unroll 1
-    for (int r0 = 0; r0 < row.R; r0 += RW) {            // a step a wave
-      const int r = r0 + wave, step = s * row.R + r;
-      const bool in = r < row.R && step < row.steps;
-      const int base = in ? chunk_base(row, step) : 0;
-      double w[N], t = 0;
-      int end = -1;
-      if (in) {
-        Chunk<Z> q;
-        F v[N];
-        load_chunk<Z>(q, row, step);
-        chunk_values<Z>(v, q, row, step);
-        const F lim = limit.template of<N>(v, base);
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          w[j] = weight(v[j], v[j] >= lim);
-          if (w[j] > 0) end = base + j;
-          t += w[j];
-        }
-      }
-      double all;
-      const double upto = before + block_scan(t, sh.wave_d, all);
-      const uint64_t who = last ? 0 : __ballot(t > 0 && upto > target);
-      if (who && lane == (int)__builtin_ctzll(who)) {
-        double c = upto - t;
-        int pick = -1;
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-          if (w[j] > 0 && !(pick >= 0 && c > target)) c += w[j], pick = base + j;
-        atomicMin((unsigned int*)&sh.at, (unsigned int)pick);      // (-1 is the largest)
-      }
-      const uint64_t some = __ballot(end >= 0);
-      if (some && lane == 63 - (int)__builtin_clzll(some)) atomicMax(&sh.n, end);
-      __syncthreads();
-      if (sh.at >= 0) break;
-      before += all;
-    }
-    return sh.at >= 0 ? sh.at : sh.n;
-  }
-};
-
-// Any row of more than 1024 classes with temperature above 0, by one workgroup.  Not inlined: a row in a thousand comes here,
-// and its registers would cost every other.
-template <typename Z>
-__device__ __attribute__((noinline)) int slow_row(const Z* p, int V, int R, typename Key<Z>::type top, double u, double T, double P,
-                                                  double M, int k) {
-  typedef typename Key<Z>::val_t F;
-  __shared__ RowShared<Z> sh;
-  const RowArgs a = {u, T, P, M, k};
-  const RowScale<Z> sc(top, a);
-  __syncthreads();
-  if (threadIdx.x < 32) sh.pow2[threadIdx.x] = exp2((double)threadIdx.x / 32.0);
-  constexpr int N = Chunk<Z>::N;
-  const RowView<Z> row = {p, V, (int)(((int64_t)V + 64 * N - 1) / (64 * N)), R, (int)(threadIdx.x >> 6), RW, sc.inf};
-  RowSampler<Z> r = {sh, row, sc.m, RowWeight<F>(sc.m, T, sh.pow2), sc.floor};
-  Cut<F> cut = {-__builtin_inff(), -1};
-  if (k) cut = r.template select<false>(cut, (double)k);
-  if (P < 1.0) cut = r.template select<true>(cut, P);
-  r.segment_sums(cut, sc.least);
-  return r.draw(cut, sc.least, u);
-}
-
-// ---- the launches -------------------------------------------------------------------------------------------------
-
-struct Geometry {
-  int V, steps, R, segs, per_seg;      // per_seg: groups a segment (a power of two)
-  int most;                            // top-k up to this many is taken from the list
-};
-
-template <typename Z>
-Geometry geometry(int V) {
-  constexpr int N = Chunk<Z>::N;
-  Geometry g;
-  g.V = V;
-  g.steps = (int)(((int64_t)V + 64 * N - 1) / (64 * N));
-  g.R = max((g.steps + SEGS - 1) / SEGS, max(1, min(4, g.steps / 64)));
-  g.segs = (g.steps + g.R - 1) / g.R;
-  g.per_seg = 64;
-  while (g.per_seg * g.segs > GROUPS) g.per_seg /= 2;
-  // k of n groups' maxima bound the k-th largest by an element with about -n ln(1 - k / n) above it
-  const int groups = g.per_seg * g.segs;
-  g.most = V <= LONG_CAP ? V : groups - groups / 128;
-  return g;
-}
-
-// A row's part of the workspace.
-template <typename Z>
-struct RowWork {
-  typedef typename Key<Z>::type K;
-  K maxima[GROUPS];
-  unsigned long long counts[COUNTS];              // number << 33 + sum of the places within the bin
-  double seg[SEGS], above[SEGS], rest[SEGS];      // kept for certain; those before min-p; the others
-  K key[LONG_CAP];
-  uint32_t idx[LONG_CAP];
-  int n;                                          // elements that asked for a place in the list
-  int first, last;                                // window: bins; first > last: none was found
-};
-
-enum Path { DONE_BY_MAX, LIST, WINDOW, PLAIN, SLOW };
-
-__device__ __forceinline__ Path row_path(const RowArgs& a, const Geometry& g) {
-  if (!(a.T > 0.0)) return DONE_BY_MAX;
-  if (a.k) return a.k <= g.most ? LIST : SLOW;
-  return a.P < 1.0 ? WINDOW : PLAIN;
-}
-
-constexpr int TB = 256, TW = TB / 64;
-
-// the largest key of the groups' maxima, in every thread of a workgroup of WAVES waves
-template <int WAVES, typename K>
-__device__ __forceinline__ K largest(const K* maxima, int n, K* buf) {
-  K m = 0;
-  for (int i = threadIdx.x; i < n; i += WAVES * 64) m = maxima[i] > m ? maxima[i] : m;
-  m = wave_max(m);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = m;
-  __syncthreads();
-  m = buf[0];
-#pragma unroll
-  for (int i = 1; i < WAVES; ++i) m = buf[i] > m ? buf[i] : m;
-  return m;
-}
-
-template <typename Z>
-__global__ __launch_bounds__(TB) void row_maxima_kernel(const Z* __restrict__ logits, int64_t ld, Geometry g,
-                                                        RowWork<Z>* __restrict__ work) {
-  typedef typename Key<Z>::val_t F;
-  constexpr int N = Chunk<Z>::N;
-  RowWork<Z>& w = work[blockIdx.y];
-  const int lane = threadIdx.x & 63;
-  if (blockIdx.x == 0 && threadIdx.x == 0) w.n = 0, w.first = 1, w.last = 0;
-  for (int i = blockIdx.x * TB + threadIdx.x; i < COUNTS; i += gridDim.x * TB) w.counts[i] = 0;
-  const RowView<Z> row = {logits + (int64_t)blockIdx.y * ld, g.V, g.steps, g.R, (int)(blockIdx.x * TW + (threadIdx.x >> 6)),
-                          (int)(gridDim.x * TW), false};
-  F mine = -__builtin_inff();
-  const int wide = 64 / g.per_seg;
-  walk<Z>(row, [&](F(&v)[N], int) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) mine = v[j] > mine ? v[j] : mine;
-  }, [&](int s) {
-    for (int d = 1; d < wide; d <<= 1) {
-      const F o = __shfl_xor(mine, d);
-      mine = o > mine ? o : mine;
-    }
-    if (lane % wide == 0) w.maxima[s * g.per_seg + lane / wide] = Key<Z>::of(mine);
-    mine = -__builtin_inff();
-  });
-}
-
-// Places for the lanes' `mask`ed elements in the row's list: the first one of this lane.
-__device__ __forceinline__ int list_places(int* n, uint32_t mask) {
-  const int c = __popc(mask), upto = wave_scan(c), all = from_lane(upto, 63);
-  int at = 0;
-  if ((threadIdx.x & 63) == 0) at = atomicAdd(n, all);
-  return from_lane(at, 0) + upto - c;
-}
-
-template <typename Z>
-__global__ __launch_bounds__(TB) void row_collect_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args, Geometry g,
-                                                         RowWork<Z>* __restrict__ work, int64_t row0) {
-  typedef typename Key<Z>::type K;
-  typedef typename Key<Z>::val_t F;
-  constexpr int N = Chunk<Z>::N;
-  __shared__ K buf[TW];
-  __shared__ uint64_t counts[2][TW];
-  RowWork<Z>& w = work[blockIdx.y];
-  const RowArgs a = row_args(args, row0 + blockIdx.y, g.V);
-  if (row_path(a, g) != LIST) return;
-  const int groups = g.segs * g.per_seg;
-  const K top = largest<TW>(w.maxima, groups, buf);
-  const RowScale<Z> sc(top, a);
-  K bound = 0;
-  if (a.k <= groups) {      // the k-th largest of the maxima, its upper 16 (64-bit keys: 24) bits
-    K key[GROUPS / TB];
-#pragma unroll
-    for (int i = 0; i < GROUPS / TB; ++i) {
-      const int at = i * TB + threadIdx.x;
-      key[i] = at < groups ? w.maxima[at] : (K)0;
-      if (sc.inf) key[i] = Key<Z>::of(finite(value_of<Z>(key[i]), true));
-    }
-    constexpr int BITS = 8 * (int)sizeof(K), END = BITS - (BITS == 64 ? 24 : 16);
-    int turn = 0;
-#pragma unroll 1
-    for (int bit = BITS - 2; bit >= END; bit -= 2, turn ^= 1) {      // two bits at a time
-      uint32_t c[3] = {0, 0, 0};
-#pragma unroll
-      for (int i = 0; i < GROUPS / TB; ++i)
-#pragma unroll
-        for (int j = 0; j < 3; ++j) c[j] += __popcll(__ballot(key[i] >= (bound | (K)(j + 1) << bit)));
-      if ((threadIdx.x & 63) == 0) counts[turn][threadIdx.x >> 6] = c[0] | (uint64_t)c[1] << 20 | (uint64_t)c[2] << 40;
-      __syncthreads();
-      uint64_t all = 0;
-#pragma unroll
-      for (int i = 0; i < TW; ++i) all += counts[turn][i];
-      K digit = 0;
-#pragma unroll
-      for (int j = 0; j < 3; ++j) digit += (int)(all >> (20 * j) & 0xFFFFF) >= a.k;
-      bound |= digit << bit;
-    }
-  }
-  const K lowest = Key<Z>::of(sc.floor);
-  const F lim = bound > lowest ? value_of<Z>(bound) : sc.floor;
-  const RowView<Z> row = {logits + (int64_t)blockIdx.y * ld, g.V, g.steps, g.R, (int)(blockIdx.x * TW + (threadIdx.x >> 6)),
-                          (int)(gridDim.x * TW), sc.inf};
-  walk<Z>(row, [&](F(&v)[N], int base) {
-    uint32_t mask = 0;
-#pragma unroll
-    for (int j = 0; j < N; ++j) mask |= (uint32_t)(v[j] >= lim) << j;
-    if (__any(mask != 0)) {
-      int at = list_places(&w.n, mask);
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (mask >> j & 1) {
-          if (at < LONG_CAP) w.key[at] = Key<Z>::of(v[j]), w.idx[at] = (uint32_t)(base + j);
-          ++at;
-        }
-    }
-  }, NoEnd());
-}
-
-// Bins over what matters of a row cut by top-p: what lies further below the maximum than ln(V / (1 - P)) weighs less than
-// 1 - P of the total, and five units more make what lies behind the bins weigh nothing against a bin.
-template <typename F>
-__device__ __forceinline__ F bin_slope(const RowArgs& a, int V) {
-  return (F)fmin((double)COUNTS / (a.T * (log((double)V / (1.0 - a.P)) + 5.0)), 1e38);
-}
-// Places within a bin are counted in units of 2^-place_bits: V of them stay below 2^33.
-__device__ __forceinline__ int place_bits(int V) { return min(10, 1 + (int)__builtin_clz(V)); }
-
-// The bins the border of top-p must lie in.  With step = width of a bin in units of T, an element at place f of bin b weighs
-// e^(-(b + f) step), and e^(-y) lies between 1 - y and 1 - y + y^2 / 2; places are known to their unit and to the roundings of
-// the bin number (below 4096 2^-22 of a bin).
-__device__ __forceinline__ void find_window(const unsigned long long* counts, int beyond, double slope, const RowArgs& a, int V,
-                                            double* buf, int* found) {
-  constexpr int PER = COUNTS / RT;
-  const double step = 1.0 / (slope * a.T), unit = ldexp(1.0, -place_bits(V));
-  double least[PER], most[PER], sl = 0, sm = 0;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int bin = PER * threadIdx.x + i;
-    const double n = (double)(counts[bin] >> 33), f = (double)(counts[bin] & 0x1FFFFFFFFull) * unit;
-    const double low = fmax(f - 0.001 * n, 0.0), high = f + (unit + 0.001) * n, e = exp(-(double)bin * step);
-    least[i] = e * fmax(n - step * high, 0.0);
-    most[i] = e * (n - step * low + 0.5 * step * step * high);
-    sl += least[i];
-    sm += most[i];
-  }
-  double total_least, total_most;
-  double ul = block_scan(sl, buf, total_least) - sl;
-  double um = block_scan(sm, buf, total_most) - sm;
-  total_most += (double)beyond * exp(-((double)COUNTS - 0.001) * step);
-  __syncthreads();
-  if (threadIdx.x == 0) found[0] = COUNTS, found[1] = COUNTS;
-  __syncthreads();
-  const double early = a.P * total_least * (1 - 1e-9), late = a.P * total_most * (1 + 1e-9);
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    if (um < early && um + most[i] >= early) atomicMin(&found[0], PER * (int)threadIdx.x + i);
-    if (ul < late && ul + least[i] >= late) atomicMin(&found[1], PER * (int)threadIdx.x + i);
-    ul += least[i];
-    um += most[i];
-  }
-  __syncthreads();
-}
-
-// counts; where a row has one workgroup, its window too (`n` of the row's work holds, meanwhile, the elements behind the bins)
-template <typename Z>
-__global__ __launch_bounds__(RT) void row_counts_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args, Geometry g,
-                                                        RowWork<Z>* __restrict__ work, int64_t row0) {
-  typedef typename Key<Z>::type K;
-  typedef typename Key<Z>::val_t F;
-  constexpr int N = Chunk<Z>::N;
-  __shared__ unsigned long long counts[COUNTS + 64];      // the last 64: elements that are not counted
-  __shared__ K buf[RW];
-  __shared__ double dbuf[RW];
-  __shared__ int beyond, found[2];
-  RowWork<Z>& w = work[blockIdx.y];
-  const RowArgs a = row_args(args, row0 + blockIdx.y, g.V);
-  if (row_path(a, g) != WINDOW) return;
-  for (int i = threadIdx.x; i < COUNTS; i += RT) counts[i] = 0;
-  if (threadIdx.x == 0) beyond = 0;
-  const RowScale<Z> sc(largest<RW>(w.maxima, g.segs * g.per_seg, buf), a);
-  const F slope = bin_slope<F>(a, g.V), units = (F)(1 << place_bits(g.V));
-  const RowView<Z> row = {logits + (int64_t)blockIdx.y * ld, g.V, g.steps, g.R, (int)(blockIdx.x * RW + (threadIdx.x >> 6)),
-                          (int)(gridDim.x * RW), sc.inf};
-  int behind = 0;
-  const int none = COUNTS + (int)(threadIdx.x & 63);
-  walk<Z>(row, [&](F(&v)[N], int) {
-    int bin[N];
-    uint32_t place[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const F x = (sc.m - v[j]) * slope;
-      const bool in = x < F(COUNTS), is = v[j] >= sc.floor;
-      const int b = (int)x;
-      place[j] = (uint32_t)((x - (F)b) * units);
-      bin[j] = in && is ? b : none;
-      behind += is && !in;
-    }
-#pragma unroll
-    for (int j = 0; j < N; ++j) atomicAdd(&counts[bin[j]], (1ull << 33) | place[j]);
-  }, NoEnd());
-  behind = wave_sum(behind);
-  if ((threadIdx.x & 63) == 0 && behind) atomicAdd(&beyond, behind);
-  __syncthreads();
-  if (gridDim.x == 1) {
-    find_window(counts, beyond, (double)slope, a, g.V, dbuf, found);
-    if (threadIdx.x == 0) w.first = found[0], w.last = found[1] < COUNTS ? found[1] : -1;
-    return;
-  }
-  for (int i = threadIdx.x; i < COUNTS; i += RT)
-    if (counts[i]) atomicAdd(&w.counts[i], counts[i]);
-  if (threadIdx.x == 0 && beyond) atomicAdd(&w.n, beyond);
-}
-
-template <typename Z>
-__global__ __launch_bounds__(RT) void row_window_kernel(SampleArgs args, Geometry g, RowWork<Z>* __restrict__ work, int64_t row0) {
-  typedef typename Key<Z>::val_t F;
-  __shared__ double dbuf[RW];
-  __shared__ int found[2];
-  RowWork<Z>& w = work[blockIdx.x];
-  const RowArgs a = row_args(args, row0 + blockIdx.x, g.V);
-  if (row_path(a, g) != WINDOW) return;
-  find_window(w.counts, w.n, (double)bin_slope<F>(a, g.V), a, g.V, dbuf, found);
-  if (threadIdx.x == 0) w.first = found[0], w.last = found[1] < COUNTS ? found[1] : -1, w.n = 0;
-}
-
-template <typename Z>
-__global__ __launch_bounds__(TB) void row_sums_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args, Geometry g,
-                                                      RowWork<Z>* __restrict__ work, int64_t row0) {
-  typedef typename Key<Z>::type K;
-  typedef typename Key<Z>::val_t F;
-  constexpr int N = Chunk<Z>::N;
-  __shared__ K buf[TW];
-  __shared__ double pow2[32];
-  RowWork<Z>& w = work[blockIdx.y];
-  const RowArgs a = row_args(args, row0 + blockIdx.y, g.V);
-  const Path path = row_path(a, g);
-  if (path != PLAIN && path != WINDOW) return;
-  if (path == WINDOW && w.first > w.last) return;
-  if (threadIdx.x < 32) pow2[threadIdx.x] = exp2((double)threadIdx.x / 32.0);
-  const RowScale<Z> sc(largest<TW>(w.maxima, g.segs * g.per_seg, buf), a);      // (its barriers cover pow2)
-  const RowWeight<F> weight(sc.m, a.T, pow2);
-  const RowView<Z> row = {logits + (int64_t)blockIdx.y * ld, g.V, g.steps, g.R, (int)(blockIdx.x * TW + (threadIdx.x >> 6)),
-                          (int)(gridDim.x * TW), sc.inf};
-  double sum = 0;
-  if (path == PLAIN) {
-    walk<Z>(row, [&](F(&v)[N], int) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) sum += weight(v[j], v[j] >= sc.least);
-    }, [&](int s) {
-      sum = wave_sum(sum);
-      if ((threadIdx.x & 63) == 0) w.seg[s] = sum;
-      sum = 0;
-    });
-    return;
-  }
-  const F slope = bin_slope<F>(a, g.V), top = F(w.first), bottom = F(w.last + 1);
-  double above = 0, rest = 0;
-  walk<Z>(row, [&](F(&v)[N], int base) {
-    uint32_t mask = 0;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const F x = (sc.m - v[j]) * slope;
-      const bool is = v[j] >= sc.floor;
-      const double t = weight(v[j], is), c = x < top ? t : 0.0;
-      above += c;
-      rest += t - c;
-      sum += v[j] >= sc.least ? c : 0.0;
-      mask |= (uint32_t)(is && x >= top && x < bottom) << j;
-    }
-    if (__any(mask != 0)) {
-      int at = list_places(&w.n, mask);
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (mask >> j & 1) {
-          if (at < LONG_CAP) w.key[at] = Key<Z>::of(v[j]), w.idx[at] = (uint32_t)(base + j);
-          ++at;
-        }
-    }
-  }, [&](int s) {
-    sum = wave_sum(sum);
-    above = wave_sum(above);
-    rest = wave_sum(rest);
-    if ((threadIdx.x & 63) == 0) w.seg[s] = sum, w.above[s] = above, w.rest[s] = rest;
-    sum = above = rest = 0;
-  });
-}
-
-// Cuts of a row from its list of c <= LONG_CAP elements (in the workspace), by the workgroup that finishes the row.
-template <typename Z>
-struct Finish {
-  typedef typename Key<Z>::type K;
-  typedef typename Key<Z>::val_t F;
-  RowShared<Z>& sh;
-  const RowWork<Z>& w;
-  int c;
-  RowWeight<F> weight;
-  double fixed;                 // 2^S, see `whole`
-
-  // Sums that must not depend on an order are whole numbers: weights times 2^S, rounded; below 2^52 each.
-  __device__ __forceinline__ unsigned long long whole(double x) const {
-    return (unsigned long long)__double_as_longlong(x * fixed + 0x1p52) - 0x4330000000000000ull;
-  }
-
-  // The cut behind the last element with less than `target` in front of it, of the list's elements that `cut` keeps: in
-  // number, or, MASS, in weight (in units of 2^-S), of which `above0` lies in front of all of them (share: target is a share
-  // of that and theirs).  False where the list does not hold it.
-  template <bool MASS>
-  __device__ __forceinline__ bool list_cut(Cut<F>& cut, double target, bool share, double above0) {
-    unsigned long long above = MASS ? (unsigned long long)(above0 * fixed) : 0ull;
-    K lo = ~(K)0, hi = 0;
-    for (int i = threadIdx.x; i < c; i += RT) {
-      const K k = w.key[i];
-      if (cut.keeps(value_of<Z>(k), (int)w.idx[i])) lo = k < lo ? k : lo, hi = k > hi ? k : hi;
-    }
-    block_range(lo, hi);
-#pragma unroll 1
-    for (;;) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < BINS; i += RT) sh.hist[i] = 0;
-      if (threadIdx.x == 0) sh.which = -1, sh.n = 0;
-      __syncthreads();
-      int shift = 0;
-      while (((hi - lo) >> shift) >= (K)BINS) ++shift;
-      for (int i = threadIdx.x; i < c; i += RT) {
-        const K k = w.key[i];
-        if (k >= lo && k <= hi && cut.keeps(value_of<Z>(k), (int)w.idx[i]))
-          atomicAdd(&sh.hist[(int)((hi - k) >> shift)], MASS ? whole(weight(value_of<Z>(k), true)) : 1ull);
-      }
-      __syncthreads();
-      const unsigned long long v0 = sh.hist[2 * threadIdx.x], v1 = sh.hist[2 * threadIdx.x + 1];
-      unsigned long long total;
-      const unsigned long long upto = above + block_scan(v0 + v1, sh.wave_u, total), from = upto - v0 - v1;
-      if (share) target *= (double)(above + total);
-      share = false;
-      // (the first element is kept whatever lies in front of it)
-      const unsigned long long v[2] = {v0, v1};
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const unsigned long long f = e ? from + v0 : from;
-        if (v[e] && ((double)f < target || f == above) && (double)(f + v[e]) >= target) sh.which = 2 * threadIdx.x + e, sh.above = f;
-      }
-      __syncthreads();
-      const int bin = sh.which;
-      if (bin < 0) return false;
-      const K top = hi - ((K)bin << shift);
-      const K span = ((K)1 << shift) - 1, bottom = top - lo > span ? top - span : lo;
-      above = sh.above;
-      K l = ~(K)0, h = 0;
-      __syncthreads();
-      for (int i = threadIdx.x; i < c; i += RT) {
-        const K k = w.key[i];
-        const uint32_t at = w.idx[i];
-        if (k >= bottom && k <= top && cut.keeps(value_of<Z>(k), (int)at)) {
-          const int place = atomicAdd(&sh.n, 1);
-          if (place < CAP) list_put<Z>(sh, place, k, ~at);
-          l = k < l ? k : l;
-          h = k > h ? k : h;
-        }
-      }
-      block_range(l, h);
-      const int n = sh.n;
-      if (n <= CAP) break;
-      if (l == h) return false;
-      lo = l, hi = h;
-    }
-    const int n = sh.n, n2 = list_pad<Z>(sh, n);
-    list_sort<Z>(sh, n2, false);
-    sorted_cut<MASS>(cut, n, target, above);
-    return true;
-  }
-
-  // the same for the n elements of the sorted LDS list
-  template <bool MASS>
-  __device__ __forceinline__ void sorted_cut(Cut<F>& cut, int n, double target, unsigned long long above) {
-    K key[2];
-    uint32_t nidx[2];
-    unsigned long long q[2] = {0, 0}, sum;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int i = 2 * threadIdx.x + e;
-      if (i < n) {
-        list_get<Z>(sh, i, key[e], nidx[e]);
-        q[e] = MASS ? whole(weight(value_of<Z>(key[e]), true)) : 1ull;
-      }
-    }
-    unsigned long long before = above + block_scan(q[0] + q[1], sh.wave_u, sum) - q[0] - q[1];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int i = 2 * threadIdx.x + e;
-      if (i < n && ((double)before < target || i == 0) && (i == n - 1 || (double)(before + q[e]) >= target))
-        sh.cut_key = key[e], sh.cut_idx = (int)~nidx[e];
-      before += q[e];
-    }
-    __syncthreads();
-    cut = {value_of<Z>(sh.cut_key), sh.cut_idx};
-    __syncthreads();
-  }
-
-  __device__ __forceinline__ void block_range(K& lo, K& hi) {
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-      const K a = __shfl_xor(lo, s), b = __shfl_xor(hi, s);
-      lo = a < lo ? a : lo;
-      hi = b > hi ? b : hi;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.wave_lo[threadIdx.x >> 6] = lo, sh.wave_hi[threadIdx.x >> 6] = hi;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < RW; ++i) {
-      lo = sh.wave_lo[i] < lo ? sh.wave_lo[i] : lo;
-      hi = sh.wave_hi[i] > hi ? sh.wave_hi[i] : hi;
-    }
-  }
-
-  // top-k and top-p of a list that holds the k first elements
-  __device__ __forceinline__ bool top_cut(Cut<F>& cut, const RowArgs& a) {
-    if (c <= 256) {            // few enough to sort at once
-      for (int i = threadIdx.x; i < c; i += RT) list_put<Z>(sh, i, w.key[i], ~w.idx[i]);
-      list_sort<Z>(sh, list_pad<Z>(sh, c), false);
-      const int kk = min(a.k, c);
-      if (a.P < 1.0) {
-        const int i = 2 * threadIdx.x;
-        double t = 0;
-        unsigned long long sum;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          K k = 0;
-          uint32_t n;
-          if (i + e < kk) list_get<Z>(sh, i + e, k, n);
-          t += i + e < kk ? (double)whole(weight(value_of<Z>(k), true)) : 0.0;
-        }
-        block_scan((unsigned long long)t, sh.wave_u, sum);
-        sorted_cut<true>(cut, kk, a.P * (double)sum, 0);
-      } else {
-        sorted_cut<false>(cut, kk, (double)kk, 0);
-      }
-      return true;
-    }
-    if (c > a.k && !list_cut<false>(cut, (double)a.k, false, 0)) return false;
-    return !(a.P < 1.0) || list_cut<true>(cut, a.P, true, 0);
-  }
-
-  // the list's elements that `cut` keeps and that are not below `least` join their segments' sums
-  __device__ __forceinline__ void join_segments(const Cut<F>& cut, F least, int span) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < SEGS; i += RT) sh.hist[i] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < c; i += RT) {
-      const F v = value_of<Z>(w.key[i]);
-      const uint32_t at = w.idx[i];
-      if (v >= least && cut.keeps(v, (int)at)) atomicAdd(&sh.hist[at / (uint32_t)span], whole(weight(v, true)));
-    }
-    __syncthreads();
-    sh.seg[threadIdx.x] += (double)sh.hist[threadIdx.x] / fixed;
+              for (int j = 0; j < N; ++j) sum += weight(v[j], v[j] >= lim);
+            },
+            [&](int s) {
+              sum = wave_sum(sum);
+              if ((threadIdx.x & 63) == 0) sh.seg[s] = sum;
+              sum = 0;
+            });
   }
 };
 
 template <typename Z>
-__global__ __launch_bounds__(RT, 8) void row_finish_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args, Geometry g,
-                                                        RowWork<Z>* __restrict__ work, int64_t* __restrict__ label, int64_t row0) {
-  typedef typename Key<Z>::type K;
+__global__ __launch_bounds__(RT) void row_slow_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args, Geometry g,
+                                                      const RowWork<Z>* __restrict__ work, int64_t* __restrict__ label,
+                                                      int64_t row0) {
   typedef typename Key<Z>::val_t F;
-  constexpr int N = Chunk<Z>::N;
-  __shared__ RowShared<Z> sh;
+  __shared__ RowShared<Z, RT> sh;
   const int64_t i = row0 + blockIdx.x;
-  const RowWork<Z>& w = work[blockIdx.x];
+  if (label[i] != NOT_YET) return;
   const RowArgs a = row_args(args, i, g.V);
-  const Z* p = logits + (int64_t)blockIdx.x * ld;
-  if (threadIdx.x < 32) sh.pow2[threadIdx.x] = exp2((double)threadIdx.x / 32.0);
-  const int groups = g.segs * g.per_seg;
-  const K top = largest<RW>(w.maxima, groups, sh.wave_hi);
-  if (!(value_of<Z>(top) > -__builtin_inff())) {
-    if (threadIdx.x == 0) label[i] = -1;
-    return;
-  }
-  const Path path = row_path(a, g);
-  const RowScale<Z> sc(top, a);
-  RowView<Z> row = {p, g.V, g.steps, g.R, 0, 1, sc.inf};
-  int pick = -1;
-  if (path == DONE_BY_MAX) {
-    // the first segment with the maximum, by one wave
-    if (threadIdx.x == 0) sh.which = groups, sh.at = g.V;
-    __syncthreads();
-    for (int j = threadIdx.x; j < groups; j += RT)
-      if (w.maxima[j] == top) atomicMin(&sh.which, j);
-    __syncthreads();
-    const int s = sh.which / g.per_seg;
-    const F m = value_of<Z>(top);
-    row.inf = false;
-    if (threadIdx.x < 64)
-#pragma unroll 1
-      for (int r = 0; r < g.R && s * g.R + r < g.steps; ++r) {
-        Chunk<Z> q;
-        F v[N];
-        load_chunk<Z>(q, row, s * g.R + r);
-        chunk_values<Z>(v, q, row, s * g.R + r);
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-          if (v[j] == m) atomicMin(&sh.at, chunk_base(row, s * g.R + r) + j);
-      }
-    __syncthreads();
-    pick = sh.at;
-  } else {
-    const RowWeight<F> weight(sc.m, a.T, sh.pow2);
-    // S: the sum of V weights stays below 2^63
-    Finish<Z> fin = {sh, w, w.n, weight, ldexp(1.0, min(51, 30 + (int)__builtin_clz(g.V)))};
-    Cut<F> cut = {-__builtin_inff(), -1};
-    const bool listed = fin.c > 0 && fin.c <= LONG_CAP;
-    bool good = path == PLAIN;
-    sh.seg[threadIdx.x] = (path == PLAIN || path == WINDOW) && (int)threadIdx.x < g.segs ? w.seg[threadIdx.x] : 0.0;
-    if (path == LIST) {
-      good = listed && fin.top_cut(cut, a);
-    } else if (path == WINDOW && listed && w.first <= w.last) {
-      double above, rest;
-      block_scan((int)threadIdx.x < g.segs ? w.above[threadIdx.x] : 0.0, sh.wave_d, above);
-      block_scan((int)threadIdx.x < g.segs ? w.rest[threadIdx.x] : 0.0, sh.wave_d, rest);
-      // (rest holds the window's elements, which list_cut counts by itself)
-      good = fin.template list_cut<true>(cut, a.P * (above + rest) * fin.fixed, false, above);
-    }
-    if (good) {
-      if (path != PLAIN) fin.join_segments(cut, sc.least, g.R * 64 * N);
-      RowSampler<Z> r = {sh, row, sc.m, weight, sc.floor};
-      pick = r.draw(cut, sc.least, a.u);
-    } else {
-      pick = slow_row<Z>(p, g.V, g.R, top, a.u, a.T, a.P, a.M, a.k);
-    }
-  }
+  fill_pow2(sh.pow2);
+  const RowScale<Z> sc(largest<RT>(work[blockIdx.x].maxima, g.segs * g.per_seg, sh.wave_hi), a);
+  const RowSampler<Z, RT> sampler = {sh, row_part(logits + (int64_t)blockIdx.x * ld, g, threadIdx.x >> 6, RW, sc.inf), sc,
+                                     RowWeight<F>(sc.m, a.T, sh.pow2), Whole(g.V)};
+  RowCut<Z> row(sampler);
+  Cut<F> cut = {-__builtin_inff(), -1};
+  if (a.k) cut = row.template select<false>(cut, (double)a.k);
+  if (a.P < 1.0) cut = row.template select<true>(cut, a.P);
+  row.segment_sums(cut);
+  const int pick = row.draw(cut, a.u);
   if (threadIdx.x == 0) label[i] = pick;
 }
 
@@ -1568,7 +1564,7 @@ int launch_rows(const Z* z, int64_t ld, const SampleArgs& a, int64_t* label, int
                 hipStream_t st) {
   if (!ws || ws_bytes < min(rows, ROW_BATCH) * (int64_t)sizeof(RowWork<Z>)) return TTK_EWORKSPACE;
   RowWork<Z>* work = (RowWork<Z>*)ws;
-  const Geometry g = geometry<Z>(V);
+  const Geometry g = geometry<Z>(V, min(rows, ROW_BATCH));
   // what the rows can need (parameters of their own: anything)
   const bool any_t = a.temperature || a.temperature_all > 0.0, any_k = a.top_k || (a.top_k_all > 0 && a.top_k_all < V);
   const bool all_k = !a.top_k && any_k, any_p = a.top_p || a.top_p_all < 1.0;
@@ -1578,17 +1574,18 @@ int launch_rows(const Z* z, int64_t ld, const SampleArgs& a, int64_t* label, int
     // workgroups a row: enough to fill the machine, each wave with a segment at least
     const int split = (int)max((int64_t)1, min((int64_t)(g.segs + TW - 1) / TW, (1024 + n - 1) / n));
     const int wide = (int)max((int64_t)1, min((int64_t)(g.segs + RW - 1) / RW, (256 + n - 1) / n));
-    const dim3 grid((unsigned)split, (unsigned)n), big((unsigned)wide, (unsigned)n);
+    const dim3 grid((unsigned)split, (unsigned)n), big((unsigned)wide, (unsigned)n), one((unsigned)n);
     hipLaunchKernelGGL((row_maxima_kernel<Z>), grid, dim3(TB), 0, st, p, ld, g, work);
     if (any_t && any_k) hipLaunchKernelGGL((row_collect_kernel<Z>), grid, dim3(TB), 0, st, p, ld, a, g, work, r0);
     if (any_t && !all_k) {
       if (any_p) {
         hipLaunchKernelGGL((row_counts_kernel<Z>), big, dim3(RT), 0, st, p, ld, a, g, work, r0);
-        if (wide > 1) hipLaunchKernelGGL((row_window_kernel<Z>), dim3((unsigned)n), dim3(RT), 0, st, a, g, work, r0);
+        if (wide > 1) hipLaunchKernelGGL((row_window_kernel<Z>), one, dim3(RT), 0, st, a, g, work, r0);
       }
       hipLaunchKernelGGL((row_sums_kernel<Z>), grid, dim3(TB), 0, st, p, ld, a, g, work, r0);
     }
-    hipLaunchKernelGGL((row_finish_kernel<Z>), dim3((unsigned)n), dim3(RT), 0, st, p, ld, a, g, work, label, r0);
+    hipLaunchKernelGGL((row_finish_kernel<Z>), one, dim3(TB), 0, st, p, ld, a, g, work, label, r0);
+    if (any_t && (any_k || any_p)) hipLaunchKernelGGL((row_slow_kernel<Z>), one, dim3(RT), 0, st, p, ld, a, g, work, label, r0);
   }
   return hipGetLastError() == hipSuccess ? TTK_OK : TTK_ELAUNCH;
 }
