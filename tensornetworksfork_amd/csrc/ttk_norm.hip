@@ -28,15 +28,14 @@ struct Acc<double> {
 // 16 bytes of elements as one unaligned global access: rows of odd length start anywhere.
 typedef uint32_t raw_t __attribute__((ext_vector_type(4), aligned(2)));
 
+// Held as four words (elements of their own would take a register each).
 template <typename X>
 struct Vec {
+  typedef typename Acc<X>::type A;
   static constexpr int N = 16 / (int)sizeof(X);
-  union {
-    uint32_t u[4];
-    X e[N];
-  };
+  uint32_t u[4];
   __device__ __forceinline__ void load(const X* p) {
-    raw_t r = *reinterpret_cast<const raw_t*>(p);
+    const raw_t r = *reinterpret_cast<const raw_t*>(p);
     u[0] = r.x, u[1] = r.y, u[2] = r.z, u[3] = r.w;
   }
   __device__ __forceinline__ void store(X* p) const {
@@ -49,12 +48,45 @@ struct Vec {
     u[0] = u[1] = u[2] = u[3] = 0;
 #pragma unroll
     for (int j = 0; j < N; ++j)
-      if (j < n) e[j] = p[j];
+      if (j < n) put(j, p[j]);
   }
   __device__ __forceinline__ void store_some(X* p, int n) const {
 #pragma unroll
     for (int j = 0; j < N; ++j)
-      if (j < n) p[j] = e[j];
+      if (j < n) p[j] = element(j);
+  }
+  // Forgets what was computed from the elements: without it the compiler keeps every element's float beside the element
+  // across the phases of a row, which are twice to three times the registers.
+  __device__ __forceinline__ void forget() { asm volatile("" : "+v"(u[0]), "+v"(u[1]), "+v"(u[2]), "+v"(u[3])); }
+
+  __device__ __forceinline__ X element(int j) const {
+    if constexpr (sizeof(X) == 2)
+      return __builtin_bit_cast(X, (uint16_t)(u[j / 2] >> (16 * (j % 2))));
+    else if constexpr (sizeof(X) == 4)
+      return __builtin_bit_cast(X, u[j]);
+    else
+      return __builtin_bit_cast(X, (uint64_t)u[2 * j + 1] << 32 | u[2 * j]);
+  }
+  __device__ __forceinline__ void put(int j, X e) {      // into a zero
+    if constexpr (sizeof(X) == 2) {
+      u[j / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, e) << (16 * (j % 2));
+    } else if constexpr (sizeof(X) == 4) {
+      u[j] = __builtin_bit_cast(uint32_t, e);
+    } else {
+      const uint64_t b = __builtin_bit_cast(uint64_t, e);
+      u[2 * j] = (uint32_t)b, u[2 * j + 1] = (uint32_t)(b >> 32);
+    }
+  }
+  __device__ __forceinline__ A get(int j) const {
+    if constexpr (__is_same(X, __bf16))
+      return __builtin_bit_cast(float, j % 2 ? u[j / 2] & 0xFFFF0000u : u[j / 2] << 16);
+    else
+      return (A)element(j);
+  }
+  __device__ __forceinline__ void set(const A (&h)[N]) {      // rounded to the element type
+    u[0] = u[1] = u[2] = u[3] = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) put(j, (X)h[j]);
   }
 };
 
@@ -143,17 +175,26 @@ __device__ __forceinline__ A lane_sum(A v) {
   return v;
 }
 
-// Sum of two values over a workgroup of WAVES waves; `buf` holds 2 * WAVES values and may be written again after the
-// next barrier that follows.
+// Sums over a workgroup of WAVES (at most 16) waves, the same bits in every lane; `buf` holds 16 values a sum and may be
+// written again after the next barrier that follows.
+template <int WAVES, typename A>
+__device__ __forceinline__ A block_sum(A a, A* buf) {
+  const int lane = threadIdx.x & 63;
+  a = lane_sum<64>(a);
+  if (lane == 0) buf[threadIdx.x >> 6] = a;
+  __syncthreads();
+  return lane_sum<16>((lane & 15) < WAVES ? buf[lane & 15] : A(0));
+}
 template <int WAVES, typename A>
 __device__ __forceinline__ void block_sum2(A& a, A& b, A* buf) {
+  const int lane = threadIdx.x & 63;
   a = lane_sum<64>(a);
   b = lane_sum<64>(b);
-  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = a, buf[WAVES + (threadIdx.x >> 6)] = b;
+  if (lane == 0) buf[threadIdx.x >> 6] = a, buf[16 + (threadIdx.x >> 6)] = b;
   __syncthreads();
-  a = b = A(0);
-#pragma unroll
-  for (int i = 0; i < WAVES; ++i) a += buf[i], b += buf[WAVES + i];
+  const bool is = (lane & 15) < WAVES;
+  a = lane_sum<16>(is ? buf[lane & 15] : A(0));
+  b = lane_sum<16>(is ? buf[16 + (lane & 15)] : A(0));
 }
 
 // ---------------------------------------------------------------------------------------
@@ -168,23 +209,20 @@ __global__ __launch_bounds__(LONG_THREADS) void ln_fwd_long_kernel(const X* __re
                                                                    typename Acc<X>::type* __restrict__ rstd_out, int64_t rows,
                                                                    int cols, double eps, Drop drop) {
   typedef typename Acc<X>::type A;
-  __shared__ A buf[2][2 * (LONG_THREADS / 64)];
+  __shared__ A buf[2][32];
   const uint64_t e0 = drop_base(drop);
   const A scale = (A)drop.scale;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const X* xr = x + row * ldx;
-    A s = 0, unused = 0;
+    A s = 0;
     for (int c = threadIdx.x; c < cols; c += LONG_THREADS) s += (A)xr[c];
-    block_sum2<LONG_THREADS / 64>(s, unused, buf[0]);
-    const A mean = s / (A)cols;
+    const A mean = block_sum<LONG_THREADS / 64>(s, buf[0]) / (A)cols;
     A q = 0;
     for (int c = threadIdx.x; c < cols; c += LONG_THREADS) {
       const A d = (A)xr[c] - mean;
       q += d * d;
     }
-    unused = 0;
-    block_sum2<LONG_THREADS / 64>(q, unused, buf[1]);
-    const A rstd = A(1) / sqrt(q / (A)cols + (A)eps);
+    const A rstd = A(1) / sqrt(block_sum<LONG_THREADS / 64>(q, buf[1]) / (A)cols + (A)eps);
     for (int c = threadIdx.x; c < cols; c += LONG_THREADS) {
       A v = ((A)xr[c] - mean) * rstd;
       if (w) v *= (A)w[c];
@@ -203,7 +241,7 @@ __global__ __launch_bounds__(LONG_THREADS) void ln_bwd_long_kernel(const X* __re
                                                                    const typename Acc<X>::type* __restrict__ rstd_in,
                                                                    X* __restrict__ dx, int64_t rows, int cols, Drop drop) {
   typedef typename Acc<X>::type A;
-  __shared__ A buf[2][2 * (LONG_THREADS / 64)];
+  __shared__ A buf[2][32];
   const uint64_t e0 = drop_base(drop);
   const A scale = (A)drop.scale;
   int turn = 0;
@@ -320,7 +358,7 @@ __device__ __forceinline__ void load_weights(A (&out)[N], const W* w, int c, int
       Vec<W> t;
       t.load(w + c + k * M);
 #pragma unroll
-      for (int j = 0; j < M; ++j) out[k * M + j] = (A)t.e[j];
+      for (int j = 0; j < M; ++j) out[k * M + j] = (A)t.get(j);
     }
   } else {
 #pragma unroll
@@ -340,44 +378,59 @@ __device__ __forceinline__ void row_sum2(A& a, A& b, A* buf) {
 }
 template <int LANES, typename A>
 __device__ __forceinline__ A row_sum(A a, A* buf) {
-  if constexpr (LANES <= 64) {
+  if constexpr (LANES <= 64)
     return lane_sum<LANES>(a);
-  } else {
-    a = lane_sum<64>(a);
-    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = a;
-    __syncthreads();
-    a = A(0);
-#pragma unroll
-    for (int i = 0; i < LANES / 64; ++i) a += buf[i];
-    return a;
-  }
+  else
+    return block_sum<LANES / 64>(a, buf);
 }
 
 constexpr int group_threads(int lanes) { return lanes < 256 ? 256 : lanes; }
 
+// The same value, of which the compiler knows nothing: what is computed or loaded from it in a loop stays there instead of
+// taking a register for the whole kernel.
+template <typename T>
+__device__ __forceinline__ T in_loop(T v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ const T* in_loop_uniform(const T* p) {
+  asm volatile("" : "+s"(p));
+  return p;
+}
+
+// Keeps the instructions of a lane's vectors apart where there are many: interleaved they need every vector's temporaries at
+// once.
+template <int NV>
+__device__ __forceinline__ void one_by_one() {
+  if constexpr (NV > 2) __builtin_amdgcn_sched_barrier(0);
+}
+
 // weights of a lane's columns; absent ones act as `none`
+template <typename A, typename W, int N>
+__device__ __forceinline__ void load_weights_or(A (&out)[N], const W* w, int c, int cols, A none) {
+  if (w) {
+    load_weights<A, W, N>(out, w, c, cols);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) out[j] = none;
+  }
+}
 template <typename A, typename W, int LANES, int NV, int N>
 __device__ __forceinline__ void lane_weights(A (&out)[NV][N], const W* w, int lane, int cols, A none) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (w) {
-      load_weights<A, W, N>(out[i], w, (i * LANES + lane) * N, cols);
-    } else {
-#pragma unroll
-      for (int j = 0; j < N; ++j) out[i][j] = none;
-    }
-  }
+  for (int i = 0; i < NV; ++i) load_weights_or<A, W, N>(out[i], w, (i * LANES + lane) * N, cols, none);
 }
 
 template <typename X, typename W, int LANES, int NV>
-__global__ __launch_bounds__(group_threads(LANES)) void ln_fwd_group_kernel(
+__global__ __launch_bounds__(group_threads(LANES), NV <= 2 || LANES == 1024 ? 4 : NV <= 4 ? 3 : 2) void ln_fwd_group_kernel(
     const X* __restrict__ x, int64_t ldx, const W* __restrict__ w, const W* __restrict__ b, X* __restrict__ y,
     typename Acc<X>::type* __restrict__ mean_out, typename Acc<X>::type* __restrict__ rstd_out, int64_t rows, int cols, double eps,
     Drop drop) {
   typedef typename Acc<X>::type A;
   constexpr int N = Vec<X>::N, RPB = group_threads(LANES) / LANES;
-  constexpr bool HOLD = NV * N <= 8;            // weights stay in registers
-  __shared__ A buf[2][LANES > 64 ? LANES / 64 : 1];
+  constexpr bool HOLD = NV * N <= 8, WIDE = NV * N > 8;      // weights stay in registers; many elements a lane
+  __shared__ A buf[2][LANES > 64 ? 16 : 1];
   const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
   const uint64_t e0 = drop_base(drop);
   const A scale = (A)drop.scale;
@@ -386,6 +439,7 @@ __global__ __launch_bounds__(group_threads(LANES)) void ln_fwd_group_kernel(
     lane_weights<A, W, LANES, NV, N>(wv, w, lane, cols, A(1));
     lane_weights<A, W, LANES, NV, N>(bv, b, lane, cols, A(0));
   }
+  const A inv = A(1) / (A)cols;
   const int64_t step = (int64_t)gridDim.x * RPB;
   Vec<X> next[NV];
   load_row<X, LANES, NV>(next, x + ((int64_t)blockIdx.x * RPB + sub) * ldx, lane, cols, (int64_t)blockIdx.x * RPB + sub < rows);
@@ -400,34 +454,40 @@ __global__ __launch_bounds__(group_threads(LANES)) void ln_fwd_group_kernel(
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int j = 0; j < N; ++j) s += (A)v[i].e[j];
-    const A mean = row_sum<LANES>(s, buf[0]) / (A)cols;
+      for (int j = 0; j < N; ++j) s += v[i].get(j);
+    const A mean = row_sum<LANES>(s, buf[0]) * inv;
+    if constexpr (WIDE)
+#pragma unroll
+      for (int i = 0; i < NV; ++i) v[i].forget();
     A q = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const A d = (i * LANES + lane) * N + j < cols ? (A)v[i].e[j] - mean : A(0);
+        const A d = (i * LANES + lane) * N + j < cols ? v[i].get(j) - mean : A(0);
         q += d * d;
       }
-    const A rstd = A(1) / sqrt(row_sum<LANES>(q, buf[1]) / (A)cols + (A)eps);
+    const A rstd = A(1) / sqrt(row_sum<LANES>(q, buf[1]) * inv + (A)eps);
     if (!live) continue;
-    if constexpr (!HOLD) {
-      lane_weights<A, W, LANES, NV, N>(wv, w, lane, cols, A(1));
-      lane_weights<A, W, LANES, NV, N>(bv, b, lane, cols, A(0));
-    }
+    if constexpr (WIDE)
+#pragma unroll
+      for (int i = 0; i < NV; ++i) v[i].forget();
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      if constexpr (!HOLD) {
+        load_weights_or<A, W, N>(wv[i], in_loop_uniform(w), (i * LANES + lane) * N, cols, A(1));
+        load_weights_or<A, W, N>(bv[i], in_loop_uniform(b), (i * LANES + lane) * N, cols, A(0));
+      }
       A h[N];
 #pragma unroll
-      for (int j = 0; j < N; ++j) h[j] = ((A)v[i].e[j] - mean) * rstd * wv[i][j] + bv[i][j];
+      for (int j = 0; j < N; ++j) h[j] = (v[i].get(j) - mean) * rstd * wv[i][j] + bv[i][j];
       if (drop.mode) {
         const uint32_t bits = keep_bits<N>(drop, e0 + (uint64_t)row * cols + (i * LANES + lane) * N);
 #pragma unroll
         for (int j = 0; j < N; ++j) h[j] = (bits >> j & 1) ? h[j] * scale : A(0);
       }
-#pragma unroll
-      for (int j = 0; j < N; ++j) v[i].e[j] = (X)h[j];
+      v[i].set(h);
+      one_by_one<NV>();
     }
     store_row<X, LANES, NV>(v, y + row * cols, lane, cols);
     if (lane == 0 && mean_out) mean_out[row] = mean, rstd_out[row] = rstd;
@@ -441,17 +501,18 @@ __global__ __launch_bounds__(group_threads(LANES)) void ln_bwd_group_kernel(
     typename Acc<X>::type* __restrict__ part, int64_t rows, int cols, Drop drop) {
   typedef typename Acc<X>::type A;
   constexpr int N = Vec<X>::N, RPB = group_threads(LANES) / LANES;
-  constexpr bool HOLD = NV * N <= 8;
-  __shared__ A buf[2][LANES > 64 ? 2 * (LANES / 64) : 1];
+  // a row's a and h stay in registers between its two halves; the next row's loads are under way meanwhile
+  constexpr bool HOLD = NV * N * (int)sizeof(A) <= 32, AHEAD = NV * N * (int)sizeof(A) + NV * 32 <= 256;
+  __shared__ A buf[2][LANES > 64 ? 32 : 1];
   const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
   const uint64_t e0 = drop_base(drop);
-  const A scale = (A)drop.scale;
+  const A scale = (A)drop.scale, inv = A(1) / (A)cols;
   A aw[NV][N], ab[NV][N], wv[NV][N];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < N; ++j) aw[i][j] = ab[i][j] = A(0);
-  if constexpr (HOLD) lane_weights<A, W, LANES, NV, N>(wv, w, lane, cols, A(1));
+  lane_weights<A, W, LANES, NV, N>(wv, w, lane, cols, A(1));
   const int64_t step = (int64_t)gridDim.x * RPB;
   Vec<X> nx[NV], ng[NV];
   A nmean = 0, nrstd = 0;
@@ -464,47 +525,60 @@ __global__ __launch_bounds__(group_threads(LANES)) void ln_bwd_group_kernel(
   };
   fetch((int64_t)blockIdx.x * RPB + sub);
   int turn = 0;
+#pragma unroll 1
   for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += step, turn ^= 1) {
     const int64_t row = r0 + sub;
     const bool live = row < rows;
     Vec<X> xv[NV], gv[NV];
+    if (!AHEAD && r0 != (int64_t)blockIdx.x * RPB) fetch(row);
 #pragma unroll
     for (int i = 0; i < NV; ++i) xv[i] = nx[i], gv[i] = ng[i];
     const A mean = nmean, rstd = nrstd;
-    if (r0 + step < rows) fetch(row + step);
-    if constexpr (!HOLD) lane_weights<A, W, LANES, NV, N>(wv, w, lane, cols, A(1));
-    A s1 = 0, s2 = 0;
+    if (AHEAD && r0 + step < rows) fetch(row + step);
+    A s1 = 0, s2 = 0, ha[HOLD ? NV : 1][N], aa[HOLD ? NV : 1][N];
     uint32_t bits[NV];
+    // (columns behind the row have dy = 0 and add nothing)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * LANES + lane) * N;
       if (drop.mode) bits[i] = live ? keep_bits<N>(drop, e0 + (uint64_t)row * cols + c) : 0u;
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        A g = (A)gv[i].e[j];
+        A g = gv[i].get(j);
         if (drop.mode) g = (bits[i] >> j & 1) ? g * scale : A(0);
-        const A h = c + j < cols ? ((A)xv[i].e[j] - mean) * rstd : A(0);
-        const A a = g * wv[i][j];
+        const A h = (xv[i].get(j) - mean) * rstd, a = g * wv[i][j];
         s1 += a;
         s2 += a * h;
         aw[i][j] += g * h;
         ab[i][j] += g;
+        if constexpr (HOLD) ha[i][j] = h, aa[i][j] = a;
       }
+      one_by_one<NV>();
     }
     if (!dx) continue;
     row_sum2<LANES>(s1, s2, buf[turn]);
-    s1 /= (A)cols;
-    s2 /= (A)cols;
+    s1 *= inv;
+    s2 *= inv;
     if (!live) continue;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      if constexpr (!HOLD) xv[i].forget(), gv[i].forget();
+      A out[N];
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        A g = (A)gv[i].e[j];
-        if (drop.mode) g = (bits[i] >> j & 1) ? g * scale : A(0);
-        const A h = ((A)xv[i].e[j] - mean) * rstd;
-        gv[i].e[j] = (X)(rstd * (g * wv[i][j] - s1 - h * s2));
+        A h, a;
+        if constexpr (HOLD) {
+          h = ha[i][j], a = aa[i][j];
+        } else {
+          A g = gv[i].get(j);
+          if (drop.mode) g = (bits[i] >> j & 1) ? g * scale : A(0);
+          h = (xv[i].get(j) - mean) * rstd;
+          a = g * wv[i][j];
+        }
+        out[j] = rstd * (a - s1 - h * s2);
       }
+      gv[i].set(out);
+      one_by_one<NV>();
     }
     store_row<X, LANES, NV>(gv, dx + row * cols, lane, cols);
   }
@@ -552,41 +626,92 @@ __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_wave_barrier();
 }
 
-template <typename X, typename A>
-__device__ __forceinline__ void short_load(A* lds, const X* p, int n, int lane, int pad, int inv) {
-  constexpr int N = Vec<X>::N;
-  for (int i = lane * N; i < n; i += 64 * N) {
-    Vec<X> v;
-    if (i + N <= n)
-      v.load(p + i);
-    else
-      v.load_some(p + i, n - i);
+// A tile in registers: n elements from p on, 16 bytes a lane and turn.
+template <typename X, int NC>
+struct Tile {
+  static constexpr int N = Vec<X>::N, IT = NC / N;
+  Vec<X> v[IT];
+  __device__ __forceinline__ void load(const X* p, int n, int lane) {
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (i + j < n) lds[short_pos(i + j, pad, inv)] = (A)v.e[j];
+    for (int t = 0; t < IT; ++t) {
+      const int i = (t * 64 + lane) * N;
+      if (i + N <= n)
+        v[t].load(p + i);
+      else if (i < n)
+        v[t].load_some(p + i, n - i);
+    }
+  }
+};
+// N values to or from consecutive places (pad: with a gap after every row) of a tile in LDS; what lies behind n stays unused
+template <typename A, int N>
+__device__ __forceinline__ void short_put(A* lds, const A (&h)[N], int i, int pad, int inv) {
+  if (!pad) {
+    struct alignas(16) Piece { A e[16 / sizeof(A)]; };
+#pragma unroll
+    for (int k = 0; k < N; k += 16 / (int)sizeof(A)) {
+      Piece q;
+#pragma unroll
+      for (int j = 0; j < 16 / (int)sizeof(A); ++j) q.e[j] = h[k + j];
+      *reinterpret_cast<Piece*>(lds + i + k) = q;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) lds[short_pos(i + j, pad, inv)] = h[j];
+  }
+}
+template <typename A, int N>
+__device__ __forceinline__ void short_get(const A* lds, A (&h)[N], int i, int pad, int inv) {
+  if (!pad) {
+    struct alignas(16) Piece { A e[16 / sizeof(A)]; };
+#pragma unroll
+    for (int k = 0; k < N; k += 16 / (int)sizeof(A)) {
+      const Piece q = *reinterpret_cast<const Piece*>(lds + i + k);
+#pragma unroll
+      for (int j = 0; j < 16 / (int)sizeof(A); ++j) h[k + j] = q.e[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) h[j] = lds[short_pos(i + j, pad, inv)];
   }
 }
 
+// A tile of LDS: 64 rows and room for the last 16 bytes.
+template <typename A, int NC>
+constexpr int short_words() {
+  return 64 * (NC | 1) + 64;
+}
+
 template <typename X, typename W, int NC>
-__global__ __launch_bounds__(64 * SHORT_WAVES) void ln_fwd_short_kernel(
+__global__ __launch_bounds__(64 * SHORT_WAVES, 4) void ln_fwd_short_kernel(
     const X* __restrict__ x, const W* __restrict__ w, const W* __restrict__ b, X* __restrict__ y,
     typename Acc<X>::type* __restrict__ mean_out, typename Acc<X>::type* __restrict__ rstd_out, int64_t rows, int cols, double eps,
     Drop drop) {
   typedef typename Acc<X>::type A;
-  constexpr int N = Vec<X>::N;
-  __shared__ A tile[SHORT_WAVES][64 * (NC | 1)];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int N = Vec<X>::N, IT = Tile<X, NC>::IT;
+  __shared__ alignas(16) A tile[SHORT_WAVES][short_words<A, NC>()];
+  const int wave = threadIdx.x >> 6;
   A* lds = tile[wave];
   const int pad = cols % 2 == 0, pitch = cols | 1, inv = (65536 + cols - 1) / cols;
   const uint64_t e0 = drop_base(drop);
   const A scale = (A)drop.scale;
-  const int64_t tiles = (rows + 63) / 64;
-  for (int64_t t = (int64_t)blockIdx.x * SHORT_WAVES + wave; t < tiles; t += (int64_t)gridDim.x * SHORT_WAVES) {
+  const int64_t tiles = (rows + 63) / 64, step = (int64_t)gridDim.x * SHORT_WAVES;
+  auto elements = [&](int64_t t) { return (int)min((int64_t)64, rows - t * 64) * cols; };
+#pragma unroll 1
+  for (int64_t t = (int64_t)blockIdx.x * SHORT_WAVES + wave; t < tiles; t += step) {
     const int64_t row0 = t * 64;
-    const int nr = (int)min((int64_t)64, rows - row0), n = nr * cols;
-    short_load<X, A>(lds, x + row0 * cols, n, lane, pad, inv);
+    const int n = elements(t), lane = in_loop((int)(threadIdx.x & 63));
+    Tile<X, NC> in;
+    in.load(x + row0 * cols, n, lane);
+#pragma unroll
+    for (int k = 0; k < IT; ++k) {
+      const int i = (k * 64 + lane) * N;
+      A h[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) h[j] = in.v[k].get(j);
+      if (i < n) short_put<A, N>(lds, h, i, pad, inv);
+    }
     wave_lds_fence();
-    if (lane < nr) {
+    if (lane * cols < n) {
       A v[NC], s = 0, q = 0;
 #pragma unroll
       for (int c = 0; c < NC; ++c)
@@ -608,88 +733,19 @@ __global__ __launch_bounds__(64 * SHORT_WAVES) void ln_fwd_short_kernel(
     }
     wave_lds_fence();
     X* out = y + row0 * cols;
-    for (int i = lane * N; i < n; i += 64 * N) {
-      Vec<X> v;
-      const uint32_t bits = keep_bits<N>(drop, e0 + (uint64_t)row0 * cols + i);
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        A h = i + j < n ? lds[short_pos(i + j, pad, inv)] : A(0);
-        if (drop.mode) h = (bits >> j & 1) ? h * scale : A(0);
-        v.e[j] = (X)h;
-      }
-      if (i + N <= n)
-        v.store(out + i);
-      else
-        v.store_some(out + i, n - i);
-    }
-    wave_lds_fence();
-  }
-}
-
-template <typename X, typename W, int NC>
-__global__ __launch_bounds__(64 * SHORT_WAVES) void ln_bwd_short_kernel(
-    const X* __restrict__ dy, const X* __restrict__ x, const W* __restrict__ w, const typename Acc<X>::type* __restrict__ mean_in,
-    const typename Acc<X>::type* __restrict__ rstd_in, X* __restrict__ dx, typename Acc<X>::type* __restrict__ part, int64_t rows,
-    int cols, Drop drop) {
-  typedef typename Acc<X>::type A;
-  constexpr int N = Vec<X>::N;
-  __shared__ A tile[SHORT_WAVES][2][64 * (NC | 1)];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  A *lx = tile[wave][0], *lg = tile[wave][1];
-  const int pad = cols % 2 == 0, pitch = cols | 1, inv = (65536 + cols - 1) / cols;
-  const uint64_t e0 = drop_base(drop);
-  const A scale = (A)drop.scale;
-  A aw[NC], ab[NC];
+    for (int k = 0; k < IT; ++k) {
+      const int i = (k * 64 + lane) * N;
+      if (i < n) {
+        A h[N];
+        short_get<A, N>(lds, h, i, pad, inv);
+        if (drop.mode) {
+          const uint32_t bits = keep_bits<N>(drop, e0 + (uint64_t)row0 * cols + i);
 #pragma unroll
-  for (int c = 0; c < NC; ++c) aw[c] = ab[c] = A(0);
-  const int64_t tiles = (rows + 63) / 64;
-  for (int64_t t = (int64_t)blockIdx.x * SHORT_WAVES + wave; t < tiles; t += (int64_t)gridDim.x * SHORT_WAVES) {
-    const int64_t row0 = t * 64;
-    const int nr = (int)min((int64_t)64, rows - row0), n = nr * cols;
-    short_load<X, A>(lx, x + row0 * cols, n, lane, pad, inv);
-    const X* gp = dy + row0 * cols;
-    for (int i = lane * N; i < n; i += 64 * N) {
-      Vec<X> v;
-      if (i + N <= n)
-        v.load(gp + i);
-      else
-        v.load_some(gp + i, n - i);
-      const uint32_t bits = keep_bits<N>(drop, e0 + (uint64_t)row0 * cols + i);
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        A g = (A)v.e[j];
-        if (drop.mode) g = (bits >> j & 1) ? g * scale : A(0);
-        if (i + j < n) lg[short_pos(i + j, pad, inv)] = g;
-      }
-    }
-    wave_lds_fence();
-    if (lane < nr) {
-      const A mean = mean_in[row0 + lane], rstd = rstd_in[row0 + lane];
-      A h[NC], g[NC], s1 = 0, s2 = 0;
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-        if (c < cols) {
-          h[c] = (lx[lane * pitch + c] - mean) * rstd;
-          g[c] = lg[lane * pitch + c];
-          aw[c] += g[c] * h[c];
-          ab[c] += g[c];
-          if (w) g[c] *= (A)w[c];
-          s1 += g[c];
-          s2 += g[c] * h[c];
+          for (int j = 0; j < N; ++j) h[j] = (bits >> j & 1) ? h[j] * scale : A(0);
         }
-      s1 /= (A)cols;
-      s2 /= (A)cols;
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-        if (c < cols) lg[lane * pitch + c] = rstd * (g[c] - s1 - h[c] * s2);
-    }
-    wave_lds_fence();
-    if (dx) {
-      X* out = dx + row0 * cols;
-      for (int i = lane * N; i < n; i += 64 * N) {
         Vec<X> v;
-#pragma unroll
-        for (int j = 0; j < N; ++j) v.e[j] = (X)(i + j < n ? lg[short_pos(i + j, pad, inv)] : A(0));
+        v.set(h);
         if (i + N <= n)
           v.store(out + i);
         else
@@ -698,7 +754,103 @@ __global__ __launch_bounds__(64 * SHORT_WAVES) void ln_bwd_short_kernel(
     }
     wave_lds_fence();
   }
+}
+
+template <typename X, typename W, int NC>
+__global__ __launch_bounds__(64 * SHORT_WAVES, 2) void ln_bwd_short_kernel(
+    const X* __restrict__ dy, const X* __restrict__ x, const W* __restrict__ w, const typename Acc<X>::type* __restrict__ mean_in,
+    const typename Acc<X>::type* __restrict__ rstd_in, X* __restrict__ dx, typename Acc<X>::type* __restrict__ part, int64_t rows,
+    int cols, Drop drop) {
+  typedef typename Acc<X>::type A;
+  constexpr int N = Vec<X>::N, IT = Tile<X, NC>::IT;
+  __shared__ alignas(16) A tile[SHORT_WAVES][short_words<A, NC>()];
+  const int wave = threadIdx.x >> 6;
+  A* lds = tile[wave];
+  const int pad = cols % 2 == 0, pitch = cols | 1, inv = (65536 + cols - 1) / cols;
+  const uint64_t e0 = drop_base(drop);
+  const A scale = (A)drop.scale;
+  A aw[NC], ab[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) aw[c] = ab[c] = A(0);
+  const int64_t tiles = (rows + 63) / 64, step = (int64_t)gridDim.x * SHORT_WAVES;
+  auto elements = [&](int64_t t) { return (int)min((int64_t)64, rows - t * 64) * cols; };
+#pragma unroll 1
+  for (int64_t t = (int64_t)blockIdx.x * SHORT_WAVES + wave; t < tiles; t += step) {
+    const int64_t row0 = t * 64;
+    const int n = elements(t), lane = in_loop((int)(threadIdx.x & 63));
+    const bool live = lane * cols < n;
+    Tile<X, NC> nx, ng;
+    nx.load(x + row0 * cols, n, lane);
+    ng.load(dy + row0 * cols, n, lane);
+    const A mean = live ? mean_in[row0 + lane] : A(0), rstd = live ? rstd_in[row0 + lane] : A(0);
+    A h[NC], g[NC], s1 = 0, s2 = 0;
+    // both tiles change hands in the same piece of LDS: x, then dy, then dx
+#pragma unroll
+    for (int k = 0; k < IT; ++k) {
+      const int i = (k * 64 + lane) * N;
+      A f[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) f[j] = nx.v[k].get(j);
+      if (i < n) short_put<A, N>(lds, f, i, pad, inv);
+    }
+    wave_lds_fence();
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      if (c < cols) h[c] = live ? (lds[lane * pitch + c] - mean) * rstd : A(0);
+    wave_lds_fence();
+#pragma unroll
+    for (int k = 0; k < IT; ++k) {
+      const int i = (k * 64 + lane) * N;
+      A f[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) f[j] = ng.v[k].get(j);
+      if (drop.mode) {
+        const uint32_t bits = keep_bits<N>(drop, e0 + (uint64_t)row0 * cols + i);
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] = (bits >> j & 1) ? f[j] * scale : A(0);
+      }
+      if (i < n) short_put<A, N>(lds, f, i, pad, inv);
+    }
+    wave_lds_fence();
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      if (c < cols) {
+        g[c] = live ? lds[lane * pitch + c] : A(0);
+        aw[c] += g[c] * h[c];
+        ab[c] += g[c];
+        if (w) g[c] *= (A)w[c];
+        s1 += g[c];
+        s2 += g[c] * h[c];
+      }
+    wave_lds_fence();
+    if (dx) {
+      s1 /= (A)cols;
+      s2 /= (A)cols;
+      if (live)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          if (c < cols) lds[lane * pitch + c] = rstd * (g[c] - s1 - h[c] * s2);
+      wave_lds_fence();
+      X* out = dx + row0 * cols;
+#pragma unroll
+      for (int k = 0; k < IT; ++k) {
+        const int i = (k * 64 + lane) * N;
+        if (i < n) {
+          A f[N];
+          short_get<A, N>(lds, f, i, pad, inv);
+          Vec<X> v;
+          v.set(f);
+          if (i + N <= n)
+            v.store(out + i);
+          else
+            v.store_some(out + i, n - i);
+        }
+      }
+      wave_lds_fence();
+    }
+  }
   if (!part) return;
+  const int lane = threadIdx.x & 63;
   __shared__ A red[SHORT_WAVES][2][NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c)
@@ -740,41 +892,42 @@ __global__ __launch_bounds__(256) void dropout_kernel(const X* x, X* y, int64_t 
     const int64_t i = a - s;                                // a thread's elements are i .. i + E - 1
     const bool whole = i >= 0 && i + E <= n;
     Vec<X> v[V];
-    if (whole) {
 #pragma unroll
-      for (int k = 0; k < V; ++k) v[k].load(x + i + k * N);
-    } else {
-#pragma unroll
-      for (int k = 0; k < V; ++k)
-#pragma unroll
-        for (int j = 0; j < N; ++j) v[k].e[j] = i + k * N + j >= 0 && i + k * N + j < n ? x[i + k * N + j] : (X)A(0);
-    }
-    if (drop.mode == 1) {
-#pragma unroll
-      for (int q = 0; q < E / 4; ++q) {
-        uint32_t w[4];
-        philox(drop, b0 + (uint64_t)(a >> 2) + q, w);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          X& t = v[(4 * q + j) / N].e[(4 * q + j) % N];
-          t = (X)(w[j] >= drop.threshold ? (A)t * scale : A(0));
-        }
-      }
-    } else if (drop.mode == 2) {
-#pragma unroll
-      for (int k = 0; k < V; ++k)
-#pragma unroll
-        for (int j = 0; j < N; ++j) v[k].e[j] = (X)A(0);
-    }
-    if (whole) {
-#pragma unroll
-      for (int k = 0; k < V; ++k) v[k].store(y + i + k * N);
-    } else {
-#pragma unroll
-      for (int k = 0; k < V; ++k)
+    for (int k = 0; k < V; ++k) {
+      if (whole) {
+        v[k].load(x + i + k * N);
+      } else {
+        v[k].u[0] = v[k].u[1] = v[k].u[2] = v[k].u[3] = 0;
 #pragma unroll
         for (int j = 0; j < N; ++j)
-          if (i + k * N + j >= 0 && i + k * N + j < n) y[i + k * N + j] = v[k].e[j];
+          if (i + k * N + j >= 0 && i + k * N + j < n) v[k].put(j, x[i + k * N + j]);
+      }
+    }
+    if (drop.mode) {
+      uint32_t w[E / 4][4];
+      if (drop.mode == 1)
+#pragma unroll
+        for (int q = 0; q < E / 4; ++q) philox(drop, b0 + (uint64_t)(a >> 2) + q, w[q]);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        A h[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const int at = k * N + j;
+          h[j] = drop.mode == 1 && w[at / 4][at % 4] >= drop.threshold ? v[k].get(j) * scale : A(0);
+        }
+        v[k].set(h);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      if (whole) {
+        v[k].store(y + i + k * N);
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (i + k * N + j >= 0 && i + k * N + j < n) y[i + k * N + j] = v[k].element(j);
+      }
     }
   }
 }
@@ -807,7 +960,9 @@ bool types_ok(int dtype, int wdtype) {
 struct Layout {
   int lanes, nv;     // lanes 1: short dense rows, nv columns at most; lanes 0: longer than the registers hold
 };
-Layout row_layout(int dtype, int cols, bool dense) {
+// Forward: few lanes with many elements each (rows of a workgroup of 256 run beside each other).  Backward: two sums stay
+// beside every element, so wide rows take more lanes.
+Layout row_layout(int dtype, int cols, bool dense, bool backward) {
   if (dense && cols <= (dtype == 0 ? 16 : 32)) return {1, (cols + 7) / 8 * 8};
   const int n = dtype == 0 ? 2 : dtype == 1 ? 4 : 8;         // elements of a 16-byte vector
   const int64_t nvec = ((int64_t)cols + n - 1) / n;
@@ -817,10 +972,10 @@ Layout row_layout(int dtype, int cols, bool dense) {
   if (nvec <= 64) return {64, 1};
   if (nvec <= 128) return {64, 2};
   if (nvec <= 256) return half ? Layout{256, 1} : Layout{64, 4};
-  if (nvec <= 512) return half ? Layout{512, 1} : Layout{256, 2};
-  if (nvec <= 1024) return half ? Layout{1024, 1} : Layout{512, 2};
-  if (nvec <= 2048) return {1024, 2};
-  if (nvec <= 4096 && !half) return {1024, 4};
+  if (nvec <= 512) return half && backward ? Layout{512, 1} : Layout{256, 2};
+  if (nvec <= 1024) return backward ? (half ? Layout{1024, 1} : Layout{512, 2}) : Layout{256, 4};
+  if (nvec <= 2048) return backward ? (half ? Layout{512, 4} : Layout{1024, 2}) : Layout{256, 8};
+  if (nvec <= 4096 && !half) return backward ? Layout{512, 8} : Layout{1024, 4};
   return {0, 0};
 }
 
@@ -828,7 +983,8 @@ Layout row_layout(int dtype, int cols, bool dense) {
 // one partial row of column sums per workgroup).
 int row_groups(const Layout& l, int64_t rows, bool backward) {
   const int64_t rpb = l.lanes == 1 ? 64 * SHORT_WAVES : max(1, 256 / l.lanes);
-  const int per_cu = l.lanes <= 256 ? (backward ? 4 : 8) : l.lanes == 512 ? (backward ? 2 : 4) : (backward ? 1 : 2);
+  const int per_cu = l.lanes <= 256 ? (backward ? 4 : l.nv >= 4 ? 4 : 8) : l.lanes == 512 ? (backward ? (l.nv >= 4 ? 1 : 2) : 4)
+                                                                                         : (backward ? 1 : 2);
   return (int)min((rows + rpb - 1) / rpb, (int64_t)(per_cu * CUS));
 }
 
@@ -856,48 +1012,52 @@ constexpr int type_code() {
   return sizeof(X) == 8 ? 0 : sizeof(X) == 4 ? 1 : 2;      // (layouts depend on the size alone)
 }
 
-// K(LANES, NV) of a layout, S(NC) of short rows
-#define TTK_BY_LAYOUT(K, S)                                 \
-  if (l.lanes == 1) {                                       \
-    switch (l.nv) {                                         \
-      case 8: S(8); break;                                  \
-      case 16: S(16); break;                                \
-      case 24:                                              \
-        if constexpr (sizeof(X) < 8) { S(24); }             \
-        break;                                              \
-      case 32:                                              \
-        if constexpr (sizeof(X) < 8) { S(32); }             \
-        break;                                              \
-    }                                                       \
-  } else if constexpr (sizeof(X) == 2) {                    \
-    switch (l.lanes * 16 + l.nv) {                          \
-      case 16 * 16 + 1: K(16, 1); break;                    \
-      case 64 * 16 + 1: K(64, 1); break;                    \
-      case 64 * 16 + 2: K(64, 2); break;                    \
-      case 256 * 16 + 1: K(256, 1); break;                  \
-      case 512 * 16 + 1: K(512, 1); break;                  \
-      case 1024 * 16 + 1: K(1024, 1); break;                \
-      case 1024 * 16 + 2: K(1024, 2); break;                \
-    }                                                       \
-  } else {                                                  \
-    switch (l.lanes * 16 + l.nv) {                          \
-      case 16 * 16 + 1: K(16, 1); break;                    \
-      case 16 * 16 + 2: K(16, 2); break;                    \
-      case 64 * 16 + 1: K(64, 1); break;                    \
-      case 64 * 16 + 2: K(64, 2); break;                    \
-      case 64 * 16 + 4: K(64, 4); break;                    \
-      case 256 * 16 + 2: K(256, 2); break;                  \
-      case 512 * 16 + 2: K(512, 2); break;                  \
-      case 1024 * 16 + 2: K(1024, 2); break;                \
-      case 1024 * 16 + 4: K(1024, 4); break;                \
-    }                                                       \
+// S(NC) of short rows; K(LANES, NV) of the layouts forward and backward share
+#define TTK_SHORT(S)                                        \
+  switch (l.nv) {                                           \
+    case 8: S(8); break;                                    \
+    case 16: S(16); break;                                  \
+    case 24:                                                \
+      if constexpr (sizeof(X) < 8) { S(24); }               \
+      break;                                                \
+    case 32:                                                \
+      if constexpr (sizeof(X) < 8) { S(32); }               \
+      break;                                                \
+  }
+#define TTK_LAYOUT(L, V, K) \
+  case L * 16 + V: K(L, V); break
+#define TTK_FWD_LAYOUTS(K)                                                                             \
+  if constexpr (sizeof(X) == 2) {                                                                      \
+    switch (l.lanes * 16 + l.nv) {                                                                     \
+      TTK_LAYOUT(16, 1, K); TTK_LAYOUT(64, 1, K); TTK_LAYOUT(64, 2, K); TTK_LAYOUT(256, 1, K);         \
+      TTK_LAYOUT(256, 2, K); TTK_LAYOUT(256, 4, K); TTK_LAYOUT(256, 8, K);                             \
+    }                                                                                                  \
+  } else {                                                                                             \
+    switch (l.lanes * 16 + l.nv) {                                                                     \
+      TTK_LAYOUT(16, 1, K); TTK_LAYOUT(16, 2, K); TTK_LAYOUT(64, 1, K); TTK_LAYOUT(64, 2, K);          \
+      TTK_LAYOUT(64, 4, K); TTK_LAYOUT(256, 2, K); TTK_LAYOUT(256, 4, K); TTK_LAYOUT(256, 8, K);       \
+      TTK_LAYOUT(1024, 4, K);                                                                          \
+    }                                                                                                  \
+  }
+#define TTK_BWD_LAYOUTS(K)                                                                             \
+  if constexpr (sizeof(X) == 2) {                                                                      \
+    switch (l.lanes * 16 + l.nv) {                                                                     \
+      TTK_LAYOUT(16, 1, K); TTK_LAYOUT(64, 1, K); TTK_LAYOUT(64, 2, K); TTK_LAYOUT(256, 1, K);         \
+      TTK_LAYOUT(512, 1, K); TTK_LAYOUT(1024, 1, K); TTK_LAYOUT(512, 4, K);                            \
+    }                                                                                                  \
+  } else {                                                                                             \
+    switch (l.lanes * 16 + l.nv) {                                                                     \
+      TTK_LAYOUT(16, 1, K); TTK_LAYOUT(16, 2, K); TTK_LAYOUT(64, 1, K); TTK_LAYOUT(64, 2, K);          \
+      TTK_LAYOUT(64, 4, K); TTK_LAYOUT(256, 2, K); TTK_LAYOUT(512, 2, K); TTK_LAYOUT(1024, 2, K);      \
+      TTK_LAYOUT(512, 8, K);                                                                           \
+    }                                                                                                  \
   }
 
 template <typename X, typename W>
 int ln_fwd(const void* x, int64_t ldx, const void* w, const void* b, void* y, void* mean, void* rstd, int64_t rows, int cols,
            double eps, const Drop& d, hipStream_t st) {
   typedef typename Acc<X>::type A;
-  const Layout l = row_layout(type_code<X>(), cols, ldx == cols || rows == 1);
+  const Layout l = row_layout(type_code<X>(), cols, ldx == cols || rows == 1, false);
   if (!l.lanes) {
     hipLaunchKernelGGL((ln_fwd_long_kernel<X, W>), dim3((unsigned)min(rows, (int64_t)(4 * CUS))), dim3(LONG_THREADS), 0, st,
                        (const X*)x, ldx, (const W*)w, (const W*)b, (X*)y, (A*)mean, (A*)rstd, rows, cols, eps, d);
@@ -910,7 +1070,10 @@ int ln_fwd(const void* x, int64_t ldx, const void* w, const void* b, void* y, vo
 #define S(NC)                                                                                                             \
   hipLaunchKernelGGL((ln_fwd_short_kernel<X, W, NC>), grid, dim3(64 * SHORT_WAVES), 0, st, (const X*)x, (const W*)w,       \
                      (const W*)b, (X*)y, (A*)mean, (A*)rstd, rows, cols, eps, d)
-  TTK_BY_LAYOUT(K, S)
+  if (l.lanes == 1)
+    TTK_SHORT(S)
+  else
+    TTK_FWD_LAYOUTS(K)
 #undef K
 #undef S
   return status();
@@ -920,7 +1083,7 @@ template <typename X, typename W>
 int ln_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, const void* mean, const void* rstd, void* dx,
            void* dw, void* db, int64_t rows, int cols, const Drop& d, void* ws, int64_t ws_bytes, hipStream_t st) {
   typedef typename Acc<X>::type A;
-  const Layout l = row_layout(type_code<X>(), cols, (ldx == cols && lddy == cols) || rows == 1);
+  const Layout l = row_layout(type_code<X>(), cols, (ldx == cols && lddy == cols) || rows == 1, true);
   const int parts = bwd_parts(l, rows, cols);
   const bool sums = dw || db;
   if (sums && (!ws || ws_bytes < (int64_t)parts * 2 * cols * (int64_t)sizeof(A))) return TTK_EWORKSPACE;
@@ -933,7 +1096,10 @@ int ln_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void*
 #define S(NC)                                                                                                             \
   hipLaunchKernelGGL((ln_bwd_short_kernel<X, W, NC>), dim3((unsigned)parts), dim3(64 * SHORT_WAVES), 0, st, (const X*)dy,  \
                      (const X*)x, (const W*)w, (const A*)mean, (const A*)rstd, (X*)dx, part, rows, cols, d)
-    TTK_BY_LAYOUT(K, S)
+    if (l.lanes == 1)
+      TTK_SHORT(S)
+    else
+      TTK_BWD_LAYOUTS(K)
 #undef K
 #undef S
   } else if (!l.lanes) {
@@ -980,7 +1146,7 @@ int ttk_layer_norm(int dtype, int wdtype, const void* x, int64_t ldx, const void
 
 int64_t ttk_layer_norm_backward_ws_bytes(int dtype, int64_t rows, int cols) {
   if (dtype < 0 || dtype > 3 || rows < 1 || cols < 1) return TTK_EINVAL;
-  const int parts = max(bwd_parts(row_layout(dtype, cols, true), rows, cols), bwd_parts(row_layout(dtype, cols, false), rows, cols));
+  const int parts = max(bwd_parts(row_layout(dtype, cols, true, true), rows, cols), bwd_parts(row_layout(dtype, cols, false, true), rows, cols));
   return (int64_t)parts * 2 * cols * (dtype == 0 ? 8 : 4);
 }
 
