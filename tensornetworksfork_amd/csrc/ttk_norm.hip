@@ -146,6 +146,51 @@ __device__ __forceinline__ uint32_t keep_bits(const Drop& d, uint64_t e) {
   return bits >> s;
 }
 
+// Bits of the N elements from e on where the next lane has those from e + N on (N a multiple of 4, e mod 4 the same in the
+// wave): a block that reaches into the next lane's elements comes from there, and behind the wave's last lane from the scalar
+// unit.
+template <int N>
+__device__ __forceinline__ uint32_t keep_bits_wave(const Drop& d, uint64_t e) {
+  if (d.mode == 0) return ~0u;
+  if (d.mode == 2) return 0u;
+  constexpr int NB = N / 4;
+  const uint64_t b = e >> 2;
+  uint32_t bits = philox_keep4(d, b);
+#pragma unroll
+  for (int i = 1; i < NB; ++i) bits |= philox_keep4(d, b + i) << (4 * i);
+  const int s = __builtin_amdgcn_readfirstlane((int)(e & 3));
+  if (s) {
+    const uint64_t b0 = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32 |
+                        (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b);
+    const uint64_t end = b0 + 64 * NB;      // (the first lane is lane 0)
+    uint32_t c0 = (uint32_t)end, c1 = (uint32_t)(end >> 32), c2 = 0, c3 = 0, k0 = d.k0, k1 = d.k1;
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+      const uint64_t p0 = (uint64_t)c0 * 0xD2511F53u, p1 = (uint64_t)c2 * 0xCD9E8D57u;
+      c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0;
+      c1 = (uint32_t)p1;
+      c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1;
+      c3 = (uint32_t)p0;
+      k0 += 0x9E3779B9u;
+      k1 += 0xBB67AE85u;
+    }
+    const uint32_t t = d.threshold;
+    const uint32_t last = (uint32_t)(c0 >= t) | ((uint32_t)(c1 >= t) << 1) | ((uint32_t)(c2 >= t) << 2) | ((uint32_t)(c3 >= t) << 3);
+    const uint32_t next = (uint32_t)__builtin_amdgcn_update_dpp((int)last, (int)bits, 0x130, 0xf, 0xf, false);      // lane + 1
+    bits |= (next & 0xF) << N;
+  }
+  return bits >> s;
+}
+
+// Bits of a lane's N elements of a row that LANES lanes share.
+template <int N, int LANES>
+__device__ __forceinline__ uint32_t keep_bits_row(const Drop& d, uint64_t e) {
+  if constexpr (LANES >= 64 && N % 4 == 0)
+    return keep_bits_wave<N>(d, e);
+  else
+    return keep_bits<N>(d, e);
+}
+
 // ---------------------------------------------------------------------------------------
 // Sums
 // ---------------------------------------------------------------------------------------
@@ -303,8 +348,17 @@ __global__ __launch_bounds__(1024) void ln_cols_sum_kernel(const A* __restrict__
   W* out = blockIdx.y ? db : dw;
   const A* p = part + (int64_t)blockIdx.y * cols;
   double s = 0;
-  if (c < cols)
-    for (int g = ty; g < nparts; g += 16) s += (double)p[(int64_t)g * 2 * cols + c];
+  if (c < cols) {
+    int g = ty;
+    for (; g + 7 * 16 < nparts; g += 8 * 16) {      // eight loads under way
+      A v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = p[(int64_t)(g + 16 * k) * 2 * cols + c];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += (double)v[k];
+    }
+    for (; g < nparts; g += 16) s += (double)p[(int64_t)g * 2 * cols + c];
+  }
   red[ty][threadIdx.x & 63] = s;
   __syncthreads();
   if (ty == 0 && c < cols && out) {
@@ -423,13 +477,13 @@ __device__ __forceinline__ void lane_weights(A (&out)[NV][N], const W* w, int la
 }
 
 template <typename X, typename W, int LANES, int NV>
-__global__ __launch_bounds__(group_threads(LANES), NV <= 2 || LANES == 1024 ? 4 : NV <= 4 ? 3 : 2) void ln_fwd_group_kernel(
+__global__ __launch_bounds__(group_threads(LANES), NV <= 2 || LANES >= 512 ? 4 : 3) void ln_fwd_group_kernel(
     const X* __restrict__ x, int64_t ldx, const W* __restrict__ w, const W* __restrict__ b, X* __restrict__ y,
     typename Acc<X>::type* __restrict__ mean_out, typename Acc<X>::type* __restrict__ rstd_out, int64_t rows, int cols, double eps,
     Drop drop) {
   typedef typename Acc<X>::type A;
   constexpr int N = Vec<X>::N, RPB = group_threads(LANES) / LANES;
-  constexpr bool HOLD = NV * N <= 8, WIDE = NV * N > 8;      // weights stay in registers; many elements a lane
+  constexpr bool HOLD = NV * N <= 16, WIDE = NV * N > 16;      // weights stay in registers; many elements a lane
   __shared__ A buf[2][LANES > 64 ? 16 : 1];
   const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
   const uint64_t e0 = drop_base(drop);
@@ -482,7 +536,7 @@ __global__ __launch_bounds__(group_threads(LANES), NV <= 2 || LANES == 1024 ? 4 
 #pragma unroll
       for (int j = 0; j < N; ++j) h[j] = (v[i].get(j) - mean) * rstd * wv[i][j] + bv[i][j];
       if (drop.mode) {
-        const uint32_t bits = keep_bits<N>(drop, e0 + (uint64_t)row * cols + (i * LANES + lane) * N);
+        const uint32_t bits = keep_bits_row<N, LANES>(drop, e0 + (uint64_t)row * cols + (i * LANES + lane) * N);
 #pragma unroll
         for (int j = 0; j < N; ++j) h[j] = (bits >> j & 1) ? h[j] * scale : A(0);
       }
@@ -541,7 +595,7 @@ __global__ __launch_bounds__(group_threads(LANES)) void ln_bwd_group_kernel(
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * LANES + lane) * N;
-      if (drop.mode) bits[i] = live ? keep_bits<N>(drop, e0 + (uint64_t)row * cols + c) : 0u;
+      if (drop.mode) bits[i] = live ? keep_bits_row<N, LANES>(drop, e0 + (uint64_t)row * cols + c) : 0u;
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         A g = gv[i].get(j);
@@ -974,7 +1028,7 @@ Layout row_layout(int dtype, int cols, bool dense, bool backward) {
   if (nvec <= 256) return half ? Layout{256, 1} : Layout{64, 4};
   if (nvec <= 512) return half && backward ? Layout{512, 1} : Layout{256, 2};
   if (nvec <= 1024) return backward ? (half ? Layout{1024, 1} : Layout{512, 2}) : Layout{256, 4};
-  if (nvec <= 2048) return backward ? (half ? Layout{512, 4} : Layout{1024, 2}) : Layout{256, 8};
+  if (nvec <= 2048) return backward ? (half ? Layout{512, 4} : Layout{1024, 2}) : Layout{512, 4};
   if (nvec <= 4096 && !half) return backward ? Layout{512, 8} : Layout{1024, 4};
   return {0, 0};
 }
@@ -1030,12 +1084,12 @@ constexpr int type_code() {
   if constexpr (sizeof(X) == 2) {                                                                      \
     switch (l.lanes * 16 + l.nv) {                                                                     \
       TTK_LAYOUT(16, 1, K); TTK_LAYOUT(64, 1, K); TTK_LAYOUT(64, 2, K); TTK_LAYOUT(256, 1, K);         \
-      TTK_LAYOUT(256, 2, K); TTK_LAYOUT(256, 4, K); TTK_LAYOUT(256, 8, K);                             \
+      TTK_LAYOUT(256, 2, K); TTK_LAYOUT(256, 4, K); TTK_LAYOUT(512, 4, K);                             \
     }                                                                                                  \
   } else {                                                                                             \
     switch (l.lanes * 16 + l.nv) {                                                                     \
       TTK_LAYOUT(16, 1, K); TTK_LAYOUT(16, 2, K); TTK_LAYOUT(64, 1, K); TTK_LAYOUT(64, 2, K);          \
-      TTK_LAYOUT(64, 4, K); TTK_LAYOUT(256, 2, K); TTK_LAYOUT(256, 4, K); TTK_LAYOUT(256, 8, K);       \
+      TTK_LAYOUT(64, 4, K); TTK_LAYOUT(256, 2, K); TTK_LAYOUT(256, 4, K); TTK_LAYOUT(512, 4, K);       \
       TTK_LAYOUT(1024, 4, K);                                                                          \
     }                                                                                                  \
   }
