@@ -595,7 +595,7 @@ __global__ __launch_bounds__(group_threads(LANES)) void ln_bwd_group_kernel(
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * LANES + lane) * N;
-      if (drop.mode) bits[i] = live ? keep_bits_row<N, LANES>(drop, e0 + (uint64_t)row * cols + c) : 0u;
+      if (drop.mode) bits[i] = live ? keep_bits_row<N, NV == 1 ? LANES : 1>(drop, e0 + (uint64_t)row * cols + c) : 0u;
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         A g = gv[i].get(j);
@@ -746,6 +746,12 @@ __global__ __launch_bounds__(64 * SHORT_WAVES, 4) void ln_fwd_short_kernel(
   const int wave = threadIdx.x >> 6;
   A* lds = tile[wave];
   const int pad = cols % 2 == 0, pitch = cols | 1, inv = (65536 + cols - 1) / cols;
+  __shared__ alignas(16) A weights[2][NC];      // (behind the row 0; read in the tiles' loop in one go, a load a column would wait a column)
+  if (threadIdx.x < NC) {
+    weights[0][threadIdx.x] = threadIdx.x < cols ? (w ? (A)w[threadIdx.x] : A(1)) : A(0);
+    weights[1][threadIdx.x] = threadIdx.x < cols && b ? (A)b[threadIdx.x] : A(0);
+  }
+  __syncthreads();
   const uint64_t e0 = drop_base(drop);
   const A scale = (A)drop.scale;
   const int64_t tiles = (rows + 63) / 64, step = (int64_t)gridDim.x * SHORT_WAVES;
@@ -765,24 +771,29 @@ __global__ __launch_bounds__(64 * SHORT_WAVES, 4) void ln_fwd_short_kernel(
       if (i < n) short_put<A, N>(lds, h, i, pad, inv);
     }
     wave_lds_fence();
+    A v[NC], s = 0, q = 0;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) v[c] = lds[lane * pitch + c];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) s += c < cols ? v[c] : A(0);
+    const A mean = s / (A)cols;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      v[c] = c < cols ? v[c] - mean : A(0);
+      q += v[c] * v[c];
+    }
+    const A rstd = A(1) / sqrt(q / (A)cols + (A)eps);
     if (lane * cols < n) {
-      A v[NC], s = 0, q = 0;
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
-        if (c < cols) v[c] = lds[lane * pitch + c], s += v[c];
-      const A mean = s / (A)cols;
+      for (int k = 0; k < NC; k += 8) {
+        A wv[8], bv[8];
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
-        if (c < cols) v[c] -= mean, q += v[c] * v[c];
-      const A rstd = A(1) / sqrt(q / (A)cols + (A)eps);
+        for (int c = 0; c < 8; ++c) wv[c] = weights[0][k + c], bv[c] = weights[1][k + c];
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
-        if (c < cols) {
-          A h = v[c] * rstd;
-          if (w) h *= (A)w[c];
-          if (b) h += (A)b[c];
-          lds[lane * pitch + c] = h;
-        }
+        for (int c = 0; c < 8; ++c)
+          if (k + c < cols) lds[lane * pitch + k + c] = v[k + c] * rstd * wv[c] + bv[c];
+        __builtin_amdgcn_sched_barrier(0);
+      }
       if (mean_out) mean_out[row0 + lane] = mean, rstd_out[row0 + lane] = rstd;
     }
     wave_lds_fence();
@@ -821,6 +832,11 @@ __global__ __launch_bounds__(64 * SHORT_WAVES, 2) void ln_bwd_short_kernel(
   const int wave = threadIdx.x >> 6;
   A* lds = tile[wave];
   const int pad = cols % 2 == 0, pitch = cols | 1, inv = (65536 + cols - 1) / cols;
+  __shared__ alignas(16) A weights[1][NC];      // (behind the row 0; read in the tiles' loop in one go, a load a column would wait a column)
+  if (threadIdx.x < NC) {
+    weights[0][threadIdx.x] = threadIdx.x < cols ? (w ? (A)w[threadIdx.x] : A(1)) : A(0);
+  }
+  __syncthreads();
   const uint64_t e0 = drop_base(drop);
   const A scale = (A)drop.scale;
   A aw[NC], ab[NC];
@@ -831,7 +847,8 @@ __global__ __launch_bounds__(64 * SHORT_WAVES, 2) void ln_bwd_short_kernel(
 #pragma unroll 1
   for (int64_t t = (int64_t)blockIdx.x * SHORT_WAVES + wave; t < tiles; t += step) {
     const int64_t row0 = t * 64;
-    const int n = elements(t), lane = in_loop((int)(threadIdx.x & 63));
+    const int n = elements(t);
+    int lane = in_loop((int)(threadIdx.x & 63));
     const bool live = lane * cols < n;
     Tile<X, NC> nx, ng;
     nx.load(x + row0 * cols, n, lane);
@@ -849,9 +866,11 @@ __global__ __launch_bounds__(64 * SHORT_WAVES, 2) void ln_bwd_short_kernel(
     }
     wave_lds_fence();
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-      if (c < cols) h[c] = live ? (lds[lane * pitch + c] - mean) * rstd : A(0);
+    for (int c = 0; c < NC; ++c) h[c] = lds[lane * pitch + c];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) h[c] = c < cols && live ? (h[c] - mean) * rstd : A(0);
     wave_lds_fence();
+    lane = in_loop(lane);      // (places in LDS are not kept from one turn to the next: a register an element)
 #pragma unroll
     for (int k = 0; k < IT; ++k) {
       const int i = (k * 64 + lane) * N;
@@ -864,18 +883,25 @@ __global__ __launch_bounds__(64 * SHORT_WAVES, 2) void ln_bwd_short_kernel(
         for (int j = 0; j < N; ++j) f[j] = (bits >> j & 1) ? f[j] * scale : A(0);
       }
       if (i < n) short_put<A, N>(lds, f, i, pad, inv);
+      __builtin_amdgcn_sched_barrier(0);
     }
     wave_lds_fence();
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-      if (c < cols) {
-        g[c] = live ? lds[lane * pitch + c] : A(0);
+    for (int k = 0; k < NC; k += 8) {
+      A wv[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) g[k + c] = lds[lane * pitch + k + c], wv[c] = weights[0][k + c];
+#pragma unroll
+      for (int c = k; c < k + 8; ++c) {
+        g[c] = c < cols && live ? g[c] : A(0);
         aw[c] += g[c] * h[c];
         ab[c] += g[c];
-        if (w) g[c] *= (A)w[c];
+        g[c] *= wv[c - k];
         s1 += g[c];
         s2 += g[c] * h[c];
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
     wave_lds_fence();
     if (dx) {
       s1 /= (A)cols;
@@ -885,6 +911,7 @@ __global__ __launch_bounds__(64 * SHORT_WAVES, 2) void ln_bwd_short_kernel(
         for (int c = 0; c < NC; ++c)
           if (c < cols) lds[lane * pitch + c] = rstd * (g[c] - s1 - h[c] * s2);
       wave_lds_fence();
+      lane = in_loop(lane);
       X* out = dx + row0 * cols;
 #pragma unroll
       for (int k = 0; k < IT; ++k) {
