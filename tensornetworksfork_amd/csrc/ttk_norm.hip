@@ -27,6 +27,8 @@ struct Acc<double> {
 
 // 16 bytes of elements as one unaligned global access: rows of odd length start anywhere.
 typedef uint32_t raw_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t half_t __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t word_t __attribute__((aligned(2)));
 
 // Held as four words (elements of their own would take a register each).
 template <typename X>
@@ -43,17 +45,42 @@ struct Vec {
     r.x = u[0], r.y = u[1], r.z = u[2], r.w = u[3];
     *reinterpret_cast<raw_t*>(p) = r;
   }
+  __device__ __forceinline__ void clear() { u[0] = u[1] = u[2] = u[3] = 0; }
   // the first n (< N) elements one by one, the rest zero
   __device__ __forceinline__ void load_some(const X* p, int n) {
-    u[0] = u[1] = u[2] = u[3] = 0;
+    clear();
 #pragma unroll
     for (int j = 0; j < N; ++j)
       if (j < n) put(j, p[j]);
   }
+  // the first n (0 < n < N) elements, in pieces of 8, 4 and 2 bytes
   __device__ __forceinline__ void store_some(X* p, int n) const {
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (j < n) p[j] = element(j);
+    uint32_t a = u[0], b = u[1];
+    const int bytes = n * (int)sizeof(X);
+    char* q = reinterpret_cast<char*>(p);
+    if (bytes & 8) {
+      half_t r;
+      r.x = a, r.y = b;
+      *reinterpret_cast<half_t*>(q) = r;
+      q += 8, a = u[2], b = u[3];
+    }
+    if (sizeof(X) <= 4 && bytes & 4) {
+      *reinterpret_cast<word_t*>(q) = a;
+      q += 4, a = b;
+    }
+    if (sizeof(X) == 2 && bytes & 2) *reinterpret_cast<uint16_t*>(q) = (uint16_t)a;
+  }
+  // drops the first k (< N) elements: the others move down, zeros behind them
+  __device__ __forceinline__ void drop_first(int k) {
+    const int bytes = k * (int)sizeof(X);
+    if (sizeof(X) == 2 && bytes & 2) {
+      u[0] = u[0] >> 16 | u[1] << 16;
+      u[1] = u[1] >> 16 | u[2] << 16;
+      u[2] = u[2] >> 16 | u[3] << 16;
+      u[3] >>= 16;
+    }
+    if (sizeof(X) <= 4 && bytes & 4) u[0] = u[1], u[1] = u[2], u[2] = u[3], u[3] = 0;
+    if (bytes & 8) u[0] = u[2], u[1] = u[3], u[2] = u[3] = 0;
   }
   // Forgets what was computed from the elements: without it the compiler keeps every element's float beside the element
   // across the phases of a row, which are twice to three times the registers.
@@ -206,17 +233,15 @@ __device__ __forceinline__ double dpp_mov(double v) {
   return __longlong_as_double((int64_t)(((uint64_t)hi << 32) | lo));
 }
 
-// Sum over groups of LANES (16 or 64) consecutive lanes, the same bits in every lane.
+// Sum over groups of LANES (8 to 64) consecutive lanes, the same bits in every lane.
 template <int LANES, typename A>
 __device__ __forceinline__ A lane_sum(A v) {
   v += dpp_mov<0xB1>(v);    // quad_perm 1 0 3 2
   v += dpp_mov<0x4E>(v);    // quad_perm 2 3 0 1
   v += dpp_mov<0x141>(v);   // mirror within 8
-  v += dpp_mov<0x140>(v);   // mirror within 16
-  if (LANES == 64) {
-    v += __shfl_xor(v, 16);
-    v += __shfl_xor(v, 32);
-  }
+  if (LANES >= 16) v += dpp_mov<0x140>(v);   // mirror within 16
+  if (LANES >= 32) v += __shfl_xor(v, 16);
+  if (LANES >= 64) v += __shfl_xor(v, 32);
   return v;
 }
 
@@ -376,43 +401,64 @@ __global__ __launch_bounds__(1024) void ln_cols_sum_kernel(const A* __restrict__
 // The backward pass walks many rows a workgroup and keeps each lane's columns of dw and db in registers; they leave as one
 // partial row per workgroup (`part`: [workgroup][dw | db][cols]).
 // ---------------------------------------------------------------------------------------
-template <typename X, int LANES, int NV>
+// RAGGED: the row's length is no multiple of a vector's.  The vector that reaches behind the row is then loaded from where it
+// ends with the row (no load an element, no wait before the values are used) and put right by settle_row.
+template <bool RAGGED, typename X, int LANES, int NV>
 __device__ __forceinline__ void load_row(Vec<X> (&v)[NV], const X* p, int lane, int cols, bool live) {
   constexpr int N = Vec<X>::N;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * LANES + lane) * N;
-    if (live && c + N <= cols)
-      v[i].load(p + c);
-    else
+    if (RAGGED && cols < N) {
       v[i].load_some(p + c, live ? cols - c : 0);
+    } else {
+      v[i].clear();
+      if (live && c < cols) v[i].load(p + (RAGGED ? min(c, cols - N) : c));
+    }
+  }
+}
+template <bool RAGGED, typename X, int LANES, int NV>
+__device__ __forceinline__ void settle_row(Vec<X> (&v)[NV], int lane, int cols) {
+  constexpr int N = Vec<X>::N;
+  if (!RAGGED || cols < N) return;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * LANES + lane) * N;
+    if (c < cols && c + N > cols) v[i].drop_first(c + N - cols);
   }
 }
 
-template <typename X, int LANES, int NV>
+template <bool RAGGED, typename X, int LANES, int NV>
 __device__ __forceinline__ void store_row(const Vec<X> (&v)[NV], X* p, int lane, int cols) {
   constexpr int N = Vec<X>::N;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * LANES + lane) * N;
-    if (c + N <= cols)
+    if (RAGGED ? c + N <= cols : c < cols)
       v[i].store(p + c);
-    else
+    else if (RAGGED && c < cols)
       v[i].store_some(p + c, cols - c);
   }
 }
 
 // N weights from column c on (missing ones 0)
-template <typename A, typename W, int N>
+template <bool RAGGED, typename A, typename W, int N>
 __device__ __forceinline__ void load_weights(A (&out)[N], const W* w, int c, int cols) {
   constexpr int M = Vec<W>::N;
-  if (N >= M && c + N <= cols) {
+  if (N >= M && c < cols && (!RAGGED || cols >= N)) {
+    const int at = RAGGED ? min(c, cols - N) : c, k = c - at;
 #pragma unroll
-    for (int k = 0; k < N / M; ++k) {
-      Vec<W> t;
-      t.load(w + c + k * M);
+    for (int t = 0; t < N / M; ++t) {
+      Vec<W> v;
+      v.load(w + at + t * M);
 #pragma unroll
-      for (int j = 0; j < M; ++j) out[k * M + j] = (A)t.get(j);
+      for (int j = 0; j < M; ++j) out[t * M + j] = (A)v.get(j);
+    }
+    if (RAGGED && k) {      // the row's last, incomplete vector
+#pragma unroll
+      for (int b = 1; b < N; b *= 2)
+#pragma unroll
+        for (int j = 0; j < N; ++j) out[j] = k & b ? (j + b < N ? out[j + b] : A(0)) : out[j];
     }
   } else {
 #pragma unroll
@@ -461,22 +507,22 @@ __device__ __forceinline__ void one_by_one() {
 }
 
 // weights of a lane's columns; absent ones act as `none`
-template <typename A, typename W, int N>
+template <bool RAGGED, typename A, typename W, int N>
 __device__ __forceinline__ void load_weights_or(A (&out)[N], const W* w, int c, int cols, A none) {
   if (w) {
-    load_weights<A, W, N>(out, w, c, cols);
+    load_weights<RAGGED, A, W, N>(out, w, c, cols);
   } else {
 #pragma unroll
     for (int j = 0; j < N; ++j) out[j] = none;
   }
 }
-template <typename A, typename W, int LANES, int NV, int N>
+template <bool RAGGED, typename A, typename W, int LANES, int NV, int N>
 __device__ __forceinline__ void lane_weights(A (&out)[NV][N], const W* w, int lane, int cols, A none) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) load_weights_or<A, W, N>(out[i], w, (i * LANES + lane) * N, cols, none);
+  for (int i = 0; i < NV; ++i) load_weights_or<RAGGED, A, W, N>(out[i], w, (i * LANES + lane) * N, cols, none);
 }
 
-template <typename X, typename W, int LANES, int NV>
+template <typename X, typename W, int LANES, int NV, bool RAGGED>
 __global__ __launch_bounds__(group_threads(LANES), NV <= 2 || LANES >= 512 ? 4 : 3) void ln_fwd_group_kernel(
     const X* __restrict__ x, int64_t ldx, const W* __restrict__ w, const W* __restrict__ b, X* __restrict__ y,
     typename Acc<X>::type* __restrict__ mean_out, typename Acc<X>::type* __restrict__ rstd_out, int64_t rows, int cols, double eps,
@@ -490,20 +536,21 @@ __global__ __launch_bounds__(group_threads(LANES), NV <= 2 || LANES >= 512 ? 4 :
   const A scale = (A)drop.scale;
   A wv[NV][N], bv[NV][N];
   if constexpr (HOLD) {
-    lane_weights<A, W, LANES, NV, N>(wv, w, lane, cols, A(1));
-    lane_weights<A, W, LANES, NV, N>(bv, b, lane, cols, A(0));
+    lane_weights<RAGGED, A, W, LANES, NV, N>(wv, w, lane, cols, A(1));
+    lane_weights<RAGGED, A, W, LANES, NV, N>(bv, b, lane, cols, A(0));
   }
   const A inv = A(1) / (A)cols;
   const int64_t step = (int64_t)gridDim.x * RPB;
   Vec<X> next[NV];
-  load_row<X, LANES, NV>(next, x + ((int64_t)blockIdx.x * RPB + sub) * ldx, lane, cols, (int64_t)blockIdx.x * RPB + sub < rows);
+  load_row<RAGGED, X, LANES, NV>(next, x + ((int64_t)blockIdx.x * RPB + sub) * ldx, lane, cols, (int64_t)blockIdx.x * RPB + sub < rows);
   for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += step) {
     const int64_t row = r0 + sub;
     const bool live = row < rows;
     Vec<X> v[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) v[i] = next[i];
-    if (r0 + step < rows) load_row<X, LANES, NV>(next, x + (row + step) * ldx, lane, cols, row + step < rows);
+    settle_row<RAGGED, X, LANES, NV>(v, lane, cols);
+    if (r0 + step < rows) load_row<RAGGED, X, LANES, NV>(next, x + (row + step) * ldx, lane, cols, row + step < rows);
     A s = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -529,8 +576,8 @@ __global__ __launch_bounds__(group_threads(LANES), NV <= 2 || LANES >= 512 ? 4 :
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if constexpr (!HOLD) {
-        load_weights_or<A, W, N>(wv[i], in_loop_uniform(w), (i * LANES + lane) * N, cols, A(1));
-        load_weights_or<A, W, N>(bv[i], in_loop_uniform(b), (i * LANES + lane) * N, cols, A(0));
+        load_weights_or<RAGGED, A, W, N>(wv[i], in_loop_uniform(w), (i * LANES + lane) * N, cols, A(1));
+        load_weights_or<RAGGED, A, W, N>(bv[i], in_loop_uniform(b), (i * LANES + lane) * N, cols, A(0));
       }
       A h[N];
 #pragma unroll
@@ -543,12 +590,12 @@ __global__ __launch_bounds__(group_threads(LANES), NV <= 2 || LANES >= 512 ? 4 :
       v[i].set(h);
       one_by_one<NV>();
     }
-    store_row<X, LANES, NV>(v, y + row * cols, lane, cols);
+    store_row<RAGGED, X, LANES, NV>(v, y + row * cols, lane, cols);
     if (lane == 0 && mean_out) mean_out[row] = mean, rstd_out[row] = rstd;
   }
 }
 
-template <typename X, typename W, int LANES, int NV>
+template <typename X, typename W, int LANES, int NV, bool RAGGED>
 __global__ __launch_bounds__(group_threads(LANES)) void ln_bwd_group_kernel(
     const X* __restrict__ dy, int64_t lddy, const X* __restrict__ x, int64_t ldx, const W* __restrict__ w,
     const typename Acc<X>::type* __restrict__ mean_in, const typename Acc<X>::type* __restrict__ rstd_in, X* __restrict__ dx,
@@ -556,7 +603,7 @@ __global__ __launch_bounds__(group_threads(LANES)) void ln_bwd_group_kernel(
   typedef typename Acc<X>::type A;
   constexpr int N = Vec<X>::N, RPB = group_threads(LANES) / LANES;
   // a row's a and h stay in registers between its two halves; the next row's loads are under way meanwhile
-  constexpr bool HOLD = NV * N * (int)sizeof(A) <= 32, AHEAD = NV * N * (int)sizeof(A) + NV * 32 <= 256;
+  constexpr bool HOLD = NV * N * (int)sizeof(A) <= 32, AHEAD = NV * N * (int)sizeof(A) + NV * 32 <= (LANES >= 1024 ? 128 : 256);
   __shared__ A buf[2][LANES > 64 ? 32 : 1];
   const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
   const uint64_t e0 = drop_base(drop);
@@ -566,27 +613,29 @@ __global__ __launch_bounds__(group_threads(LANES)) void ln_bwd_group_kernel(
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < N; ++j) aw[i][j] = ab[i][j] = A(0);
-  lane_weights<A, W, LANES, NV, N>(wv, w, lane, cols, A(1));
+  if constexpr (AHEAD) lane_weights<RAGGED, A, W, LANES, NV, N>(wv, w, lane, cols, A(1));
   const int64_t step = (int64_t)gridDim.x * RPB;
   Vec<X> nx[NV], ng[NV];
   A nmean = 0, nrstd = 0;
   auto fetch = [&](int64_t row) {
     const bool live = row < rows;
-    load_row<X, LANES, NV>(nx, x + row * ldx, lane, cols, live);
-    load_row<X, LANES, NV>(ng, dy + row * lddy, lane, cols, live);
+    load_row<RAGGED, X, LANES, NV>(nx, x + row * ldx, lane, cols, live);
+    load_row<RAGGED, X, LANES, NV>(ng, dy + row * lddy, lane, cols, live);
     nmean = live ? mean_in[row] : A(0);
     nrstd = live ? rstd_in[row] : A(0);
   };
-  fetch((int64_t)blockIdx.x * RPB + sub);
+  if (AHEAD) fetch((int64_t)blockIdx.x * RPB + sub);
   int turn = 0;
 #pragma unroll 1
   for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += step, turn ^= 1) {
     const int64_t row = r0 + sub;
     const bool live = row < rows;
     Vec<X> xv[NV], gv[NV];
-    if (!AHEAD && r0 != (int64_t)blockIdx.x * RPB) fetch(row);
+    if (!AHEAD) fetch(row);
 #pragma unroll
     for (int i = 0; i < NV; ++i) xv[i] = nx[i], gv[i] = ng[i];
+    settle_row<RAGGED, X, LANES, NV>(xv, lane, cols);
+    settle_row<RAGGED, X, LANES, NV>(gv, lane, cols);
     const A mean = nmean, rstd = nrstd;
     if (AHEAD && r0 + step < rows) fetch(row + step);
     A s1 = 0, s2 = 0, ha[HOLD ? NV : 1][N], aa[HOLD ? NV : 1][N];
@@ -595,6 +644,7 @@ __global__ __launch_bounds__(group_threads(LANES)) void ln_bwd_group_kernel(
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * LANES + lane) * N;
+      if constexpr (!AHEAD) load_weights_or<RAGGED, A, W, N>(wv[i], in_loop_uniform(w), c, cols, A(1));
       if (drop.mode) bits[i] = live ? keep_bits_row<N, NV == 1 ? LANES : 1>(drop, e0 + (uint64_t)row * cols + c) : 0u;
 #pragma unroll
       for (int j = 0; j < N; ++j) {
@@ -617,6 +667,7 @@ __global__ __launch_bounds__(group_threads(LANES)) void ln_bwd_group_kernel(
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if constexpr (!HOLD) xv[i].forget(), gv[i].forget();
+      if constexpr (!AHEAD) load_weights_or<RAGGED, A, W, N>(wv[i], in_loop_uniform(w), (i * LANES + lane) * N, cols, A(1));
       A out[N];
 #pragma unroll
       for (int j = 0; j < N; ++j) {
@@ -634,7 +685,7 @@ __global__ __launch_bounds__(group_threads(LANES)) void ln_bwd_group_kernel(
       gv[i].set(out);
       one_by_one<NV>();
     }
-    store_row<X, LANES, NV>(gv, dx + row * cols, lane, cols);
+    store_row<RAGGED, X, LANES, NV>(gv, dx + row * cols, lane, cols);
   }
   if (!part) return;
   A* p = part + (int64_t)blockIdx.x * 2 * cols;
@@ -1044,19 +1095,20 @@ struct Layout {
 // Forward: few lanes with many elements each (rows of a workgroup of 256 run beside each other).  Backward: two sums stay
 // beside every element, so wide rows take more lanes.
 Layout row_layout(int dtype, int cols, bool dense, bool backward) {
-  if (dense && cols <= (dtype == 0 ? 16 : 32)) return {1, (cols + 7) / 8 * 8};
+  if (dense && cols <= (dtype == 0 ? 8 : dtype == 1 ? 24 : 32)) return {1, (cols + 7) / 8 * 8};
   const int n = dtype == 0 ? 2 : dtype == 1 ? 4 : 8;         // elements of a 16-byte vector
   const int64_t nvec = ((int64_t)cols + n - 1) / n;
   const bool half = n == 8;
+  if (nvec <= 8) return {8, 1};
   if (nvec <= 16) return {16, 1};
-  if (nvec <= 32 && !half) return {16, 2};
+  if (nvec <= 32) return half ? Layout{32, 1} : Layout{16, 2};
   if (nvec <= 64) return {64, 1};
   if (nvec <= 128) return {64, 2};
   if (nvec <= 256) return half ? Layout{256, 1} : Layout{64, 4};
   if (nvec <= 512) return half && backward ? Layout{512, 1} : Layout{256, 2};
-  if (nvec <= 1024) return backward ? (half ? Layout{1024, 1} : Layout{512, 2}) : Layout{256, 4};
-  if (nvec <= 2048) return backward ? (half ? Layout{512, 4} : Layout{1024, 2}) : Layout{512, 4};
-  if (nvec <= 4096 && !half) return backward ? Layout{512, 8} : Layout{1024, 4};
+  if (nvec <= 1024) return half ? (backward ? Layout{1024, 1} : Layout{512, 2}) : backward ? Layout{512, 2} : Layout{256, 4};
+  if (nvec <= 2048) return backward ? Layout{1024, 2} : Layout{512, 4};
+  if (nvec <= 4096 && !half) return Layout{1024, 4};
   return {0, 0};
 }
 
@@ -1097,12 +1149,14 @@ constexpr int type_code() {
 #define TTK_SHORT(S)                                        \
   switch (l.nv) {                                           \
     case 8: S(8); break;                                    \
-    case 16: S(16); break;                                  \
+    case 16:                                                \
+      if constexpr (sizeof(X) < 8) { S(16); }               \
+      break;                                                \
     case 24:                                                \
       if constexpr (sizeof(X) < 8) { S(24); }               \
       break;                                                \
     case 32:                                                \
-      if constexpr (sizeof(X) < 8) { S(32); }               \
+      if constexpr (sizeof(X) == 2) { S(32); }              \
       break;                                                \
   }
 #define TTK_LAYOUT(L, V, K) \
@@ -1110,12 +1164,13 @@ constexpr int type_code() {
 #define TTK_FWD_LAYOUTS(K)                                                                             \
   if constexpr (sizeof(X) == 2) {                                                                      \
     switch (l.lanes * 16 + l.nv) {                                                                     \
-      TTK_LAYOUT(16, 1, K); TTK_LAYOUT(64, 1, K); TTK_LAYOUT(64, 2, K); TTK_LAYOUT(256, 1, K);         \
-      TTK_LAYOUT(256, 2, K); TTK_LAYOUT(256, 4, K); TTK_LAYOUT(512, 4, K);                             \
+      TTK_LAYOUT(8, 1, K); TTK_LAYOUT(16, 1, K); TTK_LAYOUT(32, 1, K); TTK_LAYOUT(64, 1, K);           \
+      TTK_LAYOUT(64, 2, K); TTK_LAYOUT(256, 1, K); TTK_LAYOUT(256, 2, K); TTK_LAYOUT(512, 2, K);       \
+      TTK_LAYOUT(512, 4, K);                             \
     }                                                                                                  \
   } else {                                                                                             \
     switch (l.lanes * 16 + l.nv) {                                                                     \
-      TTK_LAYOUT(16, 1, K); TTK_LAYOUT(16, 2, K); TTK_LAYOUT(64, 1, K); TTK_LAYOUT(64, 2, K);          \
+      TTK_LAYOUT(8, 1, K); TTK_LAYOUT(16, 1, K); TTK_LAYOUT(16, 2, K); TTK_LAYOUT(64, 1, K); TTK_LAYOUT(64, 2, K);          \
       TTK_LAYOUT(64, 4, K); TTK_LAYOUT(256, 2, K); TTK_LAYOUT(256, 4, K); TTK_LAYOUT(512, 4, K);       \
       TTK_LAYOUT(1024, 4, K);                                                                          \
     }                                                                                                  \
@@ -1123,14 +1178,14 @@ constexpr int type_code() {
 #define TTK_BWD_LAYOUTS(K)                                                                             \
   if constexpr (sizeof(X) == 2) {                                                                      \
     switch (l.lanes * 16 + l.nv) {                                                                     \
-      TTK_LAYOUT(16, 1, K); TTK_LAYOUT(64, 1, K); TTK_LAYOUT(64, 2, K); TTK_LAYOUT(256, 1, K);         \
-      TTK_LAYOUT(512, 1, K); TTK_LAYOUT(1024, 1, K); TTK_LAYOUT(512, 4, K);                            \
+      TTK_LAYOUT(8, 1, K); TTK_LAYOUT(16, 1, K); TTK_LAYOUT(32, 1, K); TTK_LAYOUT(64, 1, K);           \
+      TTK_LAYOUT(64, 2, K); TTK_LAYOUT(256, 1, K); TTK_LAYOUT(512, 1, K); TTK_LAYOUT(1024, 1, K); TTK_LAYOUT(1024, 2, K);                           \
     }                                                                                                  \
   } else {                                                                                             \
     switch (l.lanes * 16 + l.nv) {                                                                     \
-      TTK_LAYOUT(16, 1, K); TTK_LAYOUT(16, 2, K); TTK_LAYOUT(64, 1, K); TTK_LAYOUT(64, 2, K);          \
+      TTK_LAYOUT(8, 1, K); TTK_LAYOUT(16, 1, K); TTK_LAYOUT(16, 2, K); TTK_LAYOUT(64, 1, K); TTK_LAYOUT(64, 2, K);          \
       TTK_LAYOUT(64, 4, K); TTK_LAYOUT(256, 2, K); TTK_LAYOUT(512, 2, K); TTK_LAYOUT(1024, 2, K);      \
-      TTK_LAYOUT(512, 8, K);                                                                           \
+      TTK_LAYOUT(1024, 4, K);                                                                          \
     }                                                                                                  \
   }
 
@@ -1145,9 +1200,10 @@ int ln_fwd(const void* x, int64_t ldx, const void* w, const void* b, void* y, vo
     return status();
   }
   const dim3 grid((unsigned)row_groups(l, rows, false));
-#define K(LANES, NV)                                                                                                      \
-  hipLaunchKernelGGL((ln_fwd_group_kernel<X, W, LANES, NV>), grid, dim3(group_threads(LANES)), 0, st, (const X*)x, ldx,    \
+#define KR(LANES, NV, R)                                                                                                  \
+  hipLaunchKernelGGL((ln_fwd_group_kernel<X, W, LANES, NV, R>), grid, dim3(group_threads(LANES)), 0, st, (const X*)x, ldx,    \
                      (const W*)w, (const W*)b, (X*)y, (A*)mean, (A*)rstd, rows, cols, eps, d)
+#define K(LANES, NV) if (cols % Vec<X>::N) KR(LANES, NV, true); else KR(LANES, NV, false)
 #define S(NC)                                                                                                             \
   hipLaunchKernelGGL((ln_fwd_short_kernel<X, W, NC>), grid, dim3(64 * SHORT_WAVES), 0, st, (const X*)x, (const W*)w,       \
                      (const W*)b, (X*)y, (A*)mean, (A*)rstd, rows, cols, eps, d)
@@ -1156,6 +1212,7 @@ int ln_fwd(const void* x, int64_t ldx, const void* w, const void* b, void* y, vo
   else
     TTK_FWD_LAYOUTS(K)
 #undef K
+#undef KR
 #undef S
   return status();
 }
@@ -1170,10 +1227,11 @@ int ln_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void*
   if (sums && (!ws || ws_bytes < (int64_t)parts * 2 * cols * (int64_t)sizeof(A))) return TTK_EWORKSPACE;
   if (l.lanes && (dx || sums)) {
     A* part = sums ? (A*)ws : (A*)nullptr;
-#define K(LANES, NV)                                                                                                      \
-  hipLaunchKernelGGL((ln_bwd_group_kernel<X, W, LANES, NV>), dim3((unsigned)parts), dim3(group_threads(LANES)), 0, st,     \
+#define KR(LANES, NV, R)                                                                                                  \
+  hipLaunchKernelGGL((ln_bwd_group_kernel<X, W, LANES, NV, R>), dim3((unsigned)parts), dim3(group_threads(LANES)), 0, st,     \
                      (const X*)dy, lddy, (const X*)x, ldx, (const W*)w, (const A*)mean, (const A*)rstd, (X*)dx, part,      \
                      rows, cols, d)
+#define K(LANES, NV) if (cols % Vec<X>::N) KR(LANES, NV, true); else KR(LANES, NV, false)
 #define S(NC)                                                                                                             \
   hipLaunchKernelGGL((ln_bwd_short_kernel<X, W, NC>), dim3((unsigned)parts), dim3(64 * SHORT_WAVES), 0, st, (const X*)dy,  \
                      (const X*)x, (const W*)w, (const A*)mean, (const A*)rstd, (X*)dx, part, rows, cols, d)
@@ -1182,6 +1240,7 @@ int ln_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void*
     else
       TTK_BWD_LAYOUTS(K)
 #undef K
+#undef KR
 #undef S
   } else if (!l.lanes) {
     if (dx)
