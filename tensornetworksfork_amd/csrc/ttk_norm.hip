@@ -1107,7 +1107,7 @@ Layout row_layout(int dtype, int cols, bool dense, bool backward) {
   if (nvec <= 256) return half ? Layout{256, 1} : Layout{64, 4};
   if (nvec <= 512) return half && backward ? Layout{512, 1} : Layout{256, 2};
   if (nvec <= 1024) return half ? (backward ? Layout{1024, 1} : Layout{512, 2}) : backward ? Layout{512, 2} : Layout{256, 4};
-  if (nvec <= 2048) return backward ? Layout{1024, 2} : Layout{512, 4};
+  if (nvec <= 2048) return backward || half ? Layout{1024, 2} : Layout{512, 4};
   if (nvec <= 4096 && !half) return Layout{1024, 4};
   return {0, 0};
 }
@@ -1166,7 +1166,7 @@ constexpr int type_code() {
     switch (l.lanes * 16 + l.nv) {                                                                     \
       TTK_LAYOUT(8, 1, K); TTK_LAYOUT(16, 1, K); TTK_LAYOUT(32, 1, K); TTK_LAYOUT(64, 1, K);           \
       TTK_LAYOUT(64, 2, K); TTK_LAYOUT(256, 1, K); TTK_LAYOUT(256, 2, K); TTK_LAYOUT(512, 2, K);       \
-      TTK_LAYOUT(512, 4, K);                             \
+      TTK_LAYOUT(1024, 2, K);                            \
     }                                                                                                  \
   } else {                                                                                             \
     switch (l.lanes * 16 + l.nv) {                                                                     \
