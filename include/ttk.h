@@ -498,7 +498,7 @@ int ttk_layer_norm_backward(int dtype, int wdtype, const void* dy, int64_t lddy,
  * lowest index; NaN counts as -inf, -inf is never drawn, +inf takes all; temperature <= 0: lowest index of the maximum;
  * a row without a logit above -inf: -1.  V <= 2^30.  top_k <= 0 or >= V, top_p >= 1, min_p <= 0 switch a cut off.
  * u: one value a row, float64 when f64 != 0 else float32; temperature / top_p / min_p: the same type, one value a row, or
- * NULL for the *_all value; top_k: one int32 a row or NULL.  ws: ttk_sample_ws_bytes bytes (none for V <= 1024). */
+ * NULL for the *_all value; top_k: one int32 a row or NULL.  ws: ttk_sample_ws_bytes bytes (none for V <= 8192). */
 int64_t ttk_sample_ws_bytes(int dtype, int64_t rows, int V);
 int ttk_sample(int dtype, const void* logits, int64_t ld, const void* u, int f64, const void* temperature,
                double temperature_all, const int32_t* top_k, int top_k_all, const void* top_p, double top_p_all,

@@ -230,33 +230,150 @@ __global__ __launch_bounds__(64) void sample_few_kernel(const Z* __restrict__ lo
 }
 
 // ---------------------------------------------------------------------------------------
-// Up to 64 E classes: a wave a row, E consecutive elements a lane.  Cuts are found bit by bit: the largest key t with
-// enough elements (or weight) at or above it.
+// Up to 64 E W classes: W waves a row, E consecutive elements a lane at most.  Cuts are found bit by bit: the largest key t
+// with enough elements (or weight) at or above it.  A search ends as soon as one element more or less is all that is open.
 // ---------------------------------------------------------------------------------------
-template <typename Z, int E>
-__global__ __launch_bounds__(256) void sample_wave_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args,
-                                                          int64_t* __restrict__ label, int64_t rows, int V) {
+typedef uint32_t raw_t __attribute__((ext_vector_type(4), aligned(2)));
+
+// What the waves of a row agree on.  Every call writes the other half of `buf`, so one barrier a call is enough.
+template <int W>
+struct RowWaves {
+  struct Part {
+    double s;
+    int n;
+  };
+  Part* buf;      // [2][W]
+  int wave, turn;
+  __device__ __forceinline__ RowWaves(Part* buf_) : buf(buf_), wave(W > 1 ? threadIdx.x >> 6 : 0), turn(0) {}
+  __device__ __forceinline__ const Part* share(double s, int n) {
+    Part* p = buf + turn * W;
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) p[wave] = Part{s, n};
+    __syncthreads();
+    return p;
+  }
+  // sums over the row's waves, and over the waves in front of this one
+  __device__ __forceinline__ void sum(int& n) {
+    if constexpr (W > 1) {
+      const Part* p = share(0.0, n);
+      n = 0;
+#pragma unroll
+      for (int i = 0; i < W; ++i) n += p[i].n;
+      n = __builtin_amdgcn_readfirstlane(n);
+    }
+  }
+  __device__ __forceinline__ void sum(double& s, int& n) {
+    if constexpr (W > 1) {
+      const Part* p = share(s, n);
+      s = 0, n = 0;
+#pragma unroll
+      for (int i = 0; i < W; ++i) s += p[i].s, n += p[i].n;
+    }
+  }
+  __device__ __forceinline__ int in_front(int n) {
+    int before = 0;
+    if constexpr (W > 1) {
+      const Part* p = share(0.0, n);
+#pragma unroll
+      for (int i = 0; i < W - 1; ++i) before += i < wave ? p[i].n : 0;
+    }
+    return before;
+  }
+  __device__ __forceinline__ double in_front(double s, double& total) {
+    double before = 0;
+    total = s;
+    if constexpr (W > 1) {
+      const Part* p = share(s, 0);
+      total = 0;
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        before += i < wave ? p[i].s : 0.0;
+        total += p[i].s;
+      }
+    }
+    return before;
+  }
+  __device__ __forceinline__ double largest(double s) {
+    if constexpr (W > 1) {
+      const Part* p = share(s, 0);
+#pragma unroll
+      for (int i = 0; i < W; ++i) s = p[i].s > s ? p[i].s : s;
+    }
+    return s;
+  }
+  // the row's largest and the first index that has it
+  __device__ __forceinline__ void largest(double& s, int& at) {
+    if constexpr (W > 1) {
+      const Part* p = share(s, at);
+      s = p[0].s, at = p[0].n;
+#pragma unroll
+      for (int i = 1; i < W; ++i)
+        if (p[i].s > s) s = p[i].s, at = p[i].n;
+    }
+  }
+  // bit i: what wave i says
+  __device__ __forceinline__ uint32_t votes(bool b) {
+    uint32_t v = b;
+    if constexpr (W > 1) {
+      const Part* p = share(0.0, b);
+      v = 0;
+#pragma unroll
+      for (int i = 0; i < W; ++i) v |= (uint32_t)p[i].n << i;
+    }
+    return v;
+  }
+};
+
+template <typename Z, int E, int W>
+__global__ __launch_bounds__(W > 1 ? 64 * W : 256) void sample_wave_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args,
+                                                                          int64_t* __restrict__ label, int64_t rows, int V) {
   typedef typename Key<Z>::type K;
   typedef typename Key<Z>::val_t F;
+  constexpr int N = 16 / (int)sizeof(Z);      // elements of a 16-byte load (any alignment)
+  __shared__ typename RowWaves<W>::Part parts[2 * W];
+  RowWaves<W> waves(parts);
   const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t row = W > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= rows) return;
   const Z* p = logits + row * ld;
-  const int e = (V + 63) / 64, c0 = lane * e;      // this lane's elements: c0 .. c0 + e - 1
+  int e = (V + 64 * W - 1) / (64 * W);
+  if (E >= N) e = (e + N - 1) / N * N;
+  const int c0 = (waves.wave * 64 + lane) * e;      // this lane's elements: c0 .. c0 + e - 1
   F z[E], m = -__builtin_inff();
   int first = 0x7FFFFFFF;
+  if constexpr (E >= N) {
+    struct Elements {
+      Z z[N];
+    };
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    z[i] = i < e && c0 + i < V ? Key<Z>::value(p[c0 + i]) : F(-__builtin_inff());
-    if (z[i] > m) m = z[i], first = c0 + i;
+    for (int i = 0; i < E; i += N) {
+      if (i < e && c0 + i + N <= V) {
+        const Elements v = __builtin_bit_cast(Elements, *reinterpret_cast<const raw_t*>(p + c0 + i));
+#pragma unroll
+        for (int j = 0; j < N; ++j) z[i + j] = Key<Z>::value(v.z[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) z[i + j] = i < e && c0 + i + j < V ? Key<Z>::value(p[c0 + i + j]) : F(-__builtin_inff());
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) z[i] = i < e && c0 + i < V ? Key<Z>::value(p[c0 + i]) : F(-__builtin_inff());
   }
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+    if (z[i] > m) m = z[i], first = c0 + i;
   const F mine = m;
   m = wave_max(m);
+  int at_m = __builtin_amdgcn_readlane(first, (int)__builtin_ctzll(__ballot(mine == m)));
+  if constexpr (W > 1) {
+    double s = (double)m;
+    waves.largest(s, at_m);
+    m = (F)s;
+  }
   const RowArgs a = row_args(args, row, V);
   if (!(m > -__builtin_inff()) || !(a.T > 0.0)) {
-    const uint64_t who = __ballot(mine == m);
-    const int f = __shfl(first, (int)__builtin_ctzll(who));
-    if (lane == 0) label[row] = m > -__builtin_inff() ? f : -1;
+    if (lane == 0 && waves.wave == 0) label[row] = m > -__builtin_inff() ? at_m : -1;
     return;
   }
   const bool inf = m == __builtin_inff();
@@ -267,8 +384,8 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const Z* __restrict__ 
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     z[i] = finite(z[i], inf);
-    key[i] = Key<Z>::of(z[i]);
     w[i] = weight(z[i]);
+    key[i] = w[i] > 0 ? Key<Z>::of(z[i]) : K(0);      // (key 0: dropped; no element that is left has it)
   }
   constexpr int BITS = 8 * (int)sizeof(K), LOW = Key<Z>::LOW;
   // keeps, of the elements with w > 0, those in front of the cut: key above t, or the first `ties` of those with key t
@@ -278,60 +395,86 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const Z* __restrict__ 
     t |= low;
 #pragma unroll
     for (int i = 0; i < E; ++i) before += w[i] > 0 && (K)(key[i] | low) == t;
-    before = wave_scan(before) - before;
+    const int upto = wave_scan(before);
+    before = upto - before + waves.in_front(__builtin_amdgcn_readlane(upto, 63));
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       const K k = key[i] | low;
-      if (k < t || (k == t && w[i] > 0 && before++ >= ties)) w[i] = 0;
+      if (k < t || (k == t && w[i] > 0 && before++ >= ties)) w[i] = 0, key[i] = 0;
     }
+  };
+  auto cut_below = [&](K t) {      // keeps what is not below t
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (key[i] < t) w[i] = 0, key[i] = 0;
   };
   if (a.k) {
     K t = 0;
     int above = 0, all = 0;
 #pragma unroll
-    for (int i = 0; i < E; ++i) all += __popcll(__ballot(z[i] > -__builtin_inff()));
+    for (int i = 0; i < E; ++i) all += __popcll(__ballot(key[i] > 0));
+    waves.sum(all);
     if (all > a.k) {
-      for (int bit = BITS - 1; bit >= LOW; --bit) {
+      bool exact = false;
+      for (int bit = BITS - 1; bit >= LOW && !exact; --bit) {
         const K cand = t | ((K)1 << bit);
         int n = 0;
 #pragma unroll
         for (int i = 0; i < E; ++i) n += __popcll(__ballot(key[i] >= cand));
+        waves.sum(n);
         if (n >= a.k)
-          t = cand;
+          t = cand, exact = n == a.k;
         else
           above = n;      // the last candidate with too few is the next key above the final t: what lies above t
       }
-      // (elements of weight 0 lie below every other: they only matter as ties, where they are never drawn)
-      cut_at(t, a.k - above);
+      if (exact)
+        cut_below(t);
+      else
+        cut_at(t, a.k - above);
     }
   }
   if (a.P < 1.0) {
     double total = 0;
+    int kept = 0;
 #pragma unroll
-    for (int i = 0; i < E; ++i) total += w[i];
+    for (int i = 0; i < E; ++i) total += w[i], kept += __popcll(__ballot(key[i] > 0));
     total = wave_sum(total);
+    waves.sum(total, kept);
     const double target = a.P * total;
     K t = 0;
     double above = 0;
-    for (int bit = BITS - 1; bit >= LOW; --bit) {
+    int n_above = 0;                             // elements (w > 0) that `above` sums, and those at or above t
+    bool one = kept == 1;
+    for (int bit = BITS - 1; bit >= LOW && !one; --bit) {
       const K cand = t | ((K)1 << bit);
       double s = 0;
+      int n = 0;
 #pragma unroll
-      for (int i = 0; i < E; ++i) s += key[i] >= cand ? w[i] : 0.0;
+      for (int i = 0; i < E; ++i) {
+        const bool in = key[i] >= cand;
+        s += in ? w[i] : 0.0;
+        n += __popcll(__ballot(in));
+      }
       s = wave_sum(s);
+      waves.sum(s, n);
       if (s >= target)
-        t = cand;
+        t = cand, kept = n;
       else
-        above = s;
+        above = s, n_above = n;
+      one = kept - n_above == 1;                 // the element that takes the sum to the target
     }
-    double wt = 0;
-    const K low = LOW ? (K)((1ull << LOW) - 1) : (K)0;
+    if (one) {
+      cut_below(t);
+    } else {
+      double wt = 0;
+      const K low = LOW ? (K)((1ull << LOW) - 1) : (K)0;
 #pragma unroll
-    for (int i = 0; i < E; ++i)
-      if ((K)(key[i] | low) == (K)(t | low) && w[i] > 0) wt = w[i];
-    wt = wave_max(wt);
-    const double need = wt > 0 ? ceil((target - above) / wt) : 1.0;
-    cut_at(t, need < 1.0 ? 1 : need > (double)V ? V : (int)need);
+      for (int i = 0; i < E; ++i)
+        if ((K)(key[i] | low) == (K)(t | low) && w[i] > 0) wt = w[i];
+      wt = waves.largest(wave_max(wt));
+      const double need = wt > 0 ? ceil((target - above) / wt) : 1.0;
+      cut_at(t, need < 1.0 ? 1 : need > (double)V ? V : (int)need);
+    }
   }
   double s = 0;
 #pragma unroll
@@ -339,10 +482,14 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const Z* __restrict__ 
     if (!(w[i] >= a.M)) w[i] = 0;
     s += w[i];
   }
-  const double upto = wave_scan(s), total = __shfl(upto, 63), target = a.u * total;
+  double upto = wave_scan(s), total;
+  upto += waves.in_front(from_lane(upto, 63), total);
+  const double target = a.u * total;
   uint64_t who = __ballot(s > 0 && upto > target);
-  const bool last = who == 0;                       // u >= 1, or rounded up to it: the last kept element
-  if (last) who = __ballot(s > 0);
+  uint32_t where = waves.votes(who != 0);
+  const bool last = where == 0;                     // u >= 1, or rounded up to it: the last kept element
+  if (last) who = __ballot(s > 0), where = waves.votes(who != 0);
+  if (waves.wave != (last ? 31 - (int)__builtin_clz(where) : (int)__builtin_ctz(where))) return;
   const int at = last ? 63 - (int)__builtin_clzll(who) : (int)__builtin_ctzll(who);
   if (lane == at) {
     double c = upto - s;
@@ -1590,24 +1737,38 @@ int launch_rows(const Z* z, int64_t ld, const SampleArgs& a, int64_t* label, int
   return hipGetLastError() == hipSuccess ? TTK_OK : TTK_ELAUNCH;
 }
 
-constexpr int WAVE_ROW = 1024;      // rows up to this long: a wave a row, no workspace
+// Rows up to this long: a wave to eight waves a row, no workspace.  Sixteen waves are slower from here on where both top-k
+// and top-p cut (1398 rows of 12000 float32, top-k 50 and top-p 0.9: 276 us against 119 us of the launches below).
+constexpr int WAVE_ROW = 8192;
 
 template <typename Z>
 int launch(const void* logits, int64_t ld, const SampleArgs& a, int64_t* label, int64_t rows, int V, void* ws, int64_t ws_bytes,
            hipStream_t st) {
   const Z* z = (const Z*)logits;
   if (V > WAVE_ROW) return launch_rows<Z>(z, ld, a, label, rows, V, ws, ws_bytes, st);
-  const int64_t groups = V <= FEW ? (rows + 63) / 64 : (rows + 3) / 4;
+  const int64_t groups = V <= FEW ? (rows + 63) / 64 : V <= 1024 ? (rows + 3) / 4 : rows;
   if (groups > 0x7FFFFFFF) return TTK_EINVAL;
   const dim3 grid((unsigned)groups);
+#define K(E, W) hipLaunchKernelGGL((sample_wave_kernel<Z, E, W>), grid, dim3(W > 1 ? 64 * W : 256), 0, st, z, ld, a, label, rows, V)
   if (V <= FEW)
     hipLaunchKernelGGL((sample_few_kernel<Z>), grid, dim3(64), 0, st, z, ld, a, label, rows, V);
+  else if (V <= 64)
+    K(1, 1);
   else if (V <= 128)
-    hipLaunchKernelGGL((sample_wave_kernel<Z, 2>), grid, dim3(256), 0, st, z, ld, a, label, rows, V);
+    K(2, 1);
+  else if (V <= 256)
+    K(4, 1);
   else if (V <= 512)
-    hipLaunchKernelGGL((sample_wave_kernel<Z, 8>), grid, dim3(256), 0, st, z, ld, a, label, rows, V);
+    K(8, 1);
+  else if (V <= 1024)
+    K(16, 1);
+  else if (V <= 2048)
+    K(16, 2);
+  else if (V <= 4096)
+    K(16, 4);
   else
-    hipLaunchKernelGGL((sample_wave_kernel<Z, 16>), grid, dim3(256), 0, st, z, ld, a, label, rows, V);
+    K(16, 8);
+#undef K
   return hipGetLastError() == hipSuccess ? TTK_OK : TTK_ELAUNCH;
 }
 
