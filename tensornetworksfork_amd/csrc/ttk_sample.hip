@@ -505,7 +505,7 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void sample_wave_kernel(const
 // ---------------------------------------------------------------------------------------
 // Many classes: a few launches over all rows, a row split over workgroups where rows are few.
 //
-//   maxima    the largest logit of each of up to 1024 groups of a row's elements (their largest is m; the k-th largest bounds
+//   maxima    the largest logit of each of up to 4096 groups of a row's elements (their largest is m; the k-th largest bounds
 //             the k-th largest element from below)
 //   collect   top-k: the elements at or above that bound, a few more than k, into the row's list
 //   counts    top-p: the number of elements in each of 4096 bins below m and the sum of their places within the bin.  The
@@ -524,7 +524,7 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void sample_wave_kernel(const
 // m + T ln(min_p).  Sums are added in a fixed order, counts are whole numbers, lists are sorted: the label does not depend on
 // the order in which workgroups run.
 // ---------------------------------------------------------------------------------------
-constexpr int BINS = 2048, COUNTS = 4096, SEGS = 1024, GROUPS = 1024, LIST_CAP = 8192;
+constexpr int BINS = 2048, COUNTS = 4096, SEGS = 1024, FEW_GROUPS = 1024, GROUPS = 4096, LIST_CAP = 8192;
 constexpr int TB = 256, TW = TB / 64;      // threads and waves of the passes and of `finish`
 constexpr int RT = 1024, RW = RT / 64;     // of `counts`, `window` and `slow`
 
@@ -1027,7 +1027,7 @@ struct Geometry {
 };
 
 template <typename Z>
-Geometry geometry(int V, int64_t rows) {
+Geometry geometry(int V, int64_t rows, const SampleArgs& a) {
   constexpr int N = Chunk<Z>::N;
   Geometry g;
   g.V = V;
@@ -1035,11 +1035,16 @@ Geometry geometry(int V, int64_t rows) {
   // segments of up to 4 steps where the machine has work enough without shorter ones
   g.R = max((g.steps + SEGS - 1) / SEGS, rows * g.steps >= 16384 ? max(1, min(4, g.steps / 64)) : 1);
   g.segs = (g.steps + g.R - 1) / g.R;
-  g.per_seg = 64;
-  while (g.per_seg * g.segs > GROUPS) g.per_seg /= 2;
-  // the k-th largest of n groups' maxima has about -n ln(1 - k / n) elements at or above it
-  const int groups = g.per_seg * g.segs;
-  g.most = V <= LIST_CAP ? V : groups - groups / 128;
+  // few groups while they do (every workgroup reads them: 1 row of 131072 bfloat16, top-k 50: 24 us with 1024, 32 with 4096;
+  // but 104 us where 1024 do not bound k)
+  for (int limit = FEW_GROUPS; limit <= GROUPS; limit += GROUPS - FEW_GROUPS) {
+    g.per_seg = 64;
+    while (g.per_seg * g.segs > limit) g.per_seg /= 2;
+    // the k-th largest of n groups' maxima has about -n ln(1 - k / n) elements at or above it
+    const int groups = g.per_seg * g.segs;
+    g.most = min(groups - groups / 128, (int)(groups * (1.0 - exp(-0.92 * LIST_CAP / groups))));
+    if (!a.top_k && (a.top_k_all >= V || a.top_k_all <= g.most)) break;
+  }
   return g;
 }
 
@@ -1070,15 +1075,34 @@ __device__ __forceinline__ RowView<Z> row_part(const Z* p, const Geometry& g, in
   return {p, g.V, g.steps, g.R, wave, waves, inf};
 }
 
+// a thread's PER of the n keys of the groups' maxima, all loads under way at a time; 0 behind them
+template <int T, int PER, typename K>
+__device__ __forceinline__ void load_maxima(K (&key)[PER], const K* maxima, int n) {
+#pragma unroll
+  for (int i = 0; i < PER; ++i) key[i] = maxima[min(i * T + (int)threadIdx.x, n - 1)];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) key[i] = i * T + (int)threadIdx.x < n ? key[i] : (K)0;
+}
+template <int PER, typename K>
+__device__ __forceinline__ K largest_of(const K (&key)[PER]) {
+  K m = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) m = key[i] > m ? key[i] : m;
+  return m;
+}
+
 // the largest key of the groups' maxima, in every thread of a workgroup of T threads
 template <int T, typename K>
 __device__ __forceinline__ K largest(const K* maxima, int n, K* buf) {
-  K m = 0;
-#pragma unroll
-  for (int i = 0; i < GROUPS / T; ++i) {
-    const int at = i * T + threadIdx.x;
-    const K k = at < n ? maxima[at] : (K)0;
-    m = k > m ? k : m;
+  K m;
+  if (n <= FEW_GROUPS) {
+    K key[FEW_GROUPS / T];
+    load_maxima<T>(key, maxima, n);
+    m = largest_of(key);
+  } else {
+    K key[GROUPS / T];
+    load_maxima<T>(key, maxima, n);
+    m = largest_of(key);
   }
   m = wave_max(m);
   __syncthreads();
@@ -1145,22 +1169,39 @@ __global__ __launch_bounds__(TB) void row_collect_kernel(const Z* __restrict__ l
   const RowScale<Z> sc(largest<TB>(w.maxima, groups, buf), a);
   K bound = 0;
   if (a.k <= groups) {      // the k-th largest of the maxima, its upper 16 (64-bit keys: 24) bits, two at a time
-    K key[GROUPS / TB];
+    constexpr int PER = GROUPS / TB, LEAST = FEW_GROUPS / TB;
+    int per = LEAST;                 // a thread's keys
+    K key[PER];
+    if (groups <= FEW_GROUPS) {
+      K few[LEAST];
+      load_maxima<TB>(few, w.maxima, groups);
 #pragma unroll
-    for (int i = 0; i < GROUPS / TB; ++i) {
-      const int at = i * TB + threadIdx.x;
-      key[i] = at < groups ? w.maxima[at] : (K)0;
-      if (sc.inf) key[i] = Key<Z>::of(finite(value_of<Z>(key[i]), true));
+      for (int i = 0; i < PER; ++i) key[i] = i < LEAST ? few[i] : (K)0;
+    } else {
+      // where few are asked for, groups are joined to as many as bound k to a few elements more
+      load_maxima<TB>(key, w.maxima, groups);
+      per = PER;
+#pragma unroll
+      for (int h = PER / 2; h >= LEAST; h /= 2)
+        if (6 * a.k <= h * TB) {
+          per = h;
+#pragma unroll
+          for (int i = 0; i < h; ++i) key[i] = key[i + h] > key[i] ? key[i + h] : key[i];
+        }
     }
+    if (sc.inf)
+#pragma unroll
+      for (int i = 0; i < PER; ++i) key[i] = Key<Z>::of(finite(value_of<Z>(key[i]), true));
     constexpr int BITS = 8 * (int)sizeof(K), END = BITS - (BITS == 64 ? 24 : 16);
     int turn = 0;
 #pragma unroll 1
     for (int bit = BITS - 2; bit >= END; bit -= 2, turn ^= 1) {
       uint32_t c[3] = {0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < GROUPS / TB; ++i)
+      for (int i = 0; i < PER; ++i)
+        if (i < per)
 #pragma unroll
-        for (int j = 0; j < 3; ++j) c[j] += __popcll(__ballot(key[i] >= (bound | (K)(j + 1) << bit)));
+          for (int j = 0; j < 3; ++j) c[j] += __popcll(__ballot(key[i] >= (bound | (K)(j + 1) << bit)));
       if ((threadIdx.x & 63) == 0) counts[turn][threadIdx.x >> 6] = c[0] | (uint64_t)c[1] << 20 | (uint64_t)c[2] << 40;
       __syncthreads();
       uint64_t all = 0;
@@ -1711,7 +1752,7 @@ int launch_rows(const Z* z, int64_t ld, const SampleArgs& a, int64_t* label, int
                 hipStream_t st) {
   if (!ws || ws_bytes < min(rows, ROW_BATCH) * (int64_t)sizeof(RowWork<Z>)) return TTK_EWORKSPACE;
   RowWork<Z>* work = (RowWork<Z>*)ws;
-  const Geometry g = geometry<Z>(V, min(rows, ROW_BATCH));
+  const Geometry g = geometry<Z>(V, min(rows, ROW_BATCH), a);
   // what the rows can need (parameters of their own: anything)
   const bool any_t = a.temperature || a.temperature_all > 0.0, any_k = a.top_k || (a.top_k_all > 0 && a.top_k_all < V);
   const bool all_k = !a.top_k && any_k, any_p = a.top_p || a.top_p_all < 1.0;
