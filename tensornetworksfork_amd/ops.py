@@ -1168,10 +1168,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, p=0.0, seed=0, offset=0, sta
         raise _lib.TTKError(f"layer_norm: eps must be finite and not negative, got {eps}")
     p, seed, off, off_dev = _drop_args(p, seed, offset, x.device)
     wt = weight if weight is not None else bias if bias is not None else x
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape)
     mean = rstd = None
     if stats:
-        mean = torch.empty(x.shape[:-1], dtype=F64 if x.dtype == F64 else torch.float32, device=x.device)
+        mean = x.new_empty(x.shape[:-1], dtype=F64 if x.dtype == F64 else torch.float32)
         rstd = torch.empty_like(mean)
     if rows:
         _launch("ttk_layer_norm", x.device, ROW_TYPES[x.dtype], ROW_TYPES[wt.dtype], x.data_ptr(), ld, wp, bp, y.data_ptr(),
@@ -1199,15 +1199,15 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, p=0.0, seed=0, offset=0,
     wdt = weight.dtype if weight is not None else wdtype if wdtype is not None else x.dtype
     if wdt != x.dtype and not (wdt == torch.float32 and x.dtype in (torch.bfloat16, torch.float16)):
         raise _lib.TTKError(f"layer_norm_backward: gradients of type {wdt} do not go with rows of {x.dtype}")
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
-    make = torch.empty if rows else torch.zeros
-    dw = make((cols,), dtype=wdt, device=x.device) if need[1] else None
-    db = make((cols,), dtype=wdt, device=x.device) if need[2] else None
+    dx = x.new_empty(x.shape) if need[0] else None
+    make = x.new_empty if rows else x.new_zeros
+    dw = make(cols, dtype=wdt) if need[1] else None
+    db = make(cols, dtype=wdt) if need[2] else None
     if rows and any(need):
         ws, nbytes = None, 0
         if need[1] or need[2]:
             nbytes = int(_lib.lib().ttk_layer_norm_backward_ws_bytes(ROW_TYPES[x.dtype], rows, cols))
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+            ws = x.new_empty(nbytes, dtype=torch.uint8)
         ptr = [t.data_ptr() if t is not None else None for t in (dx, dw, db, ws)]
         _launch("ttk_layer_norm_backward", x.device, ROW_TYPES[x.dtype], ROW_TYPES[wdt], dy.data_ptr(), lddy, x.data_ptr(), ld, wp,
                 mean.data_ptr(), rstd.data_ptr(), ptr[0], ptr[1], ptr[2], rows, cols, p, seed, off, off_dev, ptr[3], nbytes)

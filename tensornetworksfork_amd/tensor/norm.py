@@ -31,6 +31,16 @@ def _rows(t):
     return t
 
 
+def _once(backward):
+    """`backward` without gradients of its own (asking for them raises); the guard costs more than the whole check here, so
+    it is only put on where autograd records the backward pass."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
 def _recorded(*ts):
     """Whether autograd has to remember the call."""
     return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in ts)
@@ -47,7 +57,7 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         x, weight, mean, rstd, off = ctx.saved_tensors
         p, seed, offset = ctx.drop
@@ -65,7 +75,7 @@ class _Dropout(torch.autograd.Function):
         return ops.dropout(x, p, seed, offset)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         off, = ctx.saved_tensors
         p, seed, offset = ctx.drop
