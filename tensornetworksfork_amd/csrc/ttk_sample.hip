@@ -4,7 +4,8 @@
 // counts as -inf).  Elements are ordered by descending logit, ties by ascending index.  top-k keeps the first k; top-p
 // keeps the elements whose exclusive cumulative weight is below top_p times the weight top-k kept; min-p keeps w_i >= min_p
 // (the largest weight is 1).  The label is the first index, in index order, whose cumulative kept weight exceeds u times
-// the total.  T <= 0 answers with the lowest index of the maximum, a row without a logit above -inf with -1.
+// the total.  T <= 0 answers with the lowest index of the maximum (temperatures between 0 and 1e-306 act as 1e-306), a row
+// without a logit above -inf with -1.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -34,6 +35,7 @@ __device__ __forceinline__ RowArgs row_args(const SampleArgs& a, int64_t row, in
   r.u = row_value(a.u, 0.0, a.f64, row);
   if (!(r.u > 0.0)) r.u = 0.0;
   r.T = row_value(a.temperature, a.temperature_all, a.f64, row);
+  if (r.T > 0.0 && r.T < 1e-306) r.T = 1e-306;      // 32 log2(e) / T stays finite
   r.P = row_value(a.top_p, a.top_p_all, a.f64, row);
   if (!(r.P < 1.0)) r.P = 1.0;
   r.M = row_value(a.min_p, a.min_p_all, a.f64, row);
@@ -644,7 +646,7 @@ struct RowWeight {
   double m, c;
   const double* pow2;
   __device__ __forceinline__ RowWeight(F m_, double T, const double* table)
-      : m((double)m_), c(fmin(32 * 1.4426950408889634074 / T, 1e300)), pow2(table) {}
+      : m((double)m_), c(32 * 1.4426950408889634074 / T), pow2(table) {}
   __device__ __forceinline__ double operator()(F z, bool keep) const {
     const int64_t b = __double_as_longlong(((double)z - m) * c);
     const int hi = keep ? (int)(b >> 32) : (int)0xC0E13000;      // -35200: 2^-1100, which is 0
