@@ -28,12 +28,14 @@ class _Forward(torch.autograd.Function):
         ctx.engine, ctx.data, ctx.shared = tn._engine, tn._current, shared
         ctx.nodes = [(n, n.tensor, n.tensor._version) for n in _nodes(tn._engine)]
         ctx.like = [(x.dtype, x.device) for x in xs]
+        ctx.save_for_backward(*xs)              # the environments are those of these values
         return out.tensor.detach()
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         eng, d = ctx.engine, ctx.data
+        ctx.saved_tensors                       # (raises where an input was changed in place since)
         if any(n.tensor is not t or t._version != v for n, t, v in ctx.nodes):
             raise RuntimeError("a node of the tensor network has changed since the forward pass: its input gradient is gone")
         eng.net._user_guard(d)

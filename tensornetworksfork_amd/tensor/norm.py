@@ -9,7 +9,11 @@ the whole set.  `offset` may be an int64 device tensor of one element, read when
 new mask on every replay if the graph (or the caller between replays) advances it.  Its value has to stay until the backward
 pass has run; changing it in place before that raises, as for any tensor autograd has saved.
 
-Gradients of gradients are not defined here (asking for them raises).
+Gradients of gradients are not defined here (asking for them raises).  Graphs: capture the forward pass together with its
+backward pass, while no eager graph of the same leaves is alive (autograd adds up a leaf's gradient on the stream its first
+graph was recorded on, which a capture on another stream does not survive).  The modules count their masks on the host: a
+captured pass replays one mask (pass an `offset` tensor to `layer_norm` / `dropout` for new ones), and a pass that is computed
+twice, as by checkpointing, draws two; `offset` is a plain attribute, to be kept by whoever resumes a training run.
 """
 import torch
 from torch import nn

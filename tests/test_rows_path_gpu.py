@@ -127,6 +127,20 @@ def test_a_node_that_changed_before_backward_is_noticed():
 
 
 @gpu
+def test_an_input_changed_in_place_before_backward_is_noticed():
+    from tensornetworksfork_amd.tensor.layers import TensorTrainLayer
+    dev = _dev()
+    layer = TensorTrainLayer(3, 4, 5, output_shape=1, seed=3).to(dev)
+    leaf = torch.randn(11, 5, device=dev, requires_grad=True)
+    x = leaf * 1.0
+    out = layer(x)
+    with torch.no_grad():
+        x.mul_(2.0)
+    with pytest.raises(RuntimeError):
+        out.sum().backward()
+
+
+@gpu
 def test_norm_dropout_train_loss_backward_and_sampled_labels():
     """rows -> LayerNorm(weight, bias, dropout) -> [features, 1] -> train -> cross entropy -> gradients of weight, bias and
     rows, against the whole chain in 64 bits on the CPU with the same mask; then labels drawn from the logits."""
