@@ -1141,20 +1141,44 @@ __global__ __launch_bounds__(TB) void row_maxima_kernel(const Z* __restrict__ lo
           });
 }
 
-// Puts the `mask`ed elements of the wave's 16-byte pieces into the row's list.
-template <typename Z, int N>
-__device__ __forceinline__ void list_add(RowWork<Z>& w, const typename Key<Z>::val_t (&v)[N], int base, uint32_t mask) {
-  const int c = __popc(mask), upto = wave_scan(c), all = from_lane(upto, 63);
-  int at = 0;
-  if ((threadIdx.x & 63) == 0) at = atomicAdd(&w.n, all);
-  at = from_lane(at, 0) + upto - c;
+// Elements of a wave on their way into the row's list: gathered in LDS, so that the list's counter, which every wave of the
+// row adds to, is asked once a wave and not once a step of its walk.
+template <typename Z>
+struct WaveList {
+  typedef typename Key<Z>::type K;
+  static constexpr int N = Chunk<Z>::N, CAP = 64 * N;      // a step's at most
+  struct Room {
+    K key[TW][CAP];
+    uint32_t idx[TW][CAP];
+  };
+  Room& room;
+  RowWork<Z>& w;
+  int n;
+  __device__ __forceinline__ WaveList(Room& r, RowWork<Z>& work) : room(r), w(work), n(0) {}
+
+  // the `mask`ed ones of the lanes' 16 bytes
+  __device__ __forceinline__ void add(const typename Key<Z>::val_t (&v)[N], int base, uint32_t mask) {
+    const int c = __popc(mask), upto = wave_scan(c), all = from_lane(upto, 63), wave = threadIdx.x >> 6;
+    if (n + all > CAP) flush();
+    int at = n + upto - c;
 #pragma unroll
-  for (int j = 0; j < N; ++j)
-    if (mask >> j & 1) {
-      if (at < LIST_CAP) w.key[at] = Key<Z>::of(v[j]), w.idx[at] = (uint32_t)(base + j);
-      ++at;
-    }
-}
+    for (int j = 0; j < N; ++j)
+      if (mask >> j & 1) room.key[wave][at] = Key<Z>::of(v[j]), room.idx[wave][at++] = (uint32_t)(base + j);
+    n += all;
+  }
+  __device__ __forceinline__ void flush() {
+    if (n == 0) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    int at = 0;
+    if (lane == 0) at = atomicAdd(&w.n, n);
+    at = from_lane(at, 0);
+    for (int i = lane; i < n; i += 64)
+      if (at + i < LIST_CAP) w.key[at + i] = room.key[wave][i], w.idx[at + i] = room.idx[wave][i];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    n = 0;
+  }
+};
 
 template <typename Z>
 __global__ __launch_bounds__(TB) void row_collect_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args, Geometry g,
@@ -1164,6 +1188,7 @@ __global__ __launch_bounds__(TB) void row_collect_kernel(const Z* __restrict__ l
   constexpr int N = Chunk<Z>::N;
   __shared__ K buf[TW];
   __shared__ uint64_t counts[2][TW];
+  __shared__ typename WaveList<Z>::Room room;
   RowWork<Z>& w = work[blockIdx.y];
   const RowArgs a = row_args(args, row0 + blockIdx.y, g.V);
   if (row_path(a, g) != LIST) return;
@@ -1216,14 +1241,16 @@ __global__ __launch_bounds__(TB) void row_collect_kernel(const Z* __restrict__ l
     }
   }
   const F lim = bound > Key<Z>::of(sc.floor) ? value_of<Z>(bound) : sc.floor;
+  WaveList<Z> list(room, w);
   walk<Z>(row_part(logits + (int64_t)blockIdx.y * ld, g, blockIdx.x * TW + (threadIdx.x >> 6), gridDim.x * TW, sc.inf),
           [&](F(&v)[N], int base) {
             uint32_t mask = 0;
 #pragma unroll
             for (int j = 0; j < N; ++j) mask |= (uint32_t)(v[j] >= lim) << j;
-            if (__any(mask != 0)) list_add<Z, N>(w, v, base, mask);
+            if (__any(mask != 0)) list.add(v, base, mask);
           },
           NoEnd());
+  list.flush();
 }
 
 // Bins over what matters of a row cut by top-p: what lies further below the maximum than ln(V / (1 - P)) weighs less than
@@ -1335,11 +1362,13 @@ __global__ __launch_bounds__(RT) void row_window_kernel(SampleArgs args, Geometr
 // The sums of a row that top-p cuts: MIN_P where the elements min-p drops are summed apart.
 template <typename Z, bool MIN_P>
 __device__ __forceinline__ void window_sums(const RowView<Z>& row, const RowScale<Z>& sc, const RowArgs& a,
-                                            const RowWeight<typename Key<Z>::val_t>& weight, RowWork<Z>& w) {
+                                            const RowWeight<typename Key<Z>::val_t>& weight, RowWork<Z>& w,
+                                            typename WaveList<Z>::Room& room) {
   typedef typename Key<Z>::val_t F;
   constexpr int N = Chunk<Z>::N;
   const F slope = bin_slope<F>(a, row.V), top = F(w.first), bottom = F(w.last + 1);
   double sum = 0, above = 0, total = 0;
+  WaveList<Z> list(room, w);
   walk<Z>(row,
           [&](F(&v)[N], int base) {
             uint32_t mask = 0;
@@ -1353,7 +1382,7 @@ __device__ __forceinline__ void window_sums(const RowView<Z>& row, const RowScal
               if (MIN_P) sum += v[j] >= sc.least ? c : 0.0;
               mask |= (uint32_t)(is && x >= top && x < bottom) << j;
             }
-            if (__any(mask != 0)) list_add<Z, N>(w, v, base, mask);
+            if (__any(mask != 0)) list.add(v, base, mask);
           },
           [&](int s) {
             total = wave_sum(total);
@@ -1362,6 +1391,7 @@ __device__ __forceinline__ void window_sums(const RowView<Z>& row, const RowScal
             if ((threadIdx.x & 63) == 0) w.seg[s] = MIN_P ? sum : above, w.above[s] = above, w.total[s] = total;
             sum = above = total = 0;
           });
+  list.flush();
 }
 
 template <typename Z>
@@ -1372,6 +1402,7 @@ __global__ __launch_bounds__(TB) void row_sums_kernel(const Z* __restrict__ logi
   constexpr int N = Chunk<Z>::N;
   __shared__ K buf[TW];
   __shared__ double pow2[32];
+  __shared__ typename WaveList<Z>::Room room;
   RowWork<Z>& w = work[blockIdx.y];
   const RowArgs a = row_args(args, row0 + blockIdx.y, g.V);
   const Path path = row_path(a, g);
@@ -1393,9 +1424,9 @@ __global__ __launch_bounds__(TB) void row_sums_kernel(const Z* __restrict__ logi
               sum = 0;
             });
   } else if (a.M > 0) {
-    window_sums<Z, true>(row, sc, a, weight, w);
+    window_sums<Z, true>(row, sc, a, weight, w, room);
   } else {
-    window_sums<Z, false>(row, sc, a, weight, w);
+    window_sums<Z, false>(row, sc, a, weight, w, room);
   }
 }
 
