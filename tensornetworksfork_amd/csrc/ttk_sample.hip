@@ -1443,16 +1443,33 @@ struct ListCut : RowSampler<Z, TB> {
   int c;
   __device__ __forceinline__ ListCut(const Base& b, const RowWork<Z>& work) : Base(b), w(work), c(work.n) {}
 
+  // f(key, index) of a thread's share of the list, eight elements under way at a time
+  template <typename Fn>
+  __device__ __forceinline__ void each(Fn f) {
+#pragma unroll 1
+    for (int i0 = threadIdx.x; i0 < c; i0 += 8 * TB) {
+      K k[8];
+      uint32_t at[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = min(i0 + j * TB, c - 1);
+        k[j] = w.key[i], at[j] = w.idx[i];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (i0 + j * TB < c) f(k[j], at[j]);
+    }
+  }
+
   // The cut behind the last element with less than `target` in front of it, of the list's elements that `cut` keeps: in
   // number, or, MASS, in weight (units of 2^-S), of which `above` lies in front of all of them (share: target is a share of
   // theirs).  False where the list does not hold it.
   template <bool MASS>
   __device__ __forceinline__ bool cut_at(Cut<F>& cut, double target, bool share, unsigned long long above) {
     K lo = ~(K)0, hi = 0;
-    for (int i = threadIdx.x; i < c; i += TB) {
-      const K k = w.key[i];
-      if (cut.keeps(value_of<Z>(k), (int)w.idx[i])) lo = k < lo ? k : lo, hi = k > hi ? k : hi;
-    }
+    each([&](K k, uint32_t at) {
+      if (cut.keeps(value_of<Z>(k), (int)at)) lo = k < lo ? k : lo, hi = k > hi ? k : hi;
+    });
     block_range<TB>(lo, hi, sh.wave_lo, sh.wave_hi);
 #pragma unroll 1
     for (;;) {
@@ -1462,11 +1479,10 @@ struct ListCut : RowSampler<Z, TB> {
       __syncthreads();
       int shift = 0;
       while (((hi - lo) >> shift) >= (K)BINS) ++shift;
-      for (int i = threadIdx.x; i < c; i += TB) {
-        const K k = w.key[i];
-        if (k >= lo && k <= hi && cut.keeps(value_of<Z>(k), (int)w.idx[i]))
+      each([&](K k, uint32_t at) {
+        if (k >= lo && k <= hi && cut.keeps(value_of<Z>(k), (int)at))
           atomicAdd(&sh.hist[(int)((hi - k) >> shift)], MASS ? whole(weight(value_of<Z>(k), true)) : 1ull);
-      }
+      });
       __syncthreads();
       const int bin = this->border_bin(above, target, share);
       share = false;
@@ -1475,16 +1491,14 @@ struct ListCut : RowSampler<Z, TB> {
       const K top = hi - ((K)bin << shift), span = ((K)1 << shift) - 1, bottom = top - lo > span ? top - span : lo;
       __syncthreads();
       K l = ~(K)0, h = 0;
-      for (int i = threadIdx.x; i < c; i += TB) {
-        const K k = w.key[i];
-        const uint32_t at = w.idx[i];
+      each([&](K k, uint32_t at) {
         if (k >= bottom && k <= top && cut.keeps(value_of<Z>(k), (int)at)) {
           const int place = atomicAdd(&sh.n, 1);
           if (place < Base::CAP) list_put<Z, TB>(sh, place, {k, ~at});
           l = k < l ? k : l;
           h = k > h ? k : h;
         }
-      }
+      });
       block_range<TB>(l, h, sh.wave_lo, sh.wave_hi);
       if (sh.n <= Base::CAP) break;
       if (l == h) return false;
@@ -1524,11 +1538,10 @@ struct ListCut : RowSampler<Z, TB> {
     __syncthreads();
     for (int i = threadIdx.x; i < SEGS; i += TB) sh.hist[i] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < c; i += TB) {
-      const F v = value_of<Z>(w.key[i]);
-      const uint32_t at = w.idx[i];
+    each([&](K k, uint32_t at) {
+      const F v = value_of<Z>(k);
       if (v >= this->sc.least && cut.keeps(v, (int)at)) atomicAdd(&sh.hist[at / (uint32_t)span], whole(weight(v, true)));
-    }
+    });
     __syncthreads();
     for (int i = threadIdx.x; i < SEGS; i += TB) sh.seg[i] += (double)sh.hist[i] / whole.fixed;
   }
