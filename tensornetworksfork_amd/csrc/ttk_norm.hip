@@ -268,7 +268,11 @@ __device__ __forceinline__ void block_sum2(A& a, A& b, A* buf) {
 }
 
 // ---------------------------------------------------------------------------------------
-// Layer norm, any row length: one workgroup walks a row as often as it needs it.
+// Layer norm, any row length: one workgroup walks a row as often as it needs it (forward: sum, centred squares, output;
+// backward: the two sums, dx; the column sums in a pass of their own).  Rows longer than the registers of a workgroup hold
+// (16384 elements; float64 backward 8192).  Bound by the second and third pass, which L2 serves: 30000 columns 2.1 TB/s
+// forward and 1.8 backward of float32 traffic counted once; few rows of millions of columns leave most of the machine idle
+// (22 rows of 3 million: 0.1 TB/s).
 // ---------------------------------------------------------------------------------------
 constexpr int LONG_THREADS = 1024;
 
@@ -396,10 +400,16 @@ __global__ __launch_bounds__(1024) void ln_cols_sum_kernel(const A* __restrict__
 // ---------------------------------------------------------------------------------------
 // Layer norm, rows held in registers: LANES lanes own a row, NV vectors of 16 bytes each (vector v of lane l starts at
 // column (v LANES + l) N).  One pass over memory: both statistics come from the registers, the variance from the centred
-// values.  LANES 16 and 64: several rows a workgroup, no barrier; 256 and more: a workgroup a row.
+// values.  LANES 8 to 64: several rows a workgroup, no barrier; 256 and more: a workgroup a row.  The next row's loads are
+// under way while a row is worked on.
 //
 // The backward pass walks many rows a workgroup and keeps each lane's columns of dw and db in registers; they leave as one
-// partial row per workgroup (`part`: [workgroup][dw | db][cols]).
+// partial row per workgroup (`part`: [workgroup][dw | db][cols]), so the rows are read once and no atomic orders the sums.
+//
+// Bound by HBM (a copy reaches 5.1 to 5.4 TB/s) up to the mask of 16-bit rows, whose counter blocks cost as much as their
+// bytes.  Measured: float32 54000 x 784 with dropout, forward 60 us (339 MB, 5.7 TB/s with the 256 MB cache's help), backward
+// 113 us (508 MB, 4.5 TB/s); bfloat16 16384 x 8192 backward 155 us (805 MB, 5.2 TB/s); float16 1021 x 10007 with dropout 28 and
+// 50 us (4 rows a workgroup: latency of a row's barriers, and up to 6 counter blocks a lane and row).
 // ---------------------------------------------------------------------------------------
 // RAGGED: the row's length is no multiple of a vector's.  The vector that reaches behind the row is then loaded from where it
 // ends with the row (no load an element, no wait before the values are used) and put right by settle_row.
@@ -718,7 +728,12 @@ __global__ __launch_bounds__(group_threads(LANES)) void ln_bwd_group_kernel(
 // ---------------------------------------------------------------------------------------
 // Layer norm of short dense rows: a wave takes 64 rows at once.  The tile (one contiguous piece of memory) goes through
 // the wave's own LDS with 16-byte accesses to memory, then each lane owns one row in registers and needs no other lane;
-// rows lie an odd number of words apart in LDS.  No barrier: a wave's LDS accesses stay in order.
+// rows lie an odd number of words apart in LDS.  No barrier: a wave's LDS accesses stay in order.  (Lanes that share such a
+// row stay partly empty: 17 float32 fill 5 of 8 vectors, and every row needs its own sums across lanes.)
+//
+// Bound by HBM; backward also by its 216 registers, two waves a SIMD.  Measured at float32 2700000 x 17: forward 83 us (378 MB,
+// 4.5 TB/s), backward 131 us (572 MB, 4.4 TB/s).  Every column's work is done whether the row has it or not: with a branch a
+// column each load of a value or a weight was waited for by itself (98 and 212 us).
 // ---------------------------------------------------------------------------------------
 constexpr int SHORT_WAVES = 4;
 
@@ -797,7 +812,7 @@ __global__ __launch_bounds__(64 * SHORT_WAVES, 4) void ln_fwd_short_kernel(
   const int wave = threadIdx.x >> 6;
   A* lds = tile[wave];
   const int pad = cols % 2 == 0, pitch = cols | 1, inv = (65536 + cols - 1) / cols;
-  __shared__ alignas(16) A weights[2][NC];      // (behind the row 0; read in the tiles' loop in one go, a load a column would wait a column)
+  __shared__ alignas(16) A weights[2][NC];      // 0 behind the row
   if (threadIdx.x < NC) {
     weights[0][threadIdx.x] = threadIdx.x < cols ? (w ? (A)w[threadIdx.x] : A(1)) : A(0);
     weights[1][threadIdx.x] = threadIdx.x < cols && b ? (A)b[threadIdx.x] : A(0);
@@ -883,7 +898,7 @@ __global__ __launch_bounds__(64 * SHORT_WAVES, 2) void ln_bwd_short_kernel(
   const int wave = threadIdx.x >> 6;
   A* lds = tile[wave];
   const int pad = cols % 2 == 0, pitch = cols | 1, inv = (65536 + cols - 1) / cols;
-  __shared__ alignas(16) A weights[1][NC];      // (behind the row 0; read in the tiles' loop in one go, a load a column would wait a column)
+  __shared__ alignas(16) A weights[1][NC];      // 0 behind the row
   if (threadIdx.x < NC) {
     weights[0][threadIdx.x] = threadIdx.x < cols ? (w ? (A)w[threadIdx.x] : A(1)) : A(0);
   }
@@ -1006,6 +1021,8 @@ __global__ __launch_bounds__(64 * SHORT_WAVES, 2) void ln_bwd_short_kernel(
 // ---------------------------------------------------------------------------------------
 // Threads own whole counter blocks: a thread's elements start where e is a multiple of 4 (memory alignment does not
 // matter, see Vec), so no block is computed twice; the first and the last vector of the array may be partial.
+// Bound by HBM and, in 16 bits, nearly as much by the ten rounds of 32 x 32 -> 64 products a block: 2^27 bfloat16 111 us
+// (537 MB, 4.8 TB/s; a copy of them 104 us).
 template <typename X>
 struct DropChunk {
   static constexpr int E = sizeof(X) == 2 ? 8 : 4;         // elements a thread takes at once
@@ -1093,7 +1110,12 @@ struct Layout {
   int lanes, nv;     // lanes 1: short dense rows, nv columns at most; lanes 0: longer than the registers hold
 };
 // Forward: few lanes with many elements each (rows of a workgroup of 256 run beside each other).  Backward: two sums stay
-// beside every element, so wide rows take more lanes.
+// beside every element, so wide rows take more lanes.  Both sides of the borders, TB/s of the rows' traffic:
+//   16-bit, 64 columns: 8 lanes 4.9 forward, 4.6 backward; 16 lanes 3.1, 2.5.  16-bit, 200 columns: 32 lanes 4.7, 64 lanes 2.5
+//   float32, 32 columns, backward: 8 lanes 4.9; a lane a row 3.3 (its registers spill); 24 columns: a lane a row 4.7
+//   float64, 16 columns, backward: 8 lanes 4.7; a lane a row 3.6
+//   bfloat16, 8192 columns, forward: 512 lanes of 2 vectors 5.5; 256 of 4 3.7.  16384 columns: 1024 of 2 5.5; 512 of 4 4.5
+//   float32, 16384 columns, backward: 1024 lanes of 4 vectors 3.0 (a few registers spill); 512 of 8 2.2
 Layout row_layout(int dtype, int cols, bool dense, bool backward) {
   if (dense && cols <= (dtype == 0 ? 8 : dtype == 1 ? 24 : 32)) return {1, (cols + 7) / 8 * 8};
   const int n = dtype == 0 ? 2 : dtype == 1 ? 4 : 8;         // elements of a 16-byte vector

@@ -154,6 +154,7 @@ __device__ __forceinline__ T wave_max(T v) {
 
 // ---------------------------------------------------------------------------------------
 // Few classes: a thread a row, everything in registers; an element's place in the order is counted against all others.
+// Bound by the launch: 60000 float64 rows of 10 take 6 us (5 MB).
 // ---------------------------------------------------------------------------------------
 constexpr int FEW = 16;
 
@@ -234,6 +235,10 @@ __global__ __launch_bounds__(64) void sample_few_kernel(const Z* __restrict__ lo
 // ---------------------------------------------------------------------------------------
 // Up to 64 E W classes: W waves a row, E consecutive elements a lane at most.  Cuts are found bit by bit: the largest key t
 // with enough elements (or weight) at or above it.  A search ends as soon as one element more or less is all that is open.
+//
+// A row is read once; the time goes into the searches (an instruction or two an element and bit) and the float64 weights.
+// Measured for 16.7 million float32 logits (a copy: 13 us), 1000 and 6000 classes a row: greedy 19 and 20 us, plain 35 and
+// 49, top-k 50 52 and 87, top-p 0.9 85 and 160.  The launches that longer rows take need 954 us for top-k 50 on rows of 1025.
 // ---------------------------------------------------------------------------------------
 typedef uint32_t raw_t __attribute__((ext_vector_type(4), aligned(2)));
 
@@ -525,6 +530,11 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void sample_wave_kernel(const
 // Elements of -inf do not exist for any of this, nor do weights below 2^-1000 of the largest; min-p is a bound on the value,
 // m + T ln(min_p).  Sums are added in a fixed order, counts are whole numbers, lists are sorted: the label does not depend on
 // the order in which workgroups run.
+//
+// Measured for 512 rows of 131072 bfloat16 (134 MB, a copy of them reads in 26 us), top-p 0.95, us: maxima 14 (HBM), counts 48
+// (one 64-bit LDS atomic an element), sums 81 (about 30 float64 instructions an element, at the rate of that unit), finish 18
+// and slow 4 (latency of one workgroup a row); top-k 50: maxima 14, collect 8, finish 14.  One row alone, top-k 50: 25, four
+// launches of which each waits for the one before.  256 rows of 100003 float32 with cuts of their own: 19 + 29 + 22 + 34 + 36.
 // ---------------------------------------------------------------------------------------
 constexpr int BINS = 2048, COUNTS = 4096, SEGS = 1024, FEW_GROUPS = 1024, GROUPS = 4096, LIST_CAP = 8192;
 constexpr int TB = 256, TW = TB / 64;      // threads and waves of the passes and of `finish`
