@@ -1069,6 +1069,7 @@ struct RowWork {
   double seg[SEGS], above[SEGS], total[SEGS];     // what is kept for certain; that before min-p; all
   K key[LIST_CAP];
   uint32_t idx[LIST_CAP];
+  K top;                                          // the largest logit (rows that are listed or summed)
   int n;                                          // elements that asked for a place in the list
   int first, last;                                // window: bins; first > last: none was found
 };
@@ -1203,7 +1204,9 @@ __global__ __launch_bounds__(TB) void row_collect_kernel(const Z* __restrict__ l
   const RowArgs a = row_args(args, row0 + blockIdx.y, g.V);
   if (row_path(a, g) != LIST) return;
   const int groups = g.segs * g.per_seg;
-  const RowScale<Z> sc(largest<TB>(w.maxima, groups, buf), a);
+  const K top = largest<TB>(w.maxima, groups, buf);
+  if (blockIdx.x == 0 && threadIdx.x == 0) w.top = top;
+  const RowScale<Z> sc(top, a);
   K bound = 0;
   if (a.k <= groups) {      // the k-th largest of the maxima, its upper 16 (64-bit keys: 24) bits, two at a time
     constexpr int PER = GROUPS / TB, LEAST = FEW_GROUPS / TB;
@@ -1323,7 +1326,9 @@ __global__ __launch_bounds__(RT) void row_counts_kernel(const Z* __restrict__ lo
   if (row_path(a, g) != WINDOW) return;
   for (int i = threadIdx.x; i < COUNTS; i += RT) counts[i] = 0;
   if (threadIdx.x == 0) beyond = 0;
-  const RowScale<Z> sc(largest<RT>(w.maxima, g.segs * g.per_seg, buf), a);      // (its barriers cover the zeros)
+  const K top = largest<RT>(w.maxima, g.segs * g.per_seg, buf);      // (its barriers cover the zeros)
+  if (blockIdx.x == 0 && threadIdx.x == 0) w.top = top;
+  const RowScale<Z> sc(top, a);
   const F slope = bin_slope<F>(a, g.V), units = (F)(1 << place_bits(g.V));
   int behind = 0;
   const int none = COUNTS + (int)(threadIdx.x & 63);
@@ -1418,7 +1423,13 @@ __global__ __launch_bounds__(TB) void row_sums_kernel(const Z* __restrict__ logi
   const Path path = row_path(a, g);
   if ((path != PLAIN && path != WINDOW) || (path == WINDOW && w.first > w.last)) return;
   fill_pow2(pow2);
-  const RowScale<Z> sc(largest<TB>(w.maxima, g.segs * g.per_seg, buf), a);      // (its barriers cover pow2)
+  // (a barrier covers pow2 either way)
+  const K top = path == WINDOW ? w.top : largest<TB>(w.maxima, g.segs * g.per_seg, buf);
+  if (path == WINDOW)
+    __syncthreads();
+  else if (blockIdx.x == 0 && threadIdx.x == 0)
+    w.top = top;
+  const RowScale<Z> sc(top, a);
   const RowWeight<F> weight(sc.m, a.T, pow2);
   const RowView<Z> row = row_part(logits + (int64_t)blockIdx.y * ld, g, blockIdx.x * TW + (threadIdx.x >> 6), gridDim.x * TW, sc.inf);
   if (path == PLAIN) {
@@ -1520,24 +1531,59 @@ struct ListCut : RowSampler<Z, TB> {
     return true;
   }
 
+  // The label of a list of at most TB elements that holds the k first, a thread an element: its place in the order, and then
+  // its place by index, is counted against all others (one row, top-k 50: a sort and the segments' sums take as long as the
+  // whole of this).
+  __device__ __forceinline__ int draw_few(const RowArgs& a) {
+    const int i = threadIdx.x;
+    Item<Z> e = {0, 0};
+    double wt = 0;
+    unsigned long long q = 0, sum;
+    if (i == 0) sh.which = 0x7FFFFFFF, sh.last = -1;
+    if (i < c) e = {w.key[i], ~w.idx[i]};
+    __syncthreads();                                 // (covers the weights' table)
+    if (i < c) {
+      wt = weight(value_of<Z>(e.k), true);
+      q = whole(wt);
+      list_put<Z, TB>(sh, i, e);
+      sh.seg[i] = __longlong_as_double((long long)q);
+    }
+    __syncthreads();
+    int rank = 0;
+    unsigned long long before = 0, upto = 0, total = 0;
+#pragma unroll 4
+    for (int j = 0; j < c; ++j) {
+      const bool front = in_front<Z>(list_get<Z, TB>(sh, j), e);
+      rank += front;
+      before += front ? (unsigned long long)__double_as_longlong(sh.seg[j]) : 0;
+    }
+    bool keep = i < c && rank < a.k;
+    if (a.P < 1.0) {
+      block_scan<TB>(keep ? q : 0, sh.wave_u, sum);
+      keep = keep && (rank == 0 || (double)before < a.P * (double)sum);
+    }
+    keep = keep && value_of<Z>(e.k) >= this->sc.least;
+    __syncthreads();
+    if (i < c) sh.seg[i] = __longlong_as_double(keep ? (long long)q : 0);
+    __syncthreads();
+    const int mine = (int)~e.n;
+#pragma unroll 4
+    for (int j = 0; j < c; ++j) {
+      const unsigned long long o = (unsigned long long)__double_as_longlong(sh.seg[j]);
+      total += o;
+      upto += (int)~list_get<Z, TB>(sh, j).n <= mine ? o : 0;
+    }
+    const double target = a.u * (double)total;
+    if (keep && wt > 0) {
+      if ((double)upto > target || !(target > 0)) atomicMin(&sh.which, mine);
+      atomicMax(&sh.last, mine);
+    }
+    __syncthreads();
+    return sh.which == 0x7FFFFFFF ? sh.last : sh.which;
+  }
+
   // top-k and top-p of a list that holds the k first elements
   __device__ __forceinline__ bool top_cut(Cut<F>& cut, const RowArgs& a) {
-    if (c <= 256) {            // few enough to sort at once
-      for (int i = threadIdx.x; i < c; i += TB) list_put<Z, TB>(sh, i, {w.key[i], ~w.idx[i]});
-      list_sort<Z, TB>(sh, c);
-      const int kk = min(a.k, c);
-      if (!(a.P < 1.0)) {
-        const Item<Z> e = list_get<Z, TB>(sh, kk - 1);
-        cut = {value_of<Z>(e.k), (int)~e.n};
-        __syncthreads();
-        return true;
-      }
-      unsigned long long q = 0, sum;
-      if ((int)threadIdx.x < kk) q = whole(weight(value_of<Z>(list_get<Z, TB>(sh, threadIdx.x).k), true));
-      block_scan<TB>(q, sh.wave_u, sum);
-      cut = this->template sorted_cut<true>(kk, a.P * (double)sum, 0);
-      return true;
-    }
     if (c > a.k && !cut_at<false>(cut, (double)a.k, false, 0)) return false;
     return !(a.P < 1.0) || cut_at<true>(cut, a.P, true, 0);
   }
@@ -1574,7 +1620,7 @@ __global__ __launch_bounds__(TB) void row_finish_kernel(const Z* __restrict__ lo
   fill_pow2(sh.pow2);
   for (int s = threadIdx.x; s < SEGS; s += TB) sh.seg[s] = (path == PLAIN || path == WINDOW) && s < g.segs ? w.seg[s] : 0.0;
   const int groups = g.segs * g.per_seg;
-  const K top = largest<TB>(w.maxima, groups, sh.wave_hi);
+  const K top = path == BY_MAX || path == SLOW ? largest<TB>(w.maxima, groups, sh.wave_hi) : w.top;
   if (!(value_of<Z>(top) > -__builtin_inff())) {
     if (threadIdx.x == 0) label[i] = -1;
     return;
@@ -1609,7 +1655,9 @@ __global__ __launch_bounds__(TB) void row_finish_kernel(const Z* __restrict__ lo
     ListCut<Z> row(sampler, w);
     Cut<F> cut = {-__builtin_inff(), -1};
     bool good = path == PLAIN;
-    if (row.c > 0 && row.c <= LIST_CAP) {
+    if (path == LIST && row.c > 0 && row.c <= TB) {
+      pick = row.draw_few(a);
+    } else if (row.c > 0 && row.c <= LIST_CAP) {
       if (path == LIST) good = row.top_cut(cut, a);
       if (path == WINDOW && w.first <= w.last) {
         double above = 0, total = 0, all_above, all;
