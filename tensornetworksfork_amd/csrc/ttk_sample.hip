@@ -1460,6 +1460,7 @@ struct ListCut : RowSampler<Z, TB> {
   using Base::sh;
   using Base::weight;
   using Base::whole;
+  static constexpr int SIDE = 1024;      // histogram words from here on lie behind the list
   const RowWork<Z>& w;
   int c;
   __device__ __forceinline__ ListCut(const Base& b, const RowWork<Z>& work) : Base(b), w(work), c(work.n) {}
@@ -1482,11 +1483,47 @@ struct ListCut : RowSampler<Z, TB> {
     }
   }
 
+  // cut_at of a list of at most TB elements, a thread an element: what lies in front of it is counted over all others.
+  template <bool MASS>
+  __device__ __forceinline__ bool cut_few(Cut<F>& cut, double target, bool share, unsigned long long above) {
+    static_assert(sizeof(sh.list) <= SIDE * sizeof(sh.hist[0]) && SIDE + TB <= BINS, "the list and what its elements count for");
+    const int i = threadIdx.x;
+    Item<Z> e = {0, 0};
+    unsigned long long q = 0, sum, kept;
+    bool in = false;
+    if (i < c) {
+      e = {w.key[i], ~w.idx[i]};
+      in = cut.keeps(value_of<Z>(e.k), (int)~e.n);
+    }
+    __syncthreads();
+    if (in) q = MASS ? whole(weight(value_of<Z>(e.k), true)) : 1ull;
+    if (i < c) list_put<Z, TB>(sh, i, in ? e : Item<Z>{0, 0}), sh.hist[SIDE + i] = q;
+    block_scan<TB>(q, sh.wave_u, sum);               // (its barriers cover the list)
+    if (share) target *= (double)(above + sum);
+    int rank = 0;
+    unsigned long long before = above;
+#pragma unroll 4
+    for (int j = 0; j < c; ++j) {
+      const bool front = in_front<Z>(list_get<Z, TB>(sh, j), e);
+      rank += front;
+      before += front ? sh.hist[SIDE + j] : 0;
+    }
+    // (the very first element is kept whatever the target)
+    const bool keep = in && ((double)before < target || (rank == 0 && above == 0));
+    block_scan<TB>((unsigned long long)keep, sh.wave_u, kept);
+    if (keep && rank == (int)kept - 1) sh.cut_key = e.k, sh.cut_idx = (int)~e.n;
+    __syncthreads();
+    if (kept == 0 || (double)(above + sum) < target) return false;
+    cut = {value_of<Z>(sh.cut_key), sh.cut_idx};
+    return true;
+  }
+
   // The cut behind the last element with less than `target` in front of it, of the list's elements that `cut` keeps: in
   // number, or, MASS, in weight (units of 2^-S), of which `above` lies in front of all of them (share: target is a share of
   // theirs).  False where the list does not hold it.
   template <bool MASS>
   __device__ __forceinline__ bool cut_at(Cut<F>& cut, double target, bool share, unsigned long long above) {
+    if (c <= TB) return cut_few<MASS>(cut, target, share, above);
     K lo = ~(K)0, hi = 0;
     each([&](K k, uint32_t at) {
       if (cut.keeps(value_of<Z>(k), (int)at)) lo = k < lo ? k : lo, hi = k > hi ? k : hi;
