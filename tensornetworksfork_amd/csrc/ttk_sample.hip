@@ -1895,8 +1895,8 @@ int launch_rows(const Z* z, int64_t ld, const SampleArgs& a, int64_t* label, int
   RowWork<Z>* work = (RowWork<Z>*)ws;
   const Geometry g = geometry<Z>(V, min(rows, ROW_BATCH), a);
   // what the rows can need (parameters of their own: anything)
-  const bool any_t = a.temperature || a.temperature_all > 0.0, any_k = a.top_k || (a.top_k_all > 0 && a.top_k_all < V);
-  const bool all_k = !a.top_k && any_k, any_p = a.top_p || a.top_p_all < 1.0;
+  const bool any_t = a.temperature || a.temperature_all > 0.0, all_k = !a.top_k && a.top_k_all > 0 && a.top_k_all < V;
+  const bool any_p = a.top_p || a.top_p_all < 1.0, any_k = a.top_k || all_k || a.top_p || !(a.top_p_all > 0.0);      // (see row_args)
   for (int64_t r0 = 0; r0 < rows; r0 += ROW_BATCH) {
     const int64_t n = min(ROW_BATCH, rows - r0);
     const Z* p = z + r0 * ld;

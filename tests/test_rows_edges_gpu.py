@@ -196,6 +196,22 @@ def test_more_rows_than_share_a_workspace(V):
 
 
 @gpu
+@pytest.mark.parametrize("V", [12, 500, 3001, 20011])
+def test_top_p_of_its_own_for_every_row_and_no_top_k(V):
+    """Shares of zero and below keep one element, shares of one and above all, also where no top-k was asked for."""
+    from tensornetworksfork_amd import ops
+    dev = N._dev()
+    g = torch.Generator().manual_seed(V)
+    z = 2.0 * torch.randn(8, V, generator=g) - 40.0
+    u = torch.rand(8, generator=g)
+    P = torch.tensor([0.0, -1.0, 0.5, 1.0, 2.0, 0.9, float("nan"), 0.0])
+    for _ in range(2):
+        torch.full((1 << 22,), 255, dtype=torch.uint8, device=dev)      # (what a workspace may hold before the call)
+        got = ops.sample(z.to(dev), u.to(dev), top_p=P.to(dev)).cpu()
+        S._check(z, u, got, [dict(k=1) if float(p) <= 0 else dict(P=float(p)) if float(p) < 1 else dict() for p in P])
+
+
+@gpu
 @pytest.mark.parametrize("V", [40, 2000, 20011])
 def test_extreme_temperatures_and_shares(V):
     """Flat and needle-like distributions, float64 rows whose logits span the whole range, shares next to 0 and 1."""

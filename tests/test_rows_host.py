@@ -43,9 +43,9 @@ def test_library_refuses_bad_arguments_before_any_launch():
         assert dr(**k) == -1, k
     for k in (dict(z=None), dict(u=None), dict(out=None), dict(rows=0), dict(V=0), dict(ld=-2), dict(dt=9), dict(V=(1 << 30) + 1)):
         assert sm(**k) == -1, k
-    need = L.ttk_sample_ws_bytes(1, 2, 5000)
-    assert need > 0 and sm(V=5000) == -2 and sm(V=5000, ws=P, n=need - 1) == -2
-    assert L.ttk_sample_ws_bytes(1, 7, 1024) == 0 and L.ttk_sample_ws_bytes(4, 7, 9) == -1 and L.ttk_sample_ws_bytes(1, 0, 9) == -1
+    need = L.ttk_sample_ws_bytes(1, 2, 9000)
+    assert need > 0 and sm(V=9000) == -2 and sm(V=9000, ws=P, n=need - 1) == -2
+    assert L.ttk_sample_ws_bytes(1, 7, 8192) == 0 and L.ttk_sample_ws_bytes(4, 7, 9) == -1 and L.ttk_sample_ws_bytes(1, 0, 9) == -1
     assert L.ttk_layer_norm_backward_ws_bytes(1, 0, 4) == -1 and L.ttk_layer_norm_backward_ws_bytes(9, 4, 4) == -1
     assert L.ttk_layer_norm_backward_ws_bytes(1, 5, 7) >= 2 * 7 * 4
 
