@@ -1244,25 +1244,36 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
             or tuple(u.shape) != shape or not u.is_contiguous():
         raise _lib.TTKError(f"u: expected a contiguous float32 / float64 tensor of shape {shape} on {logits.device}")
 
-    def param(v, name, dtype, ok):
-        if isinstance(v, torch.Tensor):
-            if v.dtype != dtype or v.device != logits.device or tuple(v.shape) != shape or not v.is_contiguous():
-                raise _lib.TTKError(f"{name}: expected a number or a contiguous {dtype} tensor of shape {shape} on {logits.device}")
-            return v.data_ptr(), 0
-        if not ok(v):
-            raise _lib.TTKError(f"{name}: {v} is out of range")
-        return None, v
-    tp, t = param(temperature, "temperature", u.dtype, lambda v: 0.0 <= v < float("inf"))
-    kp, k = param(top_k, "top_k", torch.int32, lambda v: int(v) == v and v >= 0)
-    pp, pv = param(top_p, "top_p", u.dtype, lambda v: 0.0 < v <= 1.0)
-    mp, mv = param(min_p, "min_p", u.dtype, lambda v: 0.0 <= v <= 1.0)
-    label = torch.empty(shape, dtype=torch.int64, device=logits.device)
+    def pointer(v, name, dtype):
+        if v.dtype != dtype or v.device != logits.device or tuple(v.shape) != shape or not v.is_contiguous():
+            raise _lib.TTKError(f"{name}: expected a number or a contiguous {dtype} tensor of shape {shape} on {logits.device}")
+        return v.data_ptr()
+
+    t, k, p, m = temperature, top_k, top_p, min_p
+    tp = kp = pp = mp = None
+    if isinstance(t, torch.Tensor):
+        tp, t = pointer(t, "temperature", u.dtype), 0.0
+    elif not 0.0 <= t < float("inf"):
+        raise _lib.TTKError(f"temperature: {t} is out of range")
+    if isinstance(k, torch.Tensor):
+        kp, k = pointer(k, "top_k", torch.int32), 0
+    elif k < 0 or int(k) != k:
+        raise _lib.TTKError(f"top_k: {k} is out of range")
+    if isinstance(p, torch.Tensor):
+        pp, p = pointer(p, "top_p", u.dtype), 1.0
+    elif not 0.0 < p <= 1.0:
+        raise _lib.TTKError(f"top_p: {p} is out of range")
+    if isinstance(m, torch.Tensor):
+        mp, m = pointer(m, "min_p", u.dtype), 0.0
+    elif not 0.0 <= m <= 1.0:
+        raise _lib.TTKError(f"min_p: {m} is out of range")
+    label = logits.new_empty(shape, dtype=torch.int64)
     if rows:
         if V > 1 << 30:
             raise _lib.TTKError("logits: more than 2^30 classes")
-        nbytes = int(_lib.lib().ttk_sample_ws_bytes(ROW_TYPES[logits.dtype], rows, V))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
-        _launch("ttk_sample", logits.device, ROW_TYPES[logits.dtype], logits.data_ptr(), ld, u.data_ptr(), int(u.dtype == F64), tp,
-                float(t), kp, min(int(k), 0x7FFFFFFF), pp, float(pv), mp, float(mv), label.data_ptr(), rows, V,
-                ws.data_ptr() if nbytes else None, nbytes)
+        code = ROW_TYPES[logits.dtype]
+        nbytes = int(_lib.lib().ttk_sample_ws_bytes(code, rows, V))
+        ws = logits.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+        _launch("ttk_sample", logits.device, code, logits.data_ptr(), ld, u.data_ptr(), int(u.dtype == F64), tp, float(t), kp,
+                min(int(k), 0x7FFFFFFF), pp, float(p), mp, float(m), label.data_ptr(), rows, V, ws.data_ptr() if nbytes else None, nbytes)
     return label
