@@ -515,17 +515,17 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void sample_wave_kernel(const
 //   maxima    the largest logit of each of up to 4096 groups of a row's elements (their largest is m; the k-th largest bounds
 //             the k-th largest element from below)
 //   collect   top-k: the elements at or above that bound, a few more than k, into the row's list
-//   counts    top-p: the number of elements in each of 4096 bins below m and the sum of their places within the bin.  The
-//             bin's weight follows to second order in its width (relative 1e-5), so the cumulative weight is bounded from both
-//             sides, and
-//   window    the border of top-p lies in a window of a few bins
+//   counts    top-p, and top-k where the list would not hold it: the number of elements in each of 4096 bins below m and the
+//             sum of their places within the bin.  The bin's weight follows to second order in its width (relative 1e-5), so
+//             the cumulative weight is bounded from both sides, and
+//   window    the border of top-p lies in a window of a few bins, that of top-k in one
 //   sums      every weight once: float64 sums of the kept ones per segment of the row, and of the rest; the window's elements
 //             go into the row's list
 //   finish    a workgroup a row: the cut, by histograms of the list refined until the bin with the border can be sorted in LDS;
 //             what the cut keeps of the list joins the segment sums; the segment where their running sum passes u times the
 //             total, and the element in it
-//   slow      the rows whose list does not hold what it should (top-k above what the groups bound, thousands of equal
-//             logits): the same cuts by histograms over the whole row
+//   slow      the rows whose list does not hold what it should (thousands of equal logits) and those that both top-p and a
+//             top-k above what the groups bound cut: the same by histograms over the whole row
 //
 // Elements of -inf do not exist for any of this, nor do weights below 2^-1000 of the largest; min-p is a bound on the value,
 // m + T ln(min_p).  Sums are added in a fixed order, counts are whole numbers, lists are sorted: the label does not depend on
@@ -1072,13 +1072,14 @@ struct RowWork {
   K top;                                          // the largest logit (rows that are listed or summed)
   int n;                                          // elements that asked for a place in the list
   int first, last;                                // window: bins; first > last: none was found
+  int before;                                     // top-k: elements in front of the window
 };
 
 enum Path { BY_MAX, LIST, WINDOW, PLAIN, SLOW };
 
 __device__ __forceinline__ Path row_path(const RowArgs& a, const Geometry& g) {
   if (!(a.T > 0.0)) return BY_MAX;
-  if (a.k) return a.k <= g.most ? LIST : SLOW;
+  if (a.k) return a.k <= g.most ? LIST : a.P < 1.0 ? SLOW : WINDOW;
   return a.P < 1.0 ? WINDOW : PLAIN;
 }
 
@@ -1267,10 +1268,11 @@ __global__ __launch_bounds__(TB) void row_collect_kernel(const Z* __restrict__ l
 }
 
 // Bins over what matters of a row cut by top-p: what lies further below the maximum than ln(V / (1 - P)) weighs less than
-// 1 - P of the total, and five units more make what lies behind the bins weigh nothing against a bin.
+// 1 - P of the total, and five units more make what lies behind the bins weigh nothing against a bin.  Top-k alone: bins down
+// to what weighs 1e-9 / V of the total, where the k-th element mostly is.
 template <typename F>
 __device__ __forceinline__ F bin_slope(const RowArgs& a, int V) {
-  return (F)fmin((double)COUNTS / (a.T * (log((double)V / (1.0 - a.P)) + 5.0)), 1e38);
+  return (F)fmin((double)COUNTS / (a.T * (log((double)V / (a.k ? 1e-9 : 1.0 - a.P)) + 5.0)), 1e38);
 }
 // Places within a bin are counted in units of 2^-place_bits: V of them stay below 2^33.
 __device__ __forceinline__ int place_bits(int V) { return min(10, 1 + (int)__builtin_clz(V)); }
@@ -1310,6 +1312,24 @@ __device__ __forceinline__ void find_window(const unsigned long long* counts, in
   __syncthreads();
 }
 
+// The bin of the k-th element, and the number of elements in front of it.
+__device__ __forceinline__ void find_kth(const unsigned long long* counts, int k, double* buf, int* found) {
+  constexpr int PER = COUNTS / RT;
+  int n[PER], mine = 0;
+  double total;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) n[i] = (int)(counts[PER * threadIdx.x + i] >> 33), mine += n[i];
+  int before = (int)(block_scan<RT>((double)mine, buf, total)) - mine;
+  if (threadIdx.x == 0) found[0] = found[1] = COUNTS, found[2] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (before < k && before + n[i] >= k) found[0] = found[1] = PER * threadIdx.x + i, found[2] = before;
+    before += n[i];
+  }
+  __syncthreads();
+}
+
 // counts; where a row has one workgroup, its window too (`n` of the row's work holds, meanwhile, the elements behind the bins)
 template <typename Z>
 __global__ __launch_bounds__(RT) void row_counts_kernel(const Z* __restrict__ logits, int64_t ld, SampleArgs args, Geometry g,
@@ -1320,7 +1340,7 @@ __global__ __launch_bounds__(RT) void row_counts_kernel(const Z* __restrict__ lo
   __shared__ unsigned long long counts[COUNTS + 64];      // the last 64: elements that are not counted
   __shared__ K buf[RW];
   __shared__ double dbuf[RW];
-  __shared__ int beyond, found[2];
+  __shared__ int beyond, found[3];
   RowWork<Z>& w = work[blockIdx.y];
   const RowArgs a = row_args(args, row0 + blockIdx.y, g.V);
   if (row_path(a, g) != WINDOW) return;
@@ -1353,8 +1373,11 @@ __global__ __launch_bounds__(RT) void row_counts_kernel(const Z* __restrict__ lo
   if ((threadIdx.x & 63) == 0 && behind) atomicAdd(&beyond, behind);
   __syncthreads();
   if (gridDim.x == 1) {
-    find_window(counts, beyond, (double)slope, a, g.V, dbuf, found);
-    if (threadIdx.x == 0) w.first = found[0], w.last = found[1] < COUNTS ? found[1] : -1;
+    if (a.k)
+      find_kth(counts, a.k, dbuf, found);
+    else
+      find_window(counts, beyond, (double)slope, a, g.V, dbuf, found);
+    if (threadIdx.x == 0) w.first = found[0], w.last = found[1] < COUNTS ? found[1] : -1, w.before = a.k ? found[2] : 0;
     return;
   }
   for (int i = threadIdx.x; i < COUNTS; i += RT)
@@ -1366,12 +1389,16 @@ template <typename Z>
 __global__ __launch_bounds__(RT) void row_window_kernel(SampleArgs args, Geometry g, RowWork<Z>* __restrict__ work, int64_t row0) {
   typedef typename Key<Z>::val_t F;
   __shared__ double dbuf[RW];
-  __shared__ int found[2];
+  __shared__ int found[3];
   RowWork<Z>& w = work[blockIdx.x];
   const RowArgs a = row_args(args, row0 + blockIdx.x, g.V);
   if (row_path(a, g) != WINDOW) return;
-  find_window(w.counts, w.n, (double)bin_slope<F>(a, g.V), a, g.V, dbuf, found);
-  if (threadIdx.x == 0) w.first = found[0], w.last = found[1] < COUNTS ? found[1] : -1, w.n = 0;
+  if (a.k)
+    find_kth(w.counts, a.k, dbuf, found);
+  else
+    find_window(w.counts, w.n, (double)bin_slope<F>(a, g.V), a, g.V, dbuf, found);
+  if (threadIdx.x == 0)
+    w.first = found[0], w.last = found[1] < COUNTS ? found[1] : -1, w.before = a.k ? found[2] : 0, w.n = 0;
 }
 
 // The sums of a row that top-p cuts: MIN_P where the elements min-p drops are summed apart.
@@ -1696,7 +1723,9 @@ __global__ __launch_bounds__(TB) void row_finish_kernel(const Z* __restrict__ lo
       pick = row.draw_few(a);
     } else if (row.c > 0 && row.c <= LIST_CAP) {
       if (path == LIST) good = row.top_cut(cut, a);
-      if (path == WINDOW && w.first <= w.last) {
+      if (path == WINDOW && w.first <= w.last && a.k) {
+        good = row.template cut_at<false>(cut, (double)a.k, false, (unsigned long long)w.before);
+      } else if (path == WINDOW && w.first <= w.last) {
         double above = 0, total = 0, all_above, all;
         for (int s = threadIdx.x; s < g.segs; s += TB) above += w.above[s], total += w.total[s];
         block_scan<TB>(above, sh.wave_d, all_above);
@@ -1905,9 +1934,10 @@ int launch_rows(const Z* z, int64_t ld, const SampleArgs& a, int64_t* label, int
     const int wide = (int)max((int64_t)1, min((int64_t)(g.segs + RW - 1) / RW, (256 + n - 1) / n));
     const dim3 grid((unsigned)split, (unsigned)n), big((unsigned)wide, (unsigned)n), one((unsigned)n);
     hipLaunchKernelGGL((row_maxima_kernel<Z>), grid, dim3(TB), 0, st, p, ld, g, work);
-    if (any_t && any_k) hipLaunchKernelGGL((row_collect_kernel<Z>), grid, dim3(TB), 0, st, p, ld, a, g, work, r0);
-    if (any_t && !all_k) {
-      if (any_p) {
+    const bool no_list = all_k && a.top_k_all > g.most && !a.top_p && a.top_p_all > 0.0;
+    if (any_t && any_k && !no_list) hipLaunchKernelGGL((row_collect_kernel<Z>), grid, dim3(TB), 0, st, p, ld, a, g, work, r0);
+    if (any_t && (!all_k || a.top_k_all > g.most)) {
+      if (any_p || any_k) {
         hipLaunchKernelGGL((row_counts_kernel<Z>), big, dim3(RT), 0, st, p, ld, a, g, work, r0);
         if (wide > 1) hipLaunchKernelGGL((row_window_kernel<Z>), one, dim3(RT), 0, st, a, g, work, r0);
       }
