@@ -533,8 +533,8 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void sample_wave_kernel(const
 //
 // Measured for 512 rows of 131072 bfloat16 (134 MB, a copy of them reads in 26 us), top-p 0.95, us: maxima 14 (HBM), counts 48
 // (one 64-bit LDS atomic an element), sums 81 (about 30 float64 instructions an element, at the rate of that unit), finish 18
-// and slow 4 (latency of one workgroup a row); top-k 50: maxima 14, collect 8, finish 14.  One row alone, top-k 50: 25, four
-// launches of which each waits for the one before.  256 rows of 100003 float32 with cuts of their own: 19 + 29 + 22 + 34 + 36.
+// and slow 4 (latency of one workgroup a row).  One row alone, top-k 50: 20, four launches of which each waits for the one
+// before.  256 rows of 100003 float32 with cuts of their own: 19 + 29 + 22 + 34 + 34 + 4.
 // ---------------------------------------------------------------------------------------
 constexpr int BINS = 2048, COUNTS = 4096, SEGS = 1024, FEW_GROUPS = 1024, GROUPS = 4096, LIST_CAP = 8192;
 constexpr int TB = 256, TW = TB / 64;      // threads and waves of the passes and of `finish`
@@ -1035,7 +1035,7 @@ struct RowSampler {
 
 struct Geometry {
   int V, steps, R, segs, per_seg;      // per_seg: groups a segment (a power of two)
-  int most;                            // top-k up to this many is taken from the list
+  int most, alone;                     // top-k up to this many is taken from the list: with top-p, by itself
 };
 
 template <typename Z>
@@ -1055,8 +1055,12 @@ Geometry geometry(int V, int64_t rows, const SampleArgs& a) {
     // the k-th largest of n groups' maxima has about -n ln(1 - k / n) elements at or above it
     const int groups = g.per_seg * g.segs;
     g.most = min(groups - groups / 128, (int)(groups * (1.0 - exp(-0.92 * LIST_CAP / groups))));
-    if (!a.top_k && (a.top_k_all >= V || a.top_k_all <= g.most)) break;
+    if (!a.top_k && (a.top_k_all >= V || a.top_k_all <= g.most || (!a.top_p && a.top_p_all >= 1.0 && (rows <= 64 || a.top_k_all > FEW_GROUPS))))
+      break;
   }
+  // few rows, top-k alone: a list that is not short keeps the row's one workgroup busy longer than the windows' launches take (1
+  // row of 131072 float32, top-k 900: 39 us against 25, top-k 190: 28 against 25; 128 rows, top-k 900: 58 us against 70)
+  g.alone = rows <= 64 ? min(g.most, 128) : g.most;
   return g;
 }
 
@@ -1079,7 +1083,7 @@ enum Path { BY_MAX, LIST, WINDOW, PLAIN, SLOW };
 
 __device__ __forceinline__ Path row_path(const RowArgs& a, const Geometry& g) {
   if (!(a.T > 0.0)) return BY_MAX;
-  if (a.k) return a.k <= g.most ? LIST : a.P < 1.0 ? SLOW : WINDOW;
+  if (a.k) return a.k <= (a.P < 1.0 ? g.most : g.alone) ? LIST : a.P < 1.0 ? SLOW : WINDOW;
   return a.P < 1.0 ? WINDOW : PLAIN;
 }
 
@@ -1510,6 +1514,22 @@ struct ListCut : RowSampler<Z, TB> {
     }
   }
 
+  // f(element, what it counts for) of all elements of a list of at most TB, in every thread, eight under way at a time (the
+  // list is filled up to a multiple of eight with elements that sort last and count for nothing)
+  template <typename Fn>
+  __device__ __forceinline__ void all(const unsigned long long* counts, Fn f) {
+#pragma unroll 1
+    for (int j0 = 0; j0 < c; j0 += 8) {
+      Item<Z> o[8];
+      unsigned long long q[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = list_get<Z, TB>(sh, j0 + j), q[j] = counts[j0 + j];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f(o[j], q[j]);
+    }
+  }
+  __device__ __forceinline__ bool fills(int i) { return i < ((c + 7) & ~7); }
+
   // cut_at of a list of at most TB elements, a thread an element: what lies in front of it is counted over all others.
   template <bool MASS>
   __device__ __forceinline__ bool cut_few(Cut<F>& cut, double target, bool share, unsigned long long above) {
@@ -1524,17 +1544,16 @@ struct ListCut : RowSampler<Z, TB> {
     }
     __syncthreads();
     if (in) q = MASS ? whole(weight(value_of<Z>(e.k), true)) : 1ull;
-    if (i < c) list_put<Z, TB>(sh, i, in ? e : Item<Z>{0, 0}), sh.hist[SIDE + i] = q;
+    if (fills(i)) list_put<Z, TB>(sh, i, in ? e : Item<Z>{0, 0}), sh.hist[SIDE + i] = q;
     block_scan<TB>(q, sh.wave_u, sum);               // (its barriers cover the list)
     if (share) target *= (double)(above + sum);
     int rank = 0;
     unsigned long long before = above;
-#pragma unroll 4
-    for (int j = 0; j < c; ++j) {
-      const bool front = in_front<Z>(list_get<Z, TB>(sh, j), e);
+    all(sh.hist + SIDE, [&](const Item<Z>& o, unsigned long long n) {
+      const bool front = in_front<Z>(o, e);
       rank += front;
-      before += front ? sh.hist[SIDE + j] : 0;
-    }
+      before += front ? n : 0;
+    });
     // (the very first element is kept whatever the target)
     const bool keep = in && ((double)before < target || (rank == 0 && above == 0));
     block_scan<TB>((unsigned long long)keep, sh.wave_u, kept);
@@ -1609,18 +1628,16 @@ struct ListCut : RowSampler<Z, TB> {
     if (i < c) {
       wt = weight(value_of<Z>(e.k), true);
       q = whole(wt);
-      list_put<Z, TB>(sh, i, e);
-      sh.seg[i] = __longlong_as_double((long long)q);
     }
+    if (fills(i)) list_put<Z, TB>(sh, i, e), sh.hist[SIDE + i] = q;
     __syncthreads();
     int rank = 0;
     unsigned long long before = 0, upto = 0, total = 0;
-#pragma unroll 4
-    for (int j = 0; j < c; ++j) {
-      const bool front = in_front<Z>(list_get<Z, TB>(sh, j), e);
+    all(sh.hist + SIDE, [&](const Item<Z>& o, unsigned long long n) {
+      const bool front = in_front<Z>(o, e);
       rank += front;
-      before += front ? (unsigned long long)__double_as_longlong(sh.seg[j]) : 0;
-    }
+      before += front ? n : 0;
+    });
     bool keep = i < c && rank < a.k;
     if (a.P < 1.0) {
       block_scan<TB>(keep ? q : 0, sh.wave_u, sum);
@@ -1628,15 +1645,13 @@ struct ListCut : RowSampler<Z, TB> {
     }
     keep = keep && value_of<Z>(e.k) >= this->sc.least;
     __syncthreads();
-    if (i < c) sh.seg[i] = __longlong_as_double(keep ? (long long)q : 0);
+    if (fills(i)) sh.hist[SIDE + i] = keep ? q : 0;
     __syncthreads();
     const int mine = (int)~e.n;
-#pragma unroll 4
-    for (int j = 0; j < c; ++j) {
-      const unsigned long long o = (unsigned long long)__double_as_longlong(sh.seg[j]);
-      total += o;
-      upto += (int)~list_get<Z, TB>(sh, j).n <= mine ? o : 0;
-    }
+    all(sh.hist + SIDE, [&](const Item<Z>& o, unsigned long long n) {
+      total += n;
+      upto += (int)~o.n <= mine ? n : 0;
+    });
     const double target = a.u * (double)total;
     if (keep && wt > 0) {
       if ((double)upto > target || !(target > 0)) atomicMin(&sh.which, mine);
@@ -1926,6 +1941,8 @@ int launch_rows(const Z* z, int64_t ld, const SampleArgs& a, int64_t* label, int
   // what the rows can need (parameters of their own: anything)
   const bool any_t = a.temperature || a.temperature_all > 0.0, all_k = !a.top_k && a.top_k_all > 0 && a.top_k_all < V;
   const bool any_p = a.top_p || a.top_p_all < 1.0, any_k = a.top_k || all_k || a.top_p || !(a.top_p_all > 0.0);      // (see row_args)
+  const int most = !a.top_p && a.top_p_all < 1.0 ? g.most : g.alone;
+  const bool no_list = all_k && a.top_k_all > most && !a.top_p && a.top_p_all > 0.0, sums = !all_k || a.top_k_all > most;
   for (int64_t r0 = 0; r0 < rows; r0 += ROW_BATCH) {
     const int64_t n = min(ROW_BATCH, rows - r0);
     const Z* p = z + r0 * ld;
@@ -1934,9 +1951,8 @@ int launch_rows(const Z* z, int64_t ld, const SampleArgs& a, int64_t* label, int
     const int wide = (int)max((int64_t)1, min((int64_t)(g.segs + RW - 1) / RW, (256 + n - 1) / n));
     const dim3 grid((unsigned)split, (unsigned)n), big((unsigned)wide, (unsigned)n), one((unsigned)n);
     hipLaunchKernelGGL((row_maxima_kernel<Z>), grid, dim3(TB), 0, st, p, ld, g, work);
-    const bool no_list = all_k && a.top_k_all > g.most && !a.top_p && a.top_p_all > 0.0;
     if (any_t && any_k && !no_list) hipLaunchKernelGGL((row_collect_kernel<Z>), grid, dim3(TB), 0, st, p, ld, a, g, work, r0);
-    if (any_t && (!all_k || a.top_k_all > g.most)) {
+    if (any_t && sums) {
       if (any_p || any_k) {
         hipLaunchKernelGGL((row_counts_kernel<Z>), big, dim3(RT), 0, st, p, ld, a, g, work, r0);
         if (wide > 1) hipLaunchKernelGGL((row_window_kernel<Z>), one, dim3(RT), 0, st, a, g, work, r0);
