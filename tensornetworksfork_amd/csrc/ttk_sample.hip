@@ -1514,21 +1514,42 @@ struct ListCut : RowSampler<Z, TB> {
     }
   }
 
-  // f(element, what it counts for) of all elements of a list of at most TB, in every thread, eight under way at a time (the
-  // list is filled up to a multiple of eight with elements that sort last and count for nothing)
+  // f(element, what it counts for) of the n (at most TB) elements in LDS, in every thread, eight under way at a time (they are
+  // filled up to a multiple of eight with elements that sort last and count for nothing)
   template <typename Fn>
-  __device__ __forceinline__ void all(const unsigned long long* counts, Fn f) {
+  __device__ __forceinline__ void all(int n, Fn f) {
 #pragma unroll 1
-    for (int j0 = 0; j0 < c; j0 += 8) {
+    for (int j0 = 0; j0 < n; j0 += 8) {
       Item<Z> o[8];
       unsigned long long q[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o[j] = list_get<Z, TB>(sh, j0 + j), q[j] = counts[j0 + j];
+      for (int j = 0; j < 8; ++j) o[j] = list_get<Z, TB>(sh, j0 + j), q[j] = sh.hist[SIDE + j0 + j];
 #pragma unroll
       for (int j = 0; j < 8; ++j) f(o[j], q[j]);
     }
   }
-  __device__ __forceinline__ bool fills(int i) { return i < ((c + 7) & ~7); }
+  static __device__ __forceinline__ bool fills(int i, int n) { return i < ((n + 7) & ~7); }
+
+  // The last of the n elements in LDS, a thread an element (in: this thread has one), that has less than `target` in front of
+  // it, or the first of them where `first` says so; false where there is none.
+  __device__ __forceinline__ bool last_kept(Cut<F>& cut, const Item<Z>& e, bool in, int n, double target, unsigned long long above,
+                                            bool first) {
+    int rank = 0;
+    unsigned long long before = above, kept;
+    all(n, [&](const Item<Z>& o, unsigned long long q) {
+      const bool front = in_front<Z>(o, e);
+      rank += front;
+      before += front ? q : 0;
+    });
+    const bool keep = in && ((double)before < target || (rank == 0 && first));
+    block_scan<TB>((unsigned long long)keep, sh.wave_u, kept);
+    if (keep && rank == (int)kept - 1) sh.cut_key = e.k, sh.cut_idx = (int)~e.n;
+    __syncthreads();
+    if (kept == 0) return false;
+    cut = {value_of<Z>(sh.cut_key), sh.cut_idx};
+    __syncthreads();
+    return true;
+  }
 
   // cut_at of a list of at most TB elements, a thread an element: what lies in front of it is counted over all others.
   template <bool MASS>
@@ -1536,7 +1557,7 @@ struct ListCut : RowSampler<Z, TB> {
     static_assert(sizeof(sh.list) <= SIDE * sizeof(sh.hist[0]) && SIDE + TB <= BINS, "the list and what its elements count for");
     const int i = threadIdx.x;
     Item<Z> e = {0, 0};
-    unsigned long long q = 0, sum, kept;
+    unsigned long long q = 0, sum;
     bool in = false;
     if (i < c) {
       e = {w.key[i], ~w.idx[i]};
@@ -1544,24 +1565,11 @@ struct ListCut : RowSampler<Z, TB> {
     }
     __syncthreads();
     if (in) q = MASS ? whole(weight(value_of<Z>(e.k), true)) : 1ull;
-    if (fills(i)) list_put<Z, TB>(sh, i, in ? e : Item<Z>{0, 0}), sh.hist[SIDE + i] = q;
+    if (fills(i, c)) list_put<Z, TB>(sh, i, in ? e : Item<Z>{0, 0}), sh.hist[SIDE + i] = q;
     block_scan<TB>(q, sh.wave_u, sum);               // (its barriers cover the list)
     if (share) target *= (double)(above + sum);
-    int rank = 0;
-    unsigned long long before = above;
-    all(sh.hist + SIDE, [&](const Item<Z>& o, unsigned long long n) {
-      const bool front = in_front<Z>(o, e);
-      rank += front;
-      before += front ? n : 0;
-    });
     // (the very first element is kept whatever the target)
-    const bool keep = in && ((double)before < target || (rank == 0 && above == 0));
-    block_scan<TB>((unsigned long long)keep, sh.wave_u, kept);
-    if (keep && rank == (int)kept - 1) sh.cut_key = e.k, sh.cut_idx = (int)~e.n;
-    __syncthreads();
-    if (kept == 0 || (double)(above + sum) < target) return false;
-    cut = {value_of<Z>(sh.cut_key), sh.cut_idx};
-    return true;
+    return last_kept(cut, e, in, c, target, above, above == 0) && (double)(above + sum) >= target;
   }
 
   // The cut behind the last element with less than `target` in front of it, of the list's elements that `cut` keeps: in
@@ -1608,7 +1616,17 @@ struct ListCut : RowSampler<Z, TB> {
       if (l == h) return false;
       lo = l, hi = h;
     }
-    const int n = sh.n;
+    const int n = sh.n, i = threadIdx.x;
+    if (n <= TB) {
+      Item<Z> e = {0, 0};
+      if (i < n) e = list_get<Z, TB>(sh, i);
+      if (fills(i, n)) {
+        sh.hist[SIDE + i] = i >= n ? 0 : MASS ? whole(weight(value_of<Z>(e.k), true)) : 1ull;
+        if (i >= n) list_put<Z, TB>(sh, i, e);
+      }
+      __syncthreads();
+      return last_kept(cut, e, i < n, n, target, above, true);
+    }
     list_sort<Z, TB>(sh, n);
     cut = this->template sorted_cut<MASS>(n, target, above);
     return true;
@@ -1629,11 +1647,11 @@ struct ListCut : RowSampler<Z, TB> {
       wt = weight(value_of<Z>(e.k), true);
       q = whole(wt);
     }
-    if (fills(i)) list_put<Z, TB>(sh, i, e), sh.hist[SIDE + i] = q;
+    if (fills(i, c)) list_put<Z, TB>(sh, i, e), sh.hist[SIDE + i] = q;
     __syncthreads();
     int rank = 0;
     unsigned long long before = 0, upto = 0, total = 0;
-    all(sh.hist + SIDE, [&](const Item<Z>& o, unsigned long long n) {
+    all(c, [&](const Item<Z>& o, unsigned long long n) {
       const bool front = in_front<Z>(o, e);
       rank += front;
       before += front ? n : 0;
@@ -1645,10 +1663,10 @@ struct ListCut : RowSampler<Z, TB> {
     }
     keep = keep && value_of<Z>(e.k) >= this->sc.least;
     __syncthreads();
-    if (fills(i)) sh.hist[SIDE + i] = keep ? q : 0;
+    if (fills(i, c)) sh.hist[SIDE + i] = keep ? q : 0;
     __syncthreads();
     const int mine = (int)~e.n;
-    all(sh.hist + SIDE, [&](const Item<Z>& o, unsigned long long n) {
+    all(c, [&](const Item<Z>& o, unsigned long long n) {
       total += n;
       upto += (int)~o.n <= mine ? n : 0;
     });
