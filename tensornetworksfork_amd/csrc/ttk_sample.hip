@@ -521,9 +521,10 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void sample_wave_kernel(const
 //   window    the border of top-p lies in a window of a few bins, that of top-k in one
 //   sums      every weight once: float64 sums of the kept ones per segment of the row, and of the rest; the window's elements
 //             go into the row's list
-//   finish    a workgroup a row: the cut, by histograms of the list refined until the bin with the border can be sorted in LDS;
-//             what the cut keeps of the list joins the segment sums; the segment where their running sum passes u times the
-//             total, and the element in it
+//   finish    a workgroup a row: the cut, by histograms of the list refined until few elements share the border's bin, whose
+//             order is then counted (or, up to 512, sorted) in LDS; what the cut keeps of the list joins the segment sums; the
+//             segment where their running sum passes u times the total, and the element in it.  A top-k list of at most 256
+//             elements is drawn from by itself
 //   slow      the rows whose list does not hold what it should (thousands of equal logits) and those that both top-p and a
 //             top-k above what the groups bound cut: the same by histograms over the whole row
 //
@@ -531,10 +532,10 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void sample_wave_kernel(const
 // m + T ln(min_p).  Sums are added in a fixed order, counts are whole numbers, lists are sorted: the label does not depend on
 // the order in which workgroups run.
 //
-// Measured for 512 rows of 131072 bfloat16 (134 MB, a copy of them reads in 26 us), top-p 0.95, us: maxima 14 (HBM), counts 48
-// (one 64-bit LDS atomic an element), sums 81 (about 30 float64 instructions an element, at the rate of that unit), finish 18
-// and slow 4 (latency of one workgroup a row).  One row alone, top-k 50: 20, four launches of which each waits for the one
-// before.  256 rows of 100003 float32 with cuts of their own: 19 + 29 + 22 + 34 + 34 + 4.
+// Measured for 512 rows of 131072 bfloat16 (134 MB, read in 26 us at a copy's rate), top-p 0.95, us: maxima 14 (HBM), counts
+// 49 (one 64-bit LDS atomic an element), sums 82 (about 22 instructions an element, 14 of them float64, and a dozen more
+// for the window), finish 20 and slow 4 (latency of one workgroup a row).  One row alone, top-k 50: 19, four launches of
+// which each waits for the one before.  256 rows of 100003 float32 with cuts of their own: 19 + 29 + 22 + 33 + 21 + 4.
 // ---------------------------------------------------------------------------------------
 constexpr int BINS = 2048, COUNTS = 4096, SEGS = 1024, FEW_GROUPS = 1024, GROUPS = 4096, LIST_CAP = 8192;
 constexpr int TB = 256, TW = TB / 64;      // threads and waves of the passes and of `finish`
@@ -1055,8 +1056,8 @@ Geometry geometry(int V, int64_t rows, const SampleArgs& a) {
     // the k-th largest of n groups' maxima has about -n ln(1 - k / n) elements at or above it
     const int groups = g.per_seg * g.segs;
     g.most = min(groups - groups / 128, (int)(groups * (1.0 - exp(-0.92 * LIST_CAP / groups))));
-    if (!a.top_k && (a.top_k_all >= V || a.top_k_all <= g.most || (!a.top_p && a.top_p_all >= 1.0 && (rows <= 64 || a.top_k_all > FEW_GROUPS))))
-      break;
+    const bool windows = !a.top_p && a.top_p_all >= 1.0 && (rows <= 64 || a.top_k_all > FEW_GROUPS);      // do without the list
+    if (!a.top_k && (a.top_k_all >= V || a.top_k_all <= g.most || windows)) break;
   }
   // few rows, top-k alone: a list that is not short keeps the row's one workgroup busy longer than the windows' launches take (1
   // row of 131072 float32, top-k 900: 39 us against 25, top-k 190: 28 against 25; 128 rows, top-k 900: 58 us against 70)

@@ -1,3 +1,4 @@
+import gc
 import os
 import sys
 
@@ -15,3 +16,11 @@ def pytest_configure(config):
 @pytest.fixture(scope="session")
 def golden_dir():
     return os.path.join(ROOT, "tests", "golden")
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _no_garbage():
+    """Networks are cycles of nodes: what earlier modules left of them is freed here, not in the middle of a test that looks
+    at the allocated memory."""
+    gc.collect()
+    yield
