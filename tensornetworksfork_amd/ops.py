@@ -1185,32 +1185,40 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, p=0.0, seed=0, offset=0,
     (`wdtype`, or x's, where there is no weight)."""
     _row_tensor(x, "x")
     _row_tensor(dy, "dy", x.device)
-    if dy.dtype != x.dtype or dy.shape != x.shape:
-        raise _lib.TTKError(f"dy: expected {x.dtype} of shape {tuple(x.shape)}, got {dy.dtype} of shape {tuple(dy.shape)}")
-    rows, cols, ld = rows_view(x)
-    _, _, lddy = rows_view(dy, "dy")
-    wp = _norm_vector(weight, "weight", x, cols)
     stat = F64 if x.dtype == F64 else torch.float32
     for t, name in ((mean, "mean"), (rstd, "rstd")):
         _row_tensor(t, name, x.device)
         if t.dtype != stat or tuple(t.shape) != tuple(x.shape[:-1]) or not t.is_contiguous():
             raise _lib.TTKError(f"{name}: expected a contiguous {stat} tensor of shape {tuple(x.shape[:-1])}")
-    p, seed, off, off_dev = _drop_args(p, seed, offset, x.device)
+    rows_view(x)
+    _norm_vector(weight, "weight", x, x.shape[-1])
     wdt = weight.dtype if weight is not None else wdtype if wdtype is not None else x.dtype
     if wdt != x.dtype and not (wdt == torch.float32 and x.dtype in (torch.bfloat16, torch.float16)):
         raise _lib.TTKError(f"layer_norm_backward: gradients of type {wdt} do not go with rows of {x.dtype}")
+    return norm_gradients(dy, x, mean, rstd, weight, _drop_args(p, seed, offset, x.device), need, wdt)
+
+
+def norm_gradients(dy, x, mean, rstd, weight, drop, need, wdt):
+    """layer_norm_backward of operands that a layer_norm call has checked or made (all but dy); drop: what _drop_args gives."""
+    if dy.dtype != x.dtype or dy.shape != x.shape or dy.device != x.device:
+        raise _lib.TTKError(f"dy: expected {x.dtype} of shape {tuple(x.shape)} on {x.device}, got {dy.dtype} of shape {tuple(dy.shape)} "
+                            f"on {dy.device}")
+    rows, cols, ld = rows_view(x)
+    lddy = rows_view(dy, "dy")[2]
     dx = x.new_empty(x.shape) if need[0] else None
     make = x.new_empty if rows else x.new_zeros
     dw = make(cols, dtype=wdt) if need[1] else None
     db = make(cols, dtype=wdt) if need[2] else None
-    if rows and any(need):
-        ws, nbytes = None, 0
-        if need[1] or need[2]:
-            nbytes = int(_lib.lib().ttk_layer_norm_backward_ws_bytes(ROW_TYPES[x.dtype], rows, cols))
+    sums = need[1] or need[2]
+    if rows and (sums or need[0]):
+        code, ws, nbytes = ROW_TYPES[x.dtype], None, 0
+        if sums:
+            nbytes = int(_lib.lib().ttk_layer_norm_backward_ws_bytes(code, rows, cols))
             ws = x.new_empty(nbytes, dtype=torch.uint8)
-        ptr = [t.data_ptr() if t is not None else None for t in (dx, dw, db, ws)]
-        _launch("ttk_layer_norm_backward", x.device, ROW_TYPES[x.dtype], ROW_TYPES[wdt], dy.data_ptr(), lddy, x.data_ptr(), ld, wp,
-                mean.data_ptr(), rstd.data_ptr(), ptr[0], ptr[1], ptr[2], rows, cols, p, seed, off, off_dev, ptr[3], nbytes)
+        _launch("ttk_layer_norm_backward", x.device, code, ROW_TYPES[wdt], dy.data_ptr(), lddy, x.data_ptr(), ld,
+                None if weight is None else weight.data_ptr(), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr() if need[0] else None,
+                dw.data_ptr() if need[1] else None, db.data_ptr() if need[2] else None, rows, cols, *drop,
+                ws.data_ptr() if sums else None, nbytes)
     return dx, dw, db
 
 

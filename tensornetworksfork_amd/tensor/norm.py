@@ -56,17 +56,16 @@ class _LayerNorm(torch.autograd.Function):
         y, mean, rstd = ops.layer_norm(x, weight, bias, eps, p, seed, offset)
         off = offset if isinstance(offset, torch.Tensor) else None
         ctx.save_for_backward(x, weight, mean, rstd, off)
-        ctx.wdtype = bias.dtype if weight is None and bias is not None else None
-        ctx.drop = (p, seed, None if off is not None else offset)
+        ctx.wdtype = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
+        ctx.drop = (float(p), int(seed), 0 if off is not None else int(offset))
         return y
 
     @staticmethod
     @_once
     def backward(ctx, dy):
         x, weight, mean, rstd, off = ctx.saved_tensors
-        p, seed, offset = ctx.drop
-        grads = ops.layer_norm_backward(_rows(dy), x, mean, rstd, weight, p, seed, offset if off is None else off,
-                                        need=ctx.needs_input_grad[:3], wdtype=ctx.wdtype)
+        drop = (*ctx.drop, None if off is None else off.data_ptr())
+        grads = ops.norm_gradients(_rows(dy), x, mean, rstd, weight, drop, ctx.needs_input_grad, ctx.wdtype)
         return (*grads, None, None, None, None)
 
 
