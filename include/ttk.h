@@ -467,7 +467,7 @@ int ttk_chol_prepare_dense_f64(const double* A, int D, const double* scale, doub
 
 /* ---- rows in front of a model, answers behind it (ttk_norm.hip, ttk_sample.hip) ----
  * Type codes: 0 float64, 1 float32, 2 bfloat16, 3 float16.  Pointers of these entry points need the alignment of their
- * elements only; ld* = distance of two rows in elements (0: one row for all), the elements of a row are consecutive.
+ * elements only, workspaces 8 bytes; ld* = distance of two rows in elements (0: one row for all), the elements of a row are consecutive.
  *
  * Dropout: element number e = offset (+ *offset_dev, a device integer read when the kernel runs, if not NULL) + index is
  * kept iff word e mod 4 of Philox4x32-10 with key = seed and counter = (e div 4, 0, 0) is >= min(round(p 2^32), 2^32 - 1),
@@ -495,8 +495,8 @@ int ttk_layer_norm_backward(int dtype, int wdtype, const void* dy, int64_t lddy,
 
 /* One label a row drawn from softmax(logits / temperature) cut by top-k, then top-p, then min-p, with the row's random
  * number u in [0, 1): the first index whose cumulative kept weight exceeds u times the total.  Ties in the cuts go to the
- * lowest index; NaN counts as -inf, -inf is never drawn, +inf takes all; temperature <= 0: lowest index of the maximum;
- * a row without a logit above -inf: -1.  V <= 2^30.  top_k <= 0 or >= V, top_p >= 1, min_p <= 0 switch a cut off.
+ * lowest index; NaN counts as -inf, -inf is never drawn, +inf takes all; temperature <= 0: lowest index of the maximum
+ * (between 0 and 1e-306: as 1e-306); a row without a logit above -inf: -1.  V <= 2^30.  top_k <= 0 or >= V, top_p >= 1, min_p <= 0 switch a cut off.
  * u: one value a row, float64 when f64 != 0 else float32; temperature / top_p / min_p: the same type, one value a row, or
  * NULL for the *_all value; top_k: one int32 a row or NULL.  ws: ttk_sample_ws_bytes bytes (none for V <= 8192). */
 int64_t ttk_sample_ws_bytes(int dtype, int64_t rows, int V);

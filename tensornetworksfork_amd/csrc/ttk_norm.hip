@@ -1247,6 +1247,7 @@ int ln_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void*
   const int parts = bwd_parts(l, rows, cols);
   const bool sums = dw || db;
   if (sums && (!ws || ws_bytes < (int64_t)parts * 2 * cols * (int64_t)sizeof(A))) return TTK_EWORKSPACE;
+  if (sums && (uintptr_t)ws % 8) return TTK_EINVAL;
   if (l.lanes && (dx || sums)) {
     A* part = sums ? (A*)ws : (A*)nullptr;
 #define KR(LANES, NV, R)                                                                                                  \

@@ -1955,6 +1955,7 @@ template <typename Z>
 int launch_rows(const Z* z, int64_t ld, const SampleArgs& a, int64_t* label, int64_t rows, int V, void* ws, int64_t ws_bytes,
                 hipStream_t st) {
   if (!ws || ws_bytes < min(rows, ROW_BATCH) * (int64_t)sizeof(RowWork<Z>)) return TTK_EWORKSPACE;
+  if ((uintptr_t)ws % 8) return TTK_EINVAL;
   RowWork<Z>* work = (RowWork<Z>*)ws;
   const Geometry g = geometry<Z>(V, min(rows, ROW_BATCH), a);
   // what the rows can need (parameters of their own: anything)

@@ -45,6 +45,7 @@ def test_library_refuses_bad_arguments_before_any_launch():
         assert sm(**k) == -1, k
     need = L.ttk_sample_ws_bytes(1, 2, 9000)
     assert need > 0 and sm(V=9000) == -2 and sm(V=9000, ws=P, n=need - 1) == -2
+    assert sm(V=9000, ws=P + 4, n=need) == -1 and bw(ws=P + 4) == -1      # (workspaces are aligned to 8 bytes)
     assert L.ttk_sample_ws_bytes(1, 7, 8192) == 0 and L.ttk_sample_ws_bytes(4, 7, 9) == -1 and L.ttk_sample_ws_bytes(1, 0, 9) == -1
     assert L.ttk_layer_norm_backward_ws_bytes(1, 0, 4) == -1 and L.ttk_layer_norm_backward_ws_bytes(9, 4, 4) == -1
     assert L.ttk_layer_norm_backward_ws_bytes(1, 5, 7) >= 2 * 7 * 4
