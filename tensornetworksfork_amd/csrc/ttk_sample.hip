@@ -1680,9 +1680,10 @@ struct ListCut : RowSampler<Z, TB> {
     return sh.which == 0x7FFFFFFF ? sh.last : sh.which;
   }
 
-  // top-k and top-p of a list that holds the k first elements
+  // top-k and top-p of a list that holds the k first elements.  A list of just k needs its cut as well: the draw reads the row
+  // again, where the elements that are not listed stand too (a list of fewer holds everything that weighs anything).
   __device__ __forceinline__ bool top_cut(Cut<F>& cut, const RowArgs& a) {
-    if (c > a.k && !cut_at<false>(cut, (double)a.k, false, 0)) return false;
+    if (c >= a.k && !cut_at<false>(cut, (double)a.k, false, 0)) return false;
     return !(a.P < 1.0) || cut_at<true>(cut, a.P, true, 0);
   }
 

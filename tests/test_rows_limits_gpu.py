@@ -1,0 +1,50 @@
+"""Layer norm, dropout and label sampling at the ends of what their entry points accept: rows of millions of columns and up to
+2^31 - 1, sums over millions of rows, constant rows, columns behind a row, temperatures without bounds, weights far below the
+largest, lists that hold just what top-k asks for."""
+import numpy as np
+import pytest
+import torch
+
+from tests import _row_oracles as R
+from tests import test_norm_gpu as N
+from tests import test_sample_gpu as S
+
+gpu = pytest.mark.gpu
+F64, F32, BF16, F16 = torch.float64, torch.float32, torch.bfloat16, torch.float16
+
+
+@pytest.fixture(autouse=True)
+def _float32_default():
+    """Other tests of the process may have left float64 as torch's default."""
+    old = torch.get_default_dtype()
+    torch.set_default_dtype(F32)
+    yield
+    torch.set_default_dtype(old)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,V,k,rows", [(F32, 131072, 300, 65), (F32, 100003, 1000, 70), (BF16, 131072, 300, 66), (F16, 50000, 700, 65),
+                                            (F64, 20011, 300, 65), (F32, 131072, 300, 1)])
+def test_top_k_alone_of_a_list_that_holds_just_as_many(dtype, V, k, rows):
+    """k leaders in groups of their own over a background that weighs about as much: what top-k drops is never drawn."""
+    from tensornetworksfork_amd import ops
+    dev = S._dev()
+    g = torch.Generator().manual_seed(V + k)
+    z = torch.zeros(rows, V)
+    at = torch.arange(k) * (V // k)
+    z[:, at] = float(np.log(V / k))                       # (as much as the background together, before it is cut)
+    z[rows // 2:, at] += 0.25 * torch.randint(0, 4, (rows - rows // 2, k), generator=g)
+    z = z.to(dtype)
+    Z, leaders = z.to(dev), set(at.tolist())
+    K = torch.full((rows,), k, dtype=torch.int32)
+    K[1::3] = k - 1
+    K[2::3] = k + 1
+    for top_k in (k, K.to(dev)):
+        u = torch.rand(rows, generator=g, dtype=F64)
+        got = ops.sample(Z, u.to(dev), top_k=top_k).cpu()
+        if top_k is not K and isinstance(top_k, int):
+            assert set(got.tolist()) <= leaders
+        S._check(z, u, got, [dict(k=int(n)) for n in (K if top_k is not k else [k] * rows)], least=0.95)
+    # min-p above the list's smallest weights, in the same draw
+    u = torch.rand(rows, generator=g, dtype=F64)
+    S._check(z, u, ops.sample(Z, u.to(dev), top_k=k, min_p=0.7).cpu(), dict(k=k, M=0.7), least=0.95)
