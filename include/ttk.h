@@ -496,7 +496,7 @@ int ttk_layer_norm_backward(int dtype, int wdtype, const void* dy, int64_t lddy,
 /* One label a row drawn from softmax(logits / temperature) cut by top-k, then top-p, then min-p, with the row's random
  * number u in [0, 1): the first index whose cumulative kept weight exceeds u times the total.  Ties in the cuts go to the
  * lowest index; NaN counts as -inf, -inf is never drawn, +inf takes all; temperature <= 0: lowest index of the maximum
- * (between 0 and 1e-306: as 1e-306); a row without a logit above -inf: -1.  V <= 2^30.  top_k <= 0 or >= V, top_p >= 1, min_p <= 0 switch a cut off.
+ * (between 0 and 1e-306: as 1e-306; infinite: as the largest number, all weigh the same); a row without a logit above -inf: -1.  V <= 2^30.  top_k <= 0 or >= V, top_p >= 1, min_p <= 0 switch a cut off.
  * u: one value a row, float64 when f64 != 0 else float32; temperature / top_p / min_p: the same type, one value a row, or
  * NULL for the *_all value; top_k: one int32 a row or NULL.  ws: ttk_sample_ws_bytes bytes (none for V <= 8192). */
 int64_t ttk_sample_ws_bytes(int dtype, int64_t rows, int V);

@@ -4,8 +4,8 @@
 // counts as -inf).  Elements are ordered by descending logit, ties by ascending index.  top-k keeps the first k; top-p
 // keeps the elements whose exclusive cumulative weight is below top_p times the weight top-k kept; min-p keeps w_i >= min_p
 // (the largest weight is 1).  The label is the first index, in index order, whose cumulative kept weight exceeds u times
-// the total.  T <= 0 answers with the lowest index of the maximum (temperatures between 0 and 1e-306 act as 1e-306), a row
-// without a logit above -inf with -1.
+// the total.  T <= 0 answers with the lowest index of the maximum (temperatures between 0 and 1e-306 act as 1e-306, an
+// infinite one as the largest number: all weigh the same), a row without a logit above -inf with -1.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -36,6 +36,7 @@ __device__ __forceinline__ RowArgs row_args(const SampleArgs& a, int64_t row, in
   if (!(r.u > 0.0)) r.u = 0.0;
   r.T = row_value(a.temperature, a.temperature_all, a.f64, row);
   if (r.T > 0.0 && r.T < 1e-306) r.T = 1e-306;      // 32 log2(e) / T stays finite
+  if (r.T > 0x1.fffffffffffffp1023) r.T = 0x1.fffffffffffffp1023;      // (infinite times log(1) would be no number)
   r.P = row_value(a.top_p, a.top_p_all, a.f64, row);
   if (!(r.P < 1.0)) r.P = 1.0;
   r.M = row_value(a.min_p, a.min_p_all, a.f64, row);
@@ -862,7 +863,8 @@ struct RowScale {
     inf = m == __builtin_inff();
     if (inf) m = 0;
     floor = round_up<F>((double)m - 693.147 * a.T);
-    least = a.M > 0 ? round_up<F>((double)m + a.T * log(a.M)) : floor;
+    // (a weight of at least 1: one that rounds to 1 in 64 bits, as in the kernels that compare weights)
+    least = a.M > 0 ? round_up<F>((double)m + a.T * (a.M < 1.0 ? log(a.M) : -0x1p-54)) : floor;
     if (least < floor) least = floor;
   }
 };
@@ -982,6 +984,7 @@ struct RowSampler {
     __syncthreads();
     const bool to_end = sh.which == SEGS;               // u >= 1, or rounded up to it: the last kept element
     const int s = to_end ? sh.last : sh.which;
+    if (s < 0) return -1;                               // nothing is kept (the first element always is)
     if ((int)threadIdx.x == s / PS) {
       upto = from;
 #pragma unroll

@@ -1243,7 +1243,7 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     temperature 0 answers with the lowest index of the maximum (one between 0 and 1e-306 acts as 1e-306).  u is float32 or
     float64; temperature, top_p and min_p are numbers or tensors of u's type and shape, top_k a number (0: off) or an int32
     tensor of u's shape.  Out-of-range values inside tensors switch the cut off (top_k <= 0 or >= V, top_p >= 1, min_p <= 0)
-    or are clamped (top_p <= 0 keeps one element, min_p > 1 acts as 1, u outside [0, 1) answers with the first / last kept
+    or are clamped (an infinite temperature acts as the largest number, top_p <= 0 keeps one element, min_p > 1 acts as 1, u outside [0, 1) answers with the first / last kept
     element)."""
     _row_tensor(logits, "logits")
     rows, V, ld = rows_view(logits, "logits")

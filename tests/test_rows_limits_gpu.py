@@ -48,3 +48,36 @@ def test_top_k_alone_of_a_list_that_holds_just_as_many(dtype, V, k, rows):
     # min-p above the list's smallest weights, in the same draw
     u = torch.rand(rows, generator=g, dtype=F64)
     S._check(z, u, ops.sample(Z, u.to(dev), top_k=k, min_p=0.7).cpu(), dict(k=k, M=0.7), least=0.95)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F64, F32, BF16])
+@pytest.mark.parametrize("V", [3, 12, 40, 500, 3000, 8192, 8193, 40000])
+def test_temperatures_without_bounds(V, dtype):
+    """An infinite temperature makes every logit above -inf weigh the same, also where min-p asks for the largest weight; so does
+    one so large that exp((z - m) / T) is 1 in 64 bits."""
+    from tensornetworksfork_amd import ops
+    dev = S._dev()
+    MAX = np.finfo(np.float64).max                        # (what the oracle takes an infinite temperature for: -inf / inf is no number)
+    g = torch.Generator().manual_seed(V)
+    z = (2.0 * torch.randn(12, V, generator=g, dtype=F64)).to(dtype)
+    z[3, ::2] = -float("inf")
+    z[4] = -float("inf")
+    z[5, V // 2] = float("inf")
+    T = torch.full((12,), float("inf"), dtype=F64)
+    T[6:9] = 1e300
+    T[9] = 1.7e308
+    T[10] = 1.0
+    T[11] = 1e25
+    u = torch.rand(12, generator=g, dtype=F64)
+    for dt in (F64, F32):
+        t = T.to(dt)                                      # (1e300 is infinite in float32)
+        for P in (1.0, 0.30371):
+            for M in (0.0, 0.5, 1.0):
+                c = dict(temperature=t.to(dev), top_p=P, min_p=torch.full((12,), M, dtype=dt, device=dev))
+                got = ops.sample(z.to(dev), u.to(dt).to(dev), **c).cpu()
+                assert int(got[4]) == -1 and int(got[5]) == V // 2
+                S._check(z, u.to(dt), got, [dict(T=min(float(x), MAX), P=P, M=M) for x in t], least=0.9)
+        K = torch.full((12,), max(1, V // 3), dtype=torch.int32, device=dev)
+        got = ops.sample(z.to(dev), u.to(dt).to(dev), temperature=t.to(dev), top_k=K, min_p=torch.ones(12, dtype=dt, device=dev)).cpu()
+        S._check(z, u.to(dt), got, [dict(T=min(float(x), MAX), k=max(1, V // 3), M=1.0) for x in t], least=0.9)
