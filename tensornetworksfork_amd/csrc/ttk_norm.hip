@@ -368,32 +368,38 @@ __global__ __launch_bounds__(256) void ln_cols_kernel(const X* __restrict__ dy, 
   p[cols + c] = (A)sb;
 }
 
-// Partials added in a fixed order, in 64 bits.
+// Partials added in a fixed order, in 64 bits.  The launch has SUM_GROUPS workgroups at most, each walks its share of the columns
+// (a launch counts its threads in 32 bits; one of more runs a part of its workgroups without an error).
+constexpr int SUM_GROUPS = 1 << 16;
 template <typename A, typename W>
 __global__ __launch_bounds__(1024) void ln_cols_sum_kernel(const A* __restrict__ part, int nparts, int cols, W* __restrict__ dw,
                                                            W* __restrict__ db) {
   __shared__ double red[16][64];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), ty = threadIdx.x >> 6;
+  const int ty = threadIdx.x >> 6;
   W* out = blockIdx.y ? db : dw;
   const A* p = part + (int64_t)blockIdx.y * cols;
-  double s = 0;
-  if (c < cols) {
-    int g = ty;
-    for (; g + 7 * 16 < nparts; g += 8 * 16) {      // eight loads under way
-      A v[8];
+  for (int64_t c0 = (int64_t)blockIdx.x * 64; c0 < cols; c0 += (int64_t)gridDim.x * 64) {
+    const int64_t c = c0 + (threadIdx.x & 63);
+    double s = 0;
+    if (c < cols) {
+      int g = ty;
+      for (; g + 7 * 16 < nparts; g += 8 * 16) {      // eight loads under way
+        A v[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = p[(int64_t)(g + 16 * k) * 2 * cols + c];
+        for (int k = 0; k < 8; ++k) v[k] = p[(int64_t)(g + 16 * k) * 2 * cols + c];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s += (double)v[k];
+        for (int k = 0; k < 8; ++k) s += (double)v[k];
+      }
+      for (; g < nparts; g += 16) s += (double)p[(int64_t)g * 2 * cols + c];
     }
-    for (; g < nparts; g += 16) s += (double)p[(int64_t)g * 2 * cols + c];
-  }
-  red[ty][threadIdx.x & 63] = s;
-  __syncthreads();
-  if (ty == 0 && c < cols && out) {
+    red[ty][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (ty == 0 && c < cols && out) {
 #pragma unroll
-    for (int i = 1; i < 16; ++i) s += red[i][threadIdx.x & 63];
-    out[c] = (W)s;
+      for (int i = 1; i < 16; ++i) s += red[i][threadIdx.x & 63];
+      out[c] = (W)s;
+    }
+    __syncthreads();
   }
 }
 
@@ -1275,7 +1281,7 @@ int ln_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void*
                          cols_plan(rows, cols).rows_per_split, d);
   }
   if (sums)
-    hipLaunchKernelGGL((ln_cols_sum_kernel<A, W>), dim3((unsigned)((cols + 63) / 64), 2), dim3(1024), 0, st, (const A*)ws, parts,
+    hipLaunchKernelGGL((ln_cols_sum_kernel<A, W>), dim3((unsigned)min(((int64_t)cols + 63) / 64, (int64_t)SUM_GROUPS), 2), dim3(1024), 0, st, (const A*)ws, parts,
                        cols, (W*)dw, (W*)db);
   return status();
 }

@@ -81,3 +81,18 @@ def test_temperatures_without_bounds(V, dtype):
         K = torch.full((12,), max(1, V // 3), dtype=torch.int32, device=dev)
         got = ops.sample(z.to(dev), u.to(dt).to(dev), temperature=t.to(dev), top_k=K, min_p=torch.ones(12, dtype=dt, device=dev)).cpu()
         S._check(z, u.to(dt), got, [dict(T=min(float(x), MAX), k=max(1, V // 3), M=1.0) for x in t], least=0.9)
+
+
+@gpu
+def test_column_sums_of_2_28_columns():
+    """A launch counts its threads in 32 bits: the sum over the partials walks more columns than one launch of a thread each."""
+    from tensornetworksfork_amd import ops
+    dev = N._dev()
+    cols = (1 << 28) + 8256
+    x = ((torch.arange(1001, device=dev) % 13) - 6.0).repeat(cols // 1001 + 1)[:cols]
+    dy = ((torch.arange(1003, device=dev) % 5) - 2.0).repeat(cols // 1003 + 1)[:cols]
+    mean, rstd = torch.full((3,), 1.0, device=dev), torch.full((3,), 0.5, device=dev)
+    _, dw, db = ops.layer_norm_backward(dy[None].expand(3, cols), x[None].expand(3, cols), mean, rstd, need=(False, True, True))
+    assert torch.equal(db, 3 * dy) and torch.equal(dw, 3 * dy * (x - 1) * 0.5)
+    del x, dy, dw, db
+    torch.cuda.empty_cache()
