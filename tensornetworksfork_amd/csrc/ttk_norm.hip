@@ -272,7 +272,7 @@ __device__ __forceinline__ void block_sum2(A& a, A& b, A* buf) {
 // backward: the two sums, dx; the column sums in a pass of their own).  Rows longer than the registers of a workgroup hold
 // (16384 elements; float64 backward 8192).  Bound by the second and third pass, which L2 serves: 30000 columns 2.1 TB/s
 // forward and 1.8 backward of float32 traffic counted once; few rows of millions of columns leave most of the machine idle
-// (22 rows of 3 million: 0.1 TB/s).
+// (22 rows of 3 million: 0.1 TB/s).  Rows may have up to 2^31 - 1 columns, which are counted in 64 bits.
 // ---------------------------------------------------------------------------------------
 constexpr int LONG_THREADS = 1024;
 
@@ -289,15 +289,15 @@ __global__ __launch_bounds__(LONG_THREADS) void ln_fwd_long_kernel(const X* __re
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const X* xr = x + row * ldx;
     A s = 0;
-    for (int c = threadIdx.x; c < cols; c += LONG_THREADS) s += (A)xr[c];
+    for (int64_t c = threadIdx.x; c < cols; c += LONG_THREADS) s += (A)xr[c];
     const A mean = block_sum<LONG_THREADS / 64>(s, buf[0]) / (A)cols;
     A q = 0;
-    for (int c = threadIdx.x; c < cols; c += LONG_THREADS) {
+    for (int64_t c = threadIdx.x; c < cols; c += LONG_THREADS) {
       const A d = (A)xr[c] - mean;
       q += d * d;
     }
     const A rstd = A(1) / sqrt(block_sum<LONG_THREADS / 64>(q, buf[1]) / (A)cols + (A)eps);
-    for (int c = threadIdx.x; c < cols; c += LONG_THREADS) {
+    for (int64_t c = threadIdx.x; c < cols; c += LONG_THREADS) {
       A v = ((A)xr[c] - mean) * rstd;
       if (w) v *= (A)w[c];
       if (b) v += (A)b[c];
@@ -323,7 +323,7 @@ __global__ __launch_bounds__(LONG_THREADS) void ln_bwd_long_kernel(const X* __re
     const X *xr = x + row * ldx, *dr = dy + row * lddy;
     const A mean = mean_in[row], rstd = rstd_in[row];
     A s1 = 0, s2 = 0;
-    for (int c = threadIdx.x; c < cols; c += LONG_THREADS) {
+    for (int64_t c = threadIdx.x; c < cols; c += LONG_THREADS) {
       A g = (A)dr[c];
       if (drop.mode) g = (keep_bits<1>(drop, e0 + (uint64_t)row * cols + c) & 1) ? g * scale : A(0);
       const A a = w ? g * (A)w[c] : g;
@@ -333,7 +333,7 @@ __global__ __launch_bounds__(LONG_THREADS) void ln_bwd_long_kernel(const X* __re
     block_sum2<LONG_THREADS / 64>(s1, s2, buf[turn]);
     s1 /= (A)cols;
     s2 /= (A)cols;
-    for (int c = threadIdx.x; c < cols; c += LONG_THREADS) {
+    for (int64_t c = threadIdx.x; c < cols; c += LONG_THREADS) {
       A g = (A)dr[c];
       if (drop.mode) g = (keep_bits<1>(drop, e0 + (uint64_t)row * cols + c) & 1) ? g * scale : A(0);
       const A a = w ? g * (A)w[c] : g;
@@ -351,7 +351,7 @@ __global__ __launch_bounds__(256) void ln_cols_kernel(const X* __restrict__ dy, 
                                                       typename Acc<X>::type* __restrict__ part, int64_t rows, int cols,
                                                       int64_t rows_per_split, Drop drop) {
   typedef typename Acc<X>::type A;
-  const int c = blockIdx.x * 256 + threadIdx.x;
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (c >= cols) return;
   const uint64_t e0 = drop_base(drop);
   const A scale = (A)drop.scale;
@@ -1276,7 +1276,7 @@ int ln_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void*
       hipLaunchKernelGGL((ln_bwd_long_kernel<X, W>), dim3((unsigned)min(rows, (int64_t)(4 * CUS))), dim3(LONG_THREADS), 0, st,
                          (const X*)dy, lddy, (const X*)x, ldx, (const W*)w, (const A*)mean, (const A*)rstd, (X*)dx, rows, cols, d);
     if (sums)
-      hipLaunchKernelGGL((ln_cols_kernel<X>), dim3((unsigned)((cols + 255) / 256), (unsigned)parts), dim3(256), 0, st,
+      hipLaunchKernelGGL((ln_cols_kernel<X>), dim3((unsigned)(((int64_t)cols + 255) / 256), (unsigned)parts), dim3(256), 0, st,
                          (const X*)dy, lddy, (const X*)x, ldx, (const A*)mean, (const A*)rstd, (A*)ws, rows, cols,
                          cols_plan(rows, cols).rows_per_split, d);
   }

@@ -96,3 +96,53 @@ def test_column_sums_of_2_28_columns():
     assert torch.equal(db, 3 * dy) and torch.equal(dw, 3 * dy * (x - 1) * 0.5)
     del x, dy, dw, db
     torch.cuda.empty_cache()
+
+
+@gpu
+@pytest.mark.parametrize("cols", [(1 << 30) + 8, (1 << 31) - 1])
+def test_column_sums_of_rows_beyond_2_30_columns(cols):
+    """One row broadcast to three: dw = 3 dy h, db = 3 dy, exact in float32 for these values (small whole numbers and halves)."""
+    from tensornetworksfork_amd import ops
+    dev = N._dev()
+    reps = cols // 1001 + 1
+    x = ((torch.arange(1001, device=dev) % 13) - 6.0).to(BF16).repeat(reps)[:cols]
+    dy = ((torch.arange(1003, device=dev) % 5) - 2.0).to(BF16).repeat(reps)[:cols]
+    mean = torch.full((3,), 1.0, device=dev)
+    rstd = torch.full((3,), 0.5, device=dev)
+    dx, dw, db = ops.layer_norm_backward(dy[None].expand(3, cols), x[None].expand(3, cols), mean, rstd, need=(False, True, True))
+    assert dx is None
+    step = 1 << 28
+    for a in range(0, cols, step):
+        g = dy[a:a + step].float()
+        assert torch.equal(db[a:a + step].float(), 3 * g)
+        # (bfloat16 holds 3 dy (x - 1) / 2 where it has at most 8 significant bits: |3 * 2 * 7 / 2| = 21 in steps of 1 / 2)
+        assert torch.equal(dw[a:a + step].float(), 3 * g * (x[a:a + step].float() - 1) * 0.5)
+    del x, dy, dw, db, g
+    torch.cuda.empty_cache()
+
+
+@gpu
+def test_a_row_of_as_many_columns_as_are_accepted():
+    """2^31 - 1 columns of +-1 and one 0: mean 0, rstd 1 to rounding; y = x, and dx = dy - x mean(dy x) for dy = x is 0."""
+    from tensornetworksfork_amd import ops
+    dev = N._dev()
+    cols = (1 << 31) - 1
+    x = torch.ones(cols, dtype=BF16, device=dev)
+    x[::2] = -1
+    x[cols // 2] = 0
+    n = float(cols)
+    s = -1.0 - float(1 - 2 * (1 - (cols // 2) % 2))       # (one -1 more than there are +1, and the one set to 0)
+    y, mean, rstd = ops.layer_norm(x[None], eps=0.0)
+    assert abs(float(mean) - s / n) <= 2 * R.U32 * abs(s / n) + 1e-12
+    assert abs(float(rstd) - (n / (n - 1)) ** 0.5) <= 8 * R.U32
+    step = 1 << 28
+    for a in range(0, cols, step):
+        assert torch.equal(y[0, a:a + step].float().round(), x[a:a + step].float())
+    dx, dw, db = ops.layer_norm_backward(x[None], x[None], mean, rstd)
+    for a in range(0, cols, step):
+        # (x - 0 - x (1 - 1 / n) in float32, of which 1 / n is below half a step)
+        assert float(dx[0, a:a + step].float().abs().max()) <= 16 * R.U32
+        assert torch.equal(db[a:a + step], x[a:a + step])
+        assert torch.equal(dw[a:a + step].float(), x[a:a + step].float().square())
+    del x, y, dx, dw, db
+    torch.cuda.empty_cache()
