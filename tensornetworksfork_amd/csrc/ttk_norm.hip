@@ -12,6 +12,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "ttk.h"
 
 namespace {
@@ -1090,6 +1092,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(const X* x, X* y, int64_t 
 // ---------------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------------
+// (sizes on the host: std::min, the min of hip_runtime.h takes ints there)
 inline int status() { return hipGetLastError() == hipSuccess ? TTK_OK : TTK_ELAUNCH; }
 
 constexpr int CUS = 256;
@@ -1143,10 +1146,10 @@ Layout row_layout(int dtype, int cols, bool dense, bool backward) {
 // Workgroups of a launch: as many as are resident at a time, each walks its share of the rows (the backward pass leaves
 // one partial row of column sums per workgroup).
 int row_groups(const Layout& l, int64_t rows, bool backward) {
-  const int64_t rpb = l.lanes == 1 ? 64 * SHORT_WAVES : max(1, 256 / l.lanes);
+  const int64_t rpb = l.lanes == 1 ? 64 * SHORT_WAVES : std::max(1, 256 / l.lanes);
   const int per_cu = l.lanes <= 256 ? (backward ? 4 : l.nv >= 4 ? 4 : 8) : l.lanes == 512 ? (backward ? (l.nv >= 4 ? 1 : 2) : 4)
                                                                                          : (backward ? 1 : 2);
-  return (int)min((rows + rpb - 1) / rpb, (int64_t)(per_cu * CUS));
+  return (int)std::min((rows + rpb - 1) / rpb, (int64_t)(per_cu * CUS));
 }
 
 // column sums of rows the registers do not hold: a thread a column over a range of rows
@@ -1156,8 +1159,8 @@ struct ColsPlan {
 };
 ColsPlan cols_plan(int64_t rows, int cols) {
   const int64_t tiles = ((int64_t)cols + 255) / 256;
-  int64_t s = min((int64_t)1024, max((int64_t)1, 8 * CUS / tiles));
-  s = min(s, (rows + 15) / 16);
+  int64_t s = std::min((int64_t)1024, std::max((int64_t)1, 8 * CUS / tiles));
+  s = std::min(s, (rows + 15) / 16);
   ColsPlan p;
   p.rows_per_split = (rows + s - 1) / s;
   p.splits = (int)((rows + p.rows_per_split - 1) / p.rows_per_split);
@@ -1223,7 +1226,7 @@ int ln_fwd(const void* x, int64_t ldx, const void* w, const void* b, void* y, vo
   typedef typename Acc<X>::type A;
   const Layout l = row_layout(type_code<X>(), cols, ldx == cols || rows == 1, false);
   if (!l.lanes) {
-    hipLaunchKernelGGL((ln_fwd_long_kernel<X, W>), dim3((unsigned)min(rows, (int64_t)(4 * CUS))), dim3(LONG_THREADS), 0, st,
+    hipLaunchKernelGGL((ln_fwd_long_kernel<X, W>), dim3((unsigned)std::min(rows, (int64_t)(4 * CUS))), dim3(LONG_THREADS), 0, st,
                        (const X*)x, ldx, (const W*)w, (const W*)b, (X*)y, (A*)mean, (A*)rstd, rows, cols, eps, d);
     return status();
   }
@@ -1273,7 +1276,7 @@ int ln_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void*
 #undef S
   } else if (!l.lanes) {
     if (dx)
-      hipLaunchKernelGGL((ln_bwd_long_kernel<X, W>), dim3((unsigned)min(rows, (int64_t)(4 * CUS))), dim3(LONG_THREADS), 0, st,
+      hipLaunchKernelGGL((ln_bwd_long_kernel<X, W>), dim3((unsigned)std::min(rows, (int64_t)(4 * CUS))), dim3(LONG_THREADS), 0, st,
                          (const X*)dy, lddy, (const X*)x, ldx, (const W*)w, (const A*)mean, (const A*)rstd, (X*)dx, rows, cols, d);
     if (sums)
       hipLaunchKernelGGL((ln_cols_kernel<X>), dim3((unsigned)(((int64_t)cols + 255) / 256), (unsigned)parts), dim3(256), 0, st,
@@ -1281,8 +1284,8 @@ int ln_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void*
                          cols_plan(rows, cols).rows_per_split, d);
   }
   if (sums)
-    hipLaunchKernelGGL((ln_cols_sum_kernel<A, W>), dim3((unsigned)min(((int64_t)cols + 63) / 64, (int64_t)SUM_GROUPS), 2), dim3(1024), 0, st, (const A*)ws, parts,
-                       cols, (W*)dw, (W*)db);
+    hipLaunchKernelGGL((ln_cols_sum_kernel<A, W>), dim3((unsigned)std::min(((int64_t)cols + 63) / 64, (int64_t)SUM_GROUPS), 2), dim3(1024), 0, st,
+                       (const A*)ws, parts, cols, (W*)dw, (W*)db);
   return status();
 }
 
@@ -1315,7 +1318,7 @@ int ttk_layer_norm(int dtype, int wdtype, const void* x, int64_t ldx, const void
 
 int64_t ttk_layer_norm_backward_ws_bytes(int dtype, int64_t rows, int cols) {
   if (dtype < 0 || dtype > 3 || rows < 1 || cols < 1) return TTK_EINVAL;
-  const int parts = max(bwd_parts(row_layout(dtype, cols, true, true), rows, cols), bwd_parts(row_layout(dtype, cols, false, true), rows, cols));
+  const int parts = std::max(bwd_parts(row_layout(dtype, cols, true, true), rows, cols), bwd_parts(row_layout(dtype, cols, false, true), rows, cols));
   return (int64_t)parts * 2 * cols * (dtype == 0 ? 8 : 4);
 }
 
@@ -1336,7 +1339,7 @@ int ttk_dropout(int dtype, const void* x, void* y, int64_t n, double p, uint64_t
   if (!x || !y || n < 1 || dtype < 0 || dtype > 3 || !make_drop(d, p, seed, offset, offset_dev)) return TTK_EINVAL;
   hipStream_t st = (hipStream_t)stream;
   const int per = 256 * (dtype < 2 ? 4 : 8);
-  const dim3 grid((unsigned)min((n + 3 + per - 1) / per, (int64_t)(16 * CUS)));
+  const dim3 grid((unsigned)std::min((n + 3 + per - 1) / per, (int64_t)(16 * CUS)));
   switch (dtype) {
     case 0: hipLaunchKernelGGL((dropout_kernel<double>), grid, dim3(256), 0, st, (const double*)x, (double*)y, n, d); break;
     case 1: hipLaunchKernelGGL((dropout_kernel<float>), grid, dim3(256), 0, st, (const float*)x, (float*)y, n, d); break;

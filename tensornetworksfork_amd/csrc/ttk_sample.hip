@@ -9,6 +9,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "ttk.h"
 
 namespace {
@@ -1049,7 +1051,7 @@ Geometry geometry(int V, int64_t rows, const SampleArgs& a) {
   g.V = V;
   g.steps = (int)(((int64_t)V + 64 * N - 1) / (64 * N));
   // segments of up to 4 steps where the machine has work enough without shorter ones
-  g.R = max((g.steps + SEGS - 1) / SEGS, rows * g.steps >= 16384 ? max(1, min(4, g.steps / 64)) : 1);
+  g.R = std::max((g.steps + SEGS - 1) / SEGS, rows * g.steps >= 16384 ? std::max(1, std::min(4, g.steps / 64)) : 1);
   g.segs = (g.steps + g.R - 1) / g.R;
   // few groups while they do (every workgroup reads them: 1 row of 131072 bfloat16, top-k 50: 24 us with 1024, 32 with 4096;
   // but 104 us where 1024 do not bound k)
@@ -1058,13 +1060,13 @@ Geometry geometry(int V, int64_t rows, const SampleArgs& a) {
     while (g.per_seg * g.segs > limit) g.per_seg /= 2;
     // the k-th largest of n groups' maxima has about -n ln(1 - k / n) elements at or above it
     const int groups = g.per_seg * g.segs;
-    g.most = min(groups - groups / 128, (int)(groups * (1.0 - exp(-0.92 * LIST_CAP / groups))));
+    g.most = std::min(groups - groups / 128, (int)(groups * (1.0 - exp(-0.92 * LIST_CAP / groups))));
     const bool windows = !a.top_p && a.top_p_all >= 1.0 && (rows <= 64 || a.top_k_all > FEW_GROUPS);      // do without the list
     if (!a.top_k && (a.top_k_all >= V || a.top_k_all <= g.most || windows)) break;
   }
   // few rows, top-k alone: a list that is not short keeps the row's one workgroup busy longer than the windows' launches take (1
   // row of 131072 float32, top-k 900: 39 us against 25, top-k 190: 28 against 25; 128 rows, top-k 900: 58 us against 70)
-  g.alone = rows <= 64 ? min(g.most, 128) : g.most;
+  g.alone = rows <= 64 ? std::min(g.most, 128) : g.most;
   return g;
 }
 
@@ -1954,25 +1956,26 @@ __global__ __launch_bounds__(RT) void row_slow_kernel(const Z* __restrict__ logi
 }
 
 constexpr int64_t ROW_BATCH = 512;      // rows that share the workspace
+// (sizes on the host: std::min, the min of hip_runtime.h takes ints there)
 
 template <typename Z>
 int launch_rows(const Z* z, int64_t ld, const SampleArgs& a, int64_t* label, int64_t rows, int V, void* ws, int64_t ws_bytes,
                 hipStream_t st) {
-  if (!ws || ws_bytes < min(rows, ROW_BATCH) * (int64_t)sizeof(RowWork<Z>)) return TTK_EWORKSPACE;
+  if (!ws || ws_bytes < std::min(rows, ROW_BATCH) * (int64_t)sizeof(RowWork<Z>)) return TTK_EWORKSPACE;
   if ((uintptr_t)ws % 8) return TTK_EINVAL;
   RowWork<Z>* work = (RowWork<Z>*)ws;
-  const Geometry g = geometry<Z>(V, min(rows, ROW_BATCH), a);
+  const Geometry g = geometry<Z>(V, std::min(rows, ROW_BATCH), a);
   // what the rows can need (parameters of their own: anything)
   const bool any_t = a.temperature || a.temperature_all > 0.0, all_k = !a.top_k && a.top_k_all > 0 && a.top_k_all < V;
   const bool any_p = a.top_p || a.top_p_all < 1.0, any_k = a.top_k || all_k || a.top_p || !(a.top_p_all > 0.0);      // (see row_args)
   const int most = !a.top_p && a.top_p_all < 1.0 ? g.most : g.alone;
   const bool no_list = all_k && a.top_k_all > most && !a.top_p && a.top_p_all > 0.0, sums = !all_k || a.top_k_all > most;
   for (int64_t r0 = 0; r0 < rows; r0 += ROW_BATCH) {
-    const int64_t n = min(ROW_BATCH, rows - r0);
+    const int64_t n = std::min(ROW_BATCH, rows - r0);
     const Z* p = z + r0 * ld;
     // workgroups a row: enough to fill the machine, each wave with a segment at least
-    const int split = (int)max((int64_t)1, min((int64_t)(g.segs + TW - 1) / TW, (1024 + n - 1) / n));
-    const int wide = (int)max((int64_t)1, min((int64_t)(g.segs + RW - 1) / RW, (256 + n - 1) / n));
+    const int split = (int)std::max((int64_t)1, std::min((int64_t)(g.segs + TW - 1) / TW, (1024 + n - 1) / n));
+    const int wide = (int)std::max((int64_t)1, std::min((int64_t)(g.segs + RW - 1) / RW, (256 + n - 1) / n));
     const dim3 grid((unsigned)split, (unsigned)n), big((unsigned)wide, (unsigned)n), one((unsigned)n);
     hipLaunchKernelGGL((row_maxima_kernel<Z>), grid, dim3(TB), 0, st, p, ld, g, work);
     if (any_t && any_k && !no_list) hipLaunchKernelGGL((row_collect_kernel<Z>), grid, dim3(TB), 0, st, p, ld, a, g, work, r0);
@@ -2031,7 +2034,7 @@ extern "C" {
 int64_t ttk_sample_ws_bytes(int dtype, int64_t rows, int V) {
   if (dtype < 0 || dtype > 3 || rows < 1 || V < 1 || V > (1 << 30)) return TTK_EINVAL;
   if (V <= WAVE_ROW) return 0;
-  return min(rows, ROW_BATCH) * (int64_t)(dtype == 0 ? sizeof(RowWork<double>) : sizeof(RowWork<float>));
+  return std::min(rows, ROW_BATCH) * (int64_t)(dtype == 0 ? sizeof(RowWork<double>) : sizeof(RowWork<float>));
 }
 
 int ttk_sample(int dtype, const void* logits, int64_t ld, const void* u, int f64, const void* temperature, double temperature_all,
