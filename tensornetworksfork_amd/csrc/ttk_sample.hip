@@ -1996,34 +1996,49 @@ int launch_rows(const Z* z, int64_t ld, const SampleArgs& a, int64_t* label, int
 // and top-p cut (1398 rows of 12000 float32, top-k 50 and top-p 0.9: 276 us against 119 us of the launches below).
 constexpr int WAVE_ROW = 8192;
 
+// The parameters from row `r` on.
+SampleArgs from_row(SampleArgs a, int64_t r) {
+  const auto at = [&](const void* p) { return p ? (const void*)((const char*)p + r * (a.f64 ? 8 : 4)) : p; };
+  a.u = at(a.u), a.temperature = at(a.temperature), a.top_p = at(a.top_p), a.min_p = at(a.min_p);
+  if (a.top_k) a.top_k += r;
+  return a;
+}
+
 template <typename Z>
-int launch(const void* logits, int64_t ld, const SampleArgs& a, int64_t* label, int64_t rows, int V, void* ws, int64_t ws_bytes,
+int launch(const void* logits, int64_t ld, const SampleArgs& args, int64_t* label, int64_t rows, int V, void* ws, int64_t ws_bytes,
            hipStream_t st) {
   const Z* z = (const Z*)logits;
-  if (V > WAVE_ROW) return launch_rows<Z>(z, ld, a, label, rows, V, ws, ws_bytes, st);
-  const int64_t groups = V <= FEW ? (rows + 63) / 64 : V <= 1024 ? (rows + 3) / 4 : rows;
-  if (groups > 0x7FFFFFFF) return TTK_EINVAL;
-  const dim3 grid((unsigned)groups);
-#define K(E, W) hipLaunchKernelGGL((sample_wave_kernel<Z, E, W>), grid, dim3(W > 1 ? 64 * W : 256), 0, st, z, ld, a, label, rows, V)
-  if (V <= FEW)
-    hipLaunchKernelGGL((sample_few_kernel<Z>), grid, dim3(64), 0, st, z, ld, a, label, rows, V);
-  else if (V <= 64)
-    K(1, 1);
-  else if (V <= 128)
-    K(2, 1);
-  else if (V <= 256)
-    K(4, 1);
-  else if (V <= 512)
-    K(8, 1);
-  else if (V <= 1024)
-    K(16, 1);
-  else if (V <= 2048)
-    K(16, 2);
-  else if (V <= 4096)
-    K(16, 4);
-  else
-    K(16, 8);
+  if (V > WAVE_ROW) return launch_rows<Z>(z, ld, args, label, rows, V, ws, ws_bytes, st);
+  // a launch counts its threads in 32 bits (one of more runs a part of its workgroups without an error): 2^31 of them at a time
+  const int threads = V <= FEW ? 1 : V <= 1024 ? 64 : V <= 2048 ? 128 : V <= 4096 ? 256 : 512;      // a row
+  const int64_t most = (1ll << 31) / threads;
+  for (int64_t r0 = 0; r0 < rows; r0 += most) {
+    const int64_t n = std::min(most, rows - r0);
+    const SampleArgs a = from_row(args, r0);
+    const dim3 grid((unsigned)(V <= FEW ? (n + 63) / 64 : V <= 1024 ? (n + 3) / 4 : n));
+#define L(THREADS, ...) hipLaunchKernelGGL((__VA_ARGS__), grid, dim3(THREADS), 0, st, z + r0 * ld, ld, a, label + r0, n, V)
+#define K(E, W) L(W > 1 ? 64 * W : 256, sample_wave_kernel<Z, E, W>)
+    if (V <= FEW)
+      L(64, sample_few_kernel<Z>);
+    else if (V <= 64)
+      K(1, 1);
+    else if (V <= 128)
+      K(2, 1);
+    else if (V <= 256)
+      K(4, 1);
+    else if (V <= 512)
+      K(8, 1);
+    else if (V <= 1024)
+      K(16, 1);
+    else if (V <= 2048)
+      K(16, 2);
+    else if (V <= 4096)
+      K(16, 4);
+    else
+      K(16, 8);
 #undef K
+#undef L
+  }
   return hipGetLastError() == hipSuccess ? TTK_OK : TTK_ELAUNCH;
 }
 

@@ -146,3 +146,31 @@ def test_a_row_of_as_many_columns_as_are_accepted():
         assert torch.equal(dw[a:a + step].float(), x[a:a + step].float().square())
     del x, y, dx, dw, db
     torch.cuda.empty_cache()
+
+
+@gpu
+@pytest.mark.parametrize("V,rows", [(3, (1 << 32) + 70), (17, (1 << 26) + 5), (1000, (1 << 26) + 5), (1025, (1 << 25) + 3), (2049, (1 << 24) + 3),
+                                    (4097, (1 << 23) + 3)])
+def test_more_rows_than_a_launch_counts_threads_for(V, rows):
+    """One row of equal logits broadcast to many: the label is floor(u V), exact in 64 bits; parameters of their own at the end."""
+    from tensornetworksfork_amd import ops
+    dev = S._dev()
+    pattern = torch.rand(1000003, generator=torch.Generator().manual_seed(V)).to(dev)
+    u = pattern.repeat(rows // pattern.numel() + 1)[:rows]
+    Z = torch.full((1, V), 0.5, dtype=BF16, device=dev).expand(rows, V)
+    if V == 3:
+        got = ops.sample(Z, u)
+    else:
+        P = torch.ones(rows, device=dev)
+        K = torch.zeros(rows, dtype=torch.int32, device=dev)
+        P[-2], K[-1] = 0.5, 2
+        got = ops.sample(Z, u, top_k=K, top_p=P)
+        # the last two rows keep ceil(V / 2) elements and two
+        for i, n in ((rows - 2, (V + 1) // 2), (rows - 1, 2)):
+            assert int(got[i]) == int(np.floor(float(u[i]) * n))
+        got, u = got[:-2], u[:-2]
+    step = 1 << 28
+    for a in range(0, got.numel(), step):
+        assert torch.equal(got[a:a + step], (u[a:a + step].double() * V).floor().long())
+    del got, u, Z
+    torch.cuda.empty_cache()
