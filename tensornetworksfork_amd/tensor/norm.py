@@ -9,7 +9,8 @@ the whole set.  `offset` may be an int64 device tensor of one element, read when
 new mask on every replay if the graph (or the caller between replays) advances it.  Its value has to stay until the backward
 pass has run; changing it in place before that raises, as for any tensor autograd has saved.
 
-Gradients of gradients are not defined here (asking for them raises).  Graphs: capture the forward pass together with its
+Gradients of gradients and forward-mode derivatives (dual tensors, torch.func.jvp) are not defined here (asking for them
+raises).  Graphs: capture the forward pass together with its
 backward pass, while no eager graph of the same leaves is alive (autograd adds up a leaf's gradient on the stream its first
 graph was recorded on, which a capture on another stream does not survive).  The modules count their masks on the host: a
 captured pass replays one mask (pass an `offset` tensor to `layer_norm` / `dropout` for new ones), and a pass that is computed
@@ -17,6 +18,7 @@ twice, as by checkpointing, draws two; `offset` is a plain attribute, to be kept
 """
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import ops
@@ -46,7 +48,9 @@ def _once(backward):
 
 
 def _recorded(*ts):
-    """Whether autograd has to remember the call."""
+    """Whether autograd has to remember the call.  Dual tensors, which require no gradient by themselves, are refused."""
+    if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise ops._lib.TTKError("layer norm and dropout have no forward-mode derivatives")
     return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in ts)
 
 

@@ -12,3 +12,33 @@ def test_sizes_beyond_32_bits_are_counted_in_64():
             assert L.ttk_sample_ws_bytes(dtype, rows, 9000) == L.ttk_sample_ws_bytes(dtype, 1 << 20, 9000) > 0
             for cols in (3, 40, 600, 5000, 16000, 20000):
                 assert L.ttk_layer_norm_backward_ws_bytes(dtype, rows, cols) >= L.ttk_layer_norm_backward_ws_bytes(dtype, 1 << 20, cols) > 0
+
+
+def _stub_kernels(monkeypatch):
+    """The rows' kernels replaced by what passes the values on: which graph autograd records is the host's matter."""
+    from tensornetworksfork_amd import ops
+    monkeypatch.setattr(ops, "layer_norm", lambda x, *a, stats=True, **k: (x.detach().clone(), x[..., 0].detach(), x[..., 0].detach()))
+    monkeypatch.setattr(ops, "dropout", lambda x, *a, **k: x.detach().clone())
+
+
+def test_forward_mode_derivatives_are_refused(monkeypatch):
+    """A dual tensor requires no gradient: without a look at its tangent the result would carry none, in silence."""
+    import torch.autograd.forward_ad as fw
+    from tensornetworksfork_amd import _lib
+    from tensornetworksfork_amd.tensor.norm import Dropout, LayerNorm, dropout, layer_norm
+    _stub_kernels(monkeypatch)
+    x, w, v = torch.randn(3, 4), torch.randn(4), torch.randn(4)
+    calls = [lambda a, b, c: layer_norm(a, b, c), lambda a, b, c: layer_norm(x, b, c), lambda a, b, c: layer_norm(x, w, c),
+             lambda a, b, c: dropout(a, 0.5, 1), lambda a, b, c: LayerNorm(4)(a), lambda a, b, c: Dropout(0.5)(a),
+             lambda a, b, c: layer_norm(a.t(), None, None), lambda a, b, c: layer_norm(a.clone().requires_grad_(True), b, c)]
+    for f in calls:
+        assert f(x, w, v) is not None
+        with fw.dual_level():
+            dual = [fw.make_dual(t, torch.ones_like(t)) for t in (x, w, v)]
+            with pytest.raises(_lib.TTKError):
+                f(*dual)
+            with torch.no_grad(), pytest.raises(_lib.TTKError):
+                f(*dual)
+            f(x, w, v)                                    # tensors without a tangent pass at any level
+    with pytest.raises(_lib.TTKError):
+        torch.func.jvp(lambda a: layer_norm(a, w, v), (x,), (x,))
