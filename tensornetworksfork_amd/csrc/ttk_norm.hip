@@ -557,7 +557,6 @@ __global__ __launch_bounds__(group_threads(LANES), NV <= 2 || LANES >= 512 ? 4 :
     lane_weights<RAGGED, A, W, LANES, NV, N>(wv, w, lane, cols, A(1));
     lane_weights<RAGGED, A, W, LANES, NV, N>(bv, b, lane, cols, A(0));
   }
-  const A inv = A(1) / (A)cols;
   const int64_t step = (int64_t)gridDim.x * RPB;
   Vec<X> next[NV];
   load_row<RAGGED, X, LANES, NV>(next, x + ((int64_t)blockIdx.x * RPB + sub) * ldx, lane, cols, (int64_t)blockIdx.x * RPB + sub < rows);
@@ -574,7 +573,7 @@ __global__ __launch_bounds__(group_threads(LANES), NV <= 2 || LANES >= 512 ? 4 :
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < N; ++j) s += v[i].get(j);
-    const A mean = row_sum<LANES>(s, buf[0]) * inv;
+    const A mean = row_sum<LANES>(s, buf[0]) / (A)cols;      // (times 1 / cols the mean of a constant row misses it)
     if constexpr (WIDE)
 #pragma unroll
       for (int i = 0; i < NV; ++i) v[i].forget();
@@ -586,7 +585,7 @@ __global__ __launch_bounds__(group_threads(LANES), NV <= 2 || LANES >= 512 ? 4 :
         const A d = (i * LANES + lane) * N + j < cols ? v[i].get(j) - mean : A(0);
         q += d * d;
       }
-    const A rstd = A(1) / sqrt(row_sum<LANES>(q, buf[1]) * inv + (A)eps);
+    const A rstd = A(1) / sqrt(row_sum<LANES>(q, buf[1]) / (A)cols + (A)eps);
     if (!live) continue;
     if constexpr (WIDE)
 #pragma unroll
@@ -625,7 +624,7 @@ __global__ __launch_bounds__(group_threads(LANES)) void ln_bwd_group_kernel(
   __shared__ A buf[2][LANES > 64 ? 32 : 1];
   const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
   const uint64_t e0 = drop_base(drop);
-  const A scale = (A)drop.scale, inv = A(1) / (A)cols;
+  const A scale = (A)drop.scale;
   A aw[NV][N], ab[NV][N], wv[NV][N];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
@@ -679,8 +678,8 @@ __global__ __launch_bounds__(group_threads(LANES)) void ln_bwd_group_kernel(
     }
     if (!dx) continue;
     row_sum2<LANES>(s1, s2, buf[turn]);
-    s1 *= inv;
-    s2 *= inv;
+    s1 /= (A)cols;
+    s2 /= (A)cols;
     if (!live) continue;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {

@@ -174,3 +174,23 @@ def test_more_rows_than_a_launch_counts_threads_for(V, rows):
         assert torch.equal(got[a:a + step], (u[a:a + step].double() * V).floor().long())
     del got, u, Z
     torch.cuda.empty_cache()
+
+
+@gpu
+@pytest.mark.parametrize("dtype,wdtype", N.TYPES)
+@pytest.mark.parametrize("cols", [7, 24, 33, 48, 100, 333, 784, 1000, 1500, 2300, 5120, 6001, 10007, 16383, 20011])
+def test_constant_rows_are_zero(cols, dtype, wdtype):
+    """Rows of one whole number: their sums are exact (below 2^24), so the mean is the number itself and y is 0, whatever the
+    layout; a constant gradient has no part that the norm passes on."""
+    from tensornetworksfork_amd import ops
+    dev = N._dev()
+    values = [255.0, 1000.0, 3.0, -7.0] if cols < 16000 else [255.0, 3.0, -7.0, 11.0]
+    x = torch.tensor(values, dtype=F64)[:, None].expand(4, cols).to(dtype).contiguous().to(dev)
+    assert max(abs(float(v)) for v in x[:, 0]) * cols < 1 << 24
+    w = torch.full((cols,), 3.0, dtype=wdtype, device=dev)
+    for ww in (None, w):
+        y, mean, rstd = ops.layer_norm(x, ww)
+        assert bool((y == 0).all()) and torch.equal(mean, x[:, 0].to(mean.dtype))
+        dy = torch.tensor([3.0, 255.0, -7.0, 1.0], dtype=F64)[:, None].expand(4, cols).to(dtype).contiguous().to(dev)
+        dx, dw, db = ops.layer_norm_backward(dy, x, mean, rstd, ww, wdtype=wdtype)
+        assert bool((dx == 0).all()) and bool((dw == 0).all()) and bool((db == 252).all())
