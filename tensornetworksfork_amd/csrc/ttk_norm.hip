@@ -2,7 +2,7 @@
 // column sums of the weight's and bias' gradient) and dropout from a counter-based generator.
 //
 // Element types: float64, float32, bfloat16, float16 in memory; statistics, products and sums are float32 (float64 for
-// float64 rows), and one rounding to the element type ends each output.
+// float64 rows, and in the sums of rows that the registers do not hold), and one rounding to the element type ends each output.
 //
 // Dropout.  Element number e = offset + index is kept iff word e mod 4 of Philox4x32-10 (J. Salmon, M. Moraes, R. Dror,
 // D. Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC 2011) with key = seed and counter = (e div 4, 0, 0) is at
@@ -285,20 +285,20 @@ __global__ __launch_bounds__(LONG_THREADS) void ln_fwd_long_kernel(const X* __re
                                                                    typename Acc<X>::type* __restrict__ rstd_out, int64_t rows,
                                                                    int cols, double eps, Drop drop) {
   typedef typename Acc<X>::type A;
-  __shared__ A buf[2][32];
+  __shared__ double buf[2][32];
   const uint64_t e0 = drop_base(drop);
   const A scale = (A)drop.scale;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const X* xr = x + row * ldx;
-    A s = 0;
+    double s = 0;      // (a lane adds cols / 1024 terms one after the other)
     for (int64_t c = threadIdx.x; c < cols; c += LONG_THREADS) s += (A)xr[c];
-    const A mean = block_sum<LONG_THREADS / 64>(s, buf[0]) / (A)cols;
-    A q = 0;
+    const A mean = (A)(block_sum<LONG_THREADS / 64>(s, buf[0]) / (double)cols);
+    double q = 0;
     for (int64_t c = threadIdx.x; c < cols; c += LONG_THREADS) {
       const A d = (A)xr[c] - mean;
       q += d * d;
     }
-    const A rstd = A(1) / sqrt(block_sum<LONG_THREADS / 64>(q, buf[1]) / (A)cols + (A)eps);
+    const A rstd = A(1) / sqrt((A)(block_sum<LONG_THREADS / 64>(q, buf[1]) / (double)cols) + (A)eps);
     for (int64_t c = threadIdx.x; c < cols; c += LONG_THREADS) {
       A v = ((A)xr[c] - mean) * rstd;
       if (w) v *= (A)w[c];
@@ -317,24 +317,23 @@ __global__ __launch_bounds__(LONG_THREADS) void ln_bwd_long_kernel(const X* __re
                                                                    const typename Acc<X>::type* __restrict__ rstd_in,
                                                                    X* __restrict__ dx, int64_t rows, int cols, Drop drop) {
   typedef typename Acc<X>::type A;
-  __shared__ A buf[2][32];
+  __shared__ double buf[2][32];
   const uint64_t e0 = drop_base(drop);
   const A scale = (A)drop.scale;
   int turn = 0;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
     const X *xr = x + row * ldx, *dr = dy + row * lddy;
     const A mean = mean_in[row], rstd = rstd_in[row];
-    A s1 = 0, s2 = 0;
+    double sum1 = 0, sum2 = 0;
     for (int64_t c = threadIdx.x; c < cols; c += LONG_THREADS) {
       A g = (A)dr[c];
       if (drop.mode) g = (keep_bits<1>(drop, e0 + (uint64_t)row * cols + c) & 1) ? g * scale : A(0);
       const A a = w ? g * (A)w[c] : g;
-      s1 += a;
-      s2 += a * (((A)xr[c] - mean) * rstd);
+      sum1 += a;
+      sum2 += a * (((A)xr[c] - mean) * rstd);
     }
-    block_sum2<LONG_THREADS / 64>(s1, s2, buf[turn]);
-    s1 /= (A)cols;
-    s2 /= (A)cols;
+    block_sum2<LONG_THREADS / 64>(sum1, sum2, buf[turn]);
+    const A s1 = (A)(sum1 / (double)cols), s2 = (A)(sum2 / (double)cols);
     for (int64_t c = threadIdx.x; c < cols; c += LONG_THREADS) {
       A g = (A)dr[c];
       if (drop.mode) g = (keep_bits<1>(drop, e0 + (uint64_t)row * cols + c) & 1) ? g * scale : A(0);

@@ -194,3 +194,22 @@ def test_constant_rows_are_zero(cols, dtype, wdtype):
         dy = torch.tensor([3.0, 255.0, -7.0, 1.0], dtype=F64)[:, None].expand(4, cols).to(dtype).contiguous().to(dev)
         dx, dw, db = ops.layer_norm_backward(dy, x, mean, rstd, ww, wdtype=wdtype)
         assert bool((dx == 0).all()) and bool((dw == 0).all()) and bool((db == 252).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cols", [200003, 3000001])
+def test_sums_of_millions_of_columns(cols, dtype):
+    """Terms of one sign, of which a running float32 sum loses a part at every step."""
+    from tensornetworksfork_amd import ops
+    dev = N._dev()
+    g = torch.Generator().manual_seed(cols)
+    x = torch.full((3, cols), 1.0 / 3, dtype=F64)
+    x[1] = 0.7 + 0.2 * torch.rand(cols, generator=g, dtype=F64)
+    x[2] += torch.where(torch.arange(cols) % 2 == 0, 0.3, -0.1).to(F64)
+    dy = torch.full((3, cols), 0.1, dtype=F64)
+    dy[1] = 0.1 + 0.2 * torch.rand(cols, generator=g, dtype=F64)
+    x, dy = x.to(dtype), dy.to(dtype)
+    y, mean, rstd = ops.layer_norm(x.to(dev), eps=1e-5)
+    N._check_forward(y, mean, rstd, x, None, None, 1e-5, dtype)
+    N._check_backward(ops.layer_norm_backward(dy.to(dev), x.to(dev), mean, rstd), dy, x, mean, rstd, None, dtype, dtype)
