@@ -656,17 +656,19 @@ __global__ __launch_bounds__(group_threads(LANES)) void ln_bwd_group_kernel(
     if (AHEAD && r0 + step < rows) fetch(row + step);
     A s1 = 0, s2 = 0, ha[HOLD ? NV : 1][N], aa[HOLD ? NV : 1][N];
     uint32_t bits[NV];
-    // (columns behind the row have dy = 0 and add nothing)
+    // Columns behind the row have dy = 0 and add nothing.  Their h is 0 as well: (0 - mean) rstd may lie beyond the type's range,
+    // and 0 times that is no number.
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * LANES + lane) * N;
+      const A mid = c < cols ? mean : A(0);
       if constexpr (!AHEAD) load_weights_or<RAGGED, A, W, N>(wv[i], in_loop_uniform(w), c, cols, A(1));
       if (drop.mode) bits[i] = live ? keep_bits_row<N, NV == 1 ? LANES : 1>(drop, e0 + (uint64_t)row * cols + c) : 0u;
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         A g = gv[i].get(j);
         if (drop.mode) g = (bits[i] >> j & 1) ? g * scale : A(0);
-        const A h = (xv[i].get(j) - mean) * rstd, a = g * wv[i][j];
+        const A d = xv[i].get(j) - mid, h = (RAGGED && c + j >= cols ? A(0) : d) * rstd, a = g * wv[i][j];
         s1 += a;
         s2 += a * h;
         aw[i][j] += g * h;

@@ -213,3 +213,31 @@ def test_sums_of_millions_of_columns(cols, dtype):
     y, mean, rstd = ops.layer_norm(x.to(dev), eps=1e-5)
     N._check_forward(y, mean, rstd, x, None, None, 1e-5, dtype)
     N._check_backward(ops.layer_norm_backward(dy.to(dev), x.to(dev), mean, rstd), dy, x, mean, rstd, None, dtype, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F64, F32, BF16])
+@pytest.mark.parametrize("cols", [5, 33, 100, 129, 300, 784, 1001, 2300, 5000, 6001, 10007, 16383])
+def test_what_stands_behind_a_row_stays_out_of_its_sums(cols, dtype):
+    """Lanes behind the row's end hold 0, which lies -mean rstd (beyond the type's range here) from the mean."""
+    from tensornetworksfork_amd import ops
+    dev = N._dev()
+    c, eps = (2.0 ** 1000, 1e-300) if dtype == F64 else (2.0 ** 80, 1e-36)
+    g = torch.Generator().manual_seed(cols)
+    x = torch.full((9, cols), c, dtype=dtype)
+    dy = torch.randn(9, cols, generator=g, dtype=F64).to(dtype)
+    w = (1 + 0.3 * torch.randn(cols, generator=g, dtype=F64)).to(dtype)
+    y, mean, rstd = ops.layer_norm(x.to(dev), eps=eps)
+    assert bool((y == 0).all()) and bool((mean.double() == c).all())
+    for p in (0.0, 0.3):
+        keep = R.keep_mask(x.numel(), p, 5, 3).reshape(x.shape)
+        gm = torch.where(keep, dy.double() / (1 - p), torch.zeros_like(dy, dtype=F64))
+        got = ops.layer_norm_backward(dy.to(dev), x.to(dev), mean, rstd, w.to(dev), p=p, seed=5, offset=3)
+        assert bool((got[1] == 0).all())
+        m, r = mean.cpu().double().unsqueeze(-1), rstd.cpu().double().unsqueeze(-1)
+        dx, _, db, _, a = R.norm_backward(gm, x, m, r, w)
+        with_max = dx.abs() <= torch.finfo(dtype).max
+        u, D = R.unit(dtype), N._depth(cols)
+        tol = r * u * (6 * a.abs() + (D + 6) * a.abs().mean(-1, keepdim=True))
+        tol = tol + R.half_step(dtype) * (dx.abs() + tol) + R.tiny(dtype)
+        assert bool((((got[0].cpu().double() - dx).abs() <= tol) | ~with_max).all())
