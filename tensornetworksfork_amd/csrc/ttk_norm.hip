@@ -1144,12 +1144,16 @@ Layout row_layout(int dtype, int cols, bool dense, bool backward) {
 }
 
 // Workgroups of a launch: as many as are resident at a time, each walks its share of the rows (the backward pass leaves
-// one partial row of column sums per workgroup).
+// one partial row of column sums per workgroup).  Backward, a lane adds LANE_ROWS rows at most in its registers' float32: the
+// partials are added in 64 bits (2^22 rows of one value: 16384 in a row were off by 800 to 2700 half steps, 480 are by 30).
+constexpr int64_t LANE_ROWS = 480;
+
 int row_groups(const Layout& l, int64_t rows, bool backward) {
   const int64_t rpb = l.lanes == 1 ? 64 * SHORT_WAVES : std::max(1, 256 / l.lanes);
   const int per_cu = l.lanes <= 256 ? (backward ? 4 : l.nv >= 4 ? 4 : 8) : l.lanes == 512 ? (backward ? (l.nv >= 4 ? 1 : 2) : 4)
                                                                                          : (backward ? 1 : 2);
-  return (int)std::min((rows + rpb - 1) / rpb, (int64_t)(per_cu * CUS));
+  const int64_t turns = (rows + rpb - 1) / rpb, resident = per_cu * CUS;
+  return (int)std::min(turns, backward ? std::max(resident, (turns + LANE_ROWS - 1) / LANE_ROWS) : resident);
 }
 
 // column sums of rows the registers do not hold: a thread a column over a range of rows

@@ -241,3 +241,22 @@ def test_what_stands_behind_a_row_stays_out_of_its_sums(cols, dtype):
         tol = r * u * (6 * a.abs() + (D + 6) * a.abs().mean(-1, keepdim=True))
         tol = tol + R.half_step(dtype) * (dx.abs() + tol) + R.tiny(dtype)
         assert bool((((got[0].cpu().double() - dx).abs() <= tol) | ~with_max).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype,cols,rows", [(F32, 4100, 1 << 22), (BF16, 9000, 1 << 21), (F32, 300, 1 << 24), (F16, 20, 1 << 26), (F32, 784, 1 << 23)])
+def test_column_sums_of_millions_of_rows(dtype, cols, rows):
+    """The same gradient in every row, of which a running float32 sum loses a part at every step (one row in memory, broadcast)."""
+    from tensornetworksfork_amd import ops
+    dev = N._dev()
+    dy = torch.full((1, cols), 1.0 / 3, dtype=F64).to(dtype)
+    x = torch.full((1, cols), 1.0, dtype=dtype)
+    x[:, ::2] = -1.0
+    X, DY = (t.to(dev).expand(rows, cols) for t in (x, dy))
+    mean, rstd = torch.full((rows,), 0.25, device=dev), torch.full((rows,), 0.7, device=dev)
+    dx, dw, db = ops.layer_norm_backward(DY, X, mean, rstd, need=(False, True, True), wdtype=F32 if dtype != F32 else None)
+    g, h = dy[0].double(), (x[0].double() - 0.25) * float(torch.tensor(0.7))
+    # 512 terms in a row in one lane, 16 across lanes and partials, 6 in a term; one rounding at the end
+    tol = (512 + 16 + 6 + 1) * R.U32
+    assert bool(((db.cpu().double() / rows - g).abs() <= tol * g.abs()).all())
+    assert bool(((dw.cpu().double() / rows - g * h).abs() <= tol * (g * h).abs()).all())

@@ -42,3 +42,20 @@ def test_forward_mode_derivatives_are_refused(monkeypatch):
             f(x, w, v)                                    # tensors without a tangent pass at any level
     with pytest.raises(_lib.TTKError):
         torch.func.jvp(lambda a: layer_norm(a, w, v), (x,), (x,))
+
+
+def test_rows_a_lane_adds_are_bounded():
+    """The backward pass leaves a partial row of sums for every 480 rows of a lane or fewer: the workspace grows with the rows."""
+    from tensornetworksfork_amd import _lib
+    L = _lib.lib()
+    for dtype in range(4):
+        size = 8 if dtype == 0 else 4
+        for cols in (1, 8, 20, 32, 33, 100, 784, 1500, 5000, 12000, 16000):
+            if dtype == 0 and cols > 8192:
+                continue                                  # (rows the registers do not hold: added in 64 bits, however many)
+            for rows in (1, 1000, 1 << 20, 1 << 24, 1 << 30):
+                parts = L.ttk_layer_norm_backward_ws_bytes(dtype, rows, cols) // (2 * cols * size)
+                assert parts * 256 * 480 >= rows      # (256 lanes a workgroup, each with a row of its own, at most)
+            # a workgroup a row: 1024 threads of 16 bytes hold no more
+            if cols >= 5000:
+                assert parts * 480 >= 1 << 30
