@@ -532,8 +532,9 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void sample_wave_kernel(const
 //             top-k above what the groups bound cut: the same by histograms over the whole row
 //
 // Elements of -inf do not exist for any of this, nor do weights below 2^-1000 of the largest; min-p is a bound on the value,
-// m + T ln(min_p).  Sums are added in a fixed order, counts are whole numbers, lists are sorted: the label does not depend on
-// the order in which workgroups run.
+// m + T ln(min_p).  Sums are added in a fixed order in float64, counts are whole numbers, lists are sorted: the label does not
+// depend on the order in which workgroups run.  Where LDS atomics add up weights these are whole numbers too: of 2^-48 of the
+// largest for the (at most 8192) elements of a list, two words each for the elements of a whole row.
 //
 // Measured for 512 rows of 131072 bfloat16 (134 MB, read in 26 us at a copy's rate), top-p 0.95, us: maxima 14 (HBM), counts
 // 49 (one 64-bit LDS atomic an element), sums 82 (about 22 instructions an element, 14 of them float64, and a dozen more
@@ -643,7 +644,8 @@ struct RowShared {
   unsigned long long wave_u[T / 64];
   K wave_lo[T / 64], wave_hi[T / 64];
   int n, at, which, last;
-  unsigned long long above;
+  unsigned long long above, above_l;
+  unsigned long long hist_l[T > 256 ? BINS : 1];             // second words (whole rows)
   K cut_key;
   int cut_idx;
 };
@@ -677,14 +679,31 @@ struct RowWeight {
   }
 };
 
-// Weights as whole numbers of 2^-S: sums that do not depend on an order.  S = 62 - log2 V, at most 51: the sum of V of them
-// stays below 2^63.
+// Weights of a list's elements as whole numbers of 2^-48: sums that do not depend on an order.  The sum of LIST_CAP = 2^13 of them
+// stays below 2^62; each is off by half a unit at most, a list by 2^-36 of the largest weight.
 struct Whole {
-  double fixed;      // 2^S
-  __device__ __forceinline__ explicit Whole(int V) : fixed(ldexp(1.0, min(51, 30 + (int)__builtin_clz(V)))) {}
+  static constexpr double FIXED = 0x1p48;
   __device__ __forceinline__ unsigned long long operator()(double w) const {      // w <= 1, rounded
-    return (unsigned long long)__double_as_longlong(w * fixed + 0x1p52) - 0x4330000000000000ull;
+    return (unsigned long long)__double_as_longlong(w * FIXED + 0x1p52) - 0x4330000000000000ull;
   }
+};
+
+// Weights of a whole row's elements in two such words: h 2^-S + l 2^-2S with S = 61 - log2 V, rounded down.  V of either stay
+// below 2^62, and V times the half unit that each weight is off by is 2^-33 of the largest weight at V = 2^30, 2^-72 at 2^17.
+struct Mass {
+  unsigned long long h, l;
+  __device__ __forceinline__ Mass operator+(const Mass& o) const { return {h + o.h, l + o.l}; }
+};
+struct TwoWords {
+  double fixed;      // 2^S <= 2^48
+  __device__ __forceinline__ explicit TwoWords(int V) : fixed(ldexp(1.0, 30 + (int)__builtin_clz(V))) {}
+  __device__ __forceinline__ Mass operator()(double w) const {      // w <= 1
+    const double x = w * fixed, h = fmax(x - 0.5, 0.0) + 0x1p52;   // 2^52 + the whole part of x, or one less where x is whole
+    const double l = (x - (h - 0x1p52)) * fixed + 0x1p52;          // 2^52 + the rest, 0 to 1, in units of 2^-S
+    constexpr unsigned long long ZERO = 0x4330000000000000ull;
+    return {(unsigned long long)__double_as_longlong(h) - ZERO, (unsigned long long)__double_as_longlong(l) - ZERO};
+  }
+  __device__ __forceinline__ double value(const Mass& m) const { return (double)m.h / fixed + (double)m.l / (fixed * fixed); }
 };
 
 template <int T, typename A>
@@ -931,6 +950,28 @@ struct RowSampler {
       if (v[e] && ((double)from < target || from == above) && (double)(from + v[e]) >= target)
         sh.which = PB * threadIdx.x + e, sh.above = from;
       from += v[e];
+    }
+    __syncthreads();
+    return sh.which;
+  }
+
+  // The same for weights in two words; sh.above and sh.above_l hold what the sum starts at.
+  __device__ __forceinline__ int border_bin(const TwoWords& two, double& target, bool share) {
+    const Mass above = {sh.above, sh.above_l};
+    Mass v[PB], mine = {0, 0}, total, from;
+#pragma unroll
+    for (int e = 0; e < PB; ++e) v[e] = {sh.hist[PB * threadIdx.x + e], sh.hist_l[PB * threadIdx.x + e]}, mine = mine + v[e];
+    if (threadIdx.x == 0) sh.which = -1;
+    from.h = above.h + block_scan<T>(mine.h, sh.wave_u, total.h) - mine.h;
+    from.l = above.l + block_scan<T>(mine.l, sh.wave_u, total.l) - mine.l;
+    if (share) target *= two.value(above + total);
+#pragma unroll
+    for (int e = 0; e < PB; ++e) {
+      const Mass to = from + v[e];
+      const bool first = from.h == above.h && from.l == above.l;
+      if ((v[e].h | v[e].l) && (two.value(from) < target || first) && two.value(to) >= target)
+        sh.which = PB * threadIdx.x + e, sh.above = from.h, sh.above_l = from.l;
+      from = to;
     }
     __syncthreads();
     return sh.which;
@@ -1559,7 +1600,7 @@ struct ListCut : RowSampler<Z, TB> {
 
   // cut_at of a list of at most TB elements, a thread an element: what lies in front of it is counted over all others.
   template <bool MASS>
-  __device__ __forceinline__ bool cut_few(Cut<F>& cut, double target, bool share, unsigned long long above) {
+  __device__ __forceinline__ bool cut_few(Cut<F>& cut, double target, bool share, unsigned long long above, bool first) {
     static_assert(sizeof(sh.list) <= SIDE * sizeof(sh.hist[0]) && SIDE + TB <= BINS, "the list and what its elements count for");
     const int i = threadIdx.x;
     Item<Z> e = {0, 0};
@@ -1575,15 +1616,17 @@ struct ListCut : RowSampler<Z, TB> {
     block_scan<TB>(q, sh.wave_u, sum);               // (its barriers cover the list)
     if (share) target *= (double)(above + sum);
     // (the very first element is kept whatever the target)
-    return last_kept(cut, e, in, c, target, above, above == 0) && (double)(above + sum) >= target;
+    return last_kept(cut, e, in, c, target, above, first) && (double)(above + sum) >= target;
   }
 
   // The cut behind the last element with less than `target` in front of it, of the list's elements that `cut` keeps: in
-  // number, or, MASS, in weight (units of 2^-S), of which `above` lies in front of all of them (share: target is a share of
-  // theirs).  False where the list does not hold it.
+  // number, of which `above` lie in front of all of them, or, MASS, in weight (units of 2^-48; share: target is a share of
+  // theirs).  first: nothing lies in front of the list, so that its first element is kept whatever the target.  False where
+  // the list does not hold it.
   template <bool MASS>
-  __device__ __forceinline__ bool cut_at(Cut<F>& cut, double target, bool share, unsigned long long above) {
-    if (c <= TB) return cut_few<MASS>(cut, target, share, above);
+  __device__ __forceinline__ bool cut_at(Cut<F>& cut, double target, bool share, unsigned long long above, bool first) {
+    if (!first && !((double)above < target)) return false;
+    if (c <= TB) return cut_few<MASS>(cut, target, share, above, first);
     K lo = ~(K)0, hi = 0;
     each([&](K k, uint32_t at) {
       if (cut.keeps(value_of<Z>(k), (int)at)) lo = k < lo ? k : lo, hi = k > hi ? k : hi;
@@ -1688,8 +1731,8 @@ struct ListCut : RowSampler<Z, TB> {
   // top-k and top-p of a list that holds the k first elements.  A list of just k needs its cut as well: the draw reads the row
   // again, where the elements that are not listed stand too (a list of fewer holds everything that weighs anything).
   __device__ __forceinline__ bool top_cut(Cut<F>& cut, const RowArgs& a) {
-    if (c >= a.k && !cut_at<false>(cut, (double)a.k, false, 0)) return false;
-    return !(a.P < 1.0) || cut_at<true>(cut, a.P, true, 0);
+    if (c >= a.k && !cut_at<false>(cut, (double)a.k, false, 0, true)) return false;
+    return !(a.P < 1.0) || cut_at<true>(cut, a.P, true, 0, true);
   }
 
   // the list's elements that `cut` and min-p keep join their segments' sums
@@ -1703,7 +1746,7 @@ struct ListCut : RowSampler<Z, TB> {
       if (v >= this->sc.least && cut.keeps(v, (int)at)) atomicAdd(&sh.hist[at / (uint32_t)span], whole(weight(v, true)));
     });
     __syncthreads();
-    for (int i = threadIdx.x; i < SEGS; i += TB) sh.seg[i] += (double)sh.hist[i] / whole.fixed;
+    for (int i = threadIdx.x; i < SEGS; i += TB) sh.seg[i] += (double)sh.hist[i] / Whole::FIXED;
   }
 };
 
@@ -1755,7 +1798,7 @@ __global__ __launch_bounds__(TB) void row_finish_kernel(const Z* __restrict__ lo
     pick = sh.at;
   } else if (path != SLOW) {
     const RowScale<Z> sc(top, a);
-    const RowSampler<Z, TB> sampler = {sh, row_part(p, g, 0, 1, sc.inf), sc, RowWeight<F>(sc.m, a.T, sh.pow2), Whole(g.V)};
+    const RowSampler<Z, TB> sampler = {sh, row_part(p, g, 0, 1, sc.inf), sc, RowWeight<F>(sc.m, a.T, sh.pow2), Whole()};
     ListCut<Z> row(sampler, w);
     Cut<F> cut = {-__builtin_inff(), -1};
     bool good = path == PLAIN;
@@ -1764,13 +1807,13 @@ __global__ __launch_bounds__(TB) void row_finish_kernel(const Z* __restrict__ lo
     } else if (row.c > 0 && row.c <= LIST_CAP) {
       if (path == LIST) good = row.top_cut(cut, a);
       if (path == WINDOW && w.first <= w.last && a.k) {
-        good = row.template cut_at<false>(cut, (double)a.k, false, (unsigned long long)w.before);
+        good = row.template cut_at<false>(cut, (double)a.k, false, (unsigned long long)w.before, w.before == 0);
       } else if (path == WINDOW && w.first <= w.last) {
         double above = 0, total = 0, all_above, all;
         for (int s = threadIdx.x; s < g.segs; s += TB) above += w.above[s], total += w.total[s];
         block_scan<TB>(above, sh.wave_d, all_above);
         block_scan<TB>(total, sh.wave_d, all);
-        good = row.template cut_at<true>(cut, a.P * all * row.whole.fixed, false, (unsigned long long)(all_above * row.whole.fixed));
+        good = row.template cut_at<true>(cut, (a.P * all - all_above) * Whole::FIXED, false, 0, all_above == 0);
       }
     }
     if (good) {
@@ -1847,12 +1890,13 @@ struct RowCut : RowSampler<Z, RT> {
   template <bool MASS>
   __device__ __forceinline__ Cut<F> select(Cut<F> cut, double target) {
     K a = MASS ? Key<Z>::of(this->sc.floor) : Key<Z>::of(-__builtin_inff()) + 1, b = Key<Z>::of(this->sc.m);
-    unsigned long long above = 0;
+    const TwoWords two(row.V);
     bool share = MASS;
+    if (threadIdx.x == 0) sh.above = sh.above_l = 0;
 #pragma unroll 1
     for (;;) {
       __syncthreads();
-      for (int i = threadIdx.x; i < BINS; i += RT) sh.hist[i] = 0;
+      for (int i = threadIdx.x; i < BINS; i += RT) sh.hist[i] = sh.hist_l[i] = 0;
       if (threadIdx.x == 0) sh.n = 0;
       __syncthreads();
       int shift = 0;
@@ -1862,16 +1906,19 @@ struct RowCut : RowSampler<Z, RT> {
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
                   const K k = Key<Z>::of(v[j]);
-                  if (k >= a && k <= b && cut.keeps(v[j], base + j))
-                    atomicAdd(&sh.hist[(int)((b - k) >> shift)], MASS ? whole(weight(v[j], true)) : 1ull);
+                  if (k >= a && k <= b && cut.keeps(v[j], base + j)) {
+                    const int bin = (int)((b - k) >> shift);
+                    const Mass q = MASS ? two(weight(v[j], true)) : Mass{1, 0};
+                    if (q.h) atomicAdd(&sh.hist[bin], q.h);
+                    if (q.l) atomicAdd(&sh.hist_l[bin], q.l);
+                  }
                 }
               },
               NoEnd());
       __syncthreads();
-      const int bin = this->border_bin(above, target, share);
+      const int bin = MASS ? this->border_bin(two, target, share) : this->border_bin(sh.above, target, false);
       share = false;
       if (bin < 0) return cut;                        // fewer elements than asked for: all stay
-      above = sh.above;
       const K top = b - ((K)bin << shift), span = ((K)1 << shift) - 1, bottom = top - a > span ? top - span : a;
       __syncthreads();
       K lo = ~(K)0, hi = 0;
@@ -1901,12 +1948,12 @@ struct RowCut : RowSampler<Z, RT> {
       const int c = sh.n;
       if (c <= Base::CAP) {
         list_sort<Z, RT>(sh, c);
-        return this->template sorted_cut<MASS>(c, target, above);
+        if (MASS) return this->template sorted_cut<true>(c, (target - two.value({sh.above, sh.above_l})) * Whole::FIXED, 0);
+        return this->template sorted_cut<false>(c, target, sh.above);
       }
       if (lo == hi) {                                 // one value: its first elements
         const F v = value_of<Z>(lo);
-        const double each = MASS ? (double)whole(weight(v, true)) : 1.0;
-        const double need = ceil((target - (double)above) / each);
+        const double need = ceil(MASS ? (target - two.value({sh.above, sh.above_l})) / weight(v, true) : target - (double)sh.above);
         return {v, nth_tie(cut, v, need < 1.0 ? 1 : need > (double)c ? c : (int)need)};
       }
       a = lo, b = hi;
@@ -1945,7 +1992,7 @@ __global__ __launch_bounds__(RT) void row_slow_kernel(const Z* __restrict__ logi
   fill_pow2(sh.pow2);
   const RowScale<Z> sc(largest<RT>(work[blockIdx.x].maxima, g.segs * g.per_seg, sh.wave_hi), a);
   const RowSampler<Z, RT> sampler = {sh, row_part(logits + (int64_t)blockIdx.x * ld, g, threadIdx.x >> 6, RW, sc.inf), sc,
-                                     RowWeight<F>(sc.m, a.T, sh.pow2), Whole(g.V)};
+                                     RowWeight<F>(sc.m, a.T, sh.pow2), Whole()};
   RowCut<Z> row(sampler);
   Cut<F> cut = {-__builtin_inff(), -1};
   if (a.k) cut = row.template select<false>(cut, (double)a.k);

@@ -260,3 +260,49 @@ def test_column_sums_of_millions_of_rows(dtype, cols, rows):
     tol = (512 + 16 + 6 + 1) * R.U32
     assert bool(((db.cpu().double() / rows - g).abs() <= tol * g.abs()).all())
     assert bool(((dw.cpu().double() / rows - g * h).abs() <= tol * (g * h).abs()).all())
+
+
+@gpu
+def test_top_p_where_the_tail_weighs_little_and_is_long():
+    """One leader and 2^26 - 1 equal logits of 2^-37 of its weight, together 2^-11: the border of top-p lies among them."""
+    from tensornetworksfork_amd import ops
+    dev = S._dev()
+    V = 1 << 26
+    w = 2.0 ** -37
+    z = torch.full((1, V), -37.0, dtype=BF16, device=dev)
+    z[0, 12345] = 0.0
+    T = float(1 / np.log(2.0))                            # weights 2^z, to a rounding of the exponent (37 2^-52)
+    total = 1 + (V - 1) * w
+    for P, u in ((1 - 2.0 ** -13, 0.99985), (0.99995, 1 - 2.0 ** -13), (0.9997, 0.9999)):
+        target = P * total
+        kept = int(np.ceil((target - 1) / w))             # elements of the tail
+        assert kept > 1 << 20
+        t = u * (1 + kept * w)
+        got = int(ops.sample(z, torch.tensor([u], dtype=F64, device=dev), temperature=T, top_p=P)[0])
+        # by index: 12345 of the tail, the leader, the rest of the tail
+        want = 12345 + (t - 12345 * w - 1) / w + 1 if t > 12345 * w + 1 else 12345
+        # one element for the whole numbers `kept` and the label each, one for the roundings: sums near 1 round at 2^-53, which is
+        # 2^-16 of an element, some thousand times
+        assert want > 12346 and abs(got - want) <= 3
+
+
+@gpu
+@pytest.mark.parametrize("V", [1 << 24, 20011])
+def test_light_elements_of_a_list_keep_their_weights(V):
+    """A leader and 899 (399) elements of 2^-38.5 of its weight, some 2^-29 of it together: u near 1 draws one of them."""
+    from tensornetworksfork_amd import ops
+    dev = S._dev()
+    rows, k = 65, 900 if V > 1 << 20 else 400
+    z = torch.full((1, V), -float("inf"))
+    at = torch.arange(k) * (V // k)
+    z[0, at] = -38.5 * float(np.log(2.0))
+    z[0, 0] = 0.0
+    w = float(np.exp(float(z[0, at[1]])))
+    Z = z.to(dev).expand(rows, V)
+    u = 1 - torch.linspace(0.1, 0.9, rows, dtype=F64) * (k - 1) * w
+    got = ops.sample(Z, u.to(dev), top_k=k).cpu()
+    t = u.numpy() * (1 + (k - 1) * w)
+    want = 1 + np.floor((t - 1) / w)
+    # a list's weights are multiples of 2^-48 of the largest, half a unit off at most: k 2^-49 / w = k 2^-10.5 elements; sums
+    # near 1 round at 2^-53, a hundred of them are 2^-7 of an element
+    assert np.all(np.abs(got.numpy() / (V // k) - want) <= k * 2.0 ** -10.5 + 1)
