@@ -531,7 +531,7 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void sample_wave_kernel(const
 //   slow      the rows whose list does not hold what it should (thousands of equal logits) and those that both top-p and a
 //             top-k above what the groups bound cut: the same by histograms over the whole row
 //
-// Elements of -inf do not exist for any of this, nor do weights below 2^-1000 of the largest; min-p is a bound on the value,
+// Elements of -inf do not exist for any of this, nor do weights that are 0 in 64 bits; min-p is a bound on the value,
 // m + T ln(min_p).  Sums are added in a fixed order in float64, counts are whole numbers, lists are sorted: the label does not
 // depend on the order in which workgroups run.  Where LDS atomics add up weights these are whole numbers too: of 2^-48 of the
 // largest for the (at most 8192) elements of a list, two words each for the elements of a whole row.
@@ -656,7 +656,7 @@ __device__ __forceinline__ void fill_pow2(double* pow2) {
 
 // The weight of Weight, with 2^(n / 32) from a table: 2^((z - m) log2(e) / T) = 2^(n div 32) pow2[n mod 32] 2^(f / 32),
 // |f| <= 1/2, the last factor by its Taylor polynomial (relative error below 3e-15).  The 32 doubles lie in 64 different
-// LDS banks.  m is finite; an element that is not kept weighs 0, one that is lies at most 1000 / log2(e) T below m.
+// LDS banks.  m is finite; an element that is not kept weighs 0, one that is lies at most 1075 / log2(e) T below m.
 template <typename F>
 struct RowWeight {
   double m, c;
@@ -878,12 +878,12 @@ struct RowScale {
   typedef typename Key<Z>::val_t F;
   F m;
   bool inf;
-  F floor, least;      // below `floor` weights are 0 (finite: -inf is below it); below `least` min-p drops
+  F floor, least;      // up to `floor` weights are 0 in 64 bits (finite: -inf is below it); below `least` min-p drops
   __device__ __forceinline__ RowScale(typename Key<Z>::type key, const RowArgs& a) {
     m = value_of<Z>(key);
     inf = m == __builtin_inff();
     if (inf) m = 0;
-    floor = round_up<F>((double)m - 693.147 * a.T);
+    floor = round_up<F>((double)m - 745.1332191019412 * a.T);      // 2^-1075, which rounds to 0
     // (a weight of at least 1: one that rounds to 1 in 64 bits, as in the kernels that compare weights)
     least = a.M > 0 ? round_up<F>((double)m + a.T * (a.M < 1.0 ? log(a.M) : -0x1p-54)) : floor;
     if (least < floor) least = floor;
@@ -1743,7 +1743,12 @@ struct ListCut : RowSampler<Z, TB> {
     __syncthreads();
     each([&](K k, uint32_t at) {
       const F v = value_of<Z>(k);
-      if (v >= this->sc.least && cut.keeps(v, (int)at)) atomicAdd(&sh.hist[at / (uint32_t)span], whole(weight(v, true)));
+      if (v >= this->sc.least && cut.keeps(v, (int)at)) {
+        // (u = 0 draws the first element that weighs anything: its segment must not look empty)
+        const double wt = weight(v, true);
+        const unsigned long long q = whole(wt);
+        if (wt > 0) atomicAdd(&sh.hist[at / (uint32_t)span], q ? q : 1);
+      }
     });
     __syncthreads();
     for (int i = threadIdx.x; i < SEGS; i += TB) sh.seg[i] += (double)sh.hist[i] / Whole::FIXED;

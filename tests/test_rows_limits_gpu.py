@@ -306,3 +306,34 @@ def test_light_elements_of_a_list_keep_their_weights(V):
     # a list's weights are multiples of 2^-48 of the largest, half a unit off at most: k 2^-49 / w = k 2^-10.5 elements; sums
     # near 1 round at 2^-53, a hundred of them are 2^-7 of an element
     assert np.all(np.abs(got.numpy() / (V // k) - want) <= k * 2.0 ** -10.5 + 1)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F64, F32, BF16])
+@pytest.mark.parametrize("V", [10, 60, 1000, 8192, 8193, 50000])
+def test_the_first_kept_element_is_drawn_at_zero(V, dtype):
+    """u = 0 draws the first kept element whose weight is above 0 in 64 bits, however little that is: on every path, down to the
+    smallest numbers there are (2^-1074)."""
+    from tensornetworksfork_amd import ops
+    dev = S._dev()
+    for depth in (10.0, 20.0, 45.0, 60.0, 500.0, 692.0, 700.0, 720.0, 738.0, 760.0):
+        g = torch.Generator().manual_seed(V)
+        z = torch.randn(67, V, generator=g, dtype=F64)
+        z[:, 2:] += 5.0
+        z[:, 0] = -900.0
+        z[:, 1] = z[:, 2:].max(dim=1).values.to(dtype).double() - depth
+        z = z.to(dtype)
+        u = torch.zeros(67, dtype=F64, device=dev)
+        first = 1 if depth < 744 else 2
+        Z = z.to(dev)
+        for kw in (dict(), dict(top_k=V - 1)) + ((dict(top_p=1 - 1e-12),) if depth < 11 else ()):
+            assert bool((ops.sample(Z, u, **kw) == first).all()), (depth, kw)
+        if V > 300:
+            # a list of 300: its lightest element is the first by index
+            y = torch.full_like(Z, -float("inf"))
+            y[:, 1] = Z[:, 1]
+            y[:, V - 299:] = Z[:, V - 299:]
+            y[:, V - 1] = Z[:, 2:].max(dim=1).values
+            for kw in (dict(top_k=300), dict(top_k=V // 2), dict(top_k=300, top_p=1 - 2.0 ** -53)):
+                want = 1 if depth < 744 and (kw.get("top_p", 1.0) == 1.0 or depth < 35) else V - 299
+                assert bool((ops.sample(y, u, **kw) == want).all()), (depth, kw)
