@@ -883,7 +883,8 @@ struct RowScale {
     m = value_of<Z>(key);
     inf = m == __builtin_inff();
     if (inf) m = 0;
-    floor = round_up<F>((double)m - 745.1332191019412 * a.T);      // 2^-1075, which rounds to 0
+    // 2^-1075, which rounds to 0; and float64 logits whose difference overflows, which weigh exp(-inf)
+    floor = round_up<F>((double)m - fmin(745.1332191019412 * a.T, 0x1.fffffffffffffp1023));
     // (a weight of at least 1: one that rounds to 1 in 64 bits, as in the kernels that compare weights)
     least = a.M > 0 ? round_up<F>((double)m + a.T * (a.M < 1.0 ? log(a.M) : -0x1p-54)) : floor;
     if (least < floor) least = floor;

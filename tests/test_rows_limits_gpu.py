@@ -337,3 +337,25 @@ def test_the_first_kept_element_is_drawn_at_zero(V, dtype):
             for kw in (dict(top_k=300), dict(top_k=V // 2), dict(top_k=300, top_p=1 - 2.0 ** -53)):
                 want = 1 if depth < 744 and (kw.get("top_p", 1.0) == 1.0 or depth < 35) else V - 299
                 assert bool((ops.sample(y, u, **kw) == want).all()), (depth, kw)
+
+
+@gpu
+@pytest.mark.parametrize("V", [12, 40, 3000, 8193, 20011])
+def test_differences_that_overflow_weigh_nothing(V):
+    """float64 logits further apart than the largest number: (z - m) / T is -inf in 64 bits whatever T is."""
+    from tensornetworksfork_amd import ops
+    dev = S._dev()
+    MAX = np.finfo(np.float64).max
+    g = torch.Generator().manual_seed(V)
+    z = torch.where(torch.rand(8, V, generator=g) > 0.5, 1.0, -1.0).to(F64) * 1.7e308
+    z[1, 3] = -0.9e307                                    # (one that does not overflow)
+    z[2] *= 0.5                                           # (none does)
+    z[3] = -1.7e308
+    z[3, V // 2] = 1.7e308
+    Z = z.to(dev)
+    for T in (1e305, 1e306, 1e307, 1.7e308, float("inf")):
+        t = torch.full((8,), T, dtype=F64, device=dev)
+        for c in (dict(), dict(P=0.30371), dict(k=max(2, V // 3)), dict(k=2, P=0.6), dict(M=0.25)):
+            u = torch.rand(8, generator=g, dtype=F64)
+            got = ops.sample(Z, u.to(dev), **{**S._kw(c), "temperature": t}).cpu()
+            S._check(z, u, got, dict(c, T=min(T, MAX)), least=0.85)
