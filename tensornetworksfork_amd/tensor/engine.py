@@ -17,6 +17,8 @@ A plain column is the special case a = b = 1 with G = X.
 Per-sample environments of a whole data set stay resident on the device (`_Data`) and are
 dropped only where a node of an earlier / later column changed.
 """
+import weakref
+
 import torch
 
 from .. import ops
@@ -391,6 +393,7 @@ class EngineBase:
         self.net = net
         self.error = None
         self.datasets = []
+        self.recorded = None
         self._gram_ws = {}
         self._abuf = {}
         self._pairs = {}
@@ -408,6 +411,23 @@ class EngineBase:
             gone = self.datasets.pop(0)
             self.drop_pairs(getattr(gone, "xs", ()))
         return d
+
+    def data_for_recorded(self, xs, shared):
+        """(inputs, data set) of a pass whose input gradient may be asked for: detached inputs and what they give.  One such data
+        set is kept, beside the cache above (a sweep's sets stay where they are), for passes on the same tensors with the same
+        contents; the tensors themselves are not kept alive."""
+        seen = self.recorded
+        if seen is not None and seen[0] == shared and len(seen[1]) == len(xs) \
+                and seen[3].xs[0].device == self.net.main_nodes[0].tensor.device \
+                and all(ref() is x and version == x._version for (ref, version), x in zip(seen[1], xs)):
+            return seen[2], seen[3]
+        det = [x.detach() for x in xs]          # new objects, which the cache above never mistakes for others
+        x = det[0] if shared else det
+        d = self.make_data(self.site_list(x))
+        if seen is not None:
+            self.drop_pairs(seen[3].xs)
+        self.recorded = (shared, [(weakref.ref(t), t._version) for t in xs], x, d)
+        return x, d
 
     def output_at(self, d, node, lp, core=None, rows=None):
         """(S, C) prediction through the local problem of `node` (the output is linear in every

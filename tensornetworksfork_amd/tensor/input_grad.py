@@ -21,11 +21,11 @@ class _Forward(torch.autograd.Function):
     @staticmethod
     def forward(ctx, layer, shared, *xs):
         tn = layer.tensor_network
-        det = [x.detach() for x in xs]          # new objects: the engine's data-set cache never mistakes them for others
-        out = tn.forward(det[0] if shared else det)
+        x, d = tn._engine.data_for_recorded(xs, shared)
+        out = tn.forward(x, _data=d)
         if layer.labels is not None:
             out.permute_first(*layer.labels)
-        ctx.engine, ctx.data, ctx.shared = tn._engine, tn._current, shared
+        ctx.engine, ctx.data, ctx.shared = tn._engine, d, shared
         ctx.nodes = [(n, n.tensor, n.tensor._version) for n in _nodes(tn._engine)]
         ctx.like = [(x.dtype, x.device) for x in xs]
         ctx.save_for_backward(*xs)              # the environments are those of these values

@@ -66,6 +66,7 @@ class TensorNetwork:
         from ..parallel import default_shard
         self._shard = default_shard() if shard == "auto" else shard
         self._engine.datasets = []
+        self._engine.recorded = None
         return self
 
     # ------------------------------------------------------------------ graph
@@ -183,7 +184,7 @@ class TensorNetwork:
     def right_update_stacks(self, node):
         """See left_update_stacks."""
 
-    def set_input(self, x):
+    def set_input(self, x, _data=None):
         """Binds the inputs to the input nodes; True if any binding changed (tensor/network.py:329-345)."""
         changed = False
         tensors = list(x) if isinstance(x, (tuple, list)) else [x] * len(self.input_nodes)
@@ -193,13 +194,16 @@ class TensorNetwork:
                 changed = True
         if changed:
             self.reset_stacks()
-        self._current = self._data_for(x)
+        self._current = self._data_for(x) if _data is None else _data
         return changed
 
     # ------------------------------------------------------------------ forward
-    def forward(self, x, to_tensor=False):
+    def forward(self, x, to_tensor=False, _data=None):
         self._require_chain()
-        self.set_input(x)
+        if _data is None:
+            self.set_input(x)
+        else:
+            self.set_input(x, _data)
         out = self._shape_output(self._predict(self._current))
         return out.tensor if to_tensor else out
 
