@@ -22,14 +22,13 @@ class _Forward(torch.autograd.Function):
     def forward(ctx, layer, shared, *xs):
         tn = layer.tensor_network
         x, d = tn._engine.data_for_recorded(xs, shared)
-        out = tn.forward(x, _data=d)
-        if layer.labels is not None:
-            out.permute_first(*layer.labels)
+        tn.set_input(x, d)
+        y = tn._predict(d)                      # (S, C), in the order of the engine's labels
         ctx.engine, ctx.data, ctx.shared = tn._engine, d, shared
         ctx.nodes = [(n, n.tensor, n.tensor._version) for n in _nodes(tn._engine)]
         ctx.like = [(x.dtype, x.device) for x in xs]
         ctx.save_for_backward(*xs)              # the environments are those of these values
-        return out.tensor.detach()
+        return y
 
     @staticmethod
     @once_differentiable
@@ -72,20 +71,22 @@ def _site_gradient(eng, d, k, g):
     return ops.gemm_rows(A, B, B.shape[1])
 
 
+def _inputs(x):
+    return [t for t in (x if isinstance(x, (list, tuple)) else [x]) if isinstance(t, torch.Tensor)]
+
+
 def wants_input_gradient(layer, x):
-    """Whether a forward pass of `layer` on `x` has to be recorded: grad mode, an input that requires it, a train whose
-    output carries its labels in the engine's order."""
+    """Whether a forward pass of `layer` on `x` has to be recorded: grad mode, an input that requires it, a tensor train."""
     from .engine import ChainEngine
-    xs = x if isinstance(x, (list, tuple)) else [x]
-    if not torch.is_grad_enabled() or not any(isinstance(t, torch.Tensor) and t.requires_grad for t in xs):
+    if not torch.is_grad_enabled() or not any(t.requires_grad for t in _inputs(x)):
         return False
-    tn = layer.tensor_network
-    if type(tn._engine) is not ChainEngine or tn._engine.cols is None:
-        return False
-    want = [lab for lab in (layer.labels or tn.output_labels) if lab in tn._engine.out_labels()]
-    return want == tn._engine.out_labels()
+    eng = layer.tensor_network._engine
+    return type(eng) is ChainEngine and eng.cols is not None
 
 
 def forward(layer, x):
     shared = not isinstance(x, (list, tuple))
-    return _Forward.apply(layer, shared, *([x] if shared else x))
+    out = layer.tensor_network._shape_output(_Forward.apply(layer, shared, *([x] if shared else x)))
+    if layer.labels is not None:
+        out.permute_first(*layer.labels)
+    return out.tensor

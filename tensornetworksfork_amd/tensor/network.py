@@ -198,12 +198,9 @@ class TensorNetwork:
         return changed
 
     # ------------------------------------------------------------------ forward
-    def forward(self, x, to_tensor=False, _data=None):
+    def forward(self, x, to_tensor=False):
         self._require_chain()
-        if _data is None:
-            self.set_input(x)
-        else:
-            self.set_input(x, _data)
+        self.set_input(x)
         out = self._shape_output(self._predict(self._current))
         return out.tensor if to_tensor else out
 

@@ -142,3 +142,22 @@ def test_recorded_passes_do_not_keep_their_inputs_graph_alive(cpu_kernels):
     del h, y
     gc.collect()
     assert ref() is None
+
+
+def test_input_gradient_with_labels_in_another_order(cpu_kernels):
+    """The output's labels may be asked for in any order; the gradient follows them."""
+    layer, x = _train(C=3)
+    g = torch.Generator().manual_seed(1)
+    plain = layer(x)
+    ref_in = x.clone().requires_grad_(True)
+    ref = _plain(layer, [ref_in] * 3)
+    assert torch.allclose(plain, ref, rtol=1e-12) and list(layer.labels) == ["s", "c1"]
+    for order in ((0, 1), (1, 0)):
+        layer.labels = [("s", "c1")[i] for i in order]
+        leaf = x.clone().requires_grad_(True)
+        y = layer(leaf)
+        assert y.requires_grad and torch.equal(y.detach(), plain.permute(order))
+        dy = torch.randn(y.shape, generator=g)
+        got, = torch.autograd.grad(y, leaf, dy)
+        want, = torch.autograd.grad(ref.permute(order), ref_in, dy, retain_graph=True)
+        assert torch.allclose(got, want, rtol=1e-10, atol=1e-12)
