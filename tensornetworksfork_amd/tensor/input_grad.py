@@ -7,7 +7,10 @@ gradient g
 which is an environment step with the core's feature axis in the place of its left bond; a conv or operator column then
 applies its feature node once more (one row GEMM).  Environments are the ones the forward pass's engine caches.
 """
+import warnings
+
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import ops
@@ -82,6 +85,17 @@ def wants_input_gradient(layer, x):
         return False
     eng = layer.tensor_network._engine
     return type(eng) is ChainEngine and eng.cols is not None
+
+
+def warn_of_lost_derivatives(x, out):
+    """Where a derivative was asked for that the pass does not have: other networks than trains, forward mode."""
+    xs = _inputs(x)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in xs) and not out.requires_grad:
+        warnings.warn("only tensor trains have a gradient with respect to their inputs: the output of this network has none",
+                      stacklevel=4)
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in xs) \
+            and forward_ad.unpack_dual(out).tangent is None:
+        warnings.warn("tensor networks have no forward-mode derivative: the output carries none", stacklevel=4)
 
 
 def forward(layer, x):

@@ -135,13 +135,17 @@ class TensorNetworkLayer(nn.Module):
         return super().cpu(*args, **kwargs)
 
     def forward(self, x, to_tensor=True):
-        """The network's output; differentiable with respect to inputs that require a gradient (tensor trains)."""
+        """The network's output; differentiable with respect to inputs that require a gradient (tensor trains; a warning tells
+        where another network's output has none).  As for any torch operation, such an output is detached before numpy()."""
         if to_tensor and input_grad.wants_input_gradient(self, x):
             return input_grad.forward(self, x)
         out = self.tensor_network.forward(x)
         if self.labels is not None:
             out.permute_first(*self.labels)
-        return out.tensor if to_tensor else out
+        if not to_tensor:
+            return out
+        input_grad.warn_of_lost_derivatives(x, out.tensor)
+        return out.tensor
 
     def num_parameters(self):
         return sum(n.tensor.numel() for n in self.tensor_network.train_nodes)

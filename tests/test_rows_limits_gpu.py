@@ -359,3 +359,30 @@ def test_differences_that_overflow_weigh_nothing(V):
             u = torch.rand(8, generator=g, dtype=F64)
             got = ops.sample(Z, u.to(dev), **{**S._kw(c), "temperature": t}).cpu()
             S._check(z, u, got, dict(c, T=min(T, MAX)), least=0.85)
+
+
+@gpu
+def test_layers_on_the_device_tell_what_has_a_gradient():
+    """A float32 train has an input gradient (against differences of a multilinear function: exact but for rounding); a CPD
+    network has none and says so; the values are those of an unrecorded pass either way."""
+    from tensornetworksfork_amd.tensor.layers import CPDLayer, TensorTrainLayer
+    dev = S._dev()
+    layer = TensorTrainLayer(3, 4, 5, output_shape=2, seed=3, dtype=F32).to(dev)
+    x = torch.randn(8, 5, generator=torch.Generator().manual_seed(2)).to(dev)
+    xs = [x.clone().requires_grad_(True), x * 0.5, x + 1.0]
+    y = layer(xs)
+    with torch.no_grad():
+        assert torch.equal(layer([t.detach() for t in xs]), y)
+    dy = torch.linspace(-1, 1, y.numel(), dtype=y.dtype, device=dev).reshape(y.shape)
+    got, = torch.autograd.grad(y, xs[0], dy)
+    assert got.dtype == F32 and got.shape == x.shape
+    # linear in each site's input: sum_j got[s, j] x[s, j] = sum_c dy[s, c] y[s, c]
+    a, b = (got.double() * x.double()).sum(1), (dy.double() * y.detach().double()).sum(1)
+    size = (got.double() * x.double()).abs().sum(1) + (dy.double() * y.detach().double()).abs().sum(1)
+    # float64 arithmetic on float32 nodes, and the gradient rounded to float32: half a step a term
+    assert bool(((a - b).abs() <= 4 * R.U32 * size).all())
+    cpd = CPDLayer(3, 4, 5, output_shape=2, seed=1).to(dev)
+    plain = cpd(x.double())
+    with pytest.warns(UserWarning, match="gradient"):
+        z = cpd(x.double().requires_grad_(True))
+    assert not z.requires_grad and torch.equal(z, plain)

@@ -161,3 +161,31 @@ def test_input_gradient_with_labels_in_another_order(cpu_kernels):
         got, = torch.autograd.grad(y, leaf, dy)
         want, = torch.autograd.grad(ref.permute(order), ref_in, dy, retain_graph=True)
         assert torch.allclose(got, want, rtol=1e-10, atol=1e-12)
+
+
+def test_networks_without_an_input_gradient_say_so(cpu_kernels, monkeypatch):
+    """Their outputs stay what they were, without a gradient: a warning tells who asked for one."""
+    import warnings
+
+    import torch.autograd.forward_ad as fw
+    from tensornetworksfork_amd.tensor.layers import CPDLayer, TensorTrainLayer
+    nets = [CPDLayer(3, 4, 5, output_shape=2, seed=1), TensorTrainLayer(3, 4, 5, output_shape=(2, 3), seed=1)]
+    train = TensorTrainLayer(3, 4, 5, output_shape=2, seed=1)
+    x = torch.randn(6, 5)
+    for net in nets + [train]:      # (kernels are nothing autograd sees: the stand-ins, which are torch operations, would be)
+        def closed(*args, predict=net.tensor_network._predict):
+            with torch.no_grad():
+                return fw.unpack_dual(predict(*args)).primal.clone()
+        monkeypatch.setattr(net.tensor_network, "_predict", closed)
+    for net in nets:
+        with warnings.catch_warnings():
+            warnings.simplefilter("error")
+            plain = net(x)
+            with torch.no_grad():
+                net(x.clone().requires_grad_(True))
+        with pytest.warns(UserWarning, match="gradient"):
+            y = net(x.clone().requires_grad_(True))
+        assert not y.requires_grad and torch.equal(y, plain)
+    for net in nets + [train]:
+        with fw.dual_level(), pytest.warns(UserWarning, match="derivative"):
+            net(fw.make_dual(x, torch.ones_like(x)))
