@@ -110,6 +110,8 @@ class RowFrontEnd:
     from (seed, element number), since the sweeps keep the environments of the rows they were given; the next fit() of the
     same estimator draws the next elements."""
 
+    layer_norm, dropout, _dropout_offset = False, 0.0, 0      # of estimators that were saved without
+
     def _init_front_end(self, layer_norm, dropout):
         if not 0.0 <= float(dropout) < 1.0:
             raise ValueError("dropout must be in [0, 1)")
