@@ -272,9 +272,11 @@ __device__ __forceinline__ void block_sum2(A& a, A& b, A* buf) {
 // ---------------------------------------------------------------------------------------
 // Layer norm, any row length: one workgroup walks a row as often as it needs it (forward: sum, centred squares, output;
 // backward: the two sums, dx; the column sums in a pass of their own).  Rows longer than the registers of a workgroup hold
-// (16384 elements; float64 backward 8192).  Bound by the second and third pass, which L2 serves: 30000 columns 2.1 TB/s
-// forward and 1.8 backward of float32 traffic counted once; few rows of millions of columns leave most of the machine idle
-// (22 rows of 3 million: 0.1 TB/s).  Rows may have up to 2^31 - 1 columns, which are counted in 64 bits.
+// (16384 elements; float64 8192).  Bound by one element a lane and load and by the second and third pass, which L2 serves:
+// 4096 rows of 30000 float32 columns 398 us forward (2.5 TB/s of traffic counted once), 417 us for dx (3.5) and 199 us for the
+// column sums; bfloat16 328, 448 and 242 us.  Few rows of millions of columns leave most of the machine idle (22 rows of 3 million
+// float32: 3.7 ms forward, 3.3 ms for dx, 0.1 and 0.2 TB/s).  Sums over a row are float64 whatever its type (a lane adds cols / 1024
+// terms one after the other; 3 % of the forward pass).  Rows may have up to 2^31 - 1 columns, which are counted in 64 bits.
 // ---------------------------------------------------------------------------------------
 constexpr int LONG_THREADS = 1024;
 
@@ -411,12 +413,14 @@ __global__ __launch_bounds__(1024) void ln_cols_sum_kernel(const A* __restrict__
 // under way while a row is worked on.
 //
 // The backward pass walks many rows a workgroup and keeps each lane's columns of dw and db in registers; they leave as one
-// partial row per workgroup (`part`: [workgroup][dw | db][cols]), so the rows are read once and no atomic orders the sums.
+// partial row per workgroup (`part`: [workgroup][dw | db][cols]), so the rows are read once and no atomic orders the sums.  In
+// the registers they are the rows' arithmetic type, float32 for 16- and 32-bit rows: float64 would take twice the registers of
+// kernels that registers bound.  A lane adds 480 rows at most before its partial is added in float64 (see row_groups).
 //
 // Bound by HBM (a copy reaches 5.1 to 5.4 TB/s) up to the mask of 16-bit rows, whose counter blocks cost as much as their
 // bytes.  Measured: float32 54000 x 784 with dropout, forward 60 us (339 MB, 5.7 TB/s with the 256 MB cache's help), backward
-// 113 us (508 MB, 4.5 TB/s); bfloat16 16384 x 8192 backward 155 us (805 MB, 5.2 TB/s); float16 1021 x 10007 with dropout 28 and
-// 50 us (4 rows a workgroup: latency of a row's barriers, and up to 6 counter blocks a lane and row).
+// 110 us (508 MB, 4.6 TB/s); bfloat16 16384 x 8192 backward 155 us (805 MB, 5.2 TB/s); float16 1021 x 10007 with dropout 29 and
+// 54 us (4 rows a workgroup: latency of a row's barriers, up to 6 counter blocks a lane and row, and backward 54 spilled registers).
 // ---------------------------------------------------------------------------------------
 // RAGGED: the row's length is no multiple of a vector's.  The vector that reaches behind the row is then loaded from where it
 // ends with the row (no load an element, no wait before the values are used) and put right by settle_row.
@@ -1124,7 +1128,16 @@ struct Layout {
 //   float32, 32 columns, backward: 8 lanes 4.9; a lane a row 3.3 (its registers spill); 24 columns: a lane a row 4.7
 //   float64, 16 columns, backward: 8 lanes 4.7; a lane a row 3.6
 //   bfloat16, 8192 columns, forward: 512 lanes of 2 vectors 5.5; 256 of 4 3.7.  16384 columns: 1024 of 2 5.5; 512 of 4 4.5
-//   float32, 16384 columns, backward: 1024 lanes of 4 vectors 3.0 (a few registers spill); 512 of 8 2.2
+//   float32, 16384 columns, backward: 1024 lanes of 4 vectors 3.0; 512 of 8 2.2
+// float64 (1 GiB of rows), as lanes x vectors, the one taken first: 128 columns 64x1 4.4 forward, 4.5 backward, 64x2 4.3, 4.7; 256
+// columns 64x2 4.5, 4.5, 64x4 4.6, 5.4; 512 columns 64x4 5.2, 5.1, 256x2 4.0, 4.5; 1024 columns 256x2 4.8, 4.6, 512x4 3.9 forward,
+// 512x2 4.7 backward; 2048 columns 256x4 5.2 forward, 512x4 5.3, 512x2 5.1 backward, 1024x2 5.6; 4096 columns 512x4 5.2 forward,
+// 1024x4 5.7, 1024x2 5.2 backward, 1024x4 2.5; 8192 columns 1024x4 5.6, 3.6.
+// float32 (512 MB), the same: 512 columns 64x2 6.2, 4.8, 256x2 3.6, 3.7; 1024 columns 64x4 6.0, 4.8, 256x2 5.0, 4.9; 2048 columns 256x2
+// 6.1, 4.7, 512x2 5.0 backward, 512x4 4.6 forward; 4096 columns 256x4 6.3 forward, 512x4 6.3, 512x2 4.8 backward, 1024x2 5.0; 8192
+// columns 512x4 6.4 forward, 1024x4 5.9, 1024x2 4.6 backward, 1024x4 2.7.
+// The backward kernels of 1024 lanes and 2 or 4 vectors spill: 19 to 81 registers of 16-bit rows, 21 (64 where the last vector is
+// incomplete) of float32, 39 (95) of float64 ones.
 Layout row_layout(int dtype, int cols, bool dense, bool backward) {
   if (dense && cols <= (dtype == 0 ? 8 : dtype == 1 ? 24 : 32)) return {1, (cols + 7) / 8 * 8};
   const int n = dtype == 0 ? 2 : dtype == 1 ? 4 : 8;         // elements of a 16-byte vector
