@@ -1159,14 +1159,18 @@ Layout row_layout(int dtype, int cols, bool dense, bool backward) {
 // Workgroups of a launch: as many as are resident at a time, each walks its share of the rows (the backward pass leaves
 // one partial row of column sums per workgroup).  Backward, a lane adds LANE_ROWS rows at most in its registers' float32: the
 // partials are added in 64 bits (2^22 rows of one value: 16384 in a row were off by 800 to 2700 half steps, 480 are by 30).
-constexpr int64_t LANE_ROWS = 480;
+// PART_BYTES of partials are enough for that with any rows and gradients that 288 GB hold (16-bit ones: 288 GB 2 / 480); of one row
+// broadcast to more, a lane adds more.  A launch counts its threads in 32 bits.
+constexpr int64_t LANE_ROWS = 480, PART_BYTES = 5ll << 28;
 
-int row_groups(const Layout& l, int64_t rows, bool backward) {
+int row_groups(const Layout& l, int64_t rows, int cols, int acc_bytes, bool backward) {
   const int64_t rpb = l.lanes == 1 ? 64 * SHORT_WAVES : std::max(1, 256 / l.lanes);
   const int per_cu = l.lanes <= 256 ? (backward ? 4 : l.nv >= 4 ? 4 : 8) : l.lanes == 512 ? (backward ? (l.nv >= 4 ? 1 : 2) : 4)
                                                                                          : (backward ? 1 : 2);
   const int64_t turns = (rows + rpb - 1) / rpb, resident = per_cu * CUS;
-  return (int)std::min(turns, backward ? std::max(resident, (turns + LANE_ROWS - 1) / LANE_ROWS) : resident);
+  if (!backward) return (int)std::min(turns, resident);
+  const int64_t most = std::min(PART_BYTES / (2ll * cols * acc_bytes), (1ll << 31) / (l.lanes == 1 ? 64 * SHORT_WAVES : group_threads(l.lanes)));
+  return (int)std::min(turns, std::max(resident, std::min(most, (turns + LANE_ROWS - 1) / LANE_ROWS)));
 }
 
 // column sums of rows the registers do not hold: a thread a column over a range of rows
@@ -1184,8 +1188,8 @@ ColsPlan cols_plan(int64_t rows, int cols) {
   return p;
 }
 
-int bwd_parts(const Layout& l, int64_t rows, int cols) {
-  return l.lanes ? row_groups(l, rows, true) : cols_plan(rows, cols).splits;
+int bwd_parts(const Layout& l, int64_t rows, int cols, int acc_bytes) {
+  return l.lanes ? row_groups(l, rows, cols, acc_bytes, true) : cols_plan(rows, cols).splits;
 }
 
 template <typename X>
@@ -1247,7 +1251,7 @@ int ln_fwd(const void* x, int64_t ldx, const void* w, const void* b, void* y, vo
                        (const X*)x, ldx, (const W*)w, (const W*)b, (X*)y, (A*)mean, (A*)rstd, rows, cols, eps, d);
     return status();
   }
-  const dim3 grid((unsigned)row_groups(l, rows, false));
+  const dim3 grid((unsigned)row_groups(l, rows, cols, (int)sizeof(A), false));
 #define KR(LANES, NV, R)                                                                                                  \
   hipLaunchKernelGGL((ln_fwd_group_kernel<X, W, LANES, NV, R>), grid, dim3(group_threads(LANES)), 0, st, (const X*)x, ldx,    \
                      (const W*)w, (const W*)b, (X*)y, (A*)mean, (A*)rstd, rows, cols, eps, d)
@@ -1270,7 +1274,7 @@ int ln_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void*
            void* dw, void* db, int64_t rows, int cols, const Drop& d, void* ws, int64_t ws_bytes, hipStream_t st) {
   typedef typename Acc<X>::type A;
   const Layout l = row_layout(type_code<X>(), cols, (ldx == cols && lddy == cols) || rows == 1, true);
-  const int parts = bwd_parts(l, rows, cols);
+  const int parts = bwd_parts(l, rows, cols, (int)sizeof(A));
   const bool sums = dw || db;
   if (sums && (!ws || ws_bytes < (int64_t)parts * 2 * cols * (int64_t)sizeof(A))) return TTK_EWORKSPACE;
   if (sums && (uintptr_t)ws % 8) return TTK_EINVAL;
@@ -1335,8 +1339,10 @@ int ttk_layer_norm(int dtype, int wdtype, const void* x, int64_t ldx, const void
 
 int64_t ttk_layer_norm_backward_ws_bytes(int dtype, int64_t rows, int cols) {
   if (dtype < 0 || dtype > 3 || rows < 1 || cols < 1) return TTK_EINVAL;
-  const int parts = std::max(bwd_parts(row_layout(dtype, cols, true, true), rows, cols), bwd_parts(row_layout(dtype, cols, false, true), rows, cols));
-  return (int64_t)parts * 2 * cols * (dtype == 0 ? 8 : 4);
+  const int size = dtype == 0 ? 8 : 4;
+  const int parts = std::max(bwd_parts(row_layout(dtype, cols, true, true), rows, cols, size),
+                             bwd_parts(row_layout(dtype, cols, false, true), rows, cols, size));
+  return (int64_t)parts * 2 * cols * size;
 }
 
 int ttk_layer_norm_backward(int dtype, int wdtype, const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w,

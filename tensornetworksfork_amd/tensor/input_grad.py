@@ -92,10 +92,10 @@ def warn_of_lost_derivatives(x, out):
     xs = _inputs(x)
     if torch.is_grad_enabled() and any(t.requires_grad for t in xs) and not out.requires_grad:
         warnings.warn("only tensor trains have a gradient with respect to their inputs: the output of this network has none",
-                      stacklevel=4)
+                      stacklevel=5)
     if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in xs) \
             and forward_ad.unpack_dual(out).tangent is None:
-        warnings.warn("tensor networks have no forward-mode derivative: the output carries none", stacklevel=4)
+        warnings.warn("tensor networks have no forward-mode derivative: the output carries none", stacklevel=5)
 
 
 def forward(layer, x):

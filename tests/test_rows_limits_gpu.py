@@ -386,3 +386,20 @@ def test_layers_on_the_device_tell_what_has_a_gradient():
     with pytest.warns(UserWarning, match="gradient"):
         z = cpd(x.double().requires_grad_(True))
     assert not z.requires_grad and torch.equal(z, plain)
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols", [((1 << 31) + 3, 20), (1 << 25, 5000), ((1 << 28) + 1, 300)])
+def test_one_row_broadcast_to_more_than_memory_holds(rows, cols):
+    """Whole numbers: every partial sum is exact however many rows a lane adds, and the workspace stays bounded."""
+    from tensornetworksfork_amd import _lib, ops
+    dev = N._dev()
+    assert _lib.lib().ttk_layer_norm_backward_ws_bytes(1, rows, cols) <= 5 << 28
+    x = (torch.arange(cols) % 3 - 1.0).to(dev)
+    dy = (torch.arange(cols) % 2 + 1.0).to(dev)
+    mean, rstd = torch.zeros(rows, device=dev), torch.ones(rows, device=dev)
+    _, dw, db = ops.layer_norm_backward(dy.expand(rows, cols), x.expand(rows, cols), mean, rstd, need=(False, True, True))
+    assert torch.equal(db.double(), (rows * dy.double()).float().double())
+    assert torch.equal(dw.double(), (rows * (dy * x).double()).float().double())
+    del mean, rstd
+    torch.cuda.empty_cache()

@@ -45,7 +45,8 @@ def test_forward_mode_derivatives_are_refused(monkeypatch):
 
 
 def test_rows_a_lane_adds_are_bounded():
-    """The backward pass leaves a partial row of sums for every 480 rows of a lane or fewer: the workspace grows with the rows."""
+    """The backward pass leaves a partial row of sums for every 480 rows of a lane or fewer: the workspace grows with the rows, as
+    far as rows and gradients fit the memory of a GPU (288 GB); rows that are one row broadcast may be more, but not the workspace."""
     from tensornetworksfork_amd import _lib
     L = _lib.lib()
     for dtype in range(4):
@@ -53,12 +54,15 @@ def test_rows_a_lane_adds_are_bounded():
         for cols in (1, 8, 20, 32, 33, 100, 784, 1500, 5000, 12000, 16000):
             if dtype == 0 and cols > 8192:
                 continue                                  # (rows the registers do not hold: added in 64 bits, however many)
-            for rows in (1, 1000, 1 << 20, 1 << 24, 1 << 30):
-                parts = L.ttk_layer_norm_backward_ws_bytes(dtype, rows, cols) // (2 * cols * size)
-                assert parts * 256 * 480 >= rows      # (256 lanes a workgroup, each with a row of its own, at most)
-            # a workgroup a row: 1024 threads of 16 bytes hold no more
-            if cols >= 5000:
-                assert parts * 480 >= 1 << 30
+            held = 288 * 10 ** 9 // (2 * cols * (8, 4, 2, 2)[dtype])
+            for rows in (1, 1000, 1 << 20, min(1 << 24, held), held, 1 << 31, 1 << 36):
+                need = L.ttk_layer_norm_backward_ws_bytes(dtype, rows, cols)
+                parts = need // (2 * cols * size)
+                assert 0 < need <= 5 << 28
+                if rows <= held:
+                    assert parts * 256 * 480 >= rows      # (256 lanes a workgroup, each with a row of its own, at most)
+                    if cols >= 5000:
+                        assert parts * 480 >= rows        # (a workgroup a row)
 
 
 @pytest.fixture
