@@ -398,6 +398,9 @@ class EngineBase:
         self._abuf = {}
         self._pairs = {}
 
+    def __getstate__(self):
+        return {**self.__dict__, "recorded": None}      # (weak references are neither saved nor copied)
+
     def data_for(self, x, shard=None):
         raw = self.site_list(x)
         for d in self.datasets:

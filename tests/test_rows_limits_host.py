@@ -211,3 +211,20 @@ def test_estimators_saved_before_the_front_end_work():
         x = torch.randn(4, 3)
         assert old._normalise(x) is x and old._drop(x) is x
         assert (old.layer_norm, old.dropout) == (False, 0.0)
+
+
+def test_layers_are_saved_and_copied_after_a_recorded_pass(cpu_kernels):
+    import copy
+    import pickle
+    layer, x = _train()
+    want = layer(x)
+    h = x.clone().requires_grad_(True) * 2.0
+    for t in (x.clone().requires_grad_(True), h):
+        layer(t)
+        for other in (pickle.loads(pickle.dumps(layer)), copy.deepcopy(layer)):
+            assert torch.equal(other(x), want)
+            leaf = x.clone().requires_grad_(True)
+            y = other(leaf)
+            got, = torch.autograd.grad(y, leaf, torch.ones_like(y))
+            y = layer(leaf)
+            assert torch.equal(got, torch.autograd.grad(y, leaf, torch.ones_like(y))[0])
