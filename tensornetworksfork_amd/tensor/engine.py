@@ -389,11 +389,12 @@ _MISSING = object()
 class EngineBase:
     """Shared plumbing of the engines behind TensorNetwork: data-set cache and solver workspaces."""
 
+    recorded = None             # (also of engines that were saved without)
+
     def __init__(self, net):
         self.net = net
         self.error = None
         self.datasets = []
-        self.recorded = None
         self._gram_ws = {}
         self._abuf = {}
         self._pairs = {}

@@ -228,3 +228,7 @@ def test_layers_are_saved_and_copied_after_a_recorded_pass(cpu_kernels):
             got, = torch.autograd.grad(y, leaf, torch.ones_like(y))
             y = layer(leaf)
             assert torch.equal(got, torch.autograd.grad(y, leaf, torch.ones_like(y))[0])
+    # one that was saved before there was such a place
+    old = copy.deepcopy(layer)
+    old.tensor_network._engine.__dict__.pop("recorded", None)
+    assert old(x.clone().requires_grad_(True)).requires_grad and torch.equal(old(x), want)
